@@ -44,6 +44,27 @@ void logprob_grad_inplace(torch::Tensor logits, torch::Tensor targets, torch::Te
                           int64_t vocab_start);
 std::vector<torch::Tensor> ppo_loss_fwd(torch::Tensor x, torch::Tensor old, torch::Tensor adv,
                                         c10::optional<torch::Tensor> w, double denom, double lo, double hi, double c);
+std::vector<torch::Tensor> token_logprob_fwd(torch::Tensor logits, c10::optional<torch::Tensor> tokens,
+                                             c10::optional<torch::Tensor> temp, double temp1, int64_t k, bool entropy,
+                                             int64_t vocab_start, bool open);
+torch::Tensor token_logprob_bwd(torch::Tensor logits, c10::optional<torch::Tensor> tokens,
+                                c10::optional<torch::Tensor> temp, double temp1, torch::Tensor stats,
+                                c10::optional<torch::Tensor> d_logp, c10::optional<torch::Tensor> d_entropy,
+                                int64_t vocab_start, int64_t vocab_total);
+std::vector<torch::Tensor> distill_rows(torch::Tensor logits, torch::Tensor ids, torch::Tensor logq,
+                                        c10::optional<torch::Tensor> weights, c10::optional<torch::Tensor> temp,
+                                        double temp1, double scale, bool tail, bool want_grad, bool inplace);
+std::vector<torch::Tensor> distill_open(torch::Tensor logits, torch::Tensor ids, torch::Tensor logq,
+                                        c10::optional<torch::Tensor> weights, c10::optional<torch::Tensor> temp,
+                                        double temp1, int64_t vocab_start, int64_t vocab_total);
+std::vector<torch::Tensor> distill_finish(torch::Tensor stats, torch::Tensor xc, torch::Tensor ids, torch::Tensor logq,
+                                          c10::optional<torch::Tensor> weights, c10::optional<torch::Tensor> temp,
+                                          double temp1, double scale, bool tail, int64_t vocab_total);
+torch::Tensor distill_grad(torch::Tensor logits, torch::Tensor ids, torch::Tensor coef, torch::Tensor fix,
+                           c10::optional<torch::Tensor> temp, double temp1, int64_t vocab_start, int64_t vocab_total,
+                           bool inplace);
+torch::Tensor weighted_rows_sum(torch::Tensor rows, c10::optional<torch::Tensor> weights, double denom);
+void scale_unless_one(torch::Tensor x, torch::Tensor num, double den);
 void adamw_step(torch::Tensor master, torch::Tensor param, torch::Tensor grad, torch::Tensor m, torch::Tensor v,
                 torch::Tensor clip, double lr, double b1, double b2, double eps, double wd, double bc1, double bc2);
 std::vector<torch::Tensor> tree_attn_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor pk,
@@ -143,6 +164,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("logprob_finalize", &logprob_finalize);
   m.def("logprob_grad_inplace", &logprob_grad_inplace);
   m.def("ppo_loss_fwd", &ppo_loss_fwd);
+  m.def("token_logprob_fwd", &token_logprob_fwd, "log-probs of given tokens, entropy and the k likeliest tokens");
+  m.def("token_logprob_bwd", &token_logprob_bwd, "gradient of log-probs and entropy with respect to the logits");
+  m.def("distill_rows", &distill_rows, "divergence from a teacher's top log-probs (+ gradient), whole vocabulary");
+  m.def("distill_open", &distill_open, "the same on a vocabulary shard: open sums");
+  m.def("distill_finish", &distill_finish, "... rows and gradient factors from the joined sums");
+  m.def("distill_grad", &distill_grad, "... the shard's gradient");
+  m.def("weighted_rows_sum", &weighted_rows_sum, "sum(w * rows) / denom, fixed order");
+  m.def("scale_unless_one", &scale_unless_one, "x *= num / den in place, skipped on the device when that is 1");
   m.def("adamw_step", &adamw_step);
   m.def("tree_attn_fwd", &tree_attn_fwd);
   m.def("tree_attn_bwd", &tree_attn_bwd);

@@ -1,0 +1,265 @@
+"""Distillation from a teacher that is known by its top log-probs.
+
+Per row, a teacher gives ``K`` token ids with log-probs ``log q_j`` (a negative id drops the entry); the
+student has ``p = softmax(x / T)`` over the whole vocabulary.  The divergence is
+
+* ``tail=True``: ``KL(q || p)`` over the given tokens and ONE class of all others,
+  ``sum_j q_j (log q_j - log p_j) + q_r (log q_r - log p_r)``, ``q_r = max(0, 1 - sum_j q_j)``;
+* ``tail=False``: ``KL(q' || p)`` with ``q' = q / sum q`` (so raw top logits do as well).
+
+With ``Q = sum_j q_j + q_r`` its gradient is ``dz_v = Q p_v - q_v`` on the given tokens and
+``(Q - q_r / p_r) p_v`` elsewhere; ``loss = sum_u w_u KL_u / denom``.
+
+The gradient of every row is known as soon as its statistics are, so the forward writes it
+(``csrc/vocab_rows.cu``): the logits are read from memory once and the gradient is written once.  The
+backward only checks that the loss was scaled by ``grad_scale`` as announced, and rescales otherwise.
+:func:`fused_lm_head_topk_distill` goes on to the LM head's own backward inside the forward, like
+:func:`~bridge_b200.ops.logprob.fused_lm_head_ppo`.
+
+Rows of weight 0 and rows without an entry have divergence 0 and gradient 0 whatever their logits hold.
+A given token (``q_j > 0``) without student probability makes the divergence infinite.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+import torch.distributed as dist
+from torch import Tensor
+
+from ._ext import kernels, on_gpu
+from .gemm import gemm
+from .token_logprob import (MAX_TOP, _LN2, _MASKED, check_ids, check_logits, join_shards, log2_scale, picked,
+                            row_floats, shard_sums, split_temperature, tp_world, unit_columns)
+
+
+# ------------------------------------------------------------------------- PyTorch form (CPU, oracle)
+def _open_reference(logits, ids, temp, temp1, vocab_start):
+    """``(R, s)`` of the columns outside the given ids and the given ids' log2-domain logits, of one shard."""
+    xc = logits.to(torch.promote_types(logits.dtype, torch.float32)) * log2_scale(temp, temp1, logits)
+    given = _given(ids, vocab_start, xc)
+    r, s, _ = shard_sums(torch.where(given, torch.full_like(xc, -math.inf), xc))
+    return torch.stack((r, s), dim=1), picked(xc, ids, vocab_start).clamp(min=_MASKED)
+
+
+def _given(ids, vocab_start, like):
+    local = ids - vocab_start
+    here = (local >= 0) & (local < like.shape[1])
+    cols = torch.where(here, local, torch.full_like(local, like.shape[1]))
+    given = torch.zeros((like.shape[0], like.shape[1] + 1), dtype=torch.bool, device=like.device)
+    return given.scatter_(1, cols, True)[:, :-1]
+
+
+def _finish_reference(stats, xc, ids, logq, weights, temp, temp1, scale, tail, total):
+    """Rows, the factor of ``2^(xc - R)`` outside the given ids, and the given ids' gradients (64 bits inside)."""
+    stats, xc, logq = stats.double(), xc.double(), logq.double()
+    valid = (ids >= 0) & (ids < total)
+    none = torch.full_like(logq, -math.inf)
+    logq = torch.where(valid, logq, none)
+    if not tail:
+        norm = torch.logsumexp(logq, dim=1, keepdim=True)
+        logq = torch.where(norm == -math.inf, none, logq - norm)
+    q = torch.exp(logq)
+    some = valid.any(dim=1)
+    if not tail:
+        some = some & (q.sum(dim=1) != 0)
+    same = (ids[:, :, None] == ids[:, None, :]) & valid[:, :, None] & valid[:, None, :]
+    first = valid & ~(torch.tril(same.int(), -1).bool().any(dim=2))
+    share = (same * q[:, None, :]).sum(dim=2)                    # the id's probability, repeats together
+    xc = torch.where(xc <= _MASKED, none, xc)
+    r = torch.where(stats[:, 1] == 0, none[:, 0], stats[:, 0]) if logq.shape[1] else stats[:, 0]
+    m = torch.maximum(r, torch.where(first, xc, none).amax(dim=1))
+    lost = m == -math.inf                                        # no student probability anywhere
+    m = torch.where(lost, torch.zeros_like(m), m)
+    rest = torch.where(stats[:, 1] == 0, torch.zeros_like(m), stats[:, 1] * torch.exp2(r - m))
+    z = torch.where(first, torch.exp2(xc - m[:, None]), torch.zeros_like(xc)).sum(dim=1) + rest
+    log2z = torch.log2(z)
+    logp = _LN2 * (xc - m[:, None] - log2z[:, None])
+    kl = torch.where(q == 0, torch.zeros_like(q), q * (logq - logp)).sum(dim=1)
+    q_rest = (1.0 - q.sum(dim=1)).clamp(min=0.0) if tail else torch.zeros_like(m)
+    total_q = q.sum(dim=1) + q_rest
+    p_rest = rest / z
+    kl = kl + torch.where(q_rest > 0, q_rest * (torch.log(q_rest) - torch.log(p_rest)), torch.zeros_like(m))
+    kl = torch.where(lost & ~torch.isnan(stats[:, 1]), torch.full_like(kl, math.inf), kl)
+    w = torch.ones_like(m) if weights is None else weights.double()
+    it = (1.0 / temp.double()) if temp is not None else torch.full_like(m, 1.0 / temp1)
+    live = some & (w != 0) & ~lost
+    f = torch.where(live, w * scale * it, torch.zeros_like(m))
+    factor = torch.where(live & (stats[:, 1] != 0), f * (total_q * p_rest - q_rest) / stats[:, 1], torch.zeros_like(m))
+    fix = torch.where(live[:, None], f[:, None] * (total_q[:, None] * torch.exp(logp) - share), torch.zeros_like(q))
+    rows = torch.where(some & (w != 0), kl, torch.zeros_like(kl))
+    return rows, torch.stack((stats[:, 0], factor), dim=1), torch.where(valid, fix, torch.zeros_like(fix))
+
+
+def _grad_reference(logits, ids, coef, fix, temp, temp1, vocab_start, total):
+    c = log2_scale(temp, temp1, logits)
+    t = logits.to(c.dtype) * c - coef[:, :1].to(c.dtype)
+    factor = coef[:, 1:].to(c.dtype)
+    given = _given(ids, vocab_start, logits)
+    g = torch.where(given | (factor == 0), torch.zeros_like(t), factor * torch.exp2(t))
+    local = ids - vocab_start
+    here = (ids >= 0) & (ids < total) & (local >= 0) & (local < logits.shape[1])
+    rows, j = torch.nonzero(here, as_tuple=True)
+    g[rows, local[rows, j]] = fix[rows, j].to(g.dtype)
+    return g.to(logits.dtype)
+
+
+# ------------------------------------------------------------------------------------------- one shard
+def _rows_and_grad(logits, ids, logq, weights, temp, temp1, scale, tail, want_grad, inplace, vocab_start, group):
+    """``(KL [U], gradient or None)`` of this rank's shard (a whole vocabulary without a group)."""
+    own, world = on_gpu(logits), tp_world(group)
+    total = logits.shape[1] * world
+    if own and world == 1:
+        rows, grad = kernels().distill_rows(logits, ids, logq, weights, temp, temp1, scale, tail, want_grad, inplace)
+        return rows, (grad if want_grad else None)
+    if own:
+        stats, xc = kernels().distill_open(logits, ids, logq, weights, temp, temp1, vocab_start, total)
+    else:
+        stats, xc = _open_reference(logits, ids, temp, temp1, vocab_start)
+    if world > 1:
+        r, s = stats.unbind(1)
+        r, s, _ = join_shards(r, s, torch.zeros_like(s), group)
+        stats = torch.stack((r, s), dim=1)
+        dist.all_reduce(xc, group=group)
+    if own:
+        rows, coef, fix = kernels().distill_finish(stats, xc, ids, logq, weights, temp, temp1, scale, tail, total)
+        grad = kernels().distill_grad(logits, ids, coef, fix, temp, temp1, vocab_start, total,
+                                      inplace) if want_grad else None
+        return rows, grad
+    rows, coef, fix = _finish_reference(stats, xc, ids, logq, weights, temp, temp1, scale, tail, total)
+    grad = _grad_reference(logits, ids, coef, fix, temp, temp1, vocab_start, total) if want_grad else None
+    return rows.to(torch.promote_types(logits.dtype, torch.float32)), grad
+
+
+def _weighted_sum(rows, weights, denom):
+    if on_gpu(rows):
+        return kernels().weighted_rows_sum(rows, weights, denom)
+    if weights is None:
+        return rows.sum() / denom
+    return torch.where(weights != 0, rows * weights.to(rows.dtype), torch.zeros_like(rows)).sum() / denom
+
+
+def _scale_by(grad, dloss, grad_scale):
+    if on_gpu(grad):
+        kernels().scale_unless_one(grad, dloss.float(), grad_scale)
+        return grad
+    return grad * (dloss / grad_scale).to(grad.dtype)
+
+
+class _TopkDistillFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ids, logq, weights, temp, temp1, tail, denom, grad_scale, vocab_start, group):
+        rows, grad = _rows_and_grad(logits, ids, logq, weights, temp, temp1, grad_scale / denom, tail,
+                                    ctx.needs_input_grad[0], False, vocab_start, group)
+        ctx.grad, ctx.grad_scale = grad, grad_scale
+        ctx.mark_non_differentiable(rows)
+        return _weighted_sum(rows, weights, denom), rows
+
+    @staticmethod
+    def backward(ctx, dloss, _drows):
+        grad, ctx.grad = ctx.grad, None        # handed on without a copy, so there is one backward
+        if grad is None:
+            raise RuntimeError("topk_distill_loss: the gradient was already taken by an earlier backward")
+        return (_scale_by(grad, dloss, ctx.grad_scale),) + (None,) * 10
+
+
+class _FusedHeadDistillFn(torch.autograd.Function):
+    """LM head + divergence with the head's backward inside the forward (see the module docstring)."""
+
+    @staticmethod
+    def forward(ctx, h, weight, ids, logq, weights, temp, temp1, tail, denom, grad_scale, vocab_start, group,
+                chunk_rows):
+        want = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
+        main = getattr(weight, "main_grad", None)
+        dh = torch.empty_like(h) if want else None
+        dw = None
+        parts = []
+        for a in range(0, h.shape[0], chunk_rows):
+            at = slice(a, min(a + chunk_rows, h.shape[0]))
+            lg = gemm(h[at], weight)
+            rows, dlg = _rows_and_grad(lg, ids[at], logq[at], None if weights is None else weights[at],
+                                       None if temp is None else temp[at], temp1, grad_scale / denom, tail, want,
+                                       want, vocab_start, group)
+            parts.append(rows)
+            if not want:
+                continue
+            dh[at] = gemm(dlg, weight, b_mn=True)                      # dlogits @ W
+            if not ctx.needs_input_grad[1]:
+                continue
+            if main is not None:                                       # W.main_grad += dlogits^T h
+                gemm(dlg, h[at], a_mn=True, b_mn=True, out=main, accumulate=True)
+            else:
+                part = gemm(dlg, h[at], a_mn=True, b_mn=True).float()
+                dw = part if dw is None else dw.add_(part)
+        rows = torch.cat(parts) if parts else torch.zeros(0, dtype=torch.float32, device=h.device)
+        if want:
+            ctx.save_for_backward(dh, dw if dw is not None else dh.new_empty(0))
+        ctx.grad_scale, ctx.has_dw = grad_scale, dw is not None
+        ctx.mark_non_differentiable(rows)
+        return _weighted_sum(rows, weights, denom), rows
+
+    @staticmethod
+    def backward(ctx, dloss, _drows):
+        dh, dw = ctx.saved_tensors
+        f = dloss.float() / ctx.grad_scale
+        return ((dh.float() * f).to(dh.dtype), (dw * f).to(dh.dtype) if ctx.has_dw else None) + (None,) * 11
+
+
+# ------------------------------------------------------------------------------------------------- API
+def _arguments(name, rows, device, ids, logq, weights, temperature, denom, grad_scale):
+    ids = check_ids(name, "teacher_ids", ids, rows, device)
+    if ids.ndim != 2 or not 1 <= ids.shape[1] <= MAX_TOP:
+        raise ValueError(f"{name}: teacher_ids must be [{rows}, K] with K in 1..{MAX_TOP}, got {tuple(ids.shape)}")
+    if logq.shape != ids.shape:
+        raise ValueError(f"{name}: teacher_logp must be {tuple(ids.shape)}, got {tuple(logq.shape)}")
+    if logq.device != device or not logq.is_floating_point():
+        raise ValueError(f"{name}: teacher_logp must be floating point on {device}")
+    for what, v in (("denom", denom), ("grad_scale", grad_scale)):
+        if not (float(v) > 0.0 and math.isfinite(float(v))):
+            raise ValueError(f"{name}: {what} must be finite and positive, got {v!r}")
+    if weights is not None:
+        weights = row_floats(name, "weights", weights, rows, device)
+    temp, temp1 = split_temperature(name, temperature, rows, device)
+    return ids, logq.detach().float().contiguous(), weights, temp, temp1
+
+
+def topk_distill_loss(logits: Tensor, teacher_ids: Tensor, teacher_logp: Tensor, *, denom: float,
+                      weights: Tensor | None = None, temperature: Tensor | float = 1.0, tail: bool = True,
+                      grad_scale: float = 1.0, vocab_start: int = 0, tp_group=None) -> tuple[Tensor, Tensor]:
+    """``(sum_u w_u KL_u / denom, KL [U])`` of a student's ``logits [U, V]``; only the loss is differentiable.
+
+    ``teacher_ids`` / ``teacher_logp`` are ``[U, K]`` (``K`` up to 256; a negative id drops the entry, an id
+    given twice counts as the sum of its probabilities in the gradient).  ``grad_scale`` announces the factor
+    by which the caller multiplies the loss before ``backward`` (a loss scale); another one costs one more
+    pass over the gradient.  ``backward`` can be called once.  With ``tp_group``, ``logits`` is this rank's
+    equal shard of the vocabulary and ``vocab_start`` its first token.
+    """
+    name = "topk_distill_loss"
+    check_logits(name, logits)
+    args = _arguments(name, logits.shape[0], logits.device, teacher_ids, teacher_logp, weights, temperature, denom,
+                      grad_scale)
+    return _TopkDistillFn.apply(unit_columns(logits), *args, bool(tail), float(denom), float(grad_scale),
+                                int(vocab_start), tp_group)
+
+
+def fused_lm_head_topk_distill(h: Tensor, weight: Tensor, teacher_ids: Tensor, teacher_logp: Tensor, *, denom: float,
+                               weights: Tensor | None = None, temperature: Tensor | float = 1.0, tail: bool = True,
+                               grad_scale: float = 1.0, vocab_start: int = 0, tp_group=None,
+                               chunk_rows: int = 4096) -> tuple[Tensor, Tensor]:
+    """:func:`topk_distill_loss` of hidden rows ``h [U, H]`` under the head ``weight [V_local, H]``.
+
+    The logits exist for ``chunk_rows`` rows at a time and become their own gradient in place; ``dW`` goes
+    into ``weight.main_grad`` where there is one, for a loss multiplied by ``grad_scale``.
+    """
+    name = "fused_lm_head_topk_distill"
+    if h.ndim != 2 or weight.ndim != 2 or h.shape[1] != weight.shape[1]:
+        raise ValueError(f"{name}: h {tuple(h.shape)} does not fit the head {tuple(weight.shape)}")
+    if chunk_rows < 1:
+        raise ValueError(f"{name}: chunk_rows must be positive")
+    args = _arguments(name, h.shape[0], h.device, teacher_ids, teacher_logp, weights, temperature, denom, grad_scale)
+    if on_gpu(h):
+        return _FusedHeadDistillFn.apply(h.contiguous(), weight, *args, bool(tail), float(denom), float(grad_scale),
+                                         int(vocab_start), tp_group, int(chunk_rows))
+    return _TopkDistillFn.apply(torch.matmul(h, weight.t()), *args, bool(tail), float(denom), float(grad_scale),
+                                int(vocab_start), tp_group)
