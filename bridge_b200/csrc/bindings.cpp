@@ -44,16 +44,21 @@ void logprob_grad_inplace(torch::Tensor logits, torch::Tensor targets, torch::Te
                           int64_t vocab_start);
 std::vector<torch::Tensor> ppo_loss_fwd(torch::Tensor x, torch::Tensor old, torch::Tensor adv,
                                         c10::optional<torch::Tensor> w, double denom, double lo, double hi, double c);
-std::vector<torch::Tensor> token_logprob_fwd(torch::Tensor logits, c10::optional<torch::Tensor> tokens,
-                                             c10::optional<torch::Tensor> temp, double temp1, int64_t k, bool entropy,
-                                             int64_t vocab_start, bool open);
+std::vector<torch::Tensor> token_logprobs(torch::Tensor logits, c10::optional<torch::Tensor> tokens,
+                                          c10::optional<torch::Tensor> temp, double temp1, int64_t k, bool entropy);
+std::vector<torch::Tensor> token_logprob_open(torch::Tensor logits, c10::optional<torch::Tensor> tokens,
+                                              c10::optional<torch::Tensor> temp, double temp1, int64_t k, bool entropy,
+                                              int64_t vocab_start);
 torch::Tensor token_logprob_bwd(torch::Tensor logits, c10::optional<torch::Tensor> tokens,
                                 c10::optional<torch::Tensor> temp, double temp1, torch::Tensor stats,
                                 c10::optional<torch::Tensor> d_logp, c10::optional<torch::Tensor> d_entropy,
                                 int64_t vocab_start, int64_t vocab_total);
-std::vector<torch::Tensor> distill_rows(torch::Tensor logits, torch::Tensor ids, torch::Tensor logq,
+std::vector<torch::Tensor> topk_distill(torch::Tensor logits, torch::Tensor ids, torch::Tensor logq,
                                         c10::optional<torch::Tensor> weights, c10::optional<torch::Tensor> temp,
-                                        double temp1, double scale, bool tail, bool want_grad, bool inplace);
+                                        double temp1, bool tail, double denom, double grad_scale);
+torch::Tensor distill_rows_inplace(torch::Tensor logits, torch::Tensor ids, torch::Tensor logq,
+                                   c10::optional<torch::Tensor> weights, c10::optional<torch::Tensor> temp,
+                                   double temp1, double scale, bool tail, bool want_grad);
 std::vector<torch::Tensor> distill_open(torch::Tensor logits, torch::Tensor ids, torch::Tensor logq,
                                         c10::optional<torch::Tensor> weights, c10::optional<torch::Tensor> temp,
                                         double temp1, int64_t vocab_start, int64_t vocab_total);
@@ -164,9 +169,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("logprob_finalize", &logprob_finalize);
   m.def("logprob_grad_inplace", &logprob_grad_inplace);
   m.def("ppo_loss_fwd", &ppo_loss_fwd);
-  m.def("token_logprob_fwd", &token_logprob_fwd, "log-probs of given tokens, entropy and the k likeliest tokens");
+  m.def("token_logprobs", &token_logprobs, "log-probs of given tokens, entropy and the k likeliest tokens (autograd)");
+  m.def("token_logprob_open", &token_logprob_open, "the same on a vocabulary shard: open sums, the shard's likeliest");
   m.def("token_logprob_bwd", &token_logprob_bwd, "gradient of log-probs and entropy with respect to the logits");
-  m.def("distill_rows", &distill_rows, "divergence from a teacher's top log-probs (+ gradient), whole vocabulary");
+  m.def("topk_distill", &topk_distill, "weighted divergence from a teacher's top log-probs (autograd)");
+  m.def("distill_rows_inplace", &distill_rows_inplace, "divergence per row; the logits become their own gradient");
   m.def("distill_open", &distill_open, "the same on a vocabulary shard: open sums");
   m.def("distill_finish", &distill_finish, "... rows and gradient factors from the joined sums");
   m.def("distill_grad", &distill_grad, "... the shard's gradient");

@@ -3,29 +3,38 @@
 //
 // Everything is written in the base-2 domain of one row: c = log2(e) / T, t = x c - R for a reference R near the
 // row's largest x c, e = 2^t, s = sum e.  Then p = e / s, ln p = ln 2 (t - log2 s), and the entropy is
-// ln 2 (log2 s - sum e t / s), whatever R is: a thread keeps its own R, raised only when a logit passes it by more
-// than 8 (sums grow by 2^8 at most), and partial (R, s, sum e t) triples are joined by rescaling.  Statistics are
-// FP32; the few numbers of a row that everything else is scaled by (log s, the given tokens' shares) are FP64.
+// ln 2 (log2 s - sum e t / s), whatever R is: every thread keeps its own R, and partial (R, s, sum e t) triples are
+// joined by rescaling.  Statistics are FP32; the few numbers of a row that everything else is scaled by (log s, the
+// given tokens' shares) are FP64.
 //
 // A logit with x c <= -1e30 (-inf, or a mask of the type's lowest value) carries no probability; a row without any
 // other has log-probs -inf, entropy 0 and gradient 0.
+//
+// A row belongs to one cluster of 1 to 8 blocks, each with a contiguous slice; the blocks exchange partial sums
+// through distributed shared memory, so no workspace and no atomics on global memory are needed and results do not
+// depend on timing.
 #include "vocab_rows.h"
 
 #include <c10/util/Exception.h>
+#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "common.cuh"
 
 namespace {
 
+namespace cg = cooperative_groups;
 using bb::DistillArgs;
 using bb::kMaxTop;
 using bb::RowType;
 using bb::TokenArgs;
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 512;   // at most, per block that holds its slice
+constexpr int kStream = 256;    // per block that streams it
+constexpr int kMaxCluster = 8;
 constexpr int kCand = 2048;     // candidates of the selection kept in shared memory
 constexpr float kMasked = -1e30f;
 constexpr float kSlack = 8.f;
@@ -46,65 +55,149 @@ __device__ __forceinline__ float ex2(float t) {
   return e;
 }
 
-// One row as units of 8 elements on 16-byte boundaries: unit i covers the aligned positions 8i .. 8i + 7, and
-// position a holds token a - shift.  Only the first and the last unit can be partly outside the row.
+// 2^d, log2 z and 1 / a in FP64 to about 1e-10, for the few numbers of a row that are on every block's critical path:
+// short dependent chains (a Taylor series of 2^f on |f| <= 1/2, the artanh series of log2 on [sqrt 1/2, sqrt 2], one
+// Newton step on an FP32 reciprocal) instead of full-precision functions.
+__device__ __forceinline__ double rcp_d(double a) {      // a within FP32's normal range
+  const double r = (double)(1.f / (float)a);
+  return r * (2.0 - a * r);
+}
+__device__ __forceinline__ double exp2_d(double d) {     // 0 below 2^-1000; no branches, so calls overlap
+  const double b = d < -1000.0 ? -1000.0 : (d > 1000.0 ? 1000.0 : d);
+  const int n = __double2int_rn(b);
+  const double f = (b - (double)n) * kLn2;
+  double p = 1.0 / 40320.0;
+  p = fma(p, f, 1.0 / 5040.0);
+  p = fma(p, f, 1.0 / 720.0);
+  p = fma(p, f, 1.0 / 120.0);
+  p = fma(p, f, 1.0 / 24.0);
+  p = fma(p, f, 1.0 / 6.0);
+  p = fma(p, f, 0.5);
+  p = fma(p, f, 1.0);
+  p = fma(p, f, 1.0);
+  p *= __hiloint2double((1023 + n) << 20, 0);
+  return d < -1000.0 ? 0.0 : (d > 1000.0 ? INFINITY : p);
+}
+__device__ __forceinline__ double log2_d(double z) {     // -inf at 0; z >= 0, normal
+  const int hi = __double2hiint(z);
+  const double m1 = __hiloint2double((hi & 0xfffff) | (1023 << 20), __double2loint(z));
+  const bool up = m1 > 1.4142135623730951;
+  const double m = up ? 0.5 * m1 : m1;
+  const int n = (hi >> 20) - 1023 + (up ? 1 : 0);
+  const double s = (m - 1.0) * rcp_d(m + 1.0), q = s * s;
+  double p = 1.0 / 13.0;
+  p = fma(p, q, 1.0 / 11.0);
+  p = fma(p, q, 1.0 / 9.0);
+  p = fma(p, q, 1.0 / 7.0);
+  p = fma(p, q, 1.0 / 5.0);
+  p = fma(p, q, 1.0 / 3.0);
+  p = fma(p, q, 1.0);
+  p = fma(2.0 * kLog2e * s, p, (double)n);
+  return z == 0.0 ? -INFINITY : (z < INFINITY ? p : z);      // (NaN and infinity as they are)
+}
+
+// ------------------------------------------------------------------------------------------------- rows
+// 16 bytes of a row: 8 elements of 16 bits, or 4 of 32.
+template <typename T>
+struct Unit {
+  static constexpr int kE = 16 / (int)sizeof(T);
+  uint4 w;
+
+  __device__ __forceinline__ T get(int j) const { return reinterpret_cast<const T*>(&w)[j]; }
+  __device__ __forceinline__ void set(int j, T v) { reinterpret_cast<T*>(&w)[j] = v; }
+  __device__ __forceinline__ void fill(T v) {
+#pragma unroll
+    for (int j = 0; j < kE; ++j) set(j, v);
+  }
+  __device__ __forceinline__ void mask(unsigned m) {      // -inf where a bit is set
+#pragma unroll
+    for (int j = 0; j < kE; ++j)
+      if (m >> j & 1u) set(j, from_f<T>(-INFINITY));
+  }
+  __device__ __forceinline__ void floats(float* f) const {
+    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+      const uint32_t h[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f[2 * j] = __uint_as_float(h[j] << 16);
+        f[2 * j + 1] = __uint_as_float(h[j] & 0xffff0000u);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kE; ++j) f[j] = to_f(get(j));
+    }
+  }
+  __device__ __forceinline__ void set_pair(int j, float a, float b) {
+    if constexpr (std::is_same_v<T, __nv_bfloat16>) reinterpret_cast<__nv_bfloat162*>(&w)[j] = __floats2bfloat162_rn(a, b);
+    else if constexpr (std::is_same_v<T, __half>) reinterpret_cast<__half2*>(&w)[j] = __floats2half2_rn(a, b);
+    else set(2 * j, a), set(2 * j + 1, b);
+  }
+  __device__ __forceinline__ float max() const {          // NaN does not count
+    if constexpr (sizeof(T) == 4) {
+      return fmaxf(fmaxf(get(0), get(1)), fmaxf(get(2), get(3)));
+    } else {
+      using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+      const T2* h = reinterpret_cast<const T2*>(&w);
+      const T2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+      return fmaxf(to_f(m.x), to_f(m.y));
+    }
+  }
+};
+
+// One row as units on 16-byte boundaries: unit i covers the aligned positions kE i .. kE i + kE - 1, and position a
+// holds token a - shift.  Only the first and the last unit can be partly outside the row.
 template <typename T>
 struct Row {
+  using V = std::remove_const_t<T>;
+  static constexpr int kE = Unit<V>::kE;
   T* p;        // aligned base: row start - shift
   int shift;   // elements between the 16-byte boundary and the row's first element
   int end;     // V + shift
   int units;
 
-  __device__ __forceinline__ Row(T* row, int V) {
+  __device__ __forceinline__ Row(T* row, int vocab) {
     shift = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
     p = row - shift;
-    end = V + shift;
-    units = (end + 7) >> 3;
+    end = vocab + shift;
+    units = (end + kE - 1) / kE;
   }
-  __device__ __forceinline__ bool full(int i) const { return 8 * i >= shift && 8 * i + 8 <= end; }
-  __device__ __forceinline__ void load(int i, float* f) const {
+  __device__ __forceinline__ bool full(int i) const { return kE * i >= shift && kE * i + kE <= end; }
+  __device__ __forceinline__ bool holds(int a) const { return a >= shift && a < end; }
+  __device__ __forceinline__ Unit<V> load(int i) const {
+    Unit<V> u;
     if (full(i)) {
-      if constexpr (sizeof(T) == 4) {
-        const float4 a = reinterpret_cast<const float4*>(p)[2 * i], b = reinterpret_cast<const float4*>(p)[2 * i + 1];
-        f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w;
-        f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-      } else {
-        const uint4 v = reinterpret_cast<const uint4*>(p)[i];
-        const T* h = reinterpret_cast<const T*>(&v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = to_f(h[j]);
-      }
+      u.w = reinterpret_cast<const uint4*>(p)[i];
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int a = 8 * i + j;
-        f[j] = (a >= shift && a < end) ? to_f(p[a]) : -INFINITY;
-      }
+      for (int j = 0; j < kE; ++j) u.set(j, holds(kE * i + j) ? p[kE * i + j] : from_f<V>(-INFINITY));
     }
+    return u;
   }
-  // `vec`: the output's rows start at the same offset from a 16-byte boundary as the input's
-  __device__ __forceinline__ void store(int i, const float* f, bool vec, int in_shift) const {
-    // positions are the INPUT's (in_shift); this row is the output's
-    const int a0 = 8 * i - in_shift + shift;
+  // Stores the unit that covers the INPUT's positions kE i ..; `vec`: this row and the input's start at the same
+  // offset from a 16-byte boundary.
+  __device__ __forceinline__ void store(int i, const Unit<V>& u, bool vec, int in_shift) const {
     if (vec && full(i)) {
-      if constexpr (sizeof(T) == 4) {
-        reinterpret_cast<float4*>(p)[2 * i] = make_float4(f[0], f[1], f[2], f[3]);
-        reinterpret_cast<float4*>(p)[2 * i + 1] = make_float4(f[4], f[5], f[6], f[7]);
-      } else {
-        uint4 v;
-        T* h = reinterpret_cast<T*>(&v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) h[j] = from_f<T>(f[j]);
-        reinterpret_cast<uint4*>(p)[i] = v;
-      }
+      reinterpret_cast<uint4*>(p)[i] = u.w;
     } else {
+      const int a0 = kE * i - in_shift + shift;
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (a0 + j >= shift && a0 + j < end) p[a0 + j] = from_f<T>(f[j]);
+      for (int j = 0; j < kE; ++j)
+        if (holds(a0 + j)) p[a0 + j] = u.get(j);
     }
   }
 };
 
+// The block's slice of the row's units.
+struct Slice {
+  int lo, hi;
+  __device__ __forceinline__ Slice(int units, int blocks, int rank) {
+    const int per = (units + blocks - 1) / blocks;
+    lo = min(units, rank * per);
+    hi = min(units, lo + per);
+  }
+};
+
+// --------------------------------------------------------------------------------------------- statistics
 struct Stat {
   float R, s, et;
 
@@ -115,41 +208,49 @@ struct Stat {
     s *= k;
     R = to;
   }
-  template <bool kEntropy>
-  __device__ __forceinline__ void push8(const float* f, float c) {
-    float top = f[0];
-#pragma unroll
-    for (int j = 1; j < 8; ++j) top = fmaxf(top, f[j]);
-    top *= c;
-    if (top > R + kSlack) raise(top);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float t = fmaf(f[j], c, -R), e = ex2(t);
-      s += e;
-      if (kEntropy) et += e * fmaxf(t, -1e4f);   // e = 0 there; -inf would make it NaN
-    }
-  }
-  __device__ __forceinline__ void join(Stat o) {
-    if (o.R > R) {
-      const Stat m = *this;
-      *this = o;
-      o = m;
-    }
-    if (o.s == 0.f) return;
-    o.raise(R);
-    s += o.s;
-    et += o.et;
-  }
 };
 
-__device__ __forceinline__ Stat warp_join(Stat a) {
+// A thread's running sums, in two chains.
+struct Sums {
+  float R, s[2], et[2];
+
+  __device__ __forceinline__ Sums() : R(kMasked), s{0.f, 0.f}, et{0.f, 0.f} {}
+  __device__ __forceinline__ void raise(float to) {
+    const float d = R - to, k = ex2(d);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Stat b;
-    b.R = __shfl_xor_sync(0xffffffffu, a.R, o);
-    b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-    b.et = __shfl_xor_sync(0xffffffffu, a.et, o);
-    a.join(b);
+    for (int j = 0; j < 2; ++j) {
+      et[j] = k * (et[j] + d * s[j]);
+      s[j] *= k;
+    }
+    R = to;
+  }
+  template <bool kEntropy, typename T>
+  __device__ __forceinline__ void add(const Unit<T>& u, float c) {
+    float f[Unit<T>::kE];
+    u.floats(f);
+#pragma unroll
+    for (int j = 0; j < Unit<T>::kE; ++j) {
+      const float t = fmaf(f[j], c, -R), e = ex2(t);
+      s[j & 1] += e;
+      if (kEntropy) et[j & 1] = fmaf(e, fmaxf(t, -1e4f), et[j & 1]);   // e = 0 there; -inf would make it NaN
+    }
+  }
+  __device__ __forceinline__ Stat get() const { return {R, s[0] + s[1], et[0] + et[1]}; }
+};
+
+__device__ __forceinline__ float warp_top(float v) {
+  asm("redux.sync.max.f32 %0, %0, 0xffffffff;" : "+f"(v));
+  return v;
+}
+
+// Sum over the first kLanes lanes' triples (the other lanes hold none), in every one of those lanes.
+template <int kLanes = 32>
+__device__ __forceinline__ Stat warp_join(Stat a) {
+  a.raise(warp_top(a.R));
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) {
+    a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+    a.et += __shfl_xor_sync(0xffffffffu, a.et, o);
   }
   return a;
 }
@@ -177,6 +278,169 @@ __device__ __forceinline__ double warp_max_d(double v) {
   return v;
 }
 
+// A block's slice on its way through shared memory.  A warp takes batches of 4 x 32 consecutive units, warp w the
+// batches w, w + warps, ...; every lane owns kGroups x 4 slots of 16 bytes that it alone fills (asynchronous copies)
+// and reads, so a warp waits for nothing but its own copies, which run kGroups batches ahead, from before the first
+// batch is needed.  With two passes the batches come once more in reverse order (what was read last is the likeliest
+// to be in L2 still), and their copies start before the first pass ends.
+constexpr int kBatch = 4, kGroups = 3, kSpan = 32 * kBatch;
+static_assert(kBatch == 4, "a batch is written out unit by unit");
+
+__device__ __forceinline__ unsigned long long evict_first() {
+  unsigned long long p;
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+__device__ __forceinline__ unsigned long long evict_normal() {
+  unsigned long long p;
+  asm("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+template <int b>
+__device__ __forceinline__ void store_streaming(uint4* p, uint4 v, unsigned long long policy) {
+  asm volatile("st.global.L2::cache_hint.v4.b32 [%0 + %6], {%1, %2, %3, %4}, %5;" ::"l"(p), "r"(v.x), "r"(v.y),
+               "r"(v.z), "r"(v.w), "l"(policy), "n"(512 * b)
+               : "memory");
+}
+
+// The batches at a slice's ends, out of the way of the others.  Lane's units i, i + 32, ..: those within [lo, hi) can be
+// copied; the others are read one element at a time (-inf outside the slice, which ends at `stop`).
+static __device__ __noinline__ void copy_edge(uint32_t to, const uint4* from, int i, int lo, int hi) {
+  for (int b = 0; b < kBatch; ++b)
+    if (i + 32 * b >= lo && i + 32 * b < hi)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 512 * b), "l"(from + 32 * b) : "memory");
+}
+template <typename T>
+__device__ __noinline__ void read_edge(uint32_t to, const T* p, int shift, int end, int i, int lo, int hi, int stop) {
+  constexpr int kE = Unit<T>::kE;
+  for (int b = 0; b < kBatch; ++b, i += 32) {
+    if (i >= lo && i < hi) continue;
+    Unit<T> u;
+#pragma unroll
+    for (int j = 0; j < kE; ++j) {
+      const int a = kE * i + j;
+      u.set(j, i < stop && a >= shift && a < end ? p[a] : from_f<T>(-INFINITY));
+    }
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + 512 * b), "r"(u.w.x), "r"(u.w.y), "r"(u.w.z),
+                 "r"(u.w.w)
+                 : "memory");
+  }
+}
+
+template <typename T>
+struct Feed {
+  static constexpr int kGroupBytes = kSpan * 16;
+  uint32_t ring;         // this lane's first slot (shared address)
+  const uint4* p;        // this lane's unit of the warp's first batch
+  int first, step;       // the warp's first unit (in the row), units between its batches
+  int lo, hi;            // units of the row that can be copied: full ones, inside the slice
+  int batches, total;    // of this warp: per pass and in all
+  int inner_lo, inner_n; // batches all of whose units can be copied: the first, and how many
+  uint32_t put, get;     // offsets of the slots to fill and to read
+
+  static __host__ __device__ size_t bytes(int threads) { return (size_t)threads / 32 * kGroups * kGroupBytes; }
+  __device__ __forceinline__ Feed(unsigned char* smem, const Row<const T>& row, Slice sl, int passes) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    ring = (uint32_t)__cvta_generic_to_shared(smem) + (warp * kGroups * kGroupBytes + lane * 16);
+    first = sl.lo + warp * kSpan;
+    step = warps * kSpan;
+    p = reinterpret_cast<const uint4*>(row.p) + first + lane;
+    lo = max(sl.lo, row.shift ? 1 : 0);
+    hi = min(sl.hi, row.end / Unit<T>::kE);
+    batches = first < sl.hi ? (sl.hi - first + step - 1) / step : 0;
+    total = batches * passes;
+    inner_lo = first < lo ? 1 : 0;
+    inner_n = max(0, (hi - first >= kSpan ? (hi - first - kSpan) / step + 1 : 0) - inner_lo);
+    put = get = 0;
+    if (passes == 0) inner_n = 0;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      if (inner(g)) issue_inner(p + g * step, total > batches ? evict_normal() : evict_first());
+      else issue(g);
+    }
+  }
+  __device__ __forceinline__ bool inner(int k) const { return (unsigned)(k - inner_lo) < (unsigned)inner_n; }
+  // unit b of a lane's batch: 512 bytes on per unit, in memory and in the slots
+  template <int b>
+  static __device__ __forceinline__ void copy(uint32_t to, const uint4* from, unsigned long long policy) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0 + %3], [%1 + %3], 16, %2;" ::"r"(to), "l"(from),
+                 "l"(policy), "n"(512 * b)
+                 : "memory");
+  }
+  template <int b>
+  static __device__ __forceinline__ void read(uint32_t from, uint4& v) {
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4 + %5];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(from), "n"(512 * b)
+                 : "memory");
+  }
+  static __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+  __device__ __forceinline__ void turn(uint32_t& at) const { at = at == (kGroups - 1) * kGroupBytes ? 0 : at + kGroupBytes; }
+  // Copies of a batch whose units are all there, `from` this lane's first.
+  __device__ __forceinline__ void issue_inner(const uint4* from, unsigned long long policy) {
+    const uint32_t to = ring + put;
+    copy<0>(to, from, policy);
+    copy<1>(to, from, policy);
+    copy<2>(to, from, policy);
+    copy<3>(to, from, policy);
+    turn(put);
+    commit();
+  }
+  // Copies of the q-th batch in order of use: what there is of it.
+  __device__ __forceinline__ void issue(int q) {
+    if (q < total) {
+      const int k = q < batches ? q : 2 * batches - 1 - q;
+      copy_edge(ring + put, p + k * step, first + k * step + (int)(threadIdx.x & 31), lo, hi);
+      turn(put);
+    }
+    commit();
+  }
+  // The next batch, which is number k of the row, is in its slots: units that could not be copied are read here (-inf
+  // outside the slice).
+  __device__ __forceinline__ void wait(int k, const Row<const T>& row, Slice sl) const {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kGroups - 1) : "memory");
+    if (!inner(k))
+      read_edge<T>(ring + get, row.p, row.shift, row.end, first + k * step + (int)(threadIdx.x & 31), lo, hi, sl.hi);
+  }
+  // -inf at position `pos` of that batch; by the lane whose slot it is
+  __device__ __forceinline__ void rule_out(int pos) const {
+    constexpr int kE = Unit<T>::kE;
+    const uint32_t at = ring + get + 512 * (pos / (32 * kE)) + (pos % kE) * (int)sizeof(T);
+    const T v = from_f<T>(-INFINITY);
+    if constexpr (sizeof(T) == 4) asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(__float_as_uint(v)) : "memory");
+    else asm volatile("st.shared.b16 [%0], %1;" ::"r"(at), "h"(reinterpret_cast<const unsigned short&>(v)) : "memory");
+  }
+  // Takes it and starts the copies of the one kGroups on.
+  __device__ __forceinline__ void take(Unit<T>* u) {
+    read<0>(ring + get, u[0].w);
+    read<1>(ring + get, u[1].w);
+    read<2>(ring + get, u[2].w);
+    read<3>(ring + get, u[3].w);
+    turn(get);
+  }
+};
+
+template <typename T, int N>
+__device__ __forceinline__ float units_max(const Unit<T>* u) {
+  if constexpr (sizeof(T) == 4) {
+    float m = u[0].max();
+#pragma unroll
+    for (int n = 1; n < N; ++n) m = fmaxf(m, u[n].max());
+    return m;
+  } else {
+    using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    T2 m[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      m[j] = reinterpret_cast<const T2*>(&u[0].w)[j];
+#pragma unroll
+      for (int n = 1; n < N; ++n) m[j] = __hmax2(m[j], reinterpret_cast<const T2*>(&u[n].w)[j]);
+    }
+    m[0] = __hmax2(__hmax2(m[0], m[1]), __hmax2(m[2], m[3]));
+    return fmaxf(to_f(m[0].x), to_f(m[0].y));
+  }
+}
+
 // Order-preserving map of FP32 to unsigned; -0 counts as +0 and NaN as -inf.
 __device__ __forceinline__ uint32_t order_key(float v) {
   v = fmaxf(v, -INFINITY) + 0.f;
@@ -185,28 +449,60 @@ __device__ __forceinline__ uint32_t order_key(float v) {
 }
 
 // ---------------------------------------------------------------------------------------------- selection
-// The k largest of a row, ties to the lower id.  `best` is the largest key that this thread saw (its stripe: units
-// tid, tid + blockDim, ...).  The k-th largest of the stripes' maxima is a bound that k elements reach, so about k
-// elements lie above it; they are gathered and ranked by counting.  Rows in which more than kCand reach the bound
-// (many equal logits) are settled exactly: the k-th largest key by bisection over the row, all above it, and the
-// first of its equals in index order.
+// The k largest of a row, ties to the lower id.  Every thread knows the largest of its own elements.  In each of the
+// cluster's C blocks the ceil(k / C)-th largest of these maxima is found by bisection; the least of the C results is
+// a bound that at least k elements of the row reach, and few more do.  They are gathered in the leading block and
+// ranked by counting.  Rows in which more than kCand reach the bound (many equal logits) are settled exactly by the
+// leading block: the k-th largest key by bisection over the row, all above it, and the first of its equals in index
+// order.
 struct Select {
   unsigned long long cand[kCand];
   int count, scan[33];
 };
 
+// A value that at least k of the block's `best` reach, and not many more (0: fewer than k threads hold any).
+__device__ __forceinline__ uint32_t kth_max(uint32_t best, bool any, int k) {
+  constexpr int kBits = 20;      // sign, exponent and 11 bits of the significand: every FP16 and BF16 value exactly
+  uint32_t bound = 0;
+  if (__syncthreads_count(any) < k) return 0;
+  for (int bit = 31; bit >= 32 - kBits; --bit) {
+    const uint32_t trial = bound | (1u << bit);
+    const int n = __syncthreads_count(any && best >= trial);
+    if (n < k) continue;
+    bound = trial;
+    if (n <= k + (k >> 3)) break;
+  }
+  return bound;
+}
+
+__device__ __forceinline__ float key_value(uint32_t key) {      // the inverse of order_key
+  return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+}
+
+__device__ __forceinline__ unsigned long long pack_key(uint32_t key, int token) {
+  return ((unsigned long long)key << 32) | (0xffffffffu - (uint32_t)token);
+}
+
 template <typename T>
-__device__ int count_ge(const Row<T>& row, uint32_t key, int* scratch) {
+__device__ __forceinline__ void offer(const Unit<T>& u, int i, uint32_t bound, const Row<const T>& row, Select* lead) {
+  constexpr int kE = Unit<T>::kE;
+#pragma unroll
+  for (int j = 0; j < kE; ++j) {
+    const uint32_t key = order_key(to_f(u.get(j)));
+    if (key >= bound && row.holds(kE * i + j)) {
+      const int at = atomicAdd(&lead->count, 1);
+      if (at < kCand) lead->cand[at] = pack_key(key, kE * i + j - row.shift);
+    }
+  }
+}
+
+template <typename T>
+__device__ int count_ge(const Row<const T>& row, uint32_t key, int* scratch) {
   int n = 0;
   for (int i = threadIdx.x; i < row.units; i += blockDim.x) {
-    float f[8];
-    row.load(i, f);
-    const bool full = row.full(i);
+    const Unit<T> u = row.load(i);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int a = 8 * i + j;
-      n += (full || (a >= row.shift && a < row.end)) && order_key(f[j]) >= key;
-    }
+    for (int j = 0; j < Unit<T>::kE; ++j) n += row.holds(Unit<T>::kE * i + j) && order_key(to_f(u.get(j))) >= key;
   }
   n = __reduce_add_sync(0xffffffffu, n);
   __syncthreads();
@@ -216,70 +512,29 @@ __device__ int count_ge(const Row<T>& row, uint32_t key, int* scratch) {
   return __reduce_add_sync(0xffffffffu, n);
 }
 
-__device__ __forceinline__ unsigned long long pack_key(uint32_t key, int token) {
-  return ((unsigned long long)key << 32) | (0xffffffffu - (uint32_t)token);
-}
-
-// Gathers the elements with key >= `key` into sel.cand (as many as fit) and returns their number.
+// One block, the whole row: sel.cand[0 .. k) holds the winners afterwards.
 template <typename T>
-__device__ int gather_ge(const Row<T>& row, uint32_t key, uint32_t best, Select& sel) {
+__device__ void select_exactly(const Row<const T>& row, int k, Select& sel) {
+  constexpr int kE = Unit<T>::kE;
+  uint32_t kth = 0;
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t trial = kth | (1u << bit);
+    if (count_ge(row, trial, sel.scan) >= k) kth = trial;
+  }
   __syncthreads();
   if (threadIdx.x == 0) sel.count = 0;
   __syncthreads();
-  if (best >= key) {
-    for (int i = threadIdx.x; i < row.units; i += blockDim.x) {
-      float f[8];
-      row.load(i, f);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int a = 8 * i + j;
-        const uint32_t k = order_key(f[j]);
-        if (k >= key && a >= row.shift && a < row.end) {
-          const int at = atomicAdd(&sel.count, 1);
-          if (at < kCand) sel.cand[at] = pack_key(k, a - row.shift);
-        }
-      }
-    }
-  }
+  for (int i = threadIdx.x; i < row.units; i += blockDim.x) offer(row.load(i), i, kth + 1, row, &sel);
   __syncthreads();
-  return sel.count;
-}
-
-// After this, sel.cand[0 .. n) holds the k winners among n >= k candidates; returns n.
-template <typename T>
-__device__ int select_candidates(const Row<T>& row, int k, uint32_t best, bool any, Select& sel) {
-  // the k-th largest of the stripes' maxima (0 when fewer than k stripes hold elements: everything)
-  uint32_t bound = 0;
-  if (__syncthreads_count(any) >= k) {
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t trial = bound | (1u << bit);
-      if (__syncthreads_count(any && best >= trial) >= k) bound = trial;
-    }
-  }
-  int n = gather_ge(row, bound, any ? best : 0u, sel);
-  if (n <= kCand) return n;
-  // exact: the k-th largest key of the row
-  uint32_t kth = bound;
-  if (count_ge(row, bound + 1, sel.scan) >= k) {
-    kth = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t trial = kth | (1u << bit);
-      if (count_ge(row, trial, sel.scan) >= k) kth = trial;
-    }
-  }
-  n = gather_ge(row, kth + 1, any ? best : 0u, sel);        // fewer than k
-  // its equals, in index order, until k are held
+  int n = sel.count;      // fewer than k; now the k-th's equals, in index order
   for (int i0 = 0; i0 < row.units && n < k; i0 += blockDim.x) {
     const int i = i0 + threadIdx.x;
-    float f[8];
     uint32_t hit = 0;
     if (i < row.units) {
-      row.load(i, f);
+      const Unit<T> u = row.load(i);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int a = 8 * i + j;
-        if (order_key(f[j]) == kth && a >= row.shift && a < row.end) hit |= 1u << j;
-      }
+      for (int j = 0; j < kE; ++j)
+        if (row.holds(kE * i + j) && order_key(to_f(u.get(j))) == kth) hit |= 1u << j;
     }
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int pos = __popc(hit);
@@ -300,18 +555,22 @@ __device__ int select_candidates(const Row<T>& row, int k, uint32_t best, bool a
     while (hit) {
       const int j = __ffs(hit) - 1;
       hit &= hit - 1;
-      if (at < k) sel.cand[at] = pack_key(kth, 8 * i + j - row.shift);
+      if (at < k) sel.cand[at] = pack_key(kth, kE * i + j - row.shift);
       ++at;
     }
     n = min(k, n + total);
   }
   __syncthreads();
-  return n;
 }
 
 // ------------------------------------------------------------------------------------- token log-probs
-__device__ __forceinline__ float row_c(const float* temp, double temp1, int row) {
-  return (float)(kLog2e / (temp ? (double)temp[row] : temp1));
+template <typename A>
+__device__ __forceinline__ double inv_temp(const A& a, int row) {
+  return a.temp ? rcp_d((double)a.temp[row]) : a.inv_temp1;
+}
+template <typename A>
+__device__ __forceinline__ float row_c(const A& a, int row) {
+  return (float)(kLog2e * inv_temp(a, row));
 }
 
 __device__ __forceinline__ float finish_logp(double x, float c, Stat st, double log2s) {
@@ -320,28 +579,15 @@ __device__ __forceinline__ float finish_logp(double x, float c, Stat st, double 
   return (float)(kLn2 * (xc - (double)st.R - log2s));
 }
 
-template <typename T, bool kEntropy, bool kTop>
-__global__ void __launch_bounds__(kThreads) token_logprob_kernel(const T* __restrict__ logits, TokenArgs a) {
-  __shared__ Stat part[32];
-  extern __shared__ __align__(16) unsigned char dyn[];
-  const int r = blockIdx.x;
-  const T* x = logits + (size_t)r * a.stride;
-  const Row<const T> row(x, a.V);
-  const float c = row_c(a.temp, a.temp1, r);
-  Stat st = Stat::none();
-  float best = -INFINITY;
-  for (int i = threadIdx.x; i < row.units; i += kThreads) {
-    float f[8];
-    row.load(i, f);
-    st.push8<kEntropy>(f, c);
-    if (kTop) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) best = fmaxf(best, f[j]);
-    }
-  }
-  st = block_join(st, part);
-  const double log2s = log2((double)st.s);
-  for (int j = threadIdx.x; j < a.n; j += kThreads) {
+struct RowPart {       // what the blocks of a cluster tell one another about a row
+  Stat st;
+  uint32_t bound;
+};
+
+// The outputs of a row but its alternatives; by the leading block.
+template <typename T, bool kEntropy>
+__device__ __forceinline__ void write_row(const TokenArgs& a, int r, const T* x, float c, Stat st, double log2s) {
+  for (int j = threadIdx.x; j < a.n; j += blockDim.x) {
     const long t = a.tokens[(size_t)r * a.n + j] - a.vocab_start;
     const bool here = t >= 0 && t < a.V;
     float v = 0.f;
@@ -350,67 +596,276 @@ __global__ void __launch_bounds__(kThreads) token_logprob_kernel(const T* __rest
   }
   if (threadIdx.x == 0) {
     const bool empty = st.s == 0.f;
-    if (a.entropy) a.entropy[r] = empty ? 0.f : (float)(kLn2 * (log2s - (double)st.et / (double)st.s));
+    const double inv = rcp_d(empty ? 1.0 : (double)st.s);
+    if (kEntropy) a.entropy[r] = empty ? 0.f : (float)(kLn2 * (log2s - (double)st.et * inv));
+    if (!a.stats) return;
     float* o = a.stats + 3 * (size_t)r;
     o[0] = st.R;
-    o[1] = a.open ? st.s : (empty ? 0.f : (float)(1.0 / (double)st.s));
-    o[2] = a.open ? st.et : (empty ? 0.f : (float)((double)st.et / (double)st.s));
+    o[1] = a.open ? st.s : (empty ? 0.f : (float)inv);
+    o[2] = a.open ? st.et : (empty ? 0.f : (float)((double)st.et * inv));
   }
-  if (kTop) {
-    Select& sel = *reinterpret_cast<Select*>(dyn);
-    const int n = select_candidates(row, a.k, order_key(best), (int)threadIdx.x < row.units, sel);
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      const unsigned long long mine = sel.cand[i];
-      int rank = 0;
-      for (int j = 0; j < n; ++j) rank += sel.cand[j] > mine;
-      if (rank < a.k) {
-        const int t = (int)(0xffffffffu - (uint32_t)mine);
-        a.top_ids[(size_t)r * a.k + rank] = t + a.vocab_start;
-        a.top_logp[(size_t)r * a.k + rank] = a.open ? to_f(x[t]) : finish_logp(to_f(x[t]), c, st, log2s);
-      }
+}
+
+// The alternatives from the gathered candidates; by the leading block.
+template <typename T>
+__device__ __forceinline__ void write_top(const TokenArgs& a, int r, const Row<const T>& row, float c, Stat st,
+                                          double log2s, Select& sel) {
+  int n = sel.count;
+  if (n > kCand) {
+    select_exactly(row, a.k, sel);
+    n = a.k;
+  }
+  // ranks by counting, `share` neighbouring lanes to a candidate
+  int share = 1;
+  while (share < 32 && 2 * share * n <= (int)blockDim.x) share *= 2;
+  const int part = threadIdx.x & (share - 1), per_pass = blockDim.x / share;
+  for (int i0 = 0; i0 < n; i0 += per_pass) {
+    const int i = i0 + threadIdx.x / share;
+    const unsigned long long own = sel.cand[min(i, n - 1)];
+    int place = 0;
+#pragma unroll 4
+    for (int j = part; j < n; j += share) place += sel.cand[j] > own;
+    for (int o = share / 2; o > 0; o >>= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
+    if (i < n && part == 0 && place < a.k) {
+      const int t = (int)(0xffffffffu - (uint32_t)own);
+      const float v = key_value((uint32_t)(own >> 32));
+      a.top_ids[(size_t)r * a.k + place] = t + a.vocab_start;
+      a.top_logp[(size_t)r * a.k + place] = a.open ? v : finish_logp(v, c, st, log2s);
     }
   }
 }
 
+// Joins the cluster's sums and bounds; afterwards the leader's `sel` takes candidates.
+__device__ __forceinline__ void join_row(RowPart& mine, Stat& st, uint32_t& bound, Select* sel,
+                                         cg::cluster_group& cl) {
+  const int blocks = (int)cl.num_blocks();
+  if (threadIdx.x == 0) {
+    mine.st = st;
+    mine.bound = bound;
+    if (sel) sel->count = 0;
+  }
+  if (blocks == 1) {
+    if (sel) __syncthreads();
+    return;
+  }
+  cl.sync();
+  const int lane = threadIdx.x & 31;
+  Stat other = Stat::none();
+  uint32_t least = 0xffffffffu;
+  if (lane < blocks) {
+    const RowPart* m = cl.map_shared_rank(&mine, lane);
+    other = m->st;
+    least = m->bound;
+  }
+  st = warp_join(other);
+  bound = __reduce_min_sync(0xffffffffu, least);
+}
+
+// Alternatives of short rows, and of few rows: the cluster holds the row in registers, kUnits units per thread, so the
+// selection does not read it again.
+template <typename T, bool kEntropy, int kUnits>
+__global__ void __launch_bounds__(kThreads, kUnits == 10 ? 1 : 3) token_top_kernel(const T* __restrict__ logits, TokenArgs a) {
+  __shared__ Stat part[32];
+  __shared__ RowPart mine;
+  extern __shared__ __align__(16) unsigned char dyn[];
+  Select* sel = reinterpret_cast<Select*>(dyn);
+  cg::cluster_group cl = cg::this_cluster();
+  const int blocks = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+  const int r = blockIdx.x / blocks;
+  const T* x = logits + (size_t)r * a.stride;
+  const Row<const T> row(x, a.V);
+  const Slice sl(row.units, blocks, rank);
+  Unit<T> u[kUnits];
+#pragma unroll
+  for (int n = 0; n < kUnits; ++n) {
+    const int i = sl.lo + threadIdx.x + n * blockDim.x;
+    if (i < sl.hi) u[n] = row.load(i);
+    else u[n].fill(from_f<T>(-INFINITY));
+  }
+  const float c = row_c(a, r);
+  const float best = units_max<T, kUnits>(u);
+  Sums sums;
+  sums.R = fmaxf(best * c, kMasked);
+#pragma unroll
+  for (int n = 0; n < kUnits; ++n) sums.template add<kEntropy>(u[n], c);
+  Stat st = block_join(sums.get(), part);
+  const bool any = sl.lo + (int)threadIdx.x < sl.hi;
+  const uint32_t best_key = order_key(best);
+  uint32_t bound = kth_max(best_key, any, (a.k + blocks - 1) / blocks);
+  join_row(mine, st, bound, sel, cl);
+  if (any && best_key >= bound) {
+    Select* lead = cl.map_shared_rank(sel, 0);
+#pragma unroll
+    for (int n = 0; n < kUnits; ++n) {
+      const int i = sl.lo + threadIdx.x + n * blockDim.x;
+      if (i < sl.hi) offer(u[n], i, bound, row, lead);
+    }
+  }
+  if (blocks > 1) cl.sync();      // the leader has every candidate, and nobody's sums are read any more
+  else __syncthreads();
+  if (rank) return;
+  const double log2s = log2_d((double)st.s);
+  write_row<T, kEntropy>(a, r, x, c, st, log2s);
+  write_top(a, r, row, c, st, log2s, *sel);
+}
+
+// Rows that stream through shared memory once.  With alternatives a warp notes the maximum of every 32 units it takes;
+// after the bound is known only those that reach it are read again.
+template <typename T, bool kEntropy, bool kTop>
+__global__ void __launch_bounds__(kStream, 4) token_stream_kernel(const T* __restrict__ logits, TokenArgs a) {
+  __shared__ Stat part[32];
+  __shared__ RowPart mine;
+  __shared__ int hits;
+  extern __shared__ __align__(16) unsigned char dyn[];
+  cg::cluster_group cl = cg::this_cluster();
+  const int blocks = (int)cl.num_blocks(), rank = (int)cl.block_rank(), lane = threadIdx.x & 31;
+  const int r = blockIdx.x / blocks;
+  const T* x = logits + (size_t)r * a.stride;
+  const Row<const T> row(x, a.V);
+  const Slice sl(row.units, blocks, rank);
+  Feed<T> feed(dyn, row, sl, 1);
+  float* strips = reinterpret_cast<float*>(dyn + max(Feed<T>::bytes(blockDim.x), sizeof(Select)));
+  const float c = row_c(a, r);
+  Sums sums;
+  float best = -INFINITY;
+  const unsigned long long policy = kTop ? evict_normal() : evict_first();
+  const uint4* from = feed.p + kGroups * feed.step;
+  float* strip = strips + (feed.first - sl.lo) / 32 + lane;
+  for (int k = 0; k < feed.batches; ++k, from += feed.step, strip += feed.step / 32) {
+    feed.wait(k, row, sl);
+    Unit<T> u[kBatch];
+    feed.take(u);
+    float top;
+    if constexpr (kTop) {
+      float m[kBatch];
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) m[b] = u[b].max();
+      top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+      best = fmaxf(best, top);
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) m[b] = warp_top(m[b]);
+      if (lane < kBatch) *strip = lane == 0 ? m[0] : (lane == 1 ? m[1] : (lane == 2 ? m[2] : m[3]));
+    } else {
+      top = units_max<T, kBatch>(u);
+    }
+    if (feed.inner(k + kGroups)) feed.issue_inner(from, policy);
+    else feed.issue(k + kGroups);
+    top *= c;
+    if (top > sums.R + kSlack) sums.raise(top);
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) sums.template add<kEntropy>(u[b], c);
+  }
+  Stat st = block_join(sums.get(), part);
+  uint32_t bound = 0;
+  Select* sel = kTop ? reinterpret_cast<Select*>(dyn) : nullptr;      // the ring's place: its copies are done
+  const int held = sl.hi - sl.lo;
+  if (kTop) bound = kth_max(order_key(best), (int)(threadIdx.x >> 5) * kSpan + lane < held, (a.k + blocks - 1) / blocks);
+  join_row(mine, st, bound, sel, cl);
+  if (kTop) {
+    Select* lead = cl.map_shared_rank(sel, 0);
+    const int count = (held + 31) / 32, warps = blockDim.x >> 5;
+    int* list = reinterpret_cast<int*>(strips);      // (a thread's own maxima are read before anything is written)
+    for (int s0 = 0; s0 < count; s0 += blockDim.x) {
+      const int s = s0 + threadIdx.x;
+      const bool hit = s < count && order_key(strips[min(s, count - 1)]) >= bound;
+      if (threadIdx.x == 0) hits = 0;
+      __syncthreads();
+      if (hit) list[s0 + atomicAdd(&hits, 1)] = s;
+      __syncthreads();
+      constexpr int kAtOnce = 4;
+      for (int h = threadIdx.x >> 5; h < hits; h += kAtOnce * warps) {
+        Unit<T> u[kAtOnce];
+        int at[kAtOnce];
+#pragma unroll
+        for (int n = 0; n < kAtOnce; ++n) {
+          at[n] = h + n * warps < hits ? sl.lo + 32 * list[s0 + h + n * warps] + lane : sl.hi;
+          if (at[n] < sl.hi) u[n] = row.load(at[n]);
+        }
+#pragma unroll
+        for (int n = 0; n < kAtOnce; ++n)
+          if (at[n] < sl.hi && order_key(u[n].max()) >= bound) offer(u[n], at[n], bound, row, lead);
+      }
+      __syncthreads();
+    }
+  }
+  if (blocks > 1) cl.sync();      // the leader has every candidate, and nobody's sums are read any more
+  else if (kTop) __syncthreads();
+  if (rank) return;
+  const double log2s = log2_d((double)st.s);
+  write_row<T, kEntropy>(a, r, x, c, st, log2s);
+  if constexpr (kTop) write_top(a, r, row, c, st, log2s, *sel);
+}
+
 // d x_v = (e / s / T) (-G - dH ln 2 (t - E[t])) + [v = t_j] g_j / T, G = sum_j g_j
 template <typename T, bool kEntropy>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kStream, 4)
     token_logprob_bwd_kernel(const T* __restrict__ logits, T* __restrict__ grad, TokenArgs a) {
   __shared__ float scratch[32];
-  const int r = blockIdx.x;
+  extern __shared__ __align__(16) unsigned char dyn[];
+  cg::cluster_group cl = cg::this_cluster();
+  const int blocks = (int)cl.num_blocks(), lane = threadIdx.x & 31;
+  const int r = blockIdx.x / blocks;
   const T* x = logits + (size_t)r * a.stride;
   T* g = grad + (size_t)r * a.V;
   const Row<const T> row(x, a.V);
   const Row<T> out(g, a.V);
+  const Slice sl(row.units, blocks, (int)cl.block_rank());
+  Feed<T> feed(dyn, row, sl, 1);
   const bool vec = row.shift == out.shift;
-  const float c = row_c(a.temp, a.temp1, r);
-  const float it = (float)(1.0 / (a.temp ? (double)a.temp[r] : a.temp1));
+  const float c = row_c(a, r);
+  const float it = (float)inv_temp(a, r);
   const float* st = a.stats + 3 * (size_t)r;
   const float R = st[0], inv = st[1], mean = st[2];
   float G = 0.f;      // a token outside the whole vocabulary (an ignored position) has no gradient
-  for (int j = threadIdx.x; j < a.n; j += kThreads) {
+  for (int j = threadIdx.x; j < a.n; j += blockDim.x) {
     const long t = a.tokens[(size_t)r * a.n + j];
     G += (t >= 0 && t < a.vocab_total) ? a.d_logp[(size_t)r * a.n + j] : 0.f;
   }
   G = bb::block_sum(G, scratch);
   const float dh = kEntropy ? a.d_entropy[r] * (float)kLn2 : 0.f;
   const float A = it * inv * (dh * mean - G), B = -it * inv * dh;
-  for (int i = threadIdx.x; i < row.units; i += kThreads) {
-    float f[8];
-    row.load(i, f);
+  const unsigned long long policy = evict_first();
+  const uint4* from = feed.p + kGroups * feed.step;
+  uint4* to = reinterpret_cast<uint4*>(out.p) + feed.first + lane;
+  for (int k = 0; k < feed.batches; ++k, from += feed.step, to += feed.step) {
+    feed.wait(k, row, sl);
+    Unit<T> u[kBatch];
+    feed.take(u);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float t = fmaf(f[j], c, -R), e = ex2(t);
-      f[j] = e * (kEntropy ? fmaf(B, fmaxf(t, -1e4f), A) : A);
+    for (int b = 0; b < kBatch; ++b) {
+      float f[Unit<T>::kE];
+      u[b].floats(f);
+#pragma unroll
+      for (int j = 0; j < Unit<T>::kE; ++j) {
+        const float t = fmaf(f[j], c, -R);
+        f[j] = ex2(t) * (kEntropy ? fmaf(B, fmaxf(t, -1e4f), A) : A);
+      }
+#pragma unroll
+      for (int j = 0; j < Unit<T>::kE; j += 2) u[b].set_pair(j / 2, f[j], f[j + 1]);
     }
-    out.store(i, f, vec, row.shift);
+    if (feed.inner(k + kGroups)) feed.issue_inner(from, policy);
+    else feed.issue(k + kGroups);
+    if (vec && feed.inner(k)) {
+      store_streaming<0>(to, u[0].w, policy);
+      store_streaming<1>(to, u[1].w, policy);
+      store_streaming<2>(to, u[2].w, policy);
+      store_streaming<3>(to, u[3].w, policy);
+    } else {
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const int i = feed.first + k * feed.step + lane + 32 * b;
+        if (i < sl.hi) out.store(i, u[b], vec, row.shift);
+      }
+    }
   }
   __syncthreads();
-  // the given tokens' columns, once per distinct token
-  for (int j = threadIdx.x; j < a.n; j += kThreads) {
+  // the given tokens' columns, once per distinct token, by the block that wrote them
+  for (int j = threadIdx.x; j < a.n; j += blockDim.x) {
     const int64_t* tk = a.tokens + (size_t)r * a.n;
     const long t = tk[j] - a.vocab_start;
     if (t < 0 || t >= a.V) continue;
+    const int unit = ((int)t + row.shift) / Unit<T>::kE;
+    if (unit < sl.lo || unit >= sl.hi) continue;
     bool first = true;
     for (int i = 0; i < j; ++i) first &= tk[i] != tk[j];
     if (!first) continue;
@@ -423,224 +878,444 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // ------------------------------------------------------------------------------------------ distillation
-struct Entries {
-  double xc[kMaxTop];      // x c of the entry, -inf where masked
-  float logq[kMaxTop];
-  float fix[kMaxTop];
-  int col[kMaxTop];        // column in this shard, or -1
-  unsigned char state[kMaxTop];   // 0 dropped, 1 first of its id, 2 repeats an earlier entry
-  float R, factor, kl;
-  int repeats;
+// Teacher side of a row, q~ = exp(log q - ref) over the entries that count, and the student's at their columns:
+// e = 2^(x c - m).  A block holds the part of its slice; the parts are summed over the cluster.
+struct Teacher {
+  double q, qlq, qxc;   // sums of q~, q~ (log q - ref), q~ x c
+  double m, z;          // max of x c, sum over distinct columns of 2^(x c - m)
 };
 
-// KL and gradient factors of a row from its entries and the (R, s) of everything else; warp 0, all lanes.
-__device__ void finish_row(Entries& en, int K, Stat rest, bool tail, double scale, double inv_temp) {
-  const int lane = threadIdx.x & 31;
-  double top = -INFINITY;      // teacher: sum of q, renormalised over the entries without a tail class
-  for (int j = lane; j < K; j += 32)
-    if (en.state[j]) top = fmax(top, (double)en.logq[j]);
-  top = warp_max_d(top);
-  double shift = 0.0;
-  if (!tail && top > -INFINITY) {
-    double z = 0.0;
-    for (int j = lane; j < K; j += 32)
-      if (en.state[j]) z += exp((double)en.logq[j] - top);
-    shift = top + log(warp_sum_d(z));
+// Everything that the gradient of a row needs.
+struct Finished {
+  float R, factor;      // columns outside the entries: factor 2^(x c - R)
+  double per_q;         // an entry's column: per_p 2^(x c - m) - per_q q~
+  double per_p, m;
+  float kl;
+};
+
+__device__ __forceinline__ Teacher no_teacher() { return {0.0, 0.0, 0.0, -INFINITY, 0.0}; }
+
+// Sum over the first kMaxCluster lanes (the others hold nothing), in those lanes.
+__device__ __forceinline__ Teacher join_blocks(Teacher t) {
+  double m = t.m;
+#pragma unroll
+  for (int o = kMaxCluster / 2; o > 0; o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
+  t.z = t.z == 0.0 ? 0.0 : t.z * exp2_d(t.m - m);
+  t.m = m;
+#pragma unroll
+  for (int o = kMaxCluster / 2; o > 0; o >>= 1) {
+    t.q += __shfl_xor_sync(0xffffffffu, t.q, o);
+    t.qlq += __shfl_xor_sync(0xffffffffu, t.qlq, o);
+    t.qxc += __shfl_xor_sync(0xffffffffu, t.qxc, o);
+    t.z += __shfl_xor_sync(0xffffffffu, t.z, o);
   }
-  double q_sum = 0.0, m = rest.s == 0.f ? -INFINITY : (double)rest.R;
-  for (int j = lane; j < K; j += 32) {
-    if (!en.state[j]) continue;
-    q_sum += exp((double)en.logq[j] - shift);
-    m = fmax(m, en.xc[j]);
-  }
-  q_sum = warp_sum_d(q_sum);
-  m = warp_max_d(m);
-  const double q_rest = tail ? fmax(0.0, 1.0 - q_sum) : 0.0;
-  const bool no_teacher = !tail && !(top > -INFINITY);
-  bool any = false;
-  for (int j = lane; j < K; j += 32) any |= en.state[j] != 0;
-  any = __any_sync(0xffffffffu, any) && !no_teacher;
-  if (!any || m == -INFINITY) {
-    // no entry: nothing to learn.  No student probability anywhere: the divergence is infinite, without gradient
-    const bool nan = rest.s != rest.s;
-    for (int j = lane; j < K; j += 32) en.fix[j] = 0.f;
-    if (lane == 0) {
-      en.R = 0.f;
-      en.factor = 0.f;
-      en.kl = !any ? 0.f : (nan ? rest.s : INFINITY);
-    }
-    return;
-  }
-  const double rest_share = rest.s == 0.f ? 0.0 : (double)rest.s * exp2((double)rest.R - m);
-  double z = 0.0;
-  for (int j = lane; j < K; j += 32)
-    if (en.state[j] == 1) z += exp2(en.xc[j] - m);
-  z = warp_sum_d(z) + rest_share;
-  const double log2z = log2(z), p_rest = rest_share / z, total = q_sum + q_rest;
-  double kl = 0.0;
-  for (int j = lane; j < K; j += 32) {
-    if (!en.state[j]) {
-      en.fix[j] = 0.f;
-      continue;
-    }
-    const double lq = (double)en.logq[j] - shift, q = exp(lq);
-    if (q > 0.0) kl += q * (lq - kLn2 * (en.xc[j] - m - log2z));
-    else if (!(q == 0.0)) kl += q;      // NaN
-    double held = q;
-    if (en.repeats && en.state[j] == 1)
-      for (int i = j + 1; i < K; ++i)
-        if (en.state[i] == 2 && en.col[i] == en.col[j]) held += exp((double)en.logq[i] - shift);
-    en.fix[j] = (float)(scale * inv_temp * (total * exp2(en.xc[j] - m) / z - held));
-  }
-  kl = warp_sum_d(kl);
-  if (lane == 0) {
-    if (q_rest > 0.0) {
-      kl += q_rest * (log(q_rest) - kLn2 * ((double)rest.R - m + log2((double)rest.s) - log2z));
-      if (rest.s == 0.f) kl = INFINITY;
-    }
-    en.kl = (float)kl;
-    en.R = rest.R;
-    en.factor = rest.s == 0.f ? 0.f : (float)(scale * inv_temp * (total * p_rest - q_rest) / (double)rest.s);
-  }
+  return t;
 }
 
-// Loads the teacher's entries of row r and marks their columns in `mask` (one byte per unit).
-template <typename T>
-__device__ void load_entries(Entries& en, const DistillArgs& a, int r, const T* x, const Row<const T>& row, float c,
-                             unsigned int* mask) {
-  const int words = (row.units + 3) >> 2;
-  for (int i = threadIdx.x; i < words; i += blockDim.x) mask[i] = 0u;
-  if (threadIdx.x == 0) en.repeats = 0;
+// `some`: the row has entries that count.  `scale` includes the row's weight and 1 / T.
+__device__ __forceinline__ Finished finish_row(const Teacher& t, Stat rest, bool some, bool tail, double scale) {
+  // (written with selects: the long FP64 chains are independent and overlap)
+  const bool out = rest.s != 0.f, in = t.z != 0.0;      // student probability outside and on the entries
+  const double Rd = out ? (double)rest.R : -INFINITY, md = in ? t.m : -INFINITY;
+  const double m = fmax(Rd, md);
+  const bool lost = m == -INFINITY;                     // none anywhere
+  const double m0 = lost ? 0.0 : m;
+  const double s = out ? (double)rest.s : 1.0;
+  const double q_rest = tail ? fmax(0.0, 1.0 - t.q) : 0.0, total = tail ? t.q + q_rest : 1.0;
+  const double q_norm = tail ? 1.0 : t.q;
+  const double log_s = log2_d(s), log_qr = log2_d(q_rest), log_norm = log2_d(q_norm);
+  const double inv_s = rcp_d(s), norm = rcp_d(q_norm);
+  const double share = out ? s * exp2_d(Rd - m0) : 0.0;
+  const double z = lost ? 1.0 : (in ? t.z * exp2_d(md - m0) : 0.0) + share;
+  const double lse = m0 + log2_d(z), inv_z = rcp_d(z), p_rest = share * inv_z;
+  double kl = norm * t.qlq - kLn2 * (log_norm + norm * t.qxc - norm * t.q * lse);
+  if (q_rest > 0.0) kl += out ? q_rest * kLn2 * (log_qr - (Rd + log_s - lse)) : INFINITY;
+  // a teacher without probability on any entry: with a tail class all of it is there, else there is nothing to learn
+  const bool nothing = !some || (!tail && t.q == 0.0);
+  const bool still = nothing || lost;
+  Finished f;
+  f.kl = nothing ? 0.f : (lost ? INFINITY : (float)kl);
+  f.R = out ? rest.R : 0.f;
+  f.factor = still || !out ? 0.f : (float)(scale * (total * p_rest - q_rest) * inv_s);
+  f.per_q = still ? 0.0 : scale * norm;
+  f.per_p = still ? 0.0 : scale * total * inv_z;
+  f.m = m0;
+  return f;
+}
+
+// The teacher's entries of a row.  Those in this block's slice are chained by where they lie (a thread's units, or a
+// warp's batch), so that whoever takes the logits there rules the entries' columns out.
+struct Entries {
+  double *xc, *q;        // of the entries in this block's slice
+  Teacher* part;         // sums of 32 entries each
+  float* logq;           // of every entry; -inf where dropped
+  int* col;              // the shard's column if it lies in this block's slice, else -1
+  int* next;             // chain, -1 at its end
+  int* heads;            // chains
+  unsigned char* later;  // repeats the column of an earlier entry
+
+  static __host__ __device__ size_t bytes(int K, int chains) {
+    return (K + 31) / 32 * sizeof(Teacher) + (size_t)K * 28 + (size_t)chains * 4 + K + 15;
+  }
+  __device__ __forceinline__ Entries(unsigned char* p, int K, int chains) {
+    part = reinterpret_cast<Teacher*>(p);
+    xc = reinterpret_cast<double*>(part + (K + 31) / 32);
+    q = xc + K;
+    logq = reinterpret_cast<float*>(q + K);
+    col = reinterpret_cast<int*>(logq + K);
+    next = col + K;
+    heads = next + K;
+    later = reinterpret_cast<unsigned char*>(heads + chains);
+  }
+};
+
+// Reads the row's entries into `en`, chains them from en.heads[place(unit)] and sums them 32 by 32; returns whether the
+// row has any that counts.  The chains are complete when it returns, the sums after the next barrier.
+template <typename T, typename Place>
+__device__ __forceinline__ bool load_entries(const Entries& en, const DistillArgs& a, int r, const T* x,
+                                             const Row<const T>& row, Slice sl, float c, int chains, Place place) {
+  const int lane = threadIdx.x & 31, padded = (a.K + 31) / 32 * 32;
+  for (int i = threadIdx.x; i < chains; i += blockDim.x) en.heads[i] = -1;
   __syncthreads();
+  bool some = false;
   for (int j = threadIdx.x; j < a.K; j += blockDim.x) {
-    const long id = a.ids[(size_t)r * a.K + j];
-    const long t = id - a.vocab_start;
-    const bool valid = id >= 0 && id < a.vocab_total, here = valid && t >= 0 && t < a.V;
-    en.logq[j] = a.logq[(size_t)r * a.K + j];
-    en.col[j] = here ? (int)t : -1;
-    en.state[j] = valid ? 1 : 0;
-    double xc = 0.0;
-    if (here) {
-      xc = (double)to_f(x[t]) * (double)c;
-      if (xc <= (double)kMasked) xc = -INFINITY;
-      const int at = (int)t + row.shift;
-      if (atomicOr(&mask[at >> 5], 1u << (at & 31)) >> (at & 31) & 1u) en.repeats = 1;
+    const size_t at = (size_t)r * a.K + j;
+    const long id = a.ids[at], t = id - a.vocab_start;
+    const float lq = a.logq[at];
+    const bool valid = id >= 0 && id < a.vocab_total;
+    const int unit = valid && t >= 0 && t < a.V ? ((int)t + row.shift) / Unit<T>::kE : -1;
+    some |= valid;
+    en.logq[j] = valid ? lq : -INFINITY;
+    en.col[j] = -1;
+    en.later[j] = 0;
+    if (unit >= sl.lo && unit < sl.hi) {
+      const double xc = (double)to_f(x[t]) * (double)c;
+      en.xc[j] = xc <= (double)kMasked ? -INFINITY : xc;
+      en.col[j] = (int)t;
+      en.next[j] = atomicExch(&en.heads[place(unit)], j);
     }
-    en.xc[j] = xc;
   }
-  __syncthreads();
-  if (en.repeats) {
-    for (int j = threadIdx.x; j < a.K; j += blockDim.x) {
-      if (en.col[j] < 0) continue;
-      for (int i = 0; i < j; ++i)
-        if (en.col[i] == en.col[j]) en.state[j] = 2;
-    }
-    __syncthreads();
+  some = __syncthreads_or(some);
+  double ref = 0.0;
+  if (!a.tail) {            // relative to the largest log q: without a tail class these may be raw logits
+    float top = -INFINITY;
+    for (int j = lane; j < a.K; j += 32) top = fmaxf(top, en.logq[j]);
+    top = warp_top(top);
+    if (top > -INFINITY) ref = (double)top;
   }
-}
-
-// g_v = k 2^(x_v c - R); k = 0 writes zeros without reading the row.
-template <typename T>
-__device__ __forceinline__ void write_gradient(const Row<const T>& row, T* g, int V, float c, float R, float k) {
-  const Row<T> out(g, V);
-  const bool vec = row.shift == out.shift;
-  for (int i = threadIdx.x; i < row.units; i += kThreads) {
-    float f[8];
-    if (k != 0.f) {
-      row.load(i, f);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = k * ex2(fmaf(f[j], c, -R));
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = 0.f;
-    }
-    out.store(i, f, vec, row.shift);
-  }
-}
-
-// One block per row: pass 1 takes the statistics of the columns outside the teacher's entries (their bits in `mask`
-// replace a logit by -inf), warp 0 finishes the row, pass 2 reads the row again and writes its gradient.
-template <typename T, bool kGrad, bool kOpen>
-__global__ void __launch_bounds__(kThreads) distill_kernel(const T* logits, T* grad, DistillArgs a) {
-  __shared__ Stat part[32];
-  __shared__ Entries en;
-  extern __shared__ __align__(16) unsigned int mask[];
-  const int r = blockIdx.x;
-  const T* x = logits + (size_t)r * a.stride;
-  const Row<const T> row(x, a.V);
-  const double inv_temp = 1.0 / (a.temp ? (double)a.temp[r] : a.temp1);
-  const float c = row_c(a.temp, a.temp1, r);
-  const float w = a.weights ? a.weights[r] : 1.f;
-  load_entries(en, a, r, x, row, c, mask);
-  Stat st = Stat::none();
-  if (w != 0.f) {
-    const unsigned char* bits = reinterpret_cast<const unsigned char*>(mask);
-    for (int i = threadIdx.x; i < row.units; i += kThreads) {
-      float f[8];
-      row.load(i, f);
-      const unsigned m = bits[i];
-      if (m) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (m >> j & 1u) f[j] = -INFINITY;
+  for (int j = threadIdx.x; j < padded; j += blockDim.x) {
+    Teacher p = no_teacher();
+    if (j < a.K && en.col[j] >= 0) {
+      const double l = (double)en.logq[j] - ref, q = exp2_d(l * kLog2e), xc = en.xc[j];
+      en.q[j] = q;
+      p.q = q;
+      p.qlq = q == 0.0 ? 0.0 : q * l;
+      p.qxc = q == 0.0 ? 0.0 : q * xc;
+      for (int e = en.heads[place((en.col[j] + row.shift) / Unit<T>::kE)]; e >= 0; e = en.next[e])
+        if (e < j && en.col[e] == en.col[j]) en.later[j] = 1;
+      if (!en.later[j] && xc > -INFINITY) {
+        p.m = xc;
+        p.z = 1.0;
       }
-      st.push8<false>(f, c);
+    }
+    const double m = warp_max_d(p.m);
+    p.z = p.z == 0.0 ? 0.0 : exp2_d(p.m - m);
+    p.m = m;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      p.q += __shfl_xor_sync(0xffffffffu, p.q, o);
+      p.qlq += __shfl_xor_sync(0xffffffffu, p.qlq, o);
+      p.qxc += __shfl_xor_sync(0xffffffffu, p.qxc, o);
+      p.z += __shfl_xor_sync(0xffffffffu, p.z, o);
+    }
+    if (lane == 0) en.part[j >> 5] = p;
+  }
+  return some;
+}
+
+struct Shared {
+  Stat warps[32];
+  struct { Stat st; Teacher teacher; } mine;
+  Finished fin;
+};
+
+// Joins the block's and the cluster's sums and finishes the row: sh.fin, and the outputs that are per row.
+template <typename T>
+__device__ __forceinline__ void finish_block(Shared& sh, const Entries& en, Stat own, const DistillArgs& a, int r, float w, bool some,
+                                             cg::cluster_group& cl) {
+  const int blocks = (int)cl.num_blocks(), rank = (int)cl.block_rank(), lane = threadIdx.x & 31;
+  Stat st = block_join(own, sh.warps);
+  Teacher t = no_teacher();
+  if (threadIdx.x < 32) {
+    if (lane < (a.K + 31) / 32) t = en.part[lane];
+    t = join_blocks(t);
+  }
+  if (blocks > 1) {
+    if (threadIdx.x == 0) {
+      sh.mine.st = st;
+      sh.mine.teacher = t;
+    }
+    cl.sync();
+    if (threadIdx.x < 32) {
+      Stat other = Stat::none();
+      t = no_teacher();
+      if (lane < blocks) {
+        const auto* m = cl.map_shared_rank(&sh.mine, lane);
+        other = m->st;
+        t = m->teacher;
+      }
+      st = warp_join<kMaxCluster>(other);
+      t = join_blocks(t);
     }
   }
-  st = block_join(st, part);
-  if (kOpen) {
-    for (int j = threadIdx.x; j < a.K; j += kThreads) a.xc[(size_t)r * a.K + j] = (float)en.xc[j];
-    if (threadIdx.x == 0) {
+  if (threadIdx.x == 0) {
+    sh.fin = finish_row(t, st, some, a.tail, (double)w * a.scale * inv_temp(a, r));
+    if (rank == 0 && a.open) {
       a.stats[2 * (size_t)r] = st.R;
       a.stats[2 * (size_t)r + 1] = st.s;
+    } else if (rank == 0) {
+      a.rows[r] = w != 0.f ? sh.fin.kl : 0.f;
     }
-    return;
   }
-  if (threadIdx.x < 32) finish_row(en, a.K, st, a.tail, (double)w * a.scale, inv_temp);
   __syncthreads();
-  if (threadIdx.x == 0) a.rows[r] = w == 0.f ? 0.f : en.kl;
-  if (!kGrad) return;
-  T* g = grad + (size_t)r * a.V;
-  write_gradient(row, g, a.V, c, en.R, w == 0.f ? 0.f : en.factor);
+  if (blocks > 1) cl.barrier_arrive();     // this block's reads of the others' sums are done
+  if (a.open)
+    for (int j = threadIdx.x; j < a.K; j += blockDim.x) {
+      const long t = a.ids[(size_t)r * a.K + j] - a.vocab_start;
+      if (en.col[j] >= 0) a.xc[(size_t)r * a.K + j] = (float)en.xc[j];
+      else if (rank == 0 && (t < 0 || t >= a.V)) a.xc[(size_t)r * a.K + j] = 0.f;
+    }
+}
+
+// The entries' own columns, over what the second pass wrote there.
+template <typename T, typename Place>
+__device__ __forceinline__ void write_entries(const Shared& sh, const Entries& en, const DistillArgs& a, T* g,
+                                              const Row<const T>& row, Place place) {
   __syncthreads();
-  if (w == 0.f) return;
-  for (int j = threadIdx.x; j < a.K; j += kThreads)
-    if (en.state[j] == 1 && en.col[j] >= 0) g[en.col[j]] = from_f<T>(en.fix[j]);
+  for (int j = threadIdx.x; j < a.K; j += blockDim.x) {
+    const int col = en.col[j];
+    if (col < 0 || en.later[j]) continue;
+    bool again = false;
+    for (int e = en.heads[place((col + row.shift) / Unit<T>::kE)]; e >= 0; e = en.next[e])
+      again |= e != j && en.col[e] == col;
+    double q = en.q[j];
+    if (again)        // in the order of the entries, whatever the chain's
+      for (int i = j + 1; i < a.K; ++i)
+        if (en.col[i] == col) q += en.q[i];
+    const double p = sh.fin.per_p * exp2_d(en.xc[j] - sh.fin.m);
+    g[col] = from_f<T>((float)(p - sh.fin.per_q * q));
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void gradient_unit(Unit<T>& u, float c, float R, float factor) {
+  float f[Unit<T>::kE];
+  u.floats(f);
+#pragma unroll
+  for (int j = 0; j < Unit<T>::kE; j += 2)
+    u.set_pair(j / 2, factor * ex2(fmaf(f[j], c, -R)), factor * ex2(fmaf(f[j + 1], c, -R)));
+}
+
+// A cluster per row, the row in registers, kUnits units per thread: the statistics of the columns outside the teacher's
+// entries, the joining, the gradient.  Short rows, and few rows, where one pass's latency is what counts.
+template <typename T, int kUnits>
+__global__ void __launch_bounds__(kThreads, kUnits == 10 ? 1 : 2) distill_kernel(const T* logits, T* grad, DistillArgs a) {
+  __shared__ Shared sh;
+  extern __shared__ __align__(16) unsigned char dyn[];
+  const Entries en(dyn, a.K, blockDim.x);
+  cg::cluster_group cl = cg::this_cluster();
+  const int blocks = (int)cl.num_blocks();
+  const int r = blockIdx.x / blocks;
+  const T* x = logits + (size_t)r * a.stride;
+  const Row<const T> row(x, a.V);
+  const Slice sl(row.units, blocks, (int)cl.block_rank());
+  const float w = a.weights ? a.weights[r] : 1.f;
+  const bool live = w != 0.f;      // rows of weight 0 are not read
+  Unit<T> u[kUnits];
+#pragma unroll
+  for (int n = 0; n < kUnits; ++n) {
+    const int i = sl.lo + threadIdx.x + n * blockDim.x;
+    if (live && i < sl.hi) u[n] = row.load(i);
+    else u[n].fill(from_f<T>(-INFINITY));
+  }
+  const float c = row_c(a, r);
+  const auto place = [&](int unit) { return (unit - sl.lo) % (int)blockDim.x; };
+  const bool some = load_entries(en, a, r, x, row, sl, c, blockDim.x, place);
+  for (int e = en.heads[threadIdx.x]; e >= 0; e = en.next[e]) {
+    const int pos = en.col[e] + row.shift - Unit<T>::kE * (sl.lo + (int)threadIdx.x);
+#pragma unroll
+    for (int n = 0; n < kUnits; ++n) {
+      const int j = pos - Unit<T>::kE * n * (int)blockDim.x;
+      if (j >= 0 && j < Unit<T>::kE) u[n].mask(1u << j);
+    }
+  }
+  Sums sums;
+  sums.R = fmaxf(units_max<T, kUnits>(u) * c, kMasked);
+#pragma unroll
+  for (int n = 0; n < kUnits; ++n) sums.template add<false>(u[n], c);
+  finish_block<T>(sh, en, sums.get(), a, r, w, some, cl);
+  if (grad) {
+    T* g = grad + (size_t)r * a.V;
+    const Row<T> out(g, a.V);
+    const bool vec = row.shift == out.shift;
+    const float R = sh.fin.R, factor = live ? sh.fin.factor : 0.f;
+#pragma unroll
+    for (int n = 0; n < kUnits; ++n) {
+      const int i = sl.lo + threadIdx.x + n * blockDim.x;
+      if (i >= sl.hi) break;
+      if (factor != 0.f) gradient_unit(u[n], c, R, factor);
+      else u[n].fill(from_f<T>(0.f));
+      out.store(i, u[n], vec, row.shift);
+    }
+    if (live) write_entries(sh, en, a, g, row, place);
+  }
+  if (blocks > 1) cl.barrier_wait();
+}
+
+// The same for many long rows: the row streams through shared memory, once for the statistics and, for the gradient,
+// once more (from L2, mostly).  The copies of the first batches are on their way while the entries are prepared, and
+// those of the second pass while the row is finished.
+template <typename T>
+__global__ void __launch_bounds__(kStream, 4) distill_stream_kernel(const T* logits, T* grad, DistillArgs a) {
+  __shared__ Shared sh;
+  extern __shared__ __align__(16) unsigned char dyn[];
+  cg::cluster_group cl = cg::this_cluster();
+  const int blocks = (int)cl.num_blocks(), lane = threadIdx.x & 31;
+  const int r = blockIdx.x / blocks;
+  const T* x = logits + (size_t)r * a.stride;
+  const Row<const T> row(x, a.V);
+  const Slice sl(row.units, blocks, (int)cl.block_rank());
+  const float w = a.weights ? a.weights[r] : 1.f;
+  const bool live = w != 0.f;
+  Feed<T> feed(dyn, row, sl, live ? (grad ? 2 : 1) : 0);
+  const int chains = (sl.hi - sl.lo + kSpan - 1) / kSpan;
+  const Entries en(dyn + Feed<T>::bytes(blockDim.x), a.K, chains);
+  const float c = row_c(a, r);
+  const auto place = [&](int unit) { return (unit - sl.lo) / kSpan; };
+  const bool some = load_entries(en, a, r, x, row, sl, c, chains, place);
+  Sums sums;
+  if (live) {
+    const int* head = en.heads + (feed.first - sl.lo) / kSpan;
+    int base = Unit<T>::kE * feed.first - row.shift;
+    const unsigned long long policy = grad ? evict_normal() : evict_first();
+    const uint4* from = feed.p + kGroups * feed.step;
+    for (int k = 0; k < feed.batches; ++k, from += feed.step) {
+      feed.wait(k, row, sl);
+      for (int e = *head; e >= 0; e = en.next[e]) {
+        const int pos = en.col[e] - base;
+        if (pos / Unit<T>::kE % 32 == lane) feed.rule_out(pos);
+      }
+      head += blockDim.x >> 5;
+      base += Unit<T>::kE * feed.step;
+      Unit<T> u[kBatch];
+      feed.take(u);
+      const float top = units_max<T, kBatch>(u) * c;
+      if (feed.inner(k + kGroups)) feed.issue_inner(from, policy);
+      else feed.issue(k + kGroups);
+      if (top > sums.R + kSlack) sums.raise(top);
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) sums.template add<false>(u[b], c);
+    }
+  }
+  finish_block<T>(sh, en, sums.get(), a, r, w, some, cl);
+  if (grad) {
+    T* g = grad + (size_t)r * a.V;
+    const Row<T> out(g, a.V);
+    const bool vec = row.shift == out.shift;
+    const float R = sh.fin.R, factor = live ? sh.fin.factor : 0.f;
+    if (factor != 0.f) {
+      const unsigned long long policy = evict_first();
+      uint4* to = reinterpret_cast<uint4*>(out.p) + feed.first + (feed.batches - 1) * feed.step + lane;
+      const uint4* from = feed.p + (feed.batches - 1 - kGroups) * feed.step;
+      for (int k = feed.batches - 1; k >= 0; --k, to -= feed.step, from -= feed.step) {
+        feed.wait(k, row, sl);
+        Unit<T> u[kBatch];
+        feed.take(u);
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) gradient_unit(u[b], c, R, factor);
+        if (feed.inner(k - kGroups)) feed.issue_inner(from, policy);
+        else feed.issue(2 * feed.batches - 1 - (k - kGroups));
+        if (vec && feed.inner(k)) {
+          store_streaming<0>(to, u[0].w, policy);
+          store_streaming<1>(to, u[1].w, policy);
+          store_streaming<2>(to, u[2].w, policy);
+          store_streaming<3>(to, u[3].w, policy);
+        } else {
+#pragma unroll
+          for (int b = 0; b < kBatch; ++b) {
+            const int i = feed.first + k * feed.step + lane + 32 * b;
+            if (i < sl.hi) out.store(i, u[b], vec, row.shift);
+          }
+        }
+      }
+    } else {      // no gradient outside the entries
+      Unit<T> u;
+      u.fill(from_f<T>(0.f));
+      for (int i = sl.lo + threadIdx.x; i < sl.hi; i += blockDim.x) out.store(i, u, vec, row.shift);
+    }
+    if (live) write_entries(sh, en, a, g, row, place);
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  if (blocks > 1) cl.barrier_wait();
 }
 
 // Vocabulary in shards: one warp per row finishes it from the joined (R, s) and x c of every entry.
 __global__ void distill_finish_kernel(DistillArgs a) {
-  __shared__ Entries en;
   const int r = blockIdx.x, lane = threadIdx.x;
   const int64_t* ids = a.ids + (size_t)r * a.K;
-  for (int j = lane; j < a.K; j += 32) {
-    const long id = ids[j];
-    en.logq[j] = a.logq[(size_t)r * a.K + j];
-    en.col[j] = (int)id;
-    const float xc = a.xc[(size_t)r * a.K + j];
-    en.xc[j] = xc <= kMasked ? -INFINITY : (double)xc;
-    bool first = true;
-    for (int i = 0; i < j; ++i) first &= ids[i] != id;
-    en.state[j] = id < 0 || id >= a.vocab_total ? 0 : (first ? 1 : 2);
+  const float *logq = a.logq + (size_t)r * a.K, *xcs = a.xc + (size_t)r * a.K;
+  const auto valid = [&](int j) { return ids[j] >= 0 && ids[j] < a.vocab_total; };
+  const auto entry = [&](int j) { return xcs[j] <= kMasked ? -INFINITY : (double)xcs[j]; };
+  float ref = 0.f;
+  bool some = false;
+  if (!a.tail) {
+    float top = -INFINITY;
+    for (int j = lane; j < a.K; j += 32)
+      if (valid(j)) top = fmaxf(top, logq[j]);
+    top = warp_top(top);
+    if (top > -INFINITY) ref = top;
   }
-  if (lane == 0) en.repeats = 1;
-  __syncwarp();
+  Teacher p = no_teacher();
+  for (int j = lane; j < a.K; j += 32) {
+    if (!valid(j)) continue;
+    some = true;
+    const double q = exp2_d(((double)logq[j] - (double)ref) * kLog2e);
+    p.q += q;
+    if (q != 0.0) {
+      p.qlq += q * ((double)logq[j] - (double)ref);
+      p.qxc += q * entry(j);
+    }
+    p.m = fmax(p.m, entry(j));
+  }
+  some = __any_sync(0xffffffffu, some);
+  p.q = warp_sum_d(p.q);
+  p.qlq = warp_sum_d(p.qlq);
+  p.qxc = warp_sum_d(p.qxc);
+  p.m = warp_max_d(p.m);
+  if (p.m > -INFINITY)
+    for (int j = lane; j < a.K; j += 32) {
+      bool first = valid(j);
+      for (int i = 0; first && i < j; ++i) first = ids[i] != ids[j];
+      if (first) p.z += exp2_d(entry(j) - p.m);
+    }
+  p.z = warp_sum_d(p.z);
   Stat st = Stat::none();
   st.R = a.stats[2 * (size_t)r];
   st.s = a.stats[2 * (size_t)r + 1];
   const float w = a.weights ? a.weights[r] : 1.f;
-  finish_row(en, a.K, st, a.tail, (double)w * a.scale, 1.0 / (a.temp ? (double)a.temp[r] : a.temp1));
-  __syncwarp();
+  const double it = inv_temp(a, r);
+  const Finished f = finish_row(p, st, some, a.tail, (double)w * a.scale * it);
   if (lane == 0) {
-    a.rows[r] = w == 0.f ? 0.f : en.kl;
-    a.coef[2 * (size_t)r] = en.R;
-    a.coef[2 * (size_t)r + 1] = w == 0.f ? 0.f : en.factor;
+    a.rows[r] = w == 0.f ? 0.f : f.kl;
+    a.coef[2 * (size_t)r] = f.R;
+    a.coef[2 * (size_t)r + 1] = w == 0.f ? 0.f : f.factor;
   }
   for (int j = lane; j < a.K; j += 32) {
-    int first = j;      // every entry of a repeated id carries the id's gradient
-    if (en.state[j] == 2)
-      for (first = 0; ids[first] != ids[j];) ++first;
-    a.fix[(size_t)r * a.K + j] = w == 0.f ? 0.f : en.fix[first];
+    double q = 0.0;        // every entry of a repeated id carries the id's gradient
+    for (int i = 0; i < a.K; ++i)
+      if (valid(i) && ids[i] == ids[j]) q += exp2_d(((double)logq[i] - (double)ref) * kLog2e);
+    const double s = f.per_p == 0.0 ? 0.0 : f.per_p * exp2_d(entry(j) - f.m);
+    a.fix[(size_t)r * a.K + j] = w == 0.f || !valid(j) ? 0.f : (float)(s - f.per_q * q);
   }
 }
 
@@ -650,10 +1325,18 @@ __global__ void __launch_bounds__(kThreads) distill_grad_kernel(const T* logits,
   const T* x = logits + (size_t)r * a.stride;
   T* g = grad + (size_t)r * a.V;
   const Row<const T> row(x, a.V);
-  const float c = row_c(a.temp, a.temp1, r);
-  write_gradient(row, g, a.V, c, a.coef[2 * (size_t)r], a.coef[2 * (size_t)r + 1]);
+  const Row<T> out(g, a.V);
+  const bool vec = row.shift == out.shift;
+  const float c = row_c(a, r), R = a.coef[2 * (size_t)r], factor = a.coef[2 * (size_t)r + 1];
+  for (int i = threadIdx.x; i < row.units; i += blockDim.x) {
+    Unit<T> v;
+    if (factor != 0.f) v = row.load(i);
+    if (factor != 0.f) gradient_unit(v, c, R, factor);
+    else v.fill(from_f<T>(0.f));
+    out.store(i, v, vec, row.shift);
+  }
   __syncthreads();
-  for (int j = threadIdx.x; j < a.K; j += kThreads) {
+  for (int j = threadIdx.x; j < a.K; j += blockDim.x) {
     const long id = a.ids[(size_t)r * a.K + j], t = id - a.vocab_start;
     if (id >= 0 && id < a.vocab_total && t >= 0 && t < a.V) g[t] = from_f<T>(a.fix[(size_t)r * a.K + j]);
   }
@@ -687,6 +1370,7 @@ __global__ void scale_unless_one_kernel(T* __restrict__ x, long n, const float* 
     x[i] = from_f<T>(to_f(x[i]) * f);
 }
 
+// -------------------------------------------------------------------------------------------------- host
 template <typename F>
 cudaError_t by_type(RowType t, F&& f) {
   if (t == RowType::f32) return f((float*)nullptr);
@@ -700,6 +1384,69 @@ cudaError_t launched() {
   return e;
 }
 
+// How a row is spread: blocks per cluster, threads per block, units held per thread (0: streamed).
+struct Shape {
+  int blocks, threads, units;
+};
+
+int units_of(int V, int width) { return (V * (long)width + 30) / 16; }   // of a row at any alignment
+
+int sm_count() {
+  static const int n = [] {
+    int dev = 0, v = 148;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev);
+    return v;
+  }();
+  return n;
+}
+
+// Rows held in registers: as few blocks as hold the row with 5 units per thread, and more while every SM still gets at
+// most one.  units = 0: too long.
+Shape held_shape(int rows, int units) {
+  int b = 1;
+  while (b < kMaxCluster && b * kThreads * 5 < units) b *= 2;
+  while (b < kMaxCluster && 2l * rows * b <= sm_count() && units >= 2 * b * 256) b *= 2;
+  for (int n : {1, 2, 5, 10}) {
+    const int t = (units + b * n - 1) / (b * n);
+    if (t <= kThreads) return {b, std::max(32, (t + 31) / 32 * 32), n};
+  }
+  return {kMaxCluster, kThreads, 0};
+}
+
+// Rows that stream: a warp per batch of units up to 8, `least` blocks per row, and more of long rows while that makes
+// no more than `most` blocks.
+Shape stream_shape(int rows, int units, int least, int most) {
+  int b = least;
+  while (b < kMaxCluster && 2l * rows * b <= most && units >= std::max(2048, 2 * b * 512)) b *= 2;
+  const int batches = ((units + b - 1) / b + kSpan - 1) / kSpan;
+  return {b, std::min(kStream, 32 * batches), 0};
+}
+
+// Whether rows are held rather than streamed: short ones always, longer ones while their blocks are resident at once
+// (up to about `per_sm` for every SM).
+bool hold(int rows, int units, int shortest, float per_sm) {
+  const Shape s = held_shape(rows, units);
+  return s.units && (units <= shortest || (float)rows * s.blocks <= per_sm * sm_count());
+}
+
+template <typename K, typename... A>
+cudaError_t launch_rows(K kernel, int rows, Shape s, size_t smem, cudaStream_t stream, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)rows * s.blocks);
+  cfg.blockDim = dim3(s.threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim = {(unsigned)s.blocks, 1, 1};
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) return e;
+  return launched();
+}
+
 }  // namespace
 
 namespace bb {
@@ -707,10 +1454,32 @@ namespace bb {
 cudaError_t launch_token_logprob(RowType t, const void* logits, const TokenArgs& a, cudaStream_t stream) {
   return by_type(t, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    auto* kern = a.k ? (a.entropy ? token_logprob_kernel<T, true, true> : token_logprob_kernel<T, false, true>)
-                     : (a.entropy ? token_logprob_kernel<T, true, false> : token_logprob_kernel<T, false, false>);
-    kern<<<(unsigned)a.U, kThreads, a.k ? sizeof(Select) : 0, stream>>>((const T*)logits, a);
-    return launched();
+    using Kernel = void (*)(const T*, TokenArgs);
+    const bool e = a.entropy != nullptr;
+    const int units = units_of(a.V, sizeof(T));
+    Shape s{0, 0, 0};
+    if (a.k && hold(a.U, units, 2560, 2.75f)) s = held_shape(a.U, units);
+    Kernel kern;
+    switch (s.units) {
+      case 1: kern = e ? token_top_kernel<T, true, 1> : token_top_kernel<T, false, 1>; break;
+      case 2: kern = e ? token_top_kernel<T, true, 2> : token_top_kernel<T, false, 2>; break;
+      case 5: kern = e ? token_top_kernel<T, true, 5> : token_top_kernel<T, false, 5>; break;
+      case 10: kern = e ? token_top_kernel<T, true, 10> : token_top_kernel<T, false, 10>; break;
+      default: {
+        s = stream_shape(a.U, units, 1, sm_count() * 4 / 3);
+        size_t smem = Feed<T>::bytes(s.threads);
+        if (a.k) {
+          kern = e ? token_stream_kernel<T, true, true> : token_stream_kernel<T, false, true>;
+          smem = std::max(smem, sizeof(Select)) + sizeof(float) * (kBatch + units / 32 / s.blocks + 2 + kStream / 32 * kBatch);
+        } else {
+          kern = e ? token_stream_kernel<T, true, false> : token_stream_kernel<T, false, false>;
+        }
+        const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (err != cudaSuccess) return err;
+        return launch_rows(kern, a.U, s, smem, stream, (const T*)logits, a);
+      }
+    }
+    return launch_rows(kern, a.U, s, sizeof(Select), stream, (const T*)logits, a);
   });
 }
 
@@ -719,29 +1488,39 @@ cudaError_t launch_token_logprob_bwd(RowType t, const void* logits, void* grad, 
   return by_type(t, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     auto* kern = a.d_entropy ? token_logprob_bwd_kernel<T, true> : token_logprob_bwd_kernel<T, false>;
-    kern<<<(unsigned)a.U, kThreads, 0, stream>>>((const T*)logits, (T*)grad, a);
-    return launched();
+    const Shape s = stream_shape(a.U, units_of(a.V, sizeof(T)), 1, sm_count() * 2);
+    const size_t smem = Feed<T>::bytes(s.threads);
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    return launch_rows(kern, a.U, s, smem, stream, (const T*)logits, (T*)grad, a);
   });
 }
 
-size_t distill_smem(long V) {   // one byte per unit, in words: (V + 7 + 7) / 8 units at most
-  return ((size_t)(V + 14) / 8 + 3) / 4 * 4;
-}
-
-cudaError_t launch_distill(RowType t, Distill mode, const void* logits, void* grad, const DistillArgs& a,
-                           cudaStream_t stream) {
+cudaError_t launch_distill(RowType t, const void* logits, void* grad, const DistillArgs& a, cudaStream_t stream) {
   return by_type(t, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    auto* kern = mode == Distill::open ? distill_kernel<T, false, true>
-                                       : (mode == Distill::loss ? distill_kernel<T, false, false>
-                                                                : distill_kernel<T, true, false>);
-    const size_t smem = distill_smem(a.V);
-    if (smem + sizeof(Entries) + 1024 > 48 * 1024) {
-      const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-      if (e != cudaSuccess) return e;
+    const int units = units_of(a.V, sizeof(T));
+    Shape s{0, 0, 0};
+    if (hold(a.U, units, 2048, 1.75f)) s = held_shape(a.U, units);
+    using Kernel = void (*)(const T*, T*, DistillArgs);
+    Kernel kern;
+    size_t smem = Entries::bytes(a.K, s.threads);
+    switch (s.units) {
+      case 1: kern = distill_kernel<T, 1>; break;
+      case 2: kern = distill_kernel<T, 2>; break;
+      case 5: kern = distill_kernel<T, 5>; break;
+      case 10: kern = distill_kernel<T, 10>; break;
+      default: {
+        kern = distill_stream_kernel<T>;
+        // with a second pass, the rows in work (4 blocks for every SM) should fit L2
+        const bool twice = grad && a.U >= 2 * sm_count() && 4l * sm_count() * units * 16 > (100l << 20);
+        s = stream_shape(a.U, units, twice ? 2 : 1, sm_count() * 4 / 3);
+        smem = Feed<T>::bytes(s.threads) + Entries::bytes(a.K, units / s.blocks / kSpan + 2);
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+      }
     }
-    kern<<<(unsigned)a.U, kThreads, smem, stream>>>((const T*)logits, (T*)grad, a);
-    return launched();
+    return launch_rows(kern, a.U, s, smem, stream, (const T*)logits, (T*)grad, a);
   });
 }
 

@@ -2,25 +2,25 @@
 #pragma once
 
 #include <cuda_runtime.h>
-#include <stddef.h>
 #include <stdint.h>
 
 namespace bb {
 
 constexpr int kMaxTop = 256;   // alternatives per row, and teacher entries per row
+constexpr int kMaxVocab = 1 << 22;   // columns: bounds what a block notes about its slice in shared memory
 
 enum class RowType { f32, f16, bf16 };
 
 struct TokenArgs {
   const int64_t* tokens;   // [U, n] or null
   const float* temp;       // [U] or null
-  double temp1;            // the temperature of every row when temp is null
+  double inv_temp1;        // 1 / T of every row when temp is null
   int U, V, n, k;
   long stride;             // elements between rows of the logits
   long vocab_start, vocab_total;
   float* logp;             // [U, n]: finished log-probs, or the tokens' x c when `open`
   float* entropy;          // [U] or null
-  float* stats;            // [U, 3]: (R, 1/s, sum e t / s), or (R, s, sum e t) when `open`
+  float* stats;            // [U, 3] or null: (R, 1/s, sum e t / s), or (R, s, sum e t) when `open`
   int64_t* top_ids;        // [U, k]
   float* top_logp;         // [U, k]: finished, or the raw logits when `open`
   const float* d_logp;     // [U, n]  (backward)
@@ -33,12 +33,12 @@ struct DistillArgs {
   const float* logq;       // [U, K]
   const float* weights;    // [U] or null
   const float* temp;       // [U] or null
-  double temp1;
+  double inv_temp1;
   double scale;            // grad_scale / denom
   int U, V, K;
   long stride;
   long vocab_start, vocab_total;
-  bool tail;
+  bool tail, open;         // open: a shard of the vocabulary, the sums are joined elsewhere
   float* rows;             // [U] divergence
   float* stats;            // [U, 2] (R, s) of the columns outside the given ids
   float* xc;               // [U, K] x c of the given ids in this shard, else 0
@@ -49,10 +49,8 @@ struct DistillArgs {
 cudaError_t launch_token_logprob(RowType t, const void* logits, const TokenArgs& a, cudaStream_t stream);
 cudaError_t launch_token_logprob_bwd(RowType t, const void* logits, void* grad, const TokenArgs& a,
                                      cudaStream_t stream);
-enum class Distill { loss, loss_and_grad, open };
-size_t distill_smem(long V);   // bytes of shared memory beside the fixed ones
-cudaError_t launch_distill(RowType t, Distill mode, const void* logits, void* grad, const DistillArgs& a,
-                           cudaStream_t stream);
+// rows (+ grad unless null), or with a.open a shard's stats and xc
+cudaError_t launch_distill(RowType t, const void* logits, void* grad, const DistillArgs& a, cudaStream_t stream);
 cudaError_t launch_distill_finish(const DistillArgs& a, cudaStream_t stream);
 cudaError_t launch_distill_grad(RowType t, const void* logits, void* grad, const DistillArgs& a, cudaStream_t stream);
 cudaError_t launch_weighted_sum(const float* rows, const float* weights, int U, double inv_denom, float* out,

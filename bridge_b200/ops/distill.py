@@ -107,12 +107,9 @@ def _grad_reference(logits, ids, coef, fix, temp, temp1, vocab_start, total):
 
 # ------------------------------------------------------------------------------------------- one shard
 def _rows_and_grad(logits, ids, logq, weights, temp, temp1, scale, tail, want_grad, inplace, vocab_start, group):
-    """``(KL [U], gradient or None)`` of this rank's shard (a whole vocabulary without a group)."""
+    """``(KL [U], gradient or None)`` of this rank's shard, in steps (and the PyTorch form)."""
     own, world = on_gpu(logits), tp_world(group)
     total = logits.shape[1] * world
-    if own and world == 1:
-        rows, grad = kernels().distill_rows(logits, ids, logq, weights, temp, temp1, scale, tail, want_grad, inplace)
-        return rows, (grad if want_grad else None)
     if own:
         stats, xc = kernels().distill_open(logits, ids, logq, weights, temp, temp1, vocab_start, total)
     else:
@@ -148,6 +145,8 @@ def _scale_by(grad, dloss, grad_scale):
 
 
 class _TopkDistillFn(torch.autograd.Function):
+    """Vocabularies in shards, and the PyTorch form."""
+
     @staticmethod
     def forward(ctx, logits, ids, logq, weights, temp, temp1, tail, denom, grad_scale, vocab_start, group):
         rows, grad = _rows_and_grad(logits, ids, logq, weights, temp, temp1, grad_scale / denom, tail,
@@ -178,9 +177,12 @@ class _FusedHeadDistillFn(torch.autograd.Function):
         for a in range(0, h.shape[0], chunk_rows):
             at = slice(a, min(a + chunk_rows, h.shape[0]))
             lg = gemm(h[at], weight)
-            rows, dlg = _rows_and_grad(lg, ids[at], logq[at], None if weights is None else weights[at],
-                                       None if temp is None else temp[at], temp1, grad_scale / denom, tail, want,
-                                       want, vocab_start, group)
+            teacher = (ids[at], logq[at], None if weights is None else weights[at], None if temp is None else temp[at],
+                       temp1, grad_scale / denom, tail, want)
+            if tp_world(group) == 1:
+                rows, dlg = kernels().distill_rows_inplace(lg, *teacher), lg
+            else:
+                rows, dlg = _rows_and_grad(lg, *teacher, want, vocab_start, group)
             parts.append(rows)
             if not want:
                 continue
@@ -221,7 +223,9 @@ def _arguments(name, rows, device, ids, logq, weights, temperature, denom, grad_
     if weights is not None:
         weights = row_floats(name, "weights", weights, rows, device)
     temp, temp1 = split_temperature(name, temperature, rows, device)
-    return ids, logq.detach().float().contiguous(), weights, temp, temp1
+    if logq.dtype != torch.float32 or not logq.is_contiguous() or logq.requires_grad:
+        logq = logq.detach().float().contiguous()
+    return ids, logq, weights, temp, temp1
 
 
 def topk_distill_loss(logits: Tensor, teacher_ids: Tensor, teacher_logp: Tensor, *, denom: float,
@@ -239,8 +243,10 @@ def topk_distill_loss(logits: Tensor, teacher_ids: Tensor, teacher_logp: Tensor,
     check_logits(name, logits)
     args = _arguments(name, logits.shape[0], logits.device, teacher_ids, teacher_logp, weights, temperature, denom,
                       grad_scale)
-    return _TopkDistillFn.apply(unit_columns(logits), *args, bool(tail), float(denom), float(grad_scale),
-                                int(vocab_start), tp_group)
+    logits = unit_columns(logits)
+    if tp_world(tp_group) == 1 and on_gpu(logits):
+        return tuple(kernels().topk_distill(logits, *args, tail, denom, grad_scale))
+    return _TopkDistillFn.apply(logits, *args, tail, float(denom), float(grad_scale), vocab_start, tp_group)
 
 
 def fused_lm_head_topk_distill(h: Tensor, weight: Tensor, teacher_ids: Tensor, teacher_logp: Tensor, *, denom: float,

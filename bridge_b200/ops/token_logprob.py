@@ -66,7 +66,7 @@ def check_ids(name: str, what: str, ids: Tensor, rows: int, device) -> Tensor:
         raise ValueError(f"{name}: {what} must be [{rows}] or [{rows}, n], got {tuple(ids.shape)}")
     if ids.device != device:
         raise ValueError(f"{name}: {what} are on {ids.device}, the logits on {device}")
-    return ids.long().contiguous()
+    return ids if ids.dtype == torch.int64 and ids.is_contiguous() else ids.long().contiguous()
 
 
 def row_floats(name: str, what: str, value: Tensor, rows: int, device) -> Tensor:
@@ -74,6 +74,8 @@ def row_floats(name: str, what: str, value: Tensor, rows: int, device) -> Tensor
         raise ValueError(f"{name}: {what} must be [{rows}], got {tuple(value.shape)}")
     if value.device != device:
         raise ValueError(f"{name}: {what} is on {value.device}, the logits on {device}")
+    if value.dtype == torch.float32 and value.is_contiguous() and not value.requires_grad:
+        return value
     return value.detach().float().contiguous()
 
 
@@ -137,6 +139,8 @@ def top_rows(x: Tensor, k: int) -> Tensor:
 
 # -------------------------------------------------------------------------------------------- autograd
 class _TokenLogprobFn(torch.autograd.Function):
+    """Vocabularies in shards, and the PyTorch form."""
+
     @staticmethod
     def forward(ctx, logits, tokens, temp, temp1, top_k, with_entropy, vocab_start, group):
         world = tp_world(group)
@@ -145,38 +149,38 @@ class _TokenLogprobFn(torch.autograd.Function):
         k = min(top_k, logits.shape[1])
         ctx.set_materialize_grads(False)
         ctx.vocab_start, ctx.total, ctx.temp1, ctx.own = vocab_start, total, temp1, own
-        if own and world == 1:
-            logp, ent, stats, ids, top = kernels().token_logprob_fwd(logits, tokens, temp, temp1, k, with_entropy,
-                                                                     vocab_start, False)
+        if own:
+            xt, sums, ids, top = kernels().token_logprob_open(logits, tokens, temp, temp1, k, with_entropy, vocab_start)
+            r, s, et = sums.unbind(1)
         else:
-            if own:
-                xt, _, sums, ids, top = kernels().token_logprob_fwd(logits, tokens, temp, temp1, k, with_entropy,
-                                                                    vocab_start, True)
-                r, s, et = sums.unbind(1)
-            else:
-                xc = logits.to(torch.promote_types(logits.dtype, torch.float32)) * log2_scale(temp, temp1, logits)
-                r, s, et = shard_sums(xc)
-                xt = picked(xc, tokens, vocab_start) if tokens is not None else xc.new_empty((xc.shape[0], 0))
+            xc = logits.to(torch.promote_types(logits.dtype, torch.float32)) * log2_scale(temp, temp1, logits)
+            r, s, et = shard_sums(xc)
+            xt = picked(xc, tokens, vocab_start) if tokens is not None else None
+            ids = top = None
+            if k:
                 ids = top_rows(logits, k)
                 top = logits.gather(1, ids).to(xc.dtype)
                 ids = ids + vocab_start
-            if world > 1:
-                r, s, et = join_shards(r, s, et, group)
+        if world > 1:
+            r, s, et = join_shards(r, s, et, group)
+            if xt is not None:
                 dist.all_reduce(xt, group=group)
+            if top_k:
                 ids, top = _join_tops(ids, top, top_k, world, group)
-            log2s = torch.log2(s)
-            full = r + log2s
+        log2s = torch.log2(s)
+        full = r + log2s
+        logp = None
+        if tokens is not None:
             logp = _finish(xt, full, s)
-            if tokens is not None:
-                logp = torch.where((tokens >= 0) & (tokens < total), logp, torch.zeros_like(logp))
-            empty = s == 0
-            one = torch.where(empty, torch.ones_like(s), s)
-            ent = torch.where(empty, torch.zeros_like(s), _LN2 * (log2s - et / one))
-            stats = torch.stack((r, torch.where(empty, torch.zeros_like(s), 1.0 / one), et / one), dim=1)
-            if top.shape[1]:
-                top = _finish(top * log2_scale(temp, temp1, top), full, s)
+            logp = torch.where((tokens >= 0) & (tokens < total), logp, torch.zeros_like(logp))
+        empty = s == 0
+        one = torch.where(empty, torch.ones_like(s), s)
+        ent = torch.where(empty, torch.zeros_like(s), _LN2 * (log2s - et / one)) if with_entropy else None
+        stats = torch.stack((r, torch.where(empty, torch.zeros_like(s), 1.0 / one), et / one), dim=1)
+        if top_k:
+            top = _finish(top * log2_scale(temp, temp1, top), full, s)
+            ctx.mark_non_differentiable(ids, top)
         ctx.save_for_backward(logits, tokens, temp, stats)
-        ctx.mark_non_differentiable(ids, top)
         return logp, ent, ids, top
 
     @staticmethod
@@ -203,15 +207,13 @@ def _finish(xc: Tensor, full: Tensor, s: Tensor) -> Tensor:
 def _join_tops(ids: Tensor, top: Tensor, k: int, world: int, group) -> tuple[Tensor, Tensor]:
     """The ``k`` best of every rank's best.  Ranks hold ascending ids and equal logits are in id order within
     a rank, so the lower position of a tie is the lower id."""
-    if k == 0:
-        return ids, top
     every_id = [torch.empty_like(ids) for _ in range(world)]
     every_top = [torch.empty_like(top) for _ in range(world)]
     dist.all_gather(every_id, ids.contiguous(), group=group)
     dist.all_gather(every_top, top.contiguous(), group=group)
     ids, top = torch.cat(every_id, dim=1), torch.cat(every_top, dim=1)
     if on_gpu(top):
-        at = kernels().token_logprob_fwd(top, None, None, 1.0, k, False, 0, True)[3]
+        at = kernels().token_logprob_open(top, None, None, 1.0, k, False, 0)[2]
     else:
         at = top_rows(top, k)
     return ids.gather(1, at), top.gather(1, at)
@@ -246,18 +248,20 @@ def token_logprobs(logits: Tensor, tokens: Tensor | None = None, temperature: Te
     name = "token_logprobs"
     check_logits(name, logits)
     rows, device = logits.shape[0], logits.device
-    total = logits.shape[1] * tp_world(tp_group)
+    world = tp_world(tp_group)
+    total = logits.shape[1] * world
     if not 0 <= top_k <= min(MAX_TOP, total):
         raise ValueError(f"{name}: top_k must be within 0..{min(MAX_TOP, total)}, got {top_k}")
-    flat = tokens is None or tokens.ndim == 1
     if tokens is not None:
         tokens = check_ids(name, "tokens", tokens, rows, device)
-        tokens = tokens[:, None] if flat else tokens
     temp, temp1 = split_temperature(name, temperature, rows, device)
-    logp, ent, ids, top = _TokenLogprobFn.apply(unit_columns(logits), tokens, temp, temp1, int(top_k),
-                                                bool(with_entropy), int(vocab_start), tp_group)
-    return TokenLogprobs(None if tokens is None else (logp[:, 0] if flat else logp), ent if with_entropy else None,
-                         ids if top_k else None, top if top_k else None)
+    logits = unit_columns(logits)
+    if world == 1 and on_gpu(logits):
+        return TokenLogprobs(*kernels().token_logprobs(logits, tokens, temp, temp1, top_k, with_entropy))
+    flat = tokens is not None and tokens.ndim == 1
+    logp, ent, ids, top = _TokenLogprobFn.apply(logits, tokens[:, None] if flat else tokens, temp, temp1, top_k,
+                                                with_entropy, vocab_start, tp_group)
+    return TokenLogprobs(logp[:, 0] if flat else logp, ent, ids, top)
 
 
 @torch.no_grad()
