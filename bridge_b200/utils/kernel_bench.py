@@ -291,8 +291,42 @@ def bench_moe(t: Timer, small: bool):
     _report("moe_combine_bwd", {"T": T, "k": k, "H": H}, ms, bytes_=(2 * T * k + T) * H * 2)
 
 
+def bench_vocab_rows(t: Timer, small: bool):
+    """Scoring with alternatives and distillation on rows of BF16 logits (vocabulary of 151936)."""
+    from bridge_b200.ops import token_logprobs, topk_distill_loss
+
+    U = 4096 if not small else 1024
+    V, k = 151936, 64
+    x = (3.0 * torch.randn(U, V, device="cuda")).to(torch.bfloat16)
+    tok = torch.randint(0, V, (U,), device="cuda")
+    nb = 2.0 * U * V
+    ms = t(lambda: token_logprobs(x, tok))
+    _report("token_logprobs", {"U": U, "V": V}, ms, bytes_=nb)
+    ms = t(lambda: token_logprobs(x, tok, top_k=k))
+    _report("token_logprobs_top", {"U": U, "V": V, "k": k}, ms, bytes_=nb)
+    r = token_logprobs(x, None, top_k=k)
+    xg = x.detach().requires_grad_()
+    d = torch.randn(U, device="cuda")
+
+    def score_fb():
+        s = token_logprobs(xg, tok)
+        torch.autograd.grad((s.logp, s.entropy), xg, (d, d))
+
+    ms = t(score_fb)
+    _report("token_logprobs_fwd_bwd", {"U": U, "V": V}, ms, bytes_=3 * nb)
+    ms = t(lambda: topk_distill_loss(x, r.top_ids, r.top_logp, denom=float(U), temperature=1.3))
+    _report("topk_distill_loss", {"U": U, "V": V, "k": k}, ms, bytes_=nb)
+
+    def distill_fb():
+        loss, _ = topk_distill_loss(xg, r.top_ids, r.top_logp, denom=float(U), temperature=1.3)
+        torch.autograd.grad(loss, xg)
+
+    ms = t(distill_fb)
+    _report("topk_distill_fwd_bwd", {"U": U, "V": V, "k": k}, ms, bytes_=2 * nb)
+
+
 OPS = {"gemm": bench_gemm, "attention": bench_attention, "elementwise": bench_elementwise,
-       "logprob": bench_logprob, "ppo": bench_ppo, "gdn": bench_gdn, "moe": bench_moe}
+       "logprob": bench_logprob, "vocab_rows": bench_vocab_rows, "ppo": bench_ppo, "gdn": bench_gdn, "moe": bench_moe}
 
 
 def main(argv=None):
