@@ -114,23 +114,21 @@ struct Unit {
     for (int j = 0; j < kE; ++j)
       if (m >> j & 1u) set(j, from_f<T>(-INFINITY));
   }
-  __device__ __forceinline__ void floats(float* f) const {
-    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
-      const uint32_t h[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        f[2 * j] = __uint_as_float(h[j] << 16);
-        f[2 * j + 1] = __uint_as_float(h[j] & 0xffff0000u);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < kE; ++j) f[j] = to_f(get(j));
-    }
+  __device__ __forceinline__ float2 pair(int j) const {
+    if constexpr (sizeof(T) == 4) return make_float2(get(2 * j), get(2 * j + 1));
+    const uint32_t h = reinterpret_cast<const uint32_t*>(&w)[j];
+    if constexpr (std::is_same_v<T, __nv_bfloat16>)
+      return make_float2(__uint_as_float(h << 16), __uint_as_float(h & 0xffff0000u));
+    else
+      return __half22float2(reinterpret_cast<const __half2&>(h));
   }
-  __device__ __forceinline__ void set_pair(int j, float a, float b) {
-    if constexpr (std::is_same_v<T, __nv_bfloat16>) reinterpret_cast<__nv_bfloat162*>(&w)[j] = __floats2bfloat162_rn(a, b);
-    else if constexpr (std::is_same_v<T, __half>) reinterpret_cast<__half2*>(&w)[j] = __floats2half2_rn(a, b);
-    else set(2 * j, a), set(2 * j + 1, b);
+  __device__ __forceinline__ void set_pair(int j, float2 f) {
+    if constexpr (std::is_same_v<T, __nv_bfloat16>)
+      reinterpret_cast<__nv_bfloat162*>(&w)[j] = __floats2bfloat162_rn(f.x, f.y);
+    else if constexpr (std::is_same_v<T, __half>)
+      reinterpret_cast<__half2*>(&w)[j] = __floats2half2_rn(f.x, f.y);
+    else
+      set(2 * j, f.x), set(2 * j + 1, f.y);
   }
   __device__ __forceinline__ float max() const {          // NaN does not count
     if constexpr (sizeof(T) == 4) {
@@ -143,6 +141,8 @@ struct Unit {
     }
   }
 };
+
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // One row as units on 16-byte boundaries: unit i covers the aligned positions kE i .. kE i + kE - 1, and position a
 // holds token a - shift.  Only the first and the last unit can be partly outside the row.
@@ -210,32 +210,31 @@ struct Stat {
   }
 };
 
-// A thread's running sums, in two chains.
+// A thread's running sums, two FP32 lanes to an instruction.
 struct Sums {
-  float R, s[2], et[2];
+  float R;
+  float2 s, et;
 
-  __device__ __forceinline__ Sums() : R(kMasked), s{0.f, 0.f}, et{0.f, 0.f} {}
+  __device__ __forceinline__ Sums() : R(kMasked), s(both(0.f)), et(both(0.f)) {}
   __device__ __forceinline__ void raise(float to) {
     const float d = R - to, k = ex2(d);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      et[j] = k * (et[j] + d * s[j]);
-      s[j] *= k;
-    }
+    et = __fmul2_rn(both(k), __ffma2_rn(both(d), s, et));
+    s = __fmul2_rn(both(k), s);
     R = to;
   }
-  template <bool kEntropy, typename T>
+  // kMask: some t may be -inf, whose e = 0 would make e t NaN
+  template <bool kEntropy, bool kMask, typename T>
   __device__ __forceinline__ void add(const Unit<T>& u, float c) {
-    float f[Unit<T>::kE];
-    u.floats(f);
 #pragma unroll
-    for (int j = 0; j < Unit<T>::kE; ++j) {
-      const float t = fmaf(f[j], c, -R), e = ex2(t);
-      s[j & 1] += e;
-      if (kEntropy) et[j & 1] = fmaf(e, fmaxf(t, -1e4f), et[j & 1]);   // e = 0 there; -inf would make it NaN
+    for (int j = 0; j < Unit<T>::kE / 2; ++j) {
+      float2 t = __ffma2_rn(u.pair(j), both(c), both(-R));
+      const float2 e = make_float2(ex2(t.x), ex2(t.y));
+      s = __fadd2_rn(s, e);
+      if (kEntropy && kMask) t = make_float2(fmaxf(t.x, -1e4f), fmaxf(t.y, -1e4f));
+      if (kEntropy) et = __ffma2_rn(e, t, et);
     }
   }
-  __device__ __forceinline__ Stat get() const { return {R, s[0] + s[1], et[0] + et[1]}; }
+  __device__ __forceinline__ Stat get() const { return {R, s.x + s.y, et.x + et.y}; }
 };
 
 __device__ __forceinline__ float warp_top(float v) {
@@ -420,12 +419,17 @@ struct Feed {
   }
 };
 
-template <typename T, int N>
-__device__ __forceinline__ float units_max(const Unit<T>* u) {
+// The largest (kSign = 1) or smallest (-1) element; NaN does not count.
+template <int kSign, typename T, int N>
+__device__ __forceinline__ float units_extreme(const Unit<T>* u) {
+  const auto pick = [](auto a, auto b) {
+    if constexpr (std::is_same_v<decltype(a), float>) return kSign > 0 ? fmaxf(a, b) : fminf(a, b);
+    else return kSign > 0 ? __hmax2(a, b) : __hmin2(a, b);
+  };
   if constexpr (sizeof(T) == 4) {
-    float m = u[0].max();
+    float m = u[0].get(0);
 #pragma unroll
-    for (int n = 1; n < N; ++n) m = fmaxf(m, u[n].max());
+    for (int i = 1; i < 4 * N; ++i) m = pick(m, u[i / 4].get(i % 4));
     return m;
   } else {
     using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
@@ -434,10 +438,29 @@ __device__ __forceinline__ float units_max(const Unit<T>* u) {
     for (int j = 0; j < 4; ++j) {
       m[j] = reinterpret_cast<const T2*>(&u[0].w)[j];
 #pragma unroll
-      for (int n = 1; n < N; ++n) m[j] = __hmax2(m[j], reinterpret_cast<const T2*>(&u[n].w)[j]);
+      for (int n = 1; n < N; ++n) m[j] = pick(m[j], reinterpret_cast<const T2*>(&u[n].w)[j]);
     }
-    m[0] = __hmax2(__hmax2(m[0], m[1]), __hmax2(m[2], m[3]));
-    return fmaxf(to_f(m[0].x), to_f(m[0].y));
+    m[0] = pick(pick(m[0], m[1]), pick(m[2], m[3]));
+    return pick(to_f(m[0].x), to_f(m[0].y));
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ float units_max(const Unit<T>* u) {
+  return units_extreme<1, T, N>(u);
+}
+// Whether some t of these units may be infinite.
+template <typename T, int N>
+__device__ __forceinline__ bool masked(const Unit<T>* u, float c) {
+  return units_extreme<-1, T, N>(u) * c < 0.1f * kMasked;
+}
+template <bool kEntropy, typename T, int N>
+__device__ __forceinline__ void add_units(Sums& sums, const Unit<T>* u, float c) {
+  if (kEntropy && masked<T, N>(u, c)) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) sums.template add<kEntropy, true>(u[n], c);
+  } else {
+#pragma unroll
+    for (int n = 0; n < N; ++n) sums.template add<kEntropy, false>(u[n], c);
   }
 }
 
@@ -686,8 +709,7 @@ __global__ void __launch_bounds__(kThreads, kUnits == 10 ? 1 : 3) token_top_kern
   const float best = units_max<T, kUnits>(u);
   Sums sums;
   sums.R = fmaxf(best * c, kMasked);
-#pragma unroll
-  for (int n = 0; n < kUnits; ++n) sums.template add<kEntropy>(u[n], c);
+  add_units<kEntropy, T, kUnits>(sums, u, c);
   Stat st = block_join(sums.get(), part);
   const bool any = sl.lo + (int)threadIdx.x < sl.hi;
   const uint32_t best_key = order_key(best);
@@ -752,8 +774,7 @@ __global__ void __launch_bounds__(kStream, 4) token_stream_kernel(const T* __res
     else feed.issue(k + kGroups);
     top *= c;
     if (top > sums.R + kSlack) sums.raise(top);
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b) sums.template add<kEntropy>(u[b], c);
+    add_units<kEntropy, T, kBatch>(sums, u, c);
   }
   Stat st = block_join(sums.get(), part);
   uint32_t bound = 0;
@@ -796,6 +817,18 @@ __global__ void __launch_bounds__(kStream, 4) token_stream_kernel(const T* __res
   if constexpr (kTop) write_top(a, r, row, c, st, log2s, *sel);
 }
 
+// u = 2^t (A + B t), t = u c - R
+template <bool kEntropy, bool kMask, typename T>
+__device__ __forceinline__ void score_gradient(Unit<T>& u, float c, float R, float A, float B) {
+#pragma unroll
+  for (int j = 0; j < Unit<T>::kE / 2; ++j) {
+    float2 t = __ffma2_rn(u.pair(j), both(c), both(-R));
+    const float2 e = make_float2(ex2(t.x), ex2(t.y));
+    if (kMask) t = make_float2(fmaxf(t.x, -1e4f), fmaxf(t.y, -1e4f));
+    u.set_pair(j, __fmul2_rn(e, kEntropy ? __ffma2_rn(both(B), t, both(A)) : both(A)));
+  }
+}
+
 // d x_v = (e / s / T) (-G - dH ln 2 (t - E[t])) + [v = t_j] g_j / T, G = sum_j g_j
 template <typename T, bool kEntropy>
 __global__ void __launch_bounds__(kStream, 4)
@@ -831,17 +864,12 @@ __global__ void __launch_bounds__(kStream, 4)
     feed.wait(k, row, sl);
     Unit<T> u[kBatch];
     feed.take(u);
+    if (kEntropy && masked<T, kBatch>(u, c)) {
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      float f[Unit<T>::kE];
-      u[b].floats(f);
+      for (int b = 0; b < kBatch; ++b) score_gradient<kEntropy, true>(u[b], c, R, A, B);
+    } else {
 #pragma unroll
-      for (int j = 0; j < Unit<T>::kE; ++j) {
-        const float t = fmaf(f[j], c, -R);
-        f[j] = ex2(t) * (kEntropy ? fmaf(B, fmaxf(t, -1e4f), A) : A);
-      }
-#pragma unroll
-      for (int j = 0; j < Unit<T>::kE; j += 2) u[b].set_pair(j / 2, f[j], f[j + 1]);
+      for (int b = 0; b < kBatch; ++b) score_gradient<kEntropy, false>(u[b], c, R, A, B);
     }
     if (feed.inner(k + kGroups)) feed.issue_inner(from, policy);
     else feed.issue(k + kGroups);
@@ -1109,11 +1137,11 @@ __device__ __forceinline__ void write_entries(const Shared& sh, const Entries& e
 
 template <typename T>
 __device__ __forceinline__ void gradient_unit(Unit<T>& u, float c, float R, float factor) {
-  float f[Unit<T>::kE];
-  u.floats(f);
 #pragma unroll
-  for (int j = 0; j < Unit<T>::kE; j += 2)
-    u.set_pair(j / 2, factor * ex2(fmaf(f[j], c, -R)), factor * ex2(fmaf(f[j + 1], c, -R)));
+  for (int j = 0; j < Unit<T>::kE / 2; ++j) {
+    const float2 t = __ffma2_rn(u.pair(j), both(c), both(-R));
+    u.set_pair(j, __fmul2_rn(make_float2(ex2(t.x), ex2(t.y)), both(factor)));
+  }
 }
 
 // A cluster per row, the row in registers, kUnits units per thread: the statistics of the columns outside the teacher's
@@ -1151,8 +1179,7 @@ __global__ void __launch_bounds__(kThreads, kUnits == 10 ? 1 : 2) distill_kernel
   }
   Sums sums;
   sums.R = fmaxf(units_max<T, kUnits>(u) * c, kMasked);
-#pragma unroll
-  for (int n = 0; n < kUnits; ++n) sums.template add<false>(u[n], c);
+  add_units<false, T, kUnits>(sums, u, c);
   finish_block<T>(sh, en, sums.get(), a, r, w, some, cl);
   if (grad) {
     T* g = grad + (size_t)r * a.V;
@@ -1213,8 +1240,7 @@ __global__ void __launch_bounds__(kStream, 4) distill_stream_kernel(const T* log
       if (feed.inner(k + kGroups)) feed.issue_inner(from, policy);
       else feed.issue(k + kGroups);
       if (top > sums.R + kSlack) sums.raise(top);
-#pragma unroll
-      for (int b = 0; b < kBatch; ++b) sums.template add<false>(u[b], c);
+      add_units<false, T, kBatch>(sums, u, c);
     }
   }
   finish_block<T>(sh, en, sums.get(), a, r, w, some, cl);
