@@ -18,7 +18,7 @@
 // 40 instructions a pass, which at 6.4 TB/s is two thirds of what the SMs can issue, so the loops are kept lean (paired
 // FP32 instructions, no checks inside a row) and everything that is per row overlaps other blocks' streaming.  B200,
 // vocabulary 151936, BF16, device time: scoring 4096 rows with entropy 0.20 ms (6.2 TB/s; 0.23 ms, 5.4 TB/s, under a
-// sustained power cap), 1024 rows with 64 alternatives 0.081 ms; gradient of the scores 0.21 ms for 2048 rows (6.0 TB/s);
+// sustained power cap), 1024 rows with 64 alternatives 0.079 ms; gradient of the scores 0.21 ms for 2048 rows (6.0 TB/s);
 // distillation loss 0.061 ms for 1024 rows, loss and gradient 0.48 ms for 4096 (5.2 TB/s of one read and one write);
 // one row with 20 alternatives 9 us, 8 rows of distillation with gradient 9 us.
 #include "vocab_rows.h"
@@ -770,7 +770,7 @@ template <typename T, bool kEntropy, bool kTop>
 __global__ void __launch_bounds__(kStream, 4) token_stream_kernel(const T* __restrict__ logits, TokenArgs a) {
   __shared__ Stat part[32];
   __shared__ RowPart mine;
-  __shared__ int hits;
+  __shared__ int hit_units;
   extern __shared__ __align__(16) unsigned char dyn[];
   cg::cluster_group cl = cg::this_cluster();
   const int blocks = (int)cl.num_blocks(), rank = (int)cl.block_rank(), lane = threadIdx.x & 31;
@@ -779,7 +779,10 @@ __global__ void __launch_bounds__(kStream, 4) token_stream_kernel(const T* __res
   const Row<const T> row(x, a.V);
   const Slice sl(row.units, blocks, rank);
   Feed<T, 1> feed(dyn, row, sl);
-  float* strips = reinterpret_cast<float*>(dyn + max(Feed<T, 1>::bytes(blockDim.x), sizeof(Select)));
+  // (the selection takes the ring's place once its copies are done)
+  float* strips = reinterpret_cast<float*>(dyn + max(Feed<T, 1>::bytes(blockDim.x), sizeof(Select) + 4 * kCand));
+  int* list = reinterpret_cast<int*>(dyn + sizeof(Select));
+  if (threadIdx.x == 0) hit_units = 0;
   const float c = row_c(a, r);
   Sums sums;
   float best = -INFINITY;
@@ -816,30 +819,35 @@ __global__ void __launch_bounds__(kStream, 4) token_stream_kernel(const T* __res
   join_row(mine, st, bound, sel, cl);
   if (kTop) {
     Select* lead = cl.map_shared_rank(sel, 0);
-    const int count = (held + 31) / 32, warps = blockDim.x >> 5;
+    const int count = (held + 31) / 32;
     const float floor = bound_value(bound);
-    int* list = reinterpret_cast<int*>(strips);      // (a thread's own maxima are read before anything is written)
-    for (int s0 = 0; s0 < count; s0 += blockDim.x) {
-      const int s = s0 + threadIdx.x;
-      const bool hit = s < count && order_key(strips[min(s, count - 1)]) >= bound;
-      if (threadIdx.x == 0) hits = 0;
-      __syncthreads();
-      if (hit) list[s0 + atomicAdd(&hits, 1)] = s;
-      __syncthreads();
-      constexpr int kAtOnce = 4;
-      for (int h = threadIdx.x >> 5; h < hits; h += kAtOnce * warps) {
+    // Units that reach the bound: first found, a warp to a strip, then taken apart, a thread to a unit.  (With the
+    // taking apart inside the strips' loop 32 lanes wait for one: 85 us, not 79, for 1024 x 151936 BF16 and k = 64.)
+    for (int s0 = 32 * (threadIdx.x >> 5); s0 < count; s0 += blockDim.x) {
+      unsigned hits = __ballot_sync(0xffffffffu, s0 + lane < count && strips[min(s0 + lane, count - 1)] >= floor);
+      while (hits) {
+        constexpr int kAtOnce = 4;
         Unit<T> u[kAtOnce];
         int at[kAtOnce];
 #pragma unroll
         for (int n = 0; n < kAtOnce; ++n) {
-          at[n] = h + n * warps < hits ? sl.lo + 32 * list[s0 + h + n * warps] + lane : sl.hi;
+          at[n] = hits ? sl.lo + 32 * (s0 + __ffs(hits) - 1) + lane : sl.hi;
+          hits &= hits - 1;
           if (at[n] < sl.hi) u[n] = row.load(at[n]);
         }
 #pragma unroll
-        for (int n = 0; n < kAtOnce; ++n)
-          if (at[n] < sl.hi && (floor == -INFINITY || u[n].max() >= floor)) offer(u[n], at[n], floor, row, lead);
+        for (int n = 0; n < kAtOnce; ++n) {
+          if (at[n] >= sl.hi || !(floor == -INFINITY || u[n].max() >= floor)) continue;
+          const int to = atomicAdd(&hit_units, 1);
+          if (to < kCand) list[to] = at[n];
+        }
       }
-      __syncthreads();
+    }
+    __syncthreads();
+    if (hit_units > kCand) {
+      if (threadIdx.x == 0) atomicAdd(&lead->count, kCand + 1);      // far too many: the exact way
+    } else {
+      for (int h = threadIdx.x; h < hit_units; h += blockDim.x) offer(row.load(list[h]), list[h], floor, row, lead);
     }
   }
   if (blocks > 1) cl.sync();      // the leader has every candidate, and nobody's sums are read any more
@@ -1538,7 +1546,7 @@ cudaError_t launch_token_logprob(RowType t, const void* logits, const TokenArgs&
         size_t smem = feed_bytes(s.threads);
         if (a.k) {
           kern = e ? token_stream_kernel<T, true, true> : token_stream_kernel<T, false, true>;
-          smem = std::max(smem, sizeof(Select)) + sizeof(float) * (kBatch + units / 32 / s.blocks + 2 + kStream / 32 * kBatch);
+          smem = std::max(smem, sizeof(Select) + 4 * kCand) + sizeof(float) * (kBatch + units / 32 / s.blocks + 2 + kStream / 32 * kBatch);
         } else {
           kern = e ? token_stream_kernel<T, true, false> : token_stream_kernel<T, false, false>;
         }
@@ -1615,7 +1623,7 @@ cudaError_t launch_weighted_sum(const float* rows, const float* weights, int U, 
 cudaError_t launch_scale_unless_one(RowType t, void* x, long n, const float* num, float den, cudaStream_t stream) {
   return by_type(t, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    const int blocks = resident_grid(scale_unless_one_kernel<T>, 512, 0, (n + 4095) / 4096);
+    const int blocks = (int)std::min<long>((n + 4095) / 4096, 4l * sm_count());
     scale_unless_one_kernel<T><<<blocks, 512, 0, stream>>>((T*)x, n, num, den);
     return launched();
   });
