@@ -3,6 +3,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <cmath>
+
 #include "vocab_rows.h"
 
 namespace {
@@ -29,6 +31,18 @@ void check_vec(const OptTensor& t, int64_t n, at::ScalarType dt, const torch::Te
   if (!t.has_value()) return;
   TORCH_CHECK(t->device() == x.device() && t->scalar_type() == dt && t->is_contiguous() && t->numel() == n, what);
 }
+// The forms that the kernels take as they are; anything else is checked and brought into them by the caller.
+bool plain_rows(const torch::Tensor& x) {
+  return x.is_cuda() && x.dim() == 2 && x.size(1) >= 1 && x.size(1) <= bb::kMaxVocab && x.size(0) < (1l << 28) &&
+         (x.size(1) == 1 || x.stride(1) == 1) &&
+         (x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf || x.scalar_type() == at::kFloat);
+}
+bool plain_floats(const OptTensor& t, const torch::Tensor& x) {
+  return !t.has_value() || (t->dim() == 1 && t->size(0) == x.size(0) && t->scalar_type() == at::kFloat &&
+                            t->is_contiguous() && t->device() == x.device() && !t->requires_grad());
+}
+bool positive(double v) { return v > 0.0 && std::isfinite(v); }
+
 template <typename V>
 V* ptr(const OptTensor& t) {
   return t.has_value() ? t->data_ptr<V>() : nullptr;
@@ -221,10 +235,17 @@ class DistillLoss : public torch::autograd::Function<DistillLoss> {
 
 }  // namespace
 
-// (log-probs, entropy, ids, their log-probs), None where not asked for.
+// (log-probs, entropy, ids, their log-probs), None where not asked for; empty where the arguments are not in the form
+// that the kernels take.
 std::vector<torch::Tensor> token_logprobs(torch::Tensor logits, OptTensor tokens, OptTensor temp, double temp1,
                                           int64_t k, bool entropy) {
-  check_scoring(logits, tokens, temp, k);
+  const bool fits = plain_rows(logits) && plain_floats(temp, logits) && positive(temp1) && k >= 0 && k <= bb::kMaxTop &&
+                    k <= logits.size(1) &&
+                    (!tokens.has_value() ||
+                     (tokens->dim() >= 1 && tokens->dim() <= 2 && tokens->size(0) == logits.size(0) &&
+                      tokens->scalar_type() == at::kLong && tokens->is_contiguous() &&
+                      tokens->device() == logits.device()));
+  if (!fits) return {};
   const bool differentiable = logits.requires_grad() && at::GradMode::is_enabled() && (tokens.has_value() || entropy);
   if (!differentiable) {
     const Scores o = score_rows(logits, tokens, temp, temp1, k, entropy, false, 0, false);
@@ -258,10 +279,17 @@ torch::Tensor token_logprob_bwd(torch::Tensor logits, OptTensor tokens, OptTenso
   return score_rows_bwd(logits, tokens, temp, temp1, stats, d_logp, d_entropy, vocab_start, vocab_total);
 }
 
-// (loss, KL [U]) of a whole vocabulary.
+// (loss, KL [U]) of a whole vocabulary; empty where the arguments are not in the form that the kernels take.
 std::vector<torch::Tensor> topk_distill(torch::Tensor logits, torch::Tensor ids, torch::Tensor logq, OptTensor weights,
                                         OptTensor temp, double temp1, bool tail, double denom, double grad_scale) {
-  check_rows(logits);
+  const auto entries = [&](const torch::Tensor& t, at::ScalarType dt) {
+    return t.dim() == 2 && t.size(0) == logits.size(0) && t.size(1) >= 1 && t.size(1) <= bb::kMaxTop &&
+           t.scalar_type() == dt && t.is_contiguous() && t.device() == logits.device() && !t.requires_grad();
+  };
+  const bool fits = plain_rows(logits) && plain_floats(temp, logits) && plain_floats(weights, logits) &&
+                    positive(temp1) && positive(denom) && positive(grad_scale) && entries(ids, at::kLong) &&
+                    entries(logq, at::kFloat) && logq.size(1) == ids.size(1);
+  if (!fits) return {};
   if (logits.requires_grad() && at::GradMode::is_enabled()) {
     const auto o = DistillLoss::apply(logits, ids, logq, weights, temp, temp1, tail, denom, grad_scale);
     return {o[0], o[1]};

@@ -239,14 +239,30 @@ def topk_distill_loss(logits: Tensor, teacher_ids: Tensor, teacher_logp: Tensor,
     pass over the gradient.  ``backward`` can be called once.  With ``tp_group``, ``logits`` is this rank's
     equal shard of the vocabulary and ``vocab_start`` its first token.
     """
+    if tp_group is None and on_gpu(logits):
+        got = _own(logits, teacher_ids, teacher_logp, weights, temperature, tail, denom, grad_scale)
+        if got:                                   # arguments that the kernels take as they are
+            return got[0], got[1]
     name = "topk_distill_loss"
     check_logits(name, logits)
     args = _arguments(name, logits.shape[0], logits.device, teacher_ids, teacher_logp, weights, temperature, denom,
                       grad_scale)
     logits = unit_columns(logits)
     if tp_world(tp_group) == 1 and on_gpu(logits):
-        return tuple(kernels().topk_distill(logits, *args, tail, denom, grad_scale))
+        got = kernels().topk_distill(logits, *args, tail, denom, grad_scale)
+        if not got:
+            raise ValueError(f"{name}: logits {tuple(logits.shape)} are larger than the kernels take")
+        return got[0], got[1]
     return _TopkDistillFn.apply(logits, *args, tail, float(denom), float(grad_scale), vocab_start, tp_group)
+
+
+def _own(logits, ids, logq, weights, temperature, tail, denom, grad_scale):
+    try:
+        if isinstance(temperature, Tensor):
+            return kernels().topk_distill(logits, ids, logq, weights, temperature, 1.0, tail, denom, grad_scale)
+        return kernels().topk_distill(logits, ids, logq, weights, None, temperature, tail, denom, grad_scale)
+    except TypeError:                             # not even the right kinds of arguments: the checks say which
+        return None
 
 
 def fused_lm_head_topk_distill(h: Tensor, weight: Tensor, teacher_ids: Tensor, teacher_logp: Tensor, *, denom: float,

@@ -245,6 +245,10 @@ def token_logprobs(logits: Tensor, tokens: Tensor | None = None, temperature: Te
     tokens.  With ``tp_group``, ``logits`` is this rank's equal shard of the vocabulary, whose first token
     is ``vocab_start``; every rank gets the whole result and its shard's gradient.
     """
+    if tp_group is None and on_gpu(logits):
+        got = _own(logits, tokens, temperature, top_k, with_entropy)
+        if got:                                   # arguments that the kernels take as they are
+            return TokenLogprobs(*got)
     name = "token_logprobs"
     check_logits(name, logits)
     rows, device = logits.shape[0], logits.device
@@ -257,11 +261,23 @@ def token_logprobs(logits: Tensor, tokens: Tensor | None = None, temperature: Te
     temp, temp1 = split_temperature(name, temperature, rows, device)
     logits = unit_columns(logits)
     if world == 1 and on_gpu(logits):
-        return TokenLogprobs(*kernels().token_logprobs(logits, tokens, temp, temp1, top_k, with_entropy))
+        got = kernels().token_logprobs(logits, tokens, temp, temp1, top_k, with_entropy)
+        if not got:
+            raise ValueError(f"{name}: logits {tuple(logits.shape)} are larger than the kernels take")
+        return TokenLogprobs(*got)
     flat = tokens is not None and tokens.ndim == 1
     logp, ent, ids, top = _TokenLogprobFn.apply(logits, tokens[:, None] if flat else tokens, temp, temp1, top_k,
                                                 with_entropy, vocab_start, tp_group)
     return TokenLogprobs(logp[:, 0] if flat else logp, ent, ids, top)
+
+
+def _own(logits, tokens, temperature, top_k, with_entropy):
+    try:
+        if isinstance(temperature, Tensor):
+            return kernels().token_logprobs(logits, tokens, temperature, 1.0, top_k, with_entropy)
+        return kernels().token_logprobs(logits, tokens, None, temperature, top_k, with_entropy)
+    except TypeError:                             # not even the right kinds of arguments: the checks say which
+        return None
 
 
 @torch.no_grad()
