@@ -199,7 +199,7 @@ struct Row {
 struct Slice {
   int lo, hi;
   __device__ __forceinline__ Slice(int units, int blocks, int rank) {
-    const int per = (units + blocks - 1) / blocks;
+    const int per = (units + blocks - 1) >> (31 - __clz(blocks));      // (blocks is a power of two)
     lo = min(units, rank * per);
     hi = min(units, lo + per);
   }
@@ -357,14 +357,15 @@ struct Feed {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     ring = (uint32_t)__cvta_generic_to_shared(smem) + (warp * kGroups * kGroupBytes + lane * 16);
     first = sl.lo + warp * kSpan;
-    step = warps * kSpan;
+    step = warps * kSpan;                       // (a power of two)
+    const int shift = 31 - __clz(step);
     p = reinterpret_cast<const uint4*>(row.p) + first + lane;
     lo = max(sl.lo, row.shift ? 1 : 0);
     hi = min(sl.hi, row.end / Unit<T>::kE);
-    batches = first < sl.hi ? (sl.hi - first + step - 1) / step : 0;
+    batches = first < sl.hi ? (sl.hi - first + step - 1) >> shift : 0;
     total = live ? batches * kPasses : 0;
     inner_lo = first < lo ? 1 : 0;
-    inner_n = max(0, (hi - first >= kSpan ? (hi - first - kSpan) / step + 1 : 0) - inner_lo);
+    inner_n = max(0, (hi - first >= kSpan ? ((hi - first - kSpan) >> shift) + 1 : 0) - inner_lo);
     put = get = 0;
     if (!live) inner_n = 0;
 #pragma unroll
@@ -1483,7 +1484,7 @@ Shape held_shape(int rows, int units) {
   return {kMaxCluster, kThreads, 0};
 }
 
-// Rows that stream: a warp per batch of units up to 8, `least` blocks per row, and more of long rows while that makes
+// Rows that stream: warps for the batches of units, up to 8 and a power of two, `least` blocks per row, and more of long rows while that makes
 // no more than `most` blocks.  1, 2, 4, 8 blocks per row, us, vocabulary 151936 BF16: scores of 8 rows 11.8, 8.9, 7.2,
 // 6.1, of 48 rows 12.1, 9.1, 9.4, 9.5, of 300 rows 24.5, 24.0, 26.7, 37.3; their gradient (whose blocks need not wait for
 // one another) of 48 rows 12.4, 8.2, 8.0, 6.8, of 148 rows 13.1, 12.4, 15.3, 15.9.
@@ -1491,7 +1492,9 @@ Shape stream_shape(int rows, int units, int least, int most) {
   int b = least;
   while (b < kMaxCluster && 2l * rows * b <= most && units >= std::max(2048, 2 * b * 512)) b *= 2;
   const int batches = ((units + b - 1) / b + kSpan - 1) / kSpan;
-  return {b, std::min(kStream, 32 * batches), 0};
+  int warps = 1;
+  while (warps < std::min(batches, kStream / 32)) warps *= 2;
+  return {b, 32 * warps, 0};
 }
 
 size_t feed_bytes(int threads) { return Feed<float, 1>::bytes(threads); }

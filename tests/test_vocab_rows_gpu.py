@@ -612,3 +612,19 @@ def test_refusals():
         ops.topk_distill_loss(x, ids.repeat(1, 65), logq.repeat(1, 65), denom=1.0)
     with pytest.raises(ValueError):
         ops.fused_lm_head_topk_distill(x, torch.randn(7, 49, device=DEV), ids, logq, denom=1.0)
+
+
+def test_vocabulary_beyond_the_kernels_is_refused():
+    ops = _ops()
+    x = torch.zeros(1, (1 << 22) + 1, device=DEV, dtype=torch.float16)
+    with pytest.raises(ValueError, match="larger"):
+        ops.token_logprobs(x)
+    with pytest.raises(ValueError, match="larger"):
+        ops.topk_distill_loss(x, torch.zeros(1, 1, dtype=torch.long, device=DEV), torch.zeros(1, 1, device=DEV),
+                              denom=1.0)
+    y = x[:, :1 << 22]
+    y[0, 4000000] = 3.0
+    r = ops.token_logprobs(y, None, top_k=2)
+    assert r.top_ids.tolist() == [[4000000, 0]]
+    _, rows = ops.topk_distill_loss(y, r.top_ids, r.top_logp, denom=1.0)
+    assert abs(float(rows[0])) < 1e-5
