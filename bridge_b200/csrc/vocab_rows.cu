@@ -288,8 +288,8 @@ __device__ __forceinline__ double warp_max_d(double v) {
 // A block's slice on its way through shared memory.  A warp takes batches of 4 x 32 consecutive units, warp w the
 // batches w, w + warps, ...; every lane owns kGroups x 4 slots of 16 bytes that it alone fills (asynchronous copies)
 // and reads, so a warp waits for nothing but its own copies, which run kGroups batches ahead, from before the first
-// batch is needed.  With two passes the batches come once more in reverse order (what was read last is the likeliest
-// to be in L2 still), and their copies start before the first pass ends.  (A lane's slots are read before the copies
+// batch is needed.  With two passes the batches come once more in reverse order: the last are in their slots still, and
+// what was read late is the likeliest to be in L2.  (A lane's slots are read before the copies
 // that refill them are issued, and those write a memory latency later.)
 //
 // 3 groups of 8 KB for 8 warps are 48 KB a block, 4 blocks an SM.  Scoring 4096 x 151936 BF16: 194 us against 267 us for
@@ -347,7 +347,7 @@ struct Feed {
   const uint4* p;        // this lane's unit of the warp's first batch
   int first, step;       // the warp's first unit (in the row), units between its batches
   int lo, hi;            // units of the row that can be copied: full ones, inside the slice
-  int batches, total;    // of this warp: per pass and in all
+  int batches, ready;    // of this warp, and of them those to copy (none of a row that is not read)
   int inner_lo, inner_n; // batches all of whose units can be copied: the first, and how many
   uint32_t put, get;     // offsets of the slots to fill and to read
 
@@ -363,7 +363,7 @@ struct Feed {
     lo = max(sl.lo, row.shift ? 1 : 0);
     hi = min(sl.hi, row.end / Unit<T>::kE);
     batches = first < sl.hi ? (sl.hi - first + step - 1) >> shift : 0;
-    total = live ? batches * kPasses : 0;
+    ready = live ? batches : 0;
     inner_lo = first < lo ? 1 : 0;
     inner_n = max(0, (hi - first >= kSpan ? ((hi - first - kSpan) >> shift) + 1 : 0) - inner_lo);
     put = get = 0;
@@ -404,10 +404,9 @@ struct Feed {
     turn(put);
     commit();
   }
-  // Copies of the q-th batch in order of use: what there is of it.
-  __device__ __forceinline__ void issue(int q) {
-    if (q < total) {
-      const int k = q < batches ? q : 2 * batches - 1 - q;
+  // Copies of batch k: what there is of it.
+  __device__ __forceinline__ void issue(int k) {
+    if (k >= 0 && k < ready) {
       copy_edge(ring + put, p + k * step, first + k * step + (int)(threadIdx.x & 31), lo, hi);
       turn(put);
     }
@@ -428,13 +427,21 @@ struct Feed {
     if constexpr (sizeof(T) == 4) asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(__float_as_uint(v)) : "memory");
     else asm volatile("st.shared.b16 [%0], %1;" ::"r"(at), "h"(reinterpret_cast<const unsigned short&>(v)) : "memory");
   }
-  // Takes it and starts the copies of the one kGroups on.
   __device__ __forceinline__ void take(Unit<T>* u) {
     read<0>(ring + get, u[0].w);
     read<1>(ring + get, u[1].w);
     read<2>(ring + get, u[2].w);
     read<3>(ring + get, u[3].w);
     turn(get);
+  }
+  // Second pass, from the last batch to the first: batch k's slots are those of k + kGroups, and the last batches are
+  // still in theirs.  The copies that follow go where this batch was.
+  __device__ __forceinline__ void take_back(int k, const Row<const T>& row, Slice sl, Unit<T>* u) {
+    put = get = get == 0 ? (kGroups - 1) * kGroupBytes : get - kGroupBytes;
+    const uint32_t here = get;
+    wait(k, row, sl);
+    take(u);
+    get = here;
   }
 };
 
@@ -1243,8 +1250,7 @@ __global__ void __launch_bounds__(kThreads, kUnits == 10 ? 1 : 2) distill_kernel
 }
 
 // The same for many long rows: the row streams through shared memory, once for the statistics and, for the gradient,
-// once more (from L2, mostly).  The copies of the first batches are on their way while the entries are prepared, and
-// those of the second pass while the row is finished.
+// once more (from L2, mostly).  The copies of the first batches are on their way while the entries are prepared.
 template <typename T, bool kGrad>
 __global__ void __launch_bounds__(kStream, 4) distill_stream_kernel(const T* logits, T* grad, DistillArgs a) {
   __shared__ Shared sh;
@@ -1298,13 +1304,12 @@ __global__ void __launch_bounds__(kStream, 4) distill_stream_kernel(const T* log
       uint4* to = reinterpret_cast<uint4*>(out.p) + feed.first + (feed.batches - 1) * feed.step + lane;
       const uint4* from = feed.p + (feed.batches - 1 - kGroups) * feed.step;
       for (int k = feed.batches - 1; k >= 0; --k, to -= feed.step, from -= feed.step) {
-        feed.wait(k, row, sl);
         Unit<T> u[kBatch];
-        feed.take(u);
+        feed.take_back(k, row, sl, u);
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) gradient_unit(u[b], c, R, factor);
         if (feed.inner(k - kGroups)) feed.issue_inner(from, policy);
-        else feed.issue(2 * feed.batches - 1 - (k - kGroups));
+        else feed.issue(k - kGroups);
         if (vec && feed.inner(k)) {
           store_streaming<0>(to, u[0].w, policy);
           store_streaming<1>(to, u[1].w, policy);
