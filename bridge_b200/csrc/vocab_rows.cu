@@ -532,9 +532,11 @@ __device__ __forceinline__ unsigned long long pack_key(uint32_t key, int token) 
   return ((unsigned long long)key << 32) | (0xffffffffu - (uint32_t)token);
 }
 
-// The value of a bound: -inf where it is below every key.
+constexpr uint32_t kLowestKey = 0x007fffffu;      // of -inf
+
+// The least value that is offered: the bound's, but -inf itself never (a row with fewer than k others is filled up).
 __device__ __forceinline__ float bound_value(uint32_t bound) {
-  return bound <= 0x007fffffu ? -INFINITY : key_value(bound);
+  return bound <= kLowestKey ? -3.402823466e38f : key_value(bound);
 }
 
 // Gives the elements of unit i that reach the bound to the leading block.
@@ -544,7 +546,7 @@ __device__ __forceinline__ void offer(const Unit<T>& u, int i, float bound, cons
   const bool full = row.full(i);
 #pragma unroll
   for (int j = 0; j < kE; ++j) {
-    const float v = fmaxf(to_f(u.get(j)), -INFINITY);      // (NaN counts as -inf)
+    const float v = to_f(u.get(j));      // (NaN counts as -inf)
     if (v >= bound && (full || row.holds(kE * i + j))) {
       const int at = atomicAdd(&lead->count, 1);
       if (at < kCand) lead->cand[at] = pack_key(order_key(v), kE * i + j - row.shift);
@@ -568,28 +570,31 @@ __device__ int count_ge(const Row<const T>& row, uint32_t key, int* scratch) {
   return __reduce_add_sync(0xffffffffu, n);
 }
 
-// One block, the whole row: sel.cand[0 .. k) holds the winners afterwards.
+// The least key of the row that is at least `bound`.
 template <typename T>
-__device__ void select_exactly(const Row<const T>& row, int k, Select& sel) {
-  constexpr int kE = Unit<T>::kE;
-  uint32_t kth = 0;
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t trial = kth | (1u << bit);
-    if (count_ge(row, trial, sel.scan) >= k) kth = trial;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) sel.count = 0;
-  __syncthreads();
+__device__ uint32_t least_ge(const Row<const T>& row, uint32_t bound, int* scratch) {
+  uint32_t least = 0xffffffffu;
   for (int i = threadIdx.x; i < row.units; i += blockDim.x) {
     const Unit<T> u = row.load(i);
 #pragma unroll
-    for (int j = 0; j < kE; ++j) {
+    for (int j = 0; j < Unit<T>::kE; ++j) {
       const uint32_t key = order_key(to_f(u.get(j)));
-      if (key > kth && row.holds(kE * i + j)) sel.cand[atomicAdd(&sel.count, 1)] = pack_key(key, kE * i + j - row.shift);
+      if (row.holds(Unit<T>::kE * i + j) && key >= bound) least = min(least, key);
     }
   }
+  least = __reduce_min_sync(0xffffffffu, least);
   __syncthreads();
-  int n = sel.count;      // fewer than k; now the k-th's equals, in index order
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = (int)least;
+  __syncthreads();
+  least = (threadIdx.x & 31) < (blockDim.x >> 5) ? (uint32_t)scratch[threadIdx.x & 31] : 0xffffffffu;
+  return __reduce_min_sync(0xffffffffu, least);
+}
+
+// One block: sel.cand[0 .. k) from the n < k candidates that are there and the first elements of key `kth`, in index
+// order.
+template <typename T>
+__device__ void fill_equals(const Row<const T>& row, uint32_t kth, int n, int k, Select& sel) {
+  constexpr int kE = Unit<T>::kE;
   for (int i0 = 0; i0 < row.units && n < k; i0 += blockDim.x) {
     const int i = i0 + threadIdx.x;
     uint32_t hit = 0;
@@ -624,6 +629,35 @@ __device__ void select_exactly(const Row<const T>& row, int k, Select& sel) {
     n = min(k, n + total);
   }
   __syncthreads();
+}
+
+// One block, the whole row, at least k of whose keys reach `bound`: sel.cand[0 .. k) holds the winners afterwards.
+// Mostly the least of those keys is the k-th largest itself, in a crowd of equals (a row of equal logits, or one whose
+// mask leaves fewer than k): two passes then; else bisection over the key's bits.
+template <typename T>
+__device__ void select_exactly(const Row<const T>& row, int k, uint32_t bound, Select& sel) {
+  constexpr int kE = Unit<T>::kE;
+  uint32_t kth = least_ge(row, bound, sel.scan);
+  if (count_ge(row, kth + 1, sel.scan) >= k) {
+    kth = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t trial = kth | (1u << bit);
+      if (count_ge(row, trial, sel.scan) >= k) kth = trial;
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) sel.count = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < row.units; i += blockDim.x) {
+    const Unit<T> u = row.load(i);
+#pragma unroll
+    for (int j = 0; j < kE; ++j) {
+      const uint32_t key = order_key(to_f(u.get(j)));
+      if (key > kth && row.holds(kE * i + j)) sel.cand[atomicAdd(&sel.count, 1)] = pack_key(key, kE * i + j - row.shift);
+    }
+  }
+  __syncthreads();
+  fill_equals(row, kth, sel.count, k, sel);
 }
 
 // ------------------------------------------------------------------------------------- token log-probs
@@ -672,10 +706,13 @@ __device__ __forceinline__ void write_row(const TokenArgs& a, int r, const T* x,
 // The alternatives from the gathered candidates; by the leading block.
 template <typename T>
 __device__ __forceinline__ void write_top(const TokenArgs& a, int r, const Row<const T>& row, float c, Stat st,
-                                          double log2s, Select& sel) {
+                                          double log2s, uint32_t bound, Select& sel) {
   int n = sel.count;
   if (n > kCand) {
-    select_exactly(row, a.k, sel);
+    select_exactly(row, a.k, bound, sel);
+    n = a.k;
+  } else if (n < a.k) {      // the others of the row are -inf
+    fill_equals(row, kLowestKey, n, a.k, sel);
     n = a.k;
   }
   // ranks by counting, `share` neighbouring lanes to a candidate
@@ -761,7 +798,8 @@ __global__ void __launch_bounds__(kThreads, kUnits == 10 ? 1 : 3) token_top_kern
 #pragma unroll
     for (int n = 0; n < kUnits; ++n) {
       const int i = sl.lo + threadIdx.x + n * blockDim.x;
-      if (i < sl.hi && (floor == -INFINITY || u[n].max() >= floor)) offer(u[n], i, floor, row, lead);
+      if (i < sl.hi && u[n].max() >= floor && *const_cast<volatile int*>(&lead->count) <= kCand)
+        offer(u[n], i, floor, row, lead);
     }
   }
   if (blocks > 1) cl.sync();      // the leader has every candidate, and nobody's sums are read any more
@@ -769,7 +807,7 @@ __global__ void __launch_bounds__(kThreads, kUnits == 10 ? 1 : 3) token_top_kern
   if (rank) return;
   const double log2s = log2_d((double)st.s);
   write_row<T, kEntropy>(a, r, x, c, st, log2s);
-  write_top(a, r, row, c, st, log2s, *sel);
+  write_top(a, r, row, c, st, log2s, bound, *sel);
 }
 
 // Rows that stream through shared memory once.  With alternatives a warp notes the maximum of every 32 units it takes;
@@ -833,7 +871,7 @@ __global__ void __launch_bounds__(kStream, 4) token_stream_kernel(const T* __res
     // taking apart inside the strips' loop 32 lanes wait for one: 85 us, not 79, for 1024 x 151936 BF16 and k = 64.)
     for (int s0 = 32 * (threadIdx.x >> 5); s0 < count; s0 += blockDim.x) {
       unsigned hits = __ballot_sync(0xffffffffu, s0 + lane < count && strips[min(s0 + lane, count - 1)] >= floor);
-      while (hits) {
+      while (hits && *const_cast<volatile int*>(&hit_units) <= kCand) {      // (beyond, the count alone decides)
         constexpr int kAtOnce = 4;
         Unit<T> u[kAtOnce];
         int at[kAtOnce];
@@ -845,7 +883,7 @@ __global__ void __launch_bounds__(kStream, 4) token_stream_kernel(const T* __res
         }
 #pragma unroll
         for (int n = 0; n < kAtOnce; ++n) {
-          if (at[n] >= sl.hi || !(floor == -INFINITY || u[n].max() >= floor)) continue;
+          if (at[n] >= sl.hi || !(u[n].max() >= floor)) continue;
           const int to = atomicAdd(&hit_units, 1);
           if (to < kCand) list[to] = at[n];
         }
@@ -863,7 +901,7 @@ __global__ void __launch_bounds__(kStream, 4) token_stream_kernel(const T* __res
   if (rank) return;
   const double log2s = log2_d((double)st.s);
   write_row<T, kEntropy>(a, r, x, c, st, log2s);
-  if constexpr (kTop) write_top(a, r, row, c, st, log2s, *sel);
+  if constexpr (kTop) write_top(a, r, row, c, st, log2s, bound, *sel);
 }
 
 // u = 2^t (A + B t), t = u c - R
