@@ -419,10 +419,9 @@ struct Feed {
     if (!inner(k))
       read_edge<T>(ring + get, row.p, row.shift, row.end, first + k * step + (int)(threadIdx.x & 31), lo, hi, sl.hi);
   }
-  // -inf at position `pos` of that batch; by the lane whose slot it is
-  __device__ __forceinline__ void rule_out(int pos) const {
-    constexpr int kE = Unit<T>::kE;
-    const uint32_t at = ring + get + 512 * (pos / (32 * kE)) + (pos % kE) * (int)sizeof(T);
+  // -inf at an offset of that batch from this lane's first slot
+  __device__ __forceinline__ void rule_out(int offset) const {
+    const uint32_t at = ring + get + offset;
     const T v = from_f<T>(-INFINITY);
     if constexpr (sizeof(T) == 4) asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(__float_as_uint(v)) : "memory");
     else asm volatile("st.shared.b16 [%0], %1;" ::"r"(at), "h"(reinterpret_cast<const unsigned short&>(v)) : "memory");
@@ -1066,11 +1065,12 @@ struct Entries {
   float* logq;           // of every entry; -inf where dropped
   int* col;              // the shard's column if it lies in this block's slice, else -1
   int* next;             // chain, -1 at its end
+  int* spot;             // where in its chain's units
   int* heads;            // chains
   unsigned char* later;  // repeats the column of an earlier entry
 
   static __host__ __device__ size_t bytes(int K, int chains) {
-    return (K + 31) / 32 * sizeof(Teacher) + (size_t)K * 28 + (size_t)chains * 4 + K + 15;
+    return (K + 31) / 32 * sizeof(Teacher) + (size_t)K * 32 + (size_t)chains * 4 + K + 15;
   }
   __device__ __forceinline__ Entries(unsigned char* p, int K, int chains) {
     part = reinterpret_cast<Teacher*>(p);
@@ -1079,16 +1079,18 @@ struct Entries {
     logq = reinterpret_cast<float*>(q + K);
     col = reinterpret_cast<int*>(logq + K);
     next = col + K;
-    heads = next + K;
+    spot = next + K;
+    heads = spot + K;
     later = reinterpret_cast<unsigned char*>(heads + chains);
   }
 };
 
 // Reads the row's entries into `en`, chains them from en.heads[place(unit)] and sums them 32 by 32; returns whether the
 // row has any that counts.  The chains are complete when it returns, the sums after the next barrier.
-template <typename T, typename Place>
+template <typename T, typename Place, typename Spot>
 __device__ __forceinline__ bool load_entries(const Entries& en, const DistillArgs& a, int r, const T* x,
-                                             const Row<const T>& row, Slice sl, float c, int chains, Place place) {
+                                             const Row<const T>& row, Slice sl, float c, int chains, Place place,
+                                             Spot spot) {
   const int lane = threadIdx.x & 31, padded = (a.K + 31) / 32 * 32;
   for (int i = threadIdx.x; i < chains; i += blockDim.x) en.heads[i] = -1;
   __syncthreads();
@@ -1107,6 +1109,7 @@ __device__ __forceinline__ bool load_entries(const Entries& en, const DistillArg
       const double xc = (double)to_f(x[t]) * (double)c;
       en.xc[j] = xc <= (double)kMasked ? -INFINITY : xc;
       en.col[j] = (int)t;
+      en.spot[j] = spot(unit, ((int)t + row.shift) % Unit<T>::kE);
       en.next[j] = atomicExch(&en.heads[place(unit)], j);
     }
   }
@@ -1256,14 +1259,13 @@ __global__ void __launch_bounds__(kThreads, kUnits == 10 ? 1 : 2) distill_kernel
   }
   const float c = row_c(a, r);
   const auto place = [&](int unit) { return (unit - sl.lo) % (int)blockDim.x; };
-  const bool some = load_entries(en, a, r, x, row, sl, c, blockDim.x, place);
+  const auto spot = [&](int unit, int j) { return (unit - sl.lo) / (int)blockDim.x * Unit<T>::kE + j; };
+  const bool some = load_entries(en, a, r, x, row, sl, c, blockDim.x, place, spot);
   for (int e = en.heads[threadIdx.x]; e >= 0; e = en.next[e]) {
-    const int pos = en.col[e] + row.shift - Unit<T>::kE * (sl.lo + (int)threadIdx.x);
+    const int at = en.spot[e];
 #pragma unroll
-    for (int n = 0; n < kUnits; ++n) {
-      const int j = pos - Unit<T>::kE * n * (int)blockDim.x;
-      if (j >= 0 && j < Unit<T>::kE) u[n].mask(1u << j);
-    }
+    for (int n = 0; n < kUnits; ++n)
+      if (at / Unit<T>::kE == n) u[n].mask(1u << at % Unit<T>::kE);
   }
   Sums sums;
   sums.R = fmaxf(units_max<T, kUnits>(u) * c, kMasked);
@@ -1307,21 +1309,24 @@ __global__ void __launch_bounds__(kStream, 4) distill_stream_kernel(const T* log
   const Entries en(dyn + Rows::bytes(blockDim.x), a.K, chains);
   const float c = row_c(a, r);
   const auto place = [&](int unit) { return (unit - sl.lo) / kSpan; };
-  const bool some = load_entries(en, a, r, x, row, sl, c, chains, place);
+  // the lane, and the offset from its first slot of the batch
+  const auto spot = [&](int unit, int j) {
+    const int n = (unit - sl.lo) % kSpan;
+    return n % 32 << 16 | (n / 32 * 512 + j * (int)sizeof(T));
+  };
+  const bool some = load_entries(en, a, r, x, row, sl, c, chains, place, spot);
   Sums sums;
   if (live) {
     const int* head = en.heads + (feed.first - sl.lo) / kSpan;
-    int base = Unit<T>::kE * feed.first - row.shift;
     const unsigned long long policy = evict_normal();
     const uint4* from = feed.p + kGroups * feed.step;
     for (int k = 0; k < feed.batches; ++k, from += feed.step) {
       feed.wait(k, row, sl);
       for (int e = *head; e >= 0; e = en.next[e]) {
-        const int pos = en.col[e] - base;
-        if (pos / Unit<T>::kE % 32 == lane) feed.rule_out(pos);
+        const int at = en.spot[e];
+        if (at >> 16 == lane) feed.rule_out(at & 0xffff);
       }
       head += blockDim.x >> 5;
-      base += Unit<T>::kE * feed.step;
       Unit<T> u[kBatch];
       feed.take(u);
       const float top = units_max<T, kBatch>(u) * c;
