@@ -17,10 +17,10 @@
 // What bounds them: reading the row.  8 BF16 logits cost 16 bytes, 8 exponentials (half a cycle of an SM) and about
 // 40 instructions a pass, which at 6.4 TB/s is two thirds of what the SMs can issue, so the loops are kept lean (paired
 // FP32 instructions, no checks inside a row) and everything that is per row overlaps other blocks' streaming.  B200,
-// vocabulary 151936, BF16, device time: scoring 4096 rows with entropy 0.20 ms (6.2 TB/s; 0.23 ms, 5.4 TB/s, under a
+// vocabulary 151936, BF16, device time: scoring 4096 rows with entropy 0.20 ms (6.2 TB/s; 0.22 ms, 5.7 TB/s, under a
 // sustained power cap), 1024 rows with 64 alternatives 0.079 ms; gradient of the scores 0.21 ms for 2048 rows (6.0 TB/s);
 // distillation loss 0.061 ms for 1024 rows, loss and gradient 0.48 ms for 4096 (5.2 TB/s of one read and one write);
-// one row with 20 alternatives 9 us, 8 rows of distillation with gradient 9 us.
+// one row with 20 alternatives 9 us, 8 rows of distillation with gradient 12 us.
 #include "vocab_rows.h"
 
 #include <c10/util/Exception.h>
@@ -339,7 +339,7 @@ __device__ __noinline__ void read_edge(uint32_t to, const T* p, int shift, int e
   }
 }
 
-// (Only two passes give L2 hints; with one, scoring is 3% faster without.)
+// (Only two passes give L2 hints: what is read once needs none.)
 template <typename T, int kPasses>
 struct Feed {
   static constexpr int kGroupBytes = kSpan * 16;
@@ -809,10 +809,73 @@ __global__ void __launch_bounds__(kThreads, kUnits == 10 ? 1 : 3) token_top_kern
   write_top(a, r, row, c, st, log2s, bound, *sel);
 }
 
-// Rows that stream through shared memory once.  With alternatives a warp notes the maximum of every 32 units it takes;
-// after the bound is known only those that reach it are read again.
-template <typename T, bool kEntropy, bool kTop>
-__global__ void __launch_bounds__(kStream, 4) token_stream_kernel(const T* __restrict__ logits, TokenArgs a) {
+// 16 bytes that are read once.  (Volatile: the compiler keeps the loads of a batch together, ahead of the arithmetic.)
+__device__ __forceinline__ uint4 read_once(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+// Scores without alternatives: a row is read once and nothing of it is needed again, so its batches come straight into
+// registers, the next while one is worked on.  Against the same pass over copies in shared memory: 203 us, not 209, for
+// 4096 x 151936 BF16; 215, not 227, where the power cap holds the clock down.  (Two batches take 73-80 registers.)
+template <typename T, bool kEntropy>
+__global__ void __launch_bounds__(kStream, 3) token_stream_kernel(const T* __restrict__ logits, TokenArgs a) {
+  __shared__ Stat part[32];
+  __shared__ RowPart mine;
+  cg::cluster_group cl = cg::this_cluster();
+  const int blocks = (int)cl.num_blocks(), rank = (int)cl.block_rank(), lane = threadIdx.x & 31;
+  const int r = blockIdx.x / blocks;
+  const T* x = logits + (size_t)r * a.stride;
+  const Row<const T> row(x, a.V);
+  const Slice sl(row.units, blocks, rank);
+  const int step = (int)(blockDim.x >> 5) * kSpan;
+  // [lo, hi): the units that are whole and in the slice
+  const int lo = max(sl.lo, row.shift ? 1 : 0), hi = min(sl.hi, row.end / Unit<T>::kE);
+  const float c = row_c(a, r);
+  Sums sums;
+  const auto fetch = [&](int first, Unit<T>* u) {      // beyond the slice: nothing but masked logits
+    if (first >= lo && first + kSpan <= hi) {
+      const uint4* p = reinterpret_cast<const uint4*>(row.p) + first + lane;
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) u[b].w = read_once(p + 32 * b);
+    } else {
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const int i = first + lane + 32 * b;
+        if (i < sl.hi) u[b] = row.load(i);
+        else u[b].fill(from_f<T>(-INFINITY));
+      }
+    }
+  };
+  const auto use = [&](const Unit<T>* u) {
+    const float top = units_max<T, kBatch>(u) * c;
+    if (top > sums.R + kSlack) sums.raise(top);
+    add_units<kEntropy, T, kBatch>(sums, u, c);
+  };
+  Unit<T> u[kBatch], v[kBatch];
+  int i = sl.lo + (int)(threadIdx.x >> 5) * kSpan;
+  fetch(i, u);
+  for (; i < sl.hi; i += 2 * step) {
+    fetch(i + step, v);
+    use(u);
+    fetch(i + 2 * step, u);
+    use(v);
+  }
+  Stat st = block_join(sums.get(), part);
+  uint32_t bound = 0;
+  join_row(mine, st, bound, nullptr, cl);
+  if (blocks > 1) cl.sync();      // nobody's sums are read any more
+  if (rank) return;
+  write_row<T, kEntropy>(a, r, x, c, st, log2_d((double)st.s));
+}
+
+// Alternatives of long rows, which stream through shared memory once.  A warp notes the maximum of every 32 units it
+// takes; after the bound is known only those that reach it are read again.
+template <typename T, bool kEntropy>
+__global__ void __launch_bounds__(kStream, 4) token_top_stream_kernel(const T* __restrict__ logits, TokenArgs a) {
   __shared__ Stat part[32];
   __shared__ RowPart mine;
   __shared__ int hit_units;
@@ -837,19 +900,14 @@ __global__ void __launch_bounds__(kStream, 4) token_stream_kernel(const T* __res
     feed.wait(k, row, sl);
     Unit<T> u[kBatch];
     feed.take(u);
-    float top;
-    if constexpr (kTop) {
-      float m[kBatch];
+    float m[kBatch];
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b) m[b] = u[b].max();
-      top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-      best = fmaxf(best, top);
+    for (int b = 0; b < kBatch; ++b) m[b] = u[b].max();
+    float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+    best = fmaxf(best, top);
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b) m[b] = warp_top(m[b]);
-      if (lane < kBatch) *strip = lane == 0 ? m[0] : (lane == 1 ? m[1] : (lane == 2 ? m[2] : m[3]));
-    } else {
-      top = units_max<T, kBatch>(u);
-    }
+    for (int b = 0; b < kBatch; ++b) m[b] = warp_top(m[b]);
+    if (lane < kBatch) *strip = lane == 0 ? m[0] : (lane == 1 ? m[1] : (lane == 2 ? m[2] : m[3]));
     if (feed.inner(k + kGroups)) feed.issue_inner(from);
     else feed.issue(k + kGroups);
     top *= c;
@@ -857,50 +915,48 @@ __global__ void __launch_bounds__(kStream, 4) token_stream_kernel(const T* __res
     add_units<kEntropy, T, kBatch>(sums, u, c);
   }
   Stat st = block_join(sums.get(), part);
-  uint32_t bound = 0;
-  Select* sel = kTop ? reinterpret_cast<Select*>(dyn) : nullptr;      // the ring's place: its copies are done
+  Select* sel = reinterpret_cast<Select*>(dyn);      // the ring's place: its copies are done
   const int held = sl.hi - sl.lo;
-  if (kTop) bound = kth_max(order_key(best), (int)(threadIdx.x >> 5) * kSpan + lane < held, (a.k + blocks - 1) / blocks);
+  uint32_t bound =
+      kth_max(order_key(best), (int)(threadIdx.x >> 5) * kSpan + lane < held, (a.k + blocks - 1) / blocks);
   join_row(mine, st, bound, sel, cl);
-  if (kTop) {
-    Select* lead = cl.map_shared_rank(sel, 0);
-    const int count = (held + 31) / 32;
-    const float floor = bound_value(bound);
-    // Units that reach the bound: first found, a warp to a strip, then taken apart, a thread to a unit.  (With the
-    // taking apart inside the strips' loop 32 lanes wait for one: 85 us, not 79, for 1024 x 151936 BF16 and k = 64.)
-    for (int s0 = 32 * (threadIdx.x >> 5); s0 < count; s0 += blockDim.x) {
-      unsigned hits = __ballot_sync(0xffffffffu, s0 + lane < count && strips[min(s0 + lane, count - 1)] >= floor);
-      while (hits && *const_cast<volatile int*>(&hit_units) <= kCand) {      // (beyond, the count alone decides)
-        constexpr int kAtOnce = 4;
-        Unit<T> u[kAtOnce];
-        int at[kAtOnce];
+  Select* lead = cl.map_shared_rank(sel, 0);
+  const int count = (held + 31) / 32;
+  const float floor = bound_value(bound);
+  // Units that reach the bound: first found, a warp to a strip, then taken apart, a thread to a unit.  (With the
+  // taking apart inside the strips' loop 32 lanes wait for one: 85 us, not 79, for 1024 x 151936 BF16 and k = 64.)
+  for (int s0 = 32 * (threadIdx.x >> 5); s0 < count; s0 += blockDim.x) {
+    unsigned hits = __ballot_sync(0xffffffffu, s0 + lane < count && strips[min(s0 + lane, count - 1)] >= floor);
+    while (hits && *const_cast<volatile int*>(&hit_units) <= kCand) {      // (beyond, the count alone decides)
+      constexpr int kAtOnce = 4;
+      Unit<T> u[kAtOnce];
+      int at[kAtOnce];
 #pragma unroll
-        for (int n = 0; n < kAtOnce; ++n) {
-          at[n] = hits ? sl.lo + 32 * (s0 + __ffs(hits) - 1) + lane : sl.hi;
-          hits &= hits - 1;
-          if (at[n] < sl.hi) u[n] = row.load(at[n]);
-        }
+      for (int n = 0; n < kAtOnce; ++n) {
+        at[n] = hits ? sl.lo + 32 * (s0 + __ffs(hits) - 1) + lane : sl.hi;
+        hits &= hits - 1;
+        if (at[n] < sl.hi) u[n] = row.load(at[n]);
+      }
 #pragma unroll
-        for (int n = 0; n < kAtOnce; ++n) {
-          if (at[n] >= sl.hi || !(u[n].max() >= floor)) continue;
-          const int to = atomicAdd(&hit_units, 1);
-          if (to < kCand) list[to] = at[n];
-        }
+      for (int n = 0; n < kAtOnce; ++n) {
+        if (at[n] >= sl.hi || !(u[n].max() >= floor)) continue;
+        const int to = atomicAdd(&hit_units, 1);
+        if (to < kCand) list[to] = at[n];
       }
     }
-    __syncthreads();
-    if (hit_units > kCand) {
-      if (threadIdx.x == 0) atomicAdd(&lead->count, kCand + 1);      // far too many: the exact way
-    } else {
-      for (int h = threadIdx.x; h < hit_units; h += blockDim.x) offer(row.load(list[h]), list[h], floor, row, lead);
-    }
+  }
+  __syncthreads();
+  if (hit_units > kCand) {
+    if (threadIdx.x == 0) atomicAdd(&lead->count, kCand + 1);      // far too many: the exact way
+  } else {
+    for (int h = threadIdx.x; h < hit_units; h += blockDim.x) offer(row.load(list[h]), list[h], floor, row, lead);
   }
   if (blocks > 1) cl.sync();      // the leader has every candidate, and nobody's sums are read any more
-  else if (kTop) __syncthreads();
+  else __syncthreads();
   if (rank) return;
   const double log2s = log2_d((double)st.s);
   write_row<T, kEntropy>(a, r, x, c, st, log2s);
-  if constexpr (kTop) write_top(a, r, row, c, st, log2s, bound, *sel);
+  write_top(a, r, row, c, st, log2s, bound, *sel);
 }
 
 // u = 2^t (A + B t), t = u c - R
@@ -1235,10 +1291,10 @@ __device__ __forceinline__ void gradient_unit(Unit<T>& u, float c, float R, floa
 }
 
 // A cluster per row, the row in registers, kUnits units per thread: the statistics of the columns outside the teacher's
-// entries, the joining, the gradient.  Short rows, and few rows, where one pass's latency is what counts: of 9 us for 8
-// rows most goes to the launch, the entries (ids, then the logits there) and the two joins, not to the 2.4 MB.
+// entries, the joining, the gradient.  Short rows, and few rows, where one pass's latency is what counts: of 8.8 us for 4
+// FP32 rows of 24000 most goes to the launch, the entries (ids, then the logits there) and two joins, not to 0.8 MB.
 template <typename T, int kUnits>
-__global__ void __launch_bounds__(kThreads, kUnits == 10 ? 1 : 2) distill_kernel(const T* logits, T* grad, DistillArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) distill_kernel(const T* logits, T* grad, DistillArgs a) {
   __shared__ Shared sh;
   extern __shared__ __align__(16) unsigned char dyn[];
   const Entries en(dyn, a.K, blockDim.x);
@@ -1532,13 +1588,15 @@ Shape held_shape(int rows, int units) {
   return {kMaxCluster, kThreads, 0};
 }
 
-// Rows that stream: warps for the batches of units, up to 8 and a power of two, `least` blocks per row, and more of long rows while that makes
-// no more than `most` blocks.  1, 2, 4, 8 blocks per row, us, vocabulary 151936 BF16: scores of 8 rows 11.8, 8.9, 7.2,
-// 6.1, of 48 rows 12.1, 9.1, 9.4, 9.5, of 300 rows 24.5, 24.0, 26.7, 37.3; their gradient (whose blocks need not wait for
-// one another) of 48 rows 12.4, 8.2, 8.0, 6.8, of 148 rows 13.1, 12.4, 15.3, 15.9.
-Shape stream_shape(int rows, int units, int least, int most) {
+// Rows that stream: warps for the batches of units, up to 8 and a power of two, `least` blocks per row, and more of long
+// rows while they have at least `part` units and three of them are resident on every SM at once.  Up to 4/3, 2, 3, 4 for
+// every SM, us, vocabulary 151936 BF16: scores of 64 rows 8.5, 7.8, 7.8, 12.2, of 74 rows 8.4, 9.5, 9.5, 12.8, of 100 rows
+// 12.4, 10.7, 9.6, 9.8, of 200 rows 16.9, 16.8, 14.1, 14.1; their gradient of 100 rows 13.4, 12.0, 10.3, 10.4, of 148 rows
+// 13.5, 12.4, 12.3, 15.2; distillation with gradient of 100 rows 26.1, 24.0, 20.6, 20.5, of 148 rows 26.2, 24.6, 24.7, 31.8.
+// At least 512 / 1024 units, 8 rows of 50257 columns: 64 entries with gradient 10.7 / 11.8, the scores' gradient 4.3 / 5.1.
+Shape stream_shape(int rows, int units, int least = 1, int part = 512) {
   int b = least;
-  while (b < kMaxCluster && 2l * rows * b <= most && units >= std::max(2048, 2 * b * 512)) b *= 2;
+  while (b < kMaxCluster && 2l * rows * b <= 3 * sm_count() && units >= std::max(2048, 2 * b * part)) b *= 2;
   const int batches = ((units + b - 1) / b + kSpan - 1) / kSpan;
   int warps = 1;
   while (warps < std::min(batches, kStream / 32)) warps *= 2;
@@ -1547,14 +1605,21 @@ Shape stream_shape(int rows, int units, int least, int most) {
 
 size_t feed_bytes(int threads) { return Feed<float, 1>::bytes(threads); }
 
-// Whether rows are held rather than streamed: short ones always, longer ones while their blocks are resident at once
-// (up to about `per_sm` for every SM).  Held / streamed, us, vocabulary 151936 BF16: 20 alternatives of 8 rows 9.7 / 14,
-// of 48 rows 15.2 / 17.7, of 148 rows 40 / 28; distillation with gradient of 8 rows 9.3 / 11.5, of 32 rows 11.6 / 13.4,
-// of 74 rows 29.6 / 25.2.  4000 rows of 12000 columns (1500 units): 63 / 103 with 20 alternatives, 88 / 99 distillation;
-// of 20000 columns (2500 units): 91 / 105 and 133 / 117.
-bool hold(int rows, int units, int shortest, float per_sm) {
-  const Shape s = held_shape(rows, units);
-  return s.units && (units <= shortest || (float)rows * s.blocks <= per_sm * sm_count());
+// Whether rows are held rather than streamed: short ones always (4000 rows held / streamed, us, BF16: of 12000 columns,
+// 1500 units, 63 / 103 with 20 alternatives, 88 / 99 distillation; of 20000, 2500 units, 91 / 105 and 133 / 117), longer
+// ones while their blocks are resident at once.
+// Alternatives take little else than the row.  Vocabulary 151936 BF16, 20 of 8 rows 10.3 / 11.7, of 32 rows 13.1 / 13.8, of
+// 48 rows 15.3 / 15.9.  With 10 units per thread an SM has room for one block, and clusters of 8 do not fill all SMs:
+// 151936 FP32, of 8 rows 9.2 / 11.0, of 16 rows 16.1 / 12.2.
+bool hold_for_top(int rows, int units, Shape s) {
+  return s.units && (units <= 2560 || 4l * rows * s.blocks <= (s.units == 10 ? 2 : 11) * sm_count());
+}
+// Distillation has the entries to prepare as well, which a block that streams does while its copies are on their way.
+// 64 entries of 16 rows with gradient, BF16: of 24000 columns 9.3 / 11.1, 50257 10.6 / 11.4, 100000 13.1 / 12.4, 151936
+// 15.1 / 13.1; of 64 rows of 24000 (1500 units in each of 2 blocks) 12.6 / 11.7; 148 of 17000 (one block) 12.3 / 14.0.
+bool hold_for_distill(int rows, int units, Shape s) {
+  if (units <= 2048) return true;
+  return 4l * rows * s.blocks <= 7 * sm_count() && (s.blocks == 1 || units <= 1024 * s.blocks);
 }
 
 template <typename K, typename... A>
@@ -1584,8 +1649,8 @@ cudaError_t launch_token_logprob(RowType t, const void* logits, const TokenArgs&
     using Kernel = void (*)(const T*, TokenArgs);
     const bool e = a.entropy != nullptr;
     const int units = units_of(a.V, sizeof(T));
-    Shape s{0, 0, 0};
-    if (a.k && hold(a.U, units, 2560, 2.75f)) s = held_shape(a.U, units);
+    Shape s = held_shape(a.U, units);
+    if (!a.k || !hold_for_top(a.U, units, s)) s.units = 0;
     Kernel kern;
     switch (s.units) {
       case 1: kern = e ? token_top_kernel<T, true, 1> : token_top_kernel<T, false, 1>; break;
@@ -1593,14 +1658,17 @@ cudaError_t launch_token_logprob(RowType t, const void* logits, const TokenArgs&
       case 5: kern = e ? token_top_kernel<T, true, 5> : token_top_kernel<T, false, 5>; break;
       case 10: kern = e ? token_top_kernel<T, true, 10> : token_top_kernel<T, false, 10>; break;
       default: {
-        s = stream_shape(a.U, units, 1, sm_count() * 4 / 3);
-        size_t smem = feed_bytes(s.threads);
-        if (a.k) {
-          kern = e ? token_stream_kernel<T, true, true> : token_stream_kernel<T, false, true>;
-          smem = std::max(smem, sizeof(Select) + 4 * kCand) + sizeof(float) * (kBatch + units / 32 / s.blocks + 2 + kStream / 32 * kBatch);
-        } else {
-          kern = e ? token_stream_kernel<T, true, false> : token_stream_kernel<T, false, false>;
+        if (!a.k) {
+          // Two batches for a warp, which are on their way at once.  Blocks of at least 512 / 1024 / 2048 units, us, BF16:
+          // 32 rows of 32000 columns 4.6 / 4.1 / 4.2, 8 of 100000 4.4 / 4.4 / 5.3.
+          s = stream_shape(a.U, units, 1, 1024);
+          kern = e ? token_stream_kernel<T, true> : token_stream_kernel<T, false>;
+          return launch_rows(kern, a.U, s, 0, stream, (const T*)logits, a);
         }
+        s = stream_shape(a.U, units);
+        size_t smem = feed_bytes(s.threads);
+        kern = e ? token_top_stream_kernel<T, true> : token_top_stream_kernel<T, false>;
+        smem = std::max(smem, sizeof(Select) + 4 * kCand) + sizeof(float) * (kBatch + units / 32 / s.blocks + 2 + kStream / 32 * kBatch);
         const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (err != cudaSuccess) return err;
         return launch_rows(kern, a.U, s, smem, stream, (const T*)logits, a);
@@ -1615,7 +1683,7 @@ cudaError_t launch_token_logprob_bwd(RowType t, const void* logits, void* grad, 
   return by_type(t, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     auto* kern = a.d_entropy ? token_logprob_bwd_kernel<T, true> : token_logprob_bwd_kernel<T, false>;
-    const Shape s = stream_shape(a.U, units_of(a.V, sizeof(T)), 1, sm_count() * 2);
+    const Shape s = stream_shape(a.U, units_of(a.V, sizeof(T)));
     const size_t smem = feed_bytes(s.threads);
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
@@ -1627,8 +1695,8 @@ cudaError_t launch_distill(RowType t, const void* logits, void* grad, const Dist
   return by_type(t, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     const int units = units_of(a.V, sizeof(T));
-    Shape s{0, 0, 0};
-    if (hold(a.U, units, 2048, 1.75f)) s = held_shape(a.U, units);
+    Shape s = held_shape(a.U, units);
+    if (!hold_for_distill(a.U, units, s)) s.units = 0;
     using Kernel = void (*)(const T*, T*, DistillArgs);
     Kernel kern;
     size_t smem = Entries::bytes(a.K, s.threads);
@@ -1636,13 +1704,12 @@ cudaError_t launch_distill(RowType t, const void* logits, void* grad, const Dist
       case 1: kern = distill_kernel<T, 1>; break;
       case 2: kern = distill_kernel<T, 2>; break;
       case 5: kern = distill_kernel<T, 5>; break;
-      case 10: kern = distill_kernel<T, 10>; break;
       default: {
         kern = grad ? distill_stream_kernel<T, true> : distill_stream_kernel<T, false>;
         // With a second pass the rows in work (4 blocks for every SM) should fit L2: 4096 x 151936 BF16 (180 MB with one
         // block per row) 529 us with one, 484 us with two; 1024 x 32003 FP32 (76 MB) 76 us with one, 93 us with two.
         const bool twice = grad && a.U >= 2 * sm_count() && 4l * sm_count() * units * 16 > (100l << 20);
-        s = stream_shape(a.U, units, twice ? 2 : 1, sm_count() * 4 / 3);
+        s = stream_shape(a.U, units, twice ? 2 : 1);
         smem = feed_bytes(s.threads) + Entries::bytes(a.K, units / s.blocks / kSpan + 2);
         const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
