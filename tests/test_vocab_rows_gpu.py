@@ -122,6 +122,38 @@ def test_token_logprobs_strides(dtype, view):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("units", [1, 31, 128, 129, 1023, 1024, 1025, 2047, 2048, 4100, 8191, 16384, 16400])
+def test_scores_alone_at_batch_edges(dtype, units):
+    """Lengths around a warp's, a block's and a cluster's batches; rows at every offset from 16 bytes, with masked ends."""
+    per = 16 // torch.empty(0, dtype=dtype).element_size()
+    for rows, short, offset in ((3, 0, 0), (9, 1, 1), (40, per - 1, per - 1)):
+        vocab = max(1, units * per - short)
+        x = _logits(rows, vocab + per + 1, dtype, seed=units)[:, offset:offset + vocab]
+        x[0, vocab // 2:] = -math.inf
+        x[1, : vocab // 2] = torch.finfo(dtype).min
+        tokens = torch.randint(0, vocab, (rows,), device=DEV)
+        tokens[0] = 0 if vocab > 1 else -1
+        tokens[1] = vocab - 1
+        tokens[2] = vocab - 1
+        r = _ops().token_logprobs(x, tokens, 1.3)
+        _check_logp(r, x, tokens[:, None], 1.3)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [2, 12, 70, 101])
+def test_long_rows_held_or_streamed(dtype, rows):
+    """Few long rows: alternatives and distillation in registers or streamed, as row count and type decide."""
+    vocab = 100003
+    x = _logits(rows, vocab, dtype, seed=rows)
+    tokens = torch.randint(0, vocab, (rows,), device=DEV)
+    r = _ops().token_logprobs(x, tokens, 1.1, top_k=17)
+    _check_logp(r, x, tokens[:, None], 1.1)
+    _check_top(r, x, 1.1, 17)
+    ids, logq = _teacher(rows, vocab, 17)
+    _check_distill(x, ids, logq, tail=True, denom=float(rows))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_masked_rows(dtype):
     """Masks of -inf and of the type's lowest value, a row with one live logit, rows with none."""
     vocab = 777
