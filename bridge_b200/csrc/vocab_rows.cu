@@ -245,8 +245,9 @@ struct Sums {
   __device__ __forceinline__ Stat get() const { return {R, s.x + s.y, et.x + et.y}; }
 };
 
+// (Volatile: it may not sink into a branch that only the lanes that use it take.)
 __device__ __forceinline__ float warp_top(float v) {
-  asm("redux.sync.max.f32 %0, %0, 0xffffffff;" : "+f"(v));
+  asm volatile("redux.sync.max.f32 %0, %0, 0xffffffff;" : "+f"(v));
   return v;
 }
 
