@@ -23,3 +23,13 @@ def test_warp_collectives_in_assembly_are_volatile():
                 seen += 1
                 assert m.group(1), f"{name}: {' '.join(m.group(2).split())[:60]}"
     assert seen > 10
+
+
+def test_slots_are_read_before_they_are_refilled():
+    """Nothing but a barrier orders a lane's read of shared memory before the asynchronous copy into the same slot that
+    it issues afterwards: reading a batch ends with one."""
+    text = dict(_sources())["vocab_rows.cu"]
+    body = re.search(r"void take\(Unit<T>\* u\) \{(.*?)\n  \}", text, re.S).group(1)
+    assert body.rindex("__syncwarp()") > body.rindex("read<3>(")
+    # and every read of a slot goes through it
+    assert len(re.findall(r"\bread<\d>\(ring", text)) == len(re.findall(r"\bread<\d>\(ring", body)) == 4
