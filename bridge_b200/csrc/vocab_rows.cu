@@ -7,8 +7,11 @@
 // joined by rescaling.  Statistics are FP32; the few numbers of a row that everything else is scaled by (log s, the
 // given tokens' shares) are FP64.
 //
-// A logit with x c <= -1e30 (-inf, or a mask of the type's lowest value) carries no probability; a row without any
-// other has log-probs -inf, entropy 0 and gradient 0.
+// A logit with x c <= -2^31 (-inf, the type's lowest value, any customary finite mask from -1e10 down) carries no
+// probability; a row without any other has log-probs -inf, entropy 0 and gradient 0.  The bound is where FP32 ends: R is
+// rounded, so t at the largest logit can be off 0 by half a unit of R's last place, 64 for |R| < 2^31 (2^64 V is still a
+// number) and hundreds above, where a thread that sees nothing but a mask of -1e10 would sum to infinity.  A row with
+// x c > 2^31 is NaN, as with an infinite logit.
 //
 // A row belongs to one cluster of 1 to 8 blocks, each with a contiguous slice; the blocks exchange partial sums
 // through distributed shared memory, so no workspace and no atomics on global memory are needed and results do not
@@ -44,7 +47,8 @@ constexpr int kThreads = 512;   // at most, per block that holds its slice
 constexpr int kStream = 256;    // per block that streams it
 constexpr int kMaxCluster = 8;
 constexpr int kCand = 2048;     // candidates of the selection kept in shared memory
-constexpr float kMasked = -1e30f;
+constexpr float kMasked = -2147483648.f;      // -2^31, of x c
+constexpr float kOverflow = -1e29f;           // x c below this may be -inf
 constexpr float kSlack = 8.f;
 constexpr double kLn2 = 0.69314718055994530942;
 constexpr double kLog2e = 1.4426950408889634074;
@@ -217,6 +221,9 @@ struct Stat {
     R = to;
   }
 };
+
+// The reference for a largest x c of `top`.
+__device__ __forceinline__ float reference(float top) { return top > -kMasked ? NAN : fmaxf(top, kMasked); }
 
 // A thread's running sums, two FP32 lanes to an instruction.
 struct Sums {
@@ -478,7 +485,7 @@ __device__ __forceinline__ float units_max(const Unit<T>* u) {
 // Whether some t of these units may be infinite.
 template <typename T, int N>
 __device__ __forceinline__ bool masked(const Unit<T>* u, float c) {
-  return units_extreme<-1, T, N>(u) * c < 0.1f * kMasked;
+  return units_extreme<-1, T, N>(u) * c < kOverflow;
 }
 template <bool kEntropy, typename T, int N>
 __device__ __forceinline__ void add_units(Sums& sums, const Unit<T>* u, float c) {
@@ -786,7 +793,7 @@ __global__ void __launch_bounds__(kThreads, kUnits == 10 ? 1 : 3) token_top_kern
   const float c = row_c(a, r);
   const float best = units_max<T, kUnits>(u);
   Sums sums;
-  sums.R = fmaxf(best * c, kMasked);
+  sums.R = reference(best * c);
   add_units<kEntropy, T, kUnits>(sums, u, c);
   Stat st = block_join(sums.get(), part);
   const bool any = sl.lo + (int)threadIdx.x < sl.hi;
@@ -854,7 +861,7 @@ __global__ void __launch_bounds__(kStream, 3) token_stream_kernel(const T* __res
   };
   const auto use = [&](const Unit<T>* u) {
     const float top = units_max<T, kBatch>(u) * c;
-    if (top > sums.R + kSlack) sums.raise(top);
+    if (top > sums.R + kSlack) sums.raise(reference(top));
     add_units<kEntropy, T, kBatch>(sums, u, c);
   };
   Unit<T> u[kBatch], v[kBatch];
@@ -913,7 +920,7 @@ __global__ void __launch_bounds__(kStream, 4) token_top_stream_kernel(const T* _
     if (feed.inner(k + kGroups)) feed.issue_inner(from);
     else feed.issue(k + kGroups);
     top *= c;
-    if (top > sums.R + kSlack) sums.raise(top);
+    if (top > sums.R + kSlack) sums.raise(reference(top));
     add_units<kEntropy, T, kBatch>(sums, u, c);
   }
   Stat st = block_join(sums.get(), part);
@@ -1326,7 +1333,7 @@ __global__ void __launch_bounds__(kThreads, 2) distill_kernel(const T* logits, T
       if (at / Unit<T>::kE == n) u[n].mask(1u << at % Unit<T>::kE);
   }
   Sums sums;
-  sums.R = fmaxf(units_max<T, kUnits>(u) * c, kMasked);
+  sums.R = reference(units_max<T, kUnits>(u) * c);
   add_units<false, T, kUnits>(sums, u, c);
   finish_block<T>(sh, en, sums.get(), a, r, w, some, cl);
   if (grad) {
@@ -1390,7 +1397,7 @@ __global__ void __launch_bounds__(kStream, 4) distill_stream_kernel(const T* log
       const float top = units_max<T, kBatch>(u) * c;
       if (feed.inner(k + kGroups)) feed.issue_inner(from, policy);
       else feed.issue(k + kGroups);
-      if (top > sums.R + kSlack) sums.raise(top);
+      if (top > sums.R + kSlack) sums.raise(reference(top));
       add_units<false, T, kBatch>(sums, u, c);
     }
   }

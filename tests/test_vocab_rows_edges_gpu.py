@@ -1,0 +1,73 @@
+"""Operators over rows of logits where they can go wrong: fills of a mask, loss factors, head-level gradients, rows whose
+entries cover all that lives, shards of the vocabulary.  Tolerances are those derived in test_vocab_rows_gpu.py, or stated
+at the test."""
+
+import math
+
+import pytest
+import torch
+
+from tests import vocab_oracle as oracle
+from tests.test_vocab_rows_gpu import (DEV, ROUND, TINY, TYPES, _check_distill, _check_grad, _check_logp, _check_top,
+                                       _close, _logits, _ops, _teacher)
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------------------ masks
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("fill", [-1e9, -1e10, -3e12, -1e20, -1e29])
+@pytest.mark.parametrize("vocab", [777, 100003])
+def test_finite_masks(dtype, fill, vocab):
+    """Masks that are neither infinite nor the type's lowest value, in rows where whole threads see nothing else."""
+    x = _logits(5, vocab, dtype, seed=vocab)
+    x[0, 100:] = fill
+    x[1, : vocab - 30] = fill
+    x[2] = fill
+    x[2, vocab // 2] = 1.5
+    x[3, ::2] = fill
+    ids, logq = _teacher(5, vocab, 6)
+    live = torch.tensor([[3, 70], [vocab - 1, vocab - 9], [vocab // 2, vocab // 2], [1, 11], [0, 5]], device=DEV)
+    ids[:, :2] = live
+    ids[2, 1] = -1
+    ids[:4, 2:] = -1                               # (a given token that the student rules out is another test's)
+    logq = torch.where(ids >= 0, logq - 1.0, logq)
+    for temp in (1.0, 0.7):
+        xg = x.detach().requires_grad_()
+        r = _ops().token_logprobs(xg, live, temp, top_k=4)
+        _check_logp(r, x, live, temp)
+        _check_top(_ops().token_logprobs(x[3:], None, temp, top_k=9), x[3:], temp, 9)
+        d, dh = torch.randn(5, 2, device=DEV), torch.randn(5, device=DEV)
+        (got,) = torch.autograd.grad((r.logp, r.entropy), xg, (d, dh))
+        size = ((d.abs().sum(1) + 32 * dh.abs()) / temp)[:, None].double()
+        _check_grad(got, oracle.token_grad(x, live, temp, d, dh), size, dtype)
+        _check_distill(x, ids, logq, tail=False, temp=temp)
+        _check_distill(x[[0, 1, 3, 4]], ids[[0, 1, 3, 4]], logq[[0, 1, 3, 4]], tail=True, temp=temp)
+
+
+@pytest.mark.parametrize("fill", [-1e10, -1e15, -1e25])
+def test_rows_of_finite_masks_carry_nothing(fill):
+    for vocab in (300, 70001):
+        x = torch.full((2, vocab), fill, device=DEV).requires_grad_()
+        r = _ops().token_logprobs(x, torch.tensor([1, 2], device=DEV), top_k=3)
+        assert bool((r.logp == -math.inf).all()) and r.entropy.tolist() == [0.0, 0.0]
+        assert r.top_ids.tolist() == [[0, 1, 2]] * 2 and bool((r.top_logp == -math.inf).all())
+        (g,) = torch.autograd.grad((r.logp, r.entropy), x, (torch.ones(2, device=DEV), torch.ones(2, device=DEV)))
+        assert not bool(g.any())
+        _, rows = _ops().topk_distill_loss(x.detach(), torch.zeros(2, 1, dtype=torch.long, device=DEV),
+                                           torch.full((2, 1), -0.5, device=DEV), denom=1.0)
+        assert rows.tolist() == [math.inf] * 2
+
+
+def test_logits_beyond_the_range_are_nan():
+    """x / T above 2^31 ln 2 has no FP32 reference near enough: NaN, as for infinite logits, in that row alone."""
+    for vocab in (300, 70001):
+        x = _logits(3, vocab, torch.float32)
+        x[1, 40] = 3e10
+        xg = x.clone().requires_grad_()
+        tokens = torch.tensor([1, 40, 3], device=DEV)
+        r = _ops().token_logprobs(xg, tokens, top_k=4)
+        assert torch.isnan(r.logp).tolist() == [False, True, False] == torch.isnan(r.entropy).tolist()
+        assert torch.equal(r.top_ids, oracle.top(x, 4))
+        (g,) = torch.autograd.grad(r.logp.sum(), xg)
+        assert bool(torch.isnan(g[1]).all()) and bool(torch.isfinite(g[::2]).all())
