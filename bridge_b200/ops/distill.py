@@ -168,8 +168,10 @@ class _FusedHeadDistillFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, h, weight, ids, logq, weights, temp, temp1, tail, denom, grad_scale, vocab_start, group,
-                chunk_rows):
-        want = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
+                chunk_rows, differentiable):
+        # (what needs a gradient is said of the inputs under no_grad too)
+        want_dh, want_dw = (differentiable and n for n in ctx.needs_input_grad[:2])
+        want = want_dh or want_dw
         main = getattr(weight, "main_grad", None)
         dh = torch.empty_like(h) if want else None
         dw = None
@@ -187,7 +189,7 @@ class _FusedHeadDistillFn(torch.autograd.Function):
             if not want:
                 continue
             dh[at] = gemm(dlg, weight, b_mn=True)                      # dlogits @ W
-            if not ctx.needs_input_grad[1]:
+            if not want_dw:
                 continue
             if main is not None:                                       # W.main_grad += dlogits^T h
                 gemm(dlg, h[at], a_mn=True, b_mn=True, out=main, accumulate=True)
@@ -205,7 +207,7 @@ class _FusedHeadDistillFn(torch.autograd.Function):
     def backward(ctx, dloss, _drows):
         dh, dw = ctx.saved_tensors
         f = dloss.float() / ctx.grad_scale
-        return ((dh.float() * f).to(dh.dtype), (dw * f).to(dh.dtype) if ctx.has_dw else None) + (None,) * 11
+        return ((dh.float() * f).to(dh.dtype), (dw * f).to(dh.dtype) if ctx.has_dw else None) + (None,) * 12
 
 
 # ------------------------------------------------------------------------------------------------- API
@@ -282,6 +284,6 @@ def fused_lm_head_topk_distill(h: Tensor, weight: Tensor, teacher_ids: Tensor, t
     args = _arguments(name, h.shape[0], h.device, teacher_ids, teacher_logp, weights, temperature, denom, grad_scale)
     if on_gpu(h):
         return _FusedHeadDistillFn.apply(h.contiguous(), weight, *args, bool(tail), float(denom), float(grad_scale),
-                                         int(vocab_start), tp_group, int(chunk_rows))
+                                         int(vocab_start), tp_group, int(chunk_rows), torch.is_grad_enabled())
     return _TopkDistillFn.apply(torch.matmul(h, weight.t()), *args, bool(tail), float(denom), float(grad_scale),
                                 int(vocab_start), tp_group)

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from bridge_b200.ops import token_logprobs
+from bridge_b200.ops import fused_lm_head_topk_distill, token_logprobs
 from tests import vocab_oracle as oracle
 from tests.test_vocab_rows_cpu import _case
 
@@ -20,3 +20,44 @@ def test_rows_of_finite_masks_carry_nothing():
     x = torch.zeros(2, 30)
     x[1, 4] = 3e10
     assert torch.isnan(token_logprobs(x, torch.tensor([1, 4])).logp).tolist() == [False, True]
+
+
+# ------------------------------------------------------------------------------------------------ heads
+def _stand_in(monkeypatch):
+    """The head-level autograd nodes on the CPU: the kernels' calls in the PyTorch form."""
+    from bridge_b200.ops import distill
+
+    class Kernels:
+        @staticmethod
+        def distill_rows_inplace(lg, ids, logq, weights, temp, temp1, scale, tail, want):
+            stats, xc = distill._open_reference(lg, ids, temp, temp1, 0)
+            rows, coef, fix = distill._finish_reference(stats, xc, ids, logq, weights, temp, temp1, scale, tail,
+                                                        lg.shape[1])
+            if want:
+                lg.copy_(distill._grad_reference(lg, ids, coef, fix, temp, temp1, 0, lg.shape[1]))
+            return rows.float()
+
+        @staticmethod
+        def weighted_rows_sum(rows, weights, denom):
+            return (rows if weights is None else rows * weights).sum() / denom
+
+    monkeypatch.setattr(distill, "on_gpu", lambda *t: True)
+    monkeypatch.setattr(distill, "kernels", lambda: Kernels)
+
+
+def _head(U=40, H=16, V=60, K=5, dtype=torch.float32):
+    g = torch.Generator().manual_seed(3)
+    h = torch.randn(U, H, generator=g).to(dtype).requires_grad_()
+    W = torch.randn(V, H, generator=g).to(dtype).requires_grad_()
+    top = torch.topk(torch.log_softmax(2 * torch.randn(U, V, generator=g), 1), K, dim=1)
+    return h, W, top.indices, top.values
+
+
+def test_head_loss_without_gradient_leaves_main_grad_alone(monkeypatch):
+    _stand_in(monkeypatch)
+    h, W, ids, logq = _head()
+    W.main_grad = torch.zeros(W.shape)
+    with torch.no_grad():
+        loss, rows = fused_lm_head_topk_distill(h, W, ids, logq, denom=40.0, chunk_rows=16)
+    assert not W.main_grad.any()
+    assert torch.allclose(rows.double(), oracle.distill((h @ W.t()).detach(), ids, logq, 1.0, True)[0], atol=1e-4)

@@ -71,3 +71,25 @@ def test_logits_beyond_the_range_are_nan():
         assert torch.equal(r.top_ids, oracle.top(x, 4))
         (g,) = torch.autograd.grad(r.logp.sum(), xg)
         assert bool(torch.isnan(g[1]).all()) and bool(torch.isfinite(g[::2]).all())
+
+
+# ------------------------------------------------------------------------------------------------ heads
+def _head(U=200, H=128, V=1000, K=8, dtype=torch.bfloat16, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    h = (torch.randn(U, H, device=DEV, generator=g) * 0.5).to(dtype)
+    W = (torch.randn(V, H, device=DEV, generator=g) * 0.2).to(dtype)
+    ids, logq = _teacher(U, V, K, seed)
+    w = 0.2 + torch.rand(U, device=DEV, generator=g)
+    return h, W, ids, logq, w
+
+
+def test_head_loss_without_gradient_leaves_main_grad_alone():
+    ops = _ops()
+    h, W, ids, logq, w = _head()
+    W.requires_grad_()
+    W.main_grad = torch.zeros(W.shape, device=DEV)
+    with torch.no_grad():
+        loss, rows = ops.fused_lm_head_topk_distill(h, W, ids, logq, denom=200.0, weights=w, chunk_rows=64)
+    assert not loss.requires_grad and not bool(W.main_grad.any())
+    want, _ = oracle.distill(h.float() @ W.detach().float().t(), ids, logq, 1.0, True)
+    _close(rows, want, 5e-2, 1e-2, "rows")
