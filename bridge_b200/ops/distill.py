@@ -13,8 +13,9 @@ With ``Q = sum_j q_j + q_r`` its gradient is ``dz_v = Q p_v - q_v`` on the given
 The gradient of every row is known as soon as its statistics are, so the forward writes it
 (``csrc/vocab_rows.cu``): the logits are read from memory once and the gradient is written once.  The
 backward only checks that the loss was scaled by ``grad_scale`` as announced, and rescales otherwise.
-:func:`fused_lm_head_topk_distill` goes on to the LM head's own backward inside the forward, like
-:func:`~bridge_b200.ops.logprob.fused_lm_head_ppo`.
+:func:`fused_lm_head_topk_distill` goes on to the LM head's own backward inside the forward and keeps
+``dh`` and, in FP32, ``dW`` for a factor that only the backward knows: a forward that is run again, or never
+followed by a backward, changes no gradient.
 
 Rows of weight 0 and rows without an entry have divergence 0 and gradient 0 whatever their logits hold.
 A given token (``q_j > 0``) without student probability makes the divergence infinite.
@@ -172,9 +173,8 @@ class _FusedHeadDistillFn(torch.autograd.Function):
         # (what needs a gradient is said of the inputs under no_grad too)
         want_dh, want_dw = (differentiable and n for n in ctx.needs_input_grad[:2])
         want = want_dh or want_dw
-        main = getattr(weight, "main_grad", None)
-        dh = torch.empty_like(h) if want else None
-        dw = None
+        dh = torch.empty_like(h) if want_dh else None
+        dw = torch.zeros(weight.shape, dtype=torch.float32, device=weight.device) if want_dw else None
         parts = []
         for a in range(0, h.shape[0], chunk_rows):
             at = slice(a, min(a + chunk_rows, h.shape[0]))
@@ -186,20 +186,14 @@ class _FusedHeadDistillFn(torch.autograd.Function):
             else:
                 rows, dlg = _rows_and_grad(lg, *teacher, want, vocab_start, group)
             parts.append(rows)
-            if not want:
-                continue
-            dh[at] = gemm(dlg, weight, b_mn=True)                      # dlogits @ W
-            if not want_dw:
-                continue
-            if main is not None:                                       # W.main_grad += dlogits^T h
-                gemm(dlg, h[at], a_mn=True, b_mn=True, out=main, accumulate=True)
-            else:
-                part = gemm(dlg, h[at], a_mn=True, b_mn=True).float()
-                dw = part if dw is None else dw.add_(part)
+            if want_dh:
+                dh[at] = gemm(dlg, weight, b_mn=True)                  # dlogits @ W
+            if want_dw:
+                gemm(dlg, h[at], a_mn=True, b_mn=True, out=dw, accumulate=True)      # += dlogits^T h
         rows = torch.cat(parts) if parts else torch.zeros(0, dtype=torch.float32, device=h.device)
-        if want:
-            ctx.save_for_backward(dh, dw if dw is not None else dh.new_empty(0))
-        ctx.grad_scale, ctx.has_dw = grad_scale, dw is not None
+        ctx.save_for_backward(dh, dw)
+        ctx.grad_scale, ctx.dtype = grad_scale, weight.dtype
+        ctx.main_grad = getattr(weight, "main_grad", None)
         ctx.mark_non_differentiable(rows)
         return _weighted_sum(rows, weights, denom), rows
 
@@ -207,7 +201,14 @@ class _FusedHeadDistillFn(torch.autograd.Function):
     def backward(ctx, dloss, _drows):
         dh, dw = ctx.saved_tensors
         f = dloss.float() / ctx.grad_scale
-        return ((dh.float() * f).to(dh.dtype), (dw * f).to(dh.dtype) if ctx.has_dw else None) + (None,) * 12
+        if dh is not None:
+            dh = (dh.float() * f).to(dh.dtype)
+        if dw is not None and ctx.main_grad is not None:
+            ctx.main_grad.addcmul_(dw.to(ctx.main_grad.dtype), f.to(ctx.main_grad.dtype))
+            dw = None
+        elif dw is not None:
+            dw = (dw * f).to(ctx.dtype)
+        return (dh, dw) + (None,) * 12
 
 
 # ------------------------------------------------------------------------------------------------- API
@@ -273,8 +274,8 @@ def fused_lm_head_topk_distill(h: Tensor, weight: Tensor, teacher_ids: Tensor, t
                                chunk_rows: int = 4096) -> tuple[Tensor, Tensor]:
     """:func:`topk_distill_loss` of hidden rows ``h [U, H]`` under the head ``weight [V_local, H]``.
 
-    The logits exist for ``chunk_rows`` rows at a time and become their own gradient in place; ``dW`` goes
-    into ``weight.main_grad`` where there is one, for a loss multiplied by ``grad_scale``.
+    The logits exist for ``chunk_rows`` rows at a time and become their own gradient in place.  ``dW`` is summed
+    in FP32 and kept for the backward, which adds it to ``weight.main_grad`` where there is one.
     """
     name = "fused_lm_head_topk_distill"
     if h.ndim != 2 or weight.ndim != 2 or h.shape[1] != weight.shape[1]:

@@ -61,3 +61,46 @@ def test_head_loss_without_gradient_leaves_main_grad_alone(monkeypatch):
         loss, rows = fused_lm_head_topk_distill(h, W, ids, logq, denom=40.0, chunk_rows=16)
     assert not W.main_grad.any()
     assert torch.allclose(rows.double(), oracle.distill((h @ W.t()).detach(), ids, logq, 1.0, True)[0], atol=1e-4)
+
+
+def _head_gradients(h, W, ids, logq, factor):
+    """In 64 bits, of ``factor`` times the loss."""
+    x = (h.detach().double() @ W.detach().double().t())
+    _, gx = oracle.distill(x, ids, logq, 1.0, True)
+    gx = gx * factor / h.shape[0]
+    return gx @ W.detach().double(), gx.t() @ h.detach().double()
+
+
+@pytest.mark.parametrize("main", [True, False])
+@pytest.mark.parametrize("announced,factor", [(1.0, 1.0), (1.0, 0.5), (4.0, 4.0), (4.0, 3.0)])
+def test_head_gradients_agree_for_any_loss_factor(monkeypatch, main, announced, factor):
+    _stand_in(monkeypatch)
+    h, W, ids, logq = _head()
+    if main:
+        W.main_grad = torch.full(W.shape, 2.0)
+    loss, _ = fused_lm_head_topk_distill(h, W, ids, logq, denom=40.0, chunk_rows=16, grad_scale=announced)
+    assert not main or bool((W.main_grad == 2.0).all())         # nothing happens to it before the backward
+    (loss * factor).backward(retain_graph=True)
+    dh, dw = _head_gradients(h, W, ids, logq, factor)
+    got = W.main_grad - 2.0 if main else W.grad
+    assert torch.allclose(h.grad.double(), dh, atol=1e-5, rtol=1e-4)
+    assert torch.allclose(got.double(), dw, atol=1e-5, rtol=1e-4)
+    loss.backward()                                              # and once more: gradients add up
+    both = _head_gradients(h, W, ids, logq, factor + 1.0)
+    got = W.main_grad - 2.0 if main else W.grad
+    assert torch.allclose(h.grad.double(), both[0], atol=1e-5, rtol=1e-4)
+    assert torch.allclose(got.double(), both[1], atol=1e-5, rtol=1e-4)
+
+
+@pytest.mark.parametrize("reentrant", [True, False])
+def test_recomputed_head_counts_once(monkeypatch, reentrant):
+    from torch.utils.checkpoint import checkpoint
+
+    _stand_in(monkeypatch)
+    h, W, ids, logq = _head()
+    W.main_grad = torch.zeros(W.shape)
+    loss = checkpoint(lambda v: fused_lm_head_topk_distill(v, W, ids, logq, denom=40.0, chunk_rows=16)[0], h,
+                      use_reentrant=reentrant)
+    loss.backward()
+    dh, dw = _head_gradients(h, W, ids, logq, 1.0)
+    assert torch.allclose(h.grad.double(), dh, atol=1e-5) and torch.allclose(W.main_grad.double(), dw, atol=1e-5)

@@ -93,3 +93,25 @@ def test_head_loss_without_gradient_leaves_main_grad_alone():
     assert not loss.requires_grad and not bool(W.main_grad.any())
     want, _ = oracle.distill(h.float() @ W.detach().float().t(), ids, logq, 1.0, True)
     _close(rows, want, 5e-2, 1e-2, "rows")
+
+
+@pytest.mark.parametrize("main", [True, False])
+@pytest.mark.parametrize("announced,factor", [(1.0, 0.5), (1.0, 1.0), (49.0, 7.0)])
+def test_head_gradients_agree_for_any_loss_factor(main, announced, factor):
+    """Tolerances of BF16 logits and their BF16 gradients, as at the other test of the head."""
+    h, W, ids, logq, w = _head()
+    h.requires_grad_()
+    W.requires_grad_()
+    if main:
+        W.main_grad = torch.full(W.shape, 2.0, device=DEV)
+    loss, _ = _ops().fused_lm_head_topk_distill(h, W, ids, logq, denom=200.0, weights=w, chunk_rows=64,
+                                                grad_scale=announced)
+    assert not main or bool((W.main_grad == 2.0).all())
+    (loss * factor).backward()
+    hd, Wd = h.detach().double(), W.detach().double()
+    _, gx = oracle.distill(hd @ Wd.t(), ids, logq, 1.0, True)
+    gx = gx * w.double()[:, None] * factor / 200.0
+    dh, dw = gx @ Wd, gx.t() @ hd
+    got = W.main_grad - 2.0 if main else W.grad
+    _close(h.grad, dh, 2e-2 * float(dh.abs().max()), 5e-2, "dh")
+    _close(got, dw, 2e-2 * float(dw.abs().max()), 5e-2, "dW")
