@@ -1252,11 +1252,12 @@ __device__ __forceinline__ void finish_block(Shared& sh, const Entries& en, Stat
     }
   }
   if (threadIdx.x == 0) {
-    sh.fin = finish_row(t, st, some, a.tail, (double)w * a.scale * inv_temp(a, r));
+    const double scale = a.num ? a.scale * ((double)a.num[0] / (double)a.den) : a.scale;
+    sh.fin = finish_row(t, st, some, a.tail, (double)w * scale * inv_temp(a, r));
     if (rank == 0 && a.open) {
       a.stats[2 * (size_t)r] = st.R;
       a.stats[2 * (size_t)r + 1] = st.s;
-    } else if (rank == 0) {
+    } else if (rank == 0 && a.rows) {
       a.rows[r] = w != 0.f ? sh.fin.kl : 0.f;
     }
   }
@@ -1299,11 +1300,15 @@ __device__ __forceinline__ void gradient_unit(Unit<T>& u, float c, float R, floa
   }
 }
 
+// Whether the gradient that is there needs no other factor (for every block of a launch alike).
+__device__ __forceinline__ bool as_announced(const DistillArgs& a) { return a.num && a.num[0] == a.den; }
+
 // A cluster per row, the row in registers, kUnits units per thread: the statistics of the columns outside the teacher's
 // entries, the joining, the gradient.  Short rows, and few rows, where one pass's latency is what counts: of 8.8 us for 4
 // FP32 rows of 24000 most goes to the launch, the entries (ids, then the logits there) and two joins, not to 0.8 MB.
 template <typename T, int kUnits>
 __global__ void __launch_bounds__(kThreads, 2) distill_kernel(const T* logits, T* grad, DistillArgs a) {
+  if (as_announced(a)) return;
   __shared__ Shared sh;
   extern __shared__ __align__(16) unsigned char dyn[];
   const Entries en(dyn, a.K, blockDim.x);
@@ -1358,6 +1363,7 @@ __global__ void __launch_bounds__(kThreads, 2) distill_kernel(const T* logits, T
 // once more (from L2, mostly).  The copies of the first batches are on their way while the entries are prepared.
 template <typename T, bool kGrad>
 __global__ void __launch_bounds__(kStream, 4) distill_stream_kernel(const T* logits, T* grad, DistillArgs a) {
+  if (as_announced(a)) return;
   __shared__ Shared sh;
   extern __shared__ __align__(16) unsigned char dyn[];
   cg::cluster_group cl = cg::this_cluster();

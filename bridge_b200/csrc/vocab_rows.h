@@ -34,12 +34,14 @@ struct DistillArgs {
   const float* weights;    // [U] or null
   const float* temp;       // [U] or null
   double inv_temp1;
-  double scale;            // grad_scale / denom
+  double scale;            // of the gradient: grad_scale / denom
+  const float* num;        // null, or the gradient is for `scale` num / den instead, and stays where that is 1
+  float den;
   int U, V, K;
   long stride;
   long vocab_start, vocab_total;
   bool tail, open;         // open: a shard of the vocabulary, the sums are joined elsewhere
-  float* rows;             // [U] divergence
+  float* rows;             // [U] divergence, or null
   float* stats;            // [U, 2] (R, s) of the columns outside the given ids
   float* xc;               // [U, K] x c of the given ids in this shard, else 0
   float* coef;             // [U, 2] (R, factor of 2^(x c - R)) of the columns outside the given ids

@@ -179,10 +179,10 @@ class ScoreRows : public torch::autograd::Function<ScoreRows> {
 
 // ------------------------------------------------------------------------------------------- distillation
 // Rows of a whole vocabulary: KL [U] and, unless `grad` is null, their gradient into it.
-void distill_into(const torch::Tensor& logits, bb::DistillArgs a, const torch::Tensor& rows, const torch::Tensor* grad) {
+void distill_into(const torch::Tensor& logits, bb::DistillArgs a, const torch::Tensor* rows, const torch::Tensor* grad) {
   if (a.U == 0) return;
   a.V = (int)logits.size(1), a.stride = logits.stride(0);
-  a.rows = rows.data_ptr<float>();
+  a.rows = rows ? rows->data_ptr<float>() : nullptr;
   check(bb::launch_distill(row_type(logits), logits.data_ptr(), grad ? grad->data_ptr() : nullptr, a,
                            at::cuda::getCurrentCUDAStream()));
 }
@@ -213,9 +213,16 @@ class DistillLoss : public torch::autograd::Function<DistillLoss> {
     auto grad = at::empty(logits.sizes(), plain);
     const auto a = distill_args(logits, ids, logq, weights, temp, temp1, grad_scale / denom, tail, 0,
                                 logits.size(1));
-    distill_into(logits, a, rows, &grad);
+    distill_into(logits, a, &rows, &grad);
     ctx->saved_data["grad"] = grad;
     ctx->saved_data["grad_scale"] = grad_scale;
+    if (logits.scalar_type() == at::kHalf) {      // what the gradient takes once more if the loss is scaled otherwise
+      const torch::Tensor none;
+      ctx->save_for_backward({logits, ids, logq, weights.value_or(none), temp.value_or(none)});
+      ctx->saved_data["temp1"] = temp1;
+      ctx->saved_data["tail"] = tail;
+      ctx->saved_data["denom"] = denom;
+    }
     ctx->mark_non_differentiable({rows});
     return {sum_rows(rows, weights, denom), rows};
   }
@@ -227,8 +234,21 @@ class DistillLoss : public torch::autograd::Function<DistillLoss> {
     auto grad = held->second.toTensor();      // handed on without a copy, so there is one backward
     ctx->saved_data.erase(held);
     const c10::cuda::CUDAGuard guard(grad.device());
-    scale_grad(grad, grads[0].to(at::kFloat), ctx->saved_data["grad_scale"].toDouble());
+    const auto dloss = grads[0].to(at::kFloat);
+    const double grad_scale = ctx->saved_data["grad_scale"].toDouble();
     const torch::Tensor none;
+    if (grad.scalar_type() == at::kHalf) {
+      // FP16 has no room for a scale after the rounding (what a loss scaler is there to save is 0 by then): the gradient
+      // is written again from the logits, unless the factor is the announced one
+      const auto saved = ctx->get_saved_variables();
+      auto a = distill_args(saved[0], saved[1], saved[2], optional(saved[3]), optional(saved[4]),
+                            ctx->saved_data["temp1"].toDouble(), grad_scale / ctx->saved_data["denom"].toDouble(),
+                            ctx->saved_data["tail"].toBool(), 0, saved[0].size(1));
+      a.num = dloss.data_ptr<float>(), a.den = (float)grad_scale;
+      distill_into(saved[0], a, nullptr, &grad);
+    } else {
+      scale_grad(grad, dloss, grad_scale);
+    }
     return {grad, none, none, none, none, none, none, none, none};
   }
 };
@@ -297,7 +317,7 @@ std::vector<torch::Tensor> topk_distill(torch::Tensor logits, torch::Tensor ids,
   const c10::cuda::CUDAGuard guard(logits.device());
   auto rows = at::empty({logits.size(0)}, logits.options().dtype(at::kFloat).requires_grad(false));
   const auto a = distill_args(logits, ids, logq, weights, temp, temp1, 1.0, tail, 0, logits.size(1));
-  distill_into(logits, a, rows, nullptr);
+  distill_into(logits, a, &rows, nullptr);
   return {sum_rows(rows, weights, denom), rows};
 }
 
@@ -309,7 +329,7 @@ torch::Tensor distill_rows_inplace(torch::Tensor logits, torch::Tensor ids, torc
   const c10::cuda::CUDAGuard guard(logits.device());
   auto rows = at::empty({logits.size(0)}, logits.options().dtype(at::kFloat));
   const auto a = distill_args(logits, ids, logq, weights, temp, temp1, scale, tail, 0, logits.size(1));
-  distill_into(logits, a, rows, want_grad ? &logits : nullptr);
+  distill_into(logits, a, &rows, want_grad ? &logits : nullptr);
   return rows;
 }
 

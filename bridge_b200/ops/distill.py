@@ -12,7 +12,9 @@ With ``Q = sum_j q_j + q_r`` its gradient is ``dz_v = Q p_v - q_v`` on the given
 
 The gradient of every row is known as soon as its statistics are, so the forward writes it
 (``csrc/vocab_rows.cu``): the logits are read from memory once and the gradient is written once.  The
-backward only checks that the loss was scaled by ``grad_scale`` as announced, and rescales otherwise.
+backward only checks that the loss was scaled by ``grad_scale`` as announced, and rescales otherwise (FP16
+gradients are written again from the logits, which they keep for that: scaling what was rounded at another
+scale would lose it).  Vocabularies in shards write theirs in the backward.
 :func:`fused_lm_head_topk_distill` goes on to the LM head's own backward inside the forward and keeps
 ``dh`` and, in FP32, ``dW`` for a factor that only the backward knows: a forward that is run again, or never
 followed by a backward, changes no gradient.
@@ -107,8 +109,8 @@ def _grad_reference(logits, ids, coef, fix, temp, temp1, vocab_start, total):
 
 
 # ------------------------------------------------------------------------------------------- one shard
-def _rows_and_grad(logits, ids, logq, weights, temp, temp1, scale, tail, want_grad, inplace, vocab_start, group):
-    """``(KL [U], gradient or None)`` of this rank's shard, in steps (and the PyTorch form)."""
+def _rows(logits, ids, logq, weights, temp, temp1, scale, tail, vocab_start, group):
+    """``(KL [U], coef, fix)`` of this rank's shard, in steps (and the PyTorch form)."""
     own, world = on_gpu(logits), tp_world(group)
     total = logits.shape[1] * world
     if own:
@@ -121,13 +123,19 @@ def _rows_and_grad(logits, ids, logq, weights, temp, temp1, scale, tail, want_gr
         stats = torch.stack((r, s), dim=1)
         dist.all_reduce(xc, group=group)
     if own:
-        rows, coef, fix = kernels().distill_finish(stats, xc, ids, logq, weights, temp, temp1, scale, tail, total)
-        grad = kernels().distill_grad(logits, ids, coef, fix, temp, temp1, vocab_start, total,
-                                      inplace) if want_grad else None
-        return rows, grad
+        return kernels().distill_finish(stats, xc, ids, logq, weights, temp, temp1, scale, tail, total)
     rows, coef, fix = _finish_reference(stats, xc, ids, logq, weights, temp, temp1, scale, tail, total)
-    grad = _grad_reference(logits, ids, coef, fix, temp, temp1, vocab_start, total) if want_grad else None
-    return rows.to(torch.promote_types(logits.dtype, torch.float32)), grad
+    return rows.to(torch.promote_types(logits.dtype, torch.float32)), coef, fix
+
+
+def _grad(logits, ids, coef, fix, temp, temp1, vocab_start, group, *, factor=None, inplace=False):
+    """The shard's gradient, ``factor`` (on the device) times what the rows were finished for."""
+    total = logits.shape[1] * tp_world(group)
+    if factor is not None:
+        coef, fix = torch.stack((coef[:, 0], coef[:, 1] * factor), dim=1), fix * factor
+    if on_gpu(logits):
+        return kernels().distill_grad(logits, ids, coef, fix, temp, temp1, vocab_start, total, inplace)
+    return _grad_reference(logits, ids, coef, fix, temp, temp1, vocab_start, total)
 
 
 def _weighted_sum(rows, weights, denom):
@@ -138,30 +146,23 @@ def _weighted_sum(rows, weights, denom):
     return torch.where(weights != 0, rows * weights.to(rows.dtype), torch.zeros_like(rows)).sum() / denom
 
 
-def _scale_by(grad, dloss, grad_scale):
-    if on_gpu(grad):
-        kernels().scale_unless_one(grad, dloss.float(), grad_scale)
-        return grad
-    return grad * (dloss / grad_scale).to(grad.dtype)
-
-
 class _TopkDistillFn(torch.autograd.Function):
     """Vocabularies in shards, and the PyTorch form."""
 
     @staticmethod
     def forward(ctx, logits, ids, logq, weights, temp, temp1, tail, denom, grad_scale, vocab_start, group):
-        rows, grad = _rows_and_grad(logits, ids, logq, weights, temp, temp1, grad_scale / denom, tail,
-                                    ctx.needs_input_grad[0], False, vocab_start, group)
-        ctx.grad, ctx.grad_scale = grad, grad_scale
+        rows, coef, fix = _rows(logits, ids, logq, weights, temp, temp1, grad_scale / denom, tail, vocab_start, group)
+        ctx.save_for_backward(logits, ids, coef, fix, temp)
+        ctx.at = temp1, vocab_start, group
+        ctx.grad_scale = grad_scale
         ctx.mark_non_differentiable(rows)
         return _weighted_sum(rows, weights, denom), rows
 
     @staticmethod
     def backward(ctx, dloss, _drows):
-        grad, ctx.grad = ctx.grad, None        # handed on without a copy, so there is one backward
-        if grad is None:
-            raise RuntimeError("topk_distill_loss: the gradient was already taken by an earlier backward")
-        return (_scale_by(grad, dloss, ctx.grad_scale),) + (None,) * 10
+        logits, ids, coef, fix, temp = ctx.saved_tensors
+        factor = dloss.to(coef.dtype) / ctx.grad_scale         # (before the one rounding to the logits' type)
+        return (_grad(logits, ids, coef, fix, temp, *ctx.at, factor=factor),) + (None,) * 10
 
 
 class _FusedHeadDistillFn(torch.autograd.Function):
@@ -184,7 +185,9 @@ class _FusedHeadDistillFn(torch.autograd.Function):
             if tp_world(group) == 1:
                 rows, dlg = kernels().distill_rows_inplace(lg, *teacher), lg
             else:
-                rows, dlg = _rows_and_grad(lg, *teacher, want, vocab_start, group)
+                rows, coef, fix = _rows(lg, *teacher[:-1], vocab_start, group)
+                if want:
+                    dlg = _grad(lg, ids[at], coef, fix, *teacher[3:5], vocab_start, group, inplace=True)
             parts.append(rows)
             if want_dh:
                 dh[at] = gemm(dlg, weight, b_mn=True)                  # dlogits @ W
@@ -239,7 +242,8 @@ def topk_distill_loss(logits: Tensor, teacher_ids: Tensor, teacher_logp: Tensor,
     ``teacher_ids`` / ``teacher_logp`` are ``[U, K]`` (``K`` up to 256; a negative id drops the entry, an id
     given twice counts as the sum of its probabilities in the gradient).  ``grad_scale`` announces the factor
     by which the caller multiplies the loss before ``backward`` (a loss scale); another one costs one more
-    pass over the gradient.  ``backward`` can be called once.  With ``tp_group``, ``logits`` is this rank's
+    pass over the gradient, with one more rounding in BF16, or for FP16 logits the gradient once more.  ``backward``
+    can be called once.  With ``tp_group``, ``logits`` is this rank's
     equal shard of the vocabulary and ``vocab_start`` its first token.
     """
     if tp_group is None and on_gpu(logits):

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from bridge_b200.ops import fused_lm_head_topk_distill, token_logprobs
+from bridge_b200.ops import fused_lm_head_topk_distill, token_logprobs, topk_distill_loss
 from tests import vocab_oracle as oracle
 from tests.test_vocab_rows_cpu import _case
 
@@ -104,3 +104,25 @@ def test_recomputed_head_counts_once(monkeypatch, reentrant):
     loss.backward()
     dh, dw = _head_gradients(h, W, ids, logq, 1.0)
     assert torch.allclose(h.grad.double(), dh, atol=1e-5) and torch.allclose(W.main_grad.double(), dw, atol=1e-5)
+
+
+# ---------------------------------------------------------------------------------------- loss factors
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_unannounced_loss_scale_is_applied_before_rounding(dtype):
+    """A gradient that underflows unscaled, as a loss scaler meets it: one rounding, of the scaled gradient."""
+    g = torch.Generator().manual_seed(0)
+    x = (3.0 * torch.randn(16, 1024, generator=g)).to(dtype).requires_grad_()
+    top = torch.topk(torch.log_softmax(2 * torch.randn(16, 1024, generator=g), 1), 8, dim=1)
+    for scale in (16384.0, 98304.0):
+        loss, _ = topk_distill_loss(x, top.indices, top.values, denom=4096.0)
+        (got,) = torch.autograd.grad(loss * scale, x)
+        _, want = oracle.distill(x.detach(), top.indices, top.values, 1.0, True)
+        want = want * scale / 4096.0
+        # the type's rounding, and 4e-6 (FP32 arithmetic) of the terms that cancel: p, and q on the given tokens
+        q = torch.zeros_like(want).scatter_(1, top.indices, top.values.double().exp())
+        terms = (torch.softmax(x.detach().double(), 1) + q) * scale / 4096.0
+        rounding = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}[dtype]
+        bound = 1.01 * rounding * want.abs() + 4e-6 * terms + 2.0 ** -25
+        assert bool(((got.double() - want).abs() <= bound).all())
+        if dtype == torch.float16:
+            assert int((got == 0).sum()) < 0.05 * got.numel()

@@ -115,3 +115,24 @@ def test_head_gradients_agree_for_any_loss_factor(main, announced, factor):
     got = W.main_grad - 2.0 if main else W.grad
     _close(h.grad, dh, 2e-2 * float(dh.abs().max()), 5e-2, "dh")
     _close(got, dw, 2e-2 * float(dw.abs().max()), 5e-2, "dW")
+
+
+# ---------------------------------------------------------------------------------------- loss factors
+@pytest.mark.parametrize("rows,vocab", [(64, 1024), (5, 30011), (400, 30000)])
+@pytest.mark.parametrize("tail", [True, False])
+@pytest.mark.parametrize("announced,factor", [(1.0, 16384.0), (49.0, 98304.0), (16384.0, 16384.0)])
+def test_unannounced_loss_scale_in_fp16(rows, vocab, tail, announced, factor):
+    """A gradient that underflows unscaled is rounded once, after the scale; the rows stay what they were."""
+    x = _logits(rows, vocab, torch.float16).requires_grad_()
+    ids, logq = _teacher(rows, vocab, 8)
+    w = 0.1 + torch.rand(rows, device=DEV)
+    w[0] = 0.0
+    loss, kl = _ops().topk_distill_loss(x, ids, logq, denom=4096.0, weights=w, grad_scale=announced, tail=tail)
+    keep = kl.clone()
+    (got,) = torch.autograd.grad(loss * factor, x, retain_graph=True)
+    _, want = oracle.distill(x.detach(), ids, logq, 1.0, tail)
+    f = w.double()[:, None] * factor / 4096.0
+    _check_grad(got, want * f, 2 * f, torch.float16)
+    assert torch.equal(kl, keep)
+    with pytest.raises(RuntimeError, match="already taken"):
+        torch.autograd.grad(loss, x)
