@@ -166,35 +166,40 @@ class _TopkDistillFn(torch.autograd.Function):
 
 
 class _FusedHeadDistillFn(torch.autograd.Function):
-    """LM head + divergence with the head's backward inside the forward (see the module docstring)."""
+    """LM head + divergence with the head's backward inside the forward (see the module docstring).
+
+    FP16 heads run it in the backward, on the chunks' logits computed again: there only the loss's own factor
+    says at which scale a gradient may be rounded."""
 
     @staticmethod
     def forward(ctx, h, weight, ids, logq, weights, temp, temp1, tail, denom, grad_scale, vocab_start, group,
                 chunk_rows, differentiable):
         # (what needs a gradient is said of the inputs under no_grad too)
         want_dh, want_dw = (differentiable and n for n in ctx.needs_input_grad[:2])
-        want = want_dh or want_dw
-        dh = torch.empty_like(h) if want_dh else None
-        dw = torch.zeros(weight.shape, dtype=torch.float32, device=weight.device) if want_dw else None
+        late = h.dtype == torch.float16 and (want_dh or want_dw)
+        want = not late and (want_dh or want_dw)
+        dh, dw = _head_gradients(h, weight, want and want_dh, want and want_dw)
         parts = []
-        for a in range(0, h.shape[0], chunk_rows):
-            at = slice(a, min(a + chunk_rows, h.shape[0]))
+        for at in _chunks(h, chunk_rows):
             lg = gemm(h[at], weight)
             teacher = (ids[at], logq[at], None if weights is None else weights[at], None if temp is None else temp[at],
-                       temp1, grad_scale / denom, tail, want)
-            if tp_world(group) == 1:
-                rows, dlg = kernels().distill_rows_inplace(lg, *teacher), lg
+                       temp1, grad_scale / denom, tail)
+            if tp_world(group) == 1 and not late:
+                parts.append((kernels().distill_rows_inplace(lg, *teacher, want), None, None))
+                dlg = lg
             else:
-                rows, coef, fix = _rows(lg, *teacher[:-1], vocab_start, group)
+                parts.append(_rows(lg, *teacher, vocab_start, group))
                 if want:
-                    dlg = _grad(lg, ids[at], coef, fix, *teacher[3:5], vocab_start, group, inplace=True)
-            parts.append(rows)
-            if want_dh:
-                dh[at] = gemm(dlg, weight, b_mn=True)                  # dlogits @ W
-            if want_dw:
-                gemm(dlg, h[at], a_mn=True, b_mn=True, out=dw, accumulate=True)      # += dlogits^T h
-        rows = torch.cat(parts) if parts else torch.zeros(0, dtype=torch.float32, device=h.device)
-        ctx.save_for_backward(dh, dw)
+                    dlg = _grad(lg, ids[at], *parts[-1][1:], *teacher[3:5], vocab_start, group, inplace=True)
+            if want:
+                _head_backward(dlg, h, weight, at, dh, dw)
+        rows = torch.cat([p[0] for p in parts]) if parts else torch.zeros(0, dtype=torch.float32, device=h.device)
+        if late and parts:
+            coef, fix = (torch.cat([p[i] for p in parts]) for i in (1, 2))
+            ctx.save_for_backward(h, weight, ids, coef, fix, temp)
+        else:
+            ctx.save_for_backward(dh, dw)
+        ctx.late = (temp1, vocab_start, group, chunk_rows) if late and parts else None
         ctx.grad_scale, ctx.dtype = grad_scale, weight.dtype
         ctx.main_grad = getattr(weight, "main_grad", None)
         ctx.mark_non_differentiable(rows)
@@ -202,16 +207,42 @@ class _FusedHeadDistillFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dloss, _drows):
-        dh, dw = ctx.saved_tensors
         f = dloss.float() / ctx.grad_scale
-        if dh is not None:
-            dh = (dh.float() * f).to(dh.dtype)
+        if ctx.late is None:
+            dh, dw = ctx.saved_tensors
+            if dh is not None:
+                dh = (dh.float() * f).to(dh.dtype)
+        else:
+            h, weight, ids, coef, fix, temp = ctx.saved_tensors
+            temp1, vocab_start, group, chunk_rows = ctx.late
+            dh, dw = _head_gradients(h, weight, *ctx.needs_input_grad[:2])
+            for at in _chunks(h, chunk_rows):
+                dlg = _grad(gemm(h[at], weight), ids[at], coef[at], fix[at], None if temp is None else temp[at], temp1,
+                            vocab_start, group, factor=f, inplace=True)
+                _head_backward(dlg, h, weight, at, dh, dw)
+            f = torch.ones_like(f)
         if dw is not None and ctx.main_grad is not None:
             ctx.main_grad.addcmul_(dw.to(ctx.main_grad.dtype), f.to(ctx.main_grad.dtype))
             dw = None
         elif dw is not None:
             dw = (dw * f).to(ctx.dtype)
         return (dh, dw) + (None,) * 12
+
+
+def _chunks(h, chunk_rows):
+    return [slice(a, min(a + chunk_rows, h.shape[0])) for a in range(0, h.shape[0], chunk_rows)]
+
+
+def _head_gradients(h, weight, want_dh, want_dw):
+    return (torch.empty_like(h) if want_dh else None,
+            torch.zeros(weight.shape, dtype=torch.float32, device=weight.device) if want_dw else None)
+
+
+def _head_backward(dlg, h, weight, at, dh, dw):
+    if dh is not None:
+        dh[at] = gemm(dlg, weight, b_mn=True)                          # dlogits @ W
+    if dw is not None:
+        gemm(dlg, h[at], a_mn=True, b_mn=True, out=dw, accumulate=True)      # += dlogits^T h
 
 
 # ------------------------------------------------------------------------------------------------- API
@@ -279,7 +310,8 @@ def fused_lm_head_topk_distill(h: Tensor, weight: Tensor, teacher_ids: Tensor, t
     """:func:`topk_distill_loss` of hidden rows ``h [U, H]`` under the head ``weight [V_local, H]``.
 
     The logits exist for ``chunk_rows`` rows at a time and become their own gradient in place.  ``dW`` is summed
-    in FP32 and kept for the backward, which adds it to ``weight.main_grad`` where there is one.
+    in FP32 and kept for the backward, which adds it to ``weight.main_grad`` where there is one.  FP16 heads compute
+    the logits once more in the backward instead, so that only scaled gradients are rounded.
     """
     name = "fused_lm_head_topk_distill"
     if h.ndim != 2 or weight.ndim != 2 or h.shape[1] != weight.shape[1]:

@@ -38,6 +38,16 @@ def _stand_in(monkeypatch):
             return rows.float()
 
         @staticmethod
+        def distill_open(logits, ids, logq, weights, temp, temp1, start, total):
+            return distill._open_reference(logits, ids, temp, temp1, start)
+
+        distill_finish = staticmethod(distill._finish_reference)
+
+        @staticmethod
+        def distill_grad(logits, ids, coef, fix, temp, temp1, start, total, inplace):
+            return distill._grad_reference(logits, ids, coef, fix, temp, temp1, start, total)
+
+        @staticmethod
         def weighted_rows_sum(rows, weights, denom):
             return (rows if weights is None else rows * weights).sum() / denom
 
@@ -126,3 +136,22 @@ def test_unannounced_loss_scale_is_applied_before_rounding(dtype):
         assert bool(((got.double() - want).abs() <= bound).all())
         if dtype == torch.float16:
             assert int((got == 0).sum()) < 0.05 * got.numel()
+
+
+@pytest.mark.parametrize("main", [True, False])
+def test_head_unannounced_loss_scale_in_fp16(monkeypatch, main):
+    """Gradients of FP16 logits under a head, which underflow unscaled: FP16 matrix products of what is rounded once."""
+    _stand_in(monkeypatch)
+    h, W, ids, logq = _head(dtype=torch.float16)
+    h, W = (0.25 * h).detach().requires_grad_(), (0.25 * W).detach().requires_grad_()
+    if main:
+        W.main_grad = torch.zeros(W.shape)
+    scale = 2.0 ** 20
+    loss, _ = fused_lm_head_topk_distill(h, W, ids, logq, denom=2.0 ** 25, chunk_rows=16)
+    (loss * scale).backward()
+    dh, dw = _head_gradients(h, W, ids, logq, scale * 40.0 / 2.0 ** 25)
+    # 60 and 40 products of at most 1/32 x 1, each with a rounding of the logits (2^-11 of 4) and its own: below 2^-6 of the
+    # largest, where the underflow of what is below 2^-25 took everything
+    assert float((h.grad.double() - dh).abs().max()) <= 2.0 ** -6 * float(dh.abs().max())
+    got = W.main_grad if main else W.grad
+    assert float((got.double() - dw).abs().max()) <= 2.0 ** -6 * float(dw.abs().max())

@@ -136,3 +136,25 @@ def test_unannounced_loss_scale_in_fp16(rows, vocab, tail, announced, factor):
     assert torch.equal(kl, keep)
     with pytest.raises(RuntimeError, match="already taken"):
         torch.autograd.grad(loss, x)
+
+
+@pytest.mark.parametrize("main", [True, False])
+@pytest.mark.parametrize("temp", [1.0, "rows"])
+def test_head_unannounced_loss_scale_in_fp16(main, temp):
+    """FP16 logits (2^-11 of their size, below 8) and FP16 products of gradients that would underflow unscaled."""
+    h, W, ids, logq, w = _head(dtype=torch.float16)
+    h.requires_grad_()
+    W.requires_grad_()
+    if main:
+        W.main_grad = torch.zeros(W.shape, device=DEV)
+    t = 0.8 + torch.rand(200, device=DEV) if temp == "rows" else temp
+    scale = 2.0 ** 20
+    loss, _ = _ops().fused_lm_head_topk_distill(h, W, ids, logq, denom=2.0 ** 25, weights=w, temperature=t, chunk_rows=64)
+    (loss * scale).backward()
+    hd, Wd = h.detach().double(), W.detach().double()
+    _, gx = oracle.distill(hd @ Wd.t(), ids, logq, t, True)
+    gx = gx * w.double()[:, None] * scale / 2.0 ** 25
+    dh, dw = gx @ Wd, gx.t() @ hd
+    got = W.main_grad if main else W.grad
+    assert float((h.grad - dh).abs().max()) <= 2.0 ** -6 * float(dh.abs().max())
+    assert float((got - dw).abs().max()) <= 2.0 ** -6 * float(dw.abs().max())
