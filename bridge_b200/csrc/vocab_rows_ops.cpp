@@ -138,6 +138,15 @@ torch::Tensor score_rows_bwd(const torch::Tensor& logits, const OptTensor& token
   return grad;
 }
 
+// Both nodes' gradients are made from sums that their forward kept: constants to a second differentiation, and nothing
+// here carries a tangent.
+void first_order(const char* name) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), name, " has no second derivative (backward was called with create_graph=True)");
+}
+void no_tangent(const torch::Tensor& x, const char* name) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!x._fw_grad(0).defined(), name, " has no forward-mode derivative");
+}
+
 OptTensor optional(const torch::Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 OptTensor upstream(const torch::Tensor& g) {
   return g.defined() ? OptTensor(g.to(at::kFloat).contiguous()) : OptTensor();
@@ -163,6 +172,7 @@ class ScoreRows : public torch::autograd::Function<ScoreRows> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
+    first_order("token_logprobs");
     const auto saved = ctx->get_saved_variables();
     const bool has_logp = ctx->saved_data["logp"].toBool();
     size_t at = 0;
@@ -228,6 +238,7 @@ class DistillLoss : public torch::autograd::Function<DistillLoss> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
+    first_order("topk_distill_loss");
     const auto held = ctx->saved_data.find("grad");
     TORCH_CHECK(held != ctx->saved_data.end(),
                 "topk_distill_loss: the gradient was already taken by an earlier backward");
@@ -266,6 +277,7 @@ std::vector<torch::Tensor> token_logprobs(torch::Tensor logits, OptTensor tokens
                       tokens->scalar_type() == at::kLong && tokens->is_contiguous() &&
                       tokens->device() == logits.device()));
   if (!fits) return {};
+  no_tangent(logits, "token_logprobs");
   const bool differentiable = logits.requires_grad() && at::GradMode::is_enabled() && (tokens.has_value() || entropy);
   if (!differentiable) {
     const Scores o = score_rows(logits, tokens, temp, temp1, k, entropy, false, 0, false);
@@ -310,6 +322,7 @@ std::vector<torch::Tensor> topk_distill(torch::Tensor logits, torch::Tensor ids,
                     positive(temp1) && positive(denom) && positive(grad_scale) && entries(ids, at::kLong) &&
                     entries(logq, at::kFloat) && logq.size(1) == ids.size(1);
   if (!fits) return {};
+  no_tangent(logits, "topk_distill_loss");
   if (logits.requires_grad() && at::GradMode::is_enabled()) {
     const auto o = DistillLoss::apply(logits, ids, logq, weights, temp, temp1, tail, denom, grad_scale);
     return {o[0], o[1]};

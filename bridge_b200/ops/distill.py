@@ -33,7 +33,7 @@ from torch import Tensor
 
 from ._ext import kernels, on_gpu
 from .gemm import gemm
-from .token_logprob import (MAX_TOP, _LN2, _MASKED, check_ids, check_logits, join_shards, log2_scale, picked,
+from .token_logprob import (MAX_TOP, _LN2, _MASKED, check_ids, check_logits, first_order, join_shards, log2_scale, picked,
                             row_floats, shard_sums, split_temperature, tp_world, unit_columns)
 
 
@@ -160,6 +160,7 @@ class _TopkDistillFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dloss, _drows):
+        first_order("topk_distill_loss")
         logits, ids, coef, fix, temp = ctx.saved_tensors
         factor = dloss.to(coef.dtype) / ctx.grad_scale         # (before the one rounding to the logits' type)
         return (_grad(logits, ids, coef, fix, temp, *ctx.at, factor=factor),) + (None,) * 10
@@ -207,6 +208,7 @@ class _FusedHeadDistillFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dloss, _drows):
+        first_order("fused_lm_head_topk_distill")
         f = dloss.float() / ctx.grad_scale
         if ctx.late is None:
             dh, dw = ctx.saved_tensors

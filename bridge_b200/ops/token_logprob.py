@@ -16,7 +16,8 @@ Edge cases: a token outside the vocabulary (a padded position) has log-prob 0 an
 of ``-inf``, or one with ``x / T`` at or below ``-2^31 ln 2`` (-1.49e9: FP32's lowest value, finite masks
 from -1e10 down), carries no probability; where a row holds nothing else its log-probs are ``-inf``, its
 entropy 0 and its gradient 0.  NaN, ``+inf`` or ``x / T`` above 1.49e9 in a row makes its log-probs and
-entropy NaN (among the alternatives NaN counts as ``-inf``).  Subnormal logits count as 0.
+entropy NaN (among the alternatives NaN counts as ``-inf``).  Subnormal logits count as 0.  There is a first derivative
+only: a backward with ``create_graph=True`` and forward-mode inputs are refused.
 """
 
 from __future__ import annotations
@@ -140,6 +141,12 @@ def top_rows(x: Tensor, k: int) -> Tensor:
 
 
 # -------------------------------------------------------------------------------------------- autograd
+def first_order(name: str) -> None:
+    """Called in a backward whose saved sums are constants: its result cannot be differentiated again."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{name} has no second derivative (backward was called with create_graph=True)")
+
+
 class _TokenLogprobFn(torch.autograd.Function):
     """Vocabularies in shards, and the PyTorch form."""
 
@@ -187,6 +194,7 @@ class _TokenLogprobFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, d_logp, d_ent, _ids, _top):
+        first_order("token_logprobs")
         logits, tokens, temp, stats = ctx.saved_tensors
         if d_logp is None and d_ent is None:
             return (None,) * 8

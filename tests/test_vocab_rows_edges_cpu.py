@@ -155,3 +155,32 @@ def test_head_unannounced_loss_scale_in_fp16(monkeypatch, main):
     assert float((h.grad.double() - dh).abs().max()) <= 2.0 ** -6 * float(dh.abs().max())
     got = W.main_grad if main else W.grad
     assert float((got.double() - dw).abs().max()) <= 2.0 ** -6 * float(dw.abs().max())
+
+
+# -------------------------------------------------------------------------------- no second derivative
+def test_second_derivatives_are_refused(monkeypatch):
+    x = torch.randn(3, 20, dtype=torch.float64, requires_grad=True)
+    tokens = torch.tensor([1, 2, 3])
+    ids, logq = torch.tensor([[0, 4]] * 3), torch.full((3, 2), -1.5)
+    r = token_logprobs(x, tokens)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(r.logp.sum() + r.entropy.sum(), x, create_graph=True)
+    loss, _ = topk_distill_loss(x, ids, logq, denom=3.0)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(loss, x, create_graph=True)
+    _stand_in(monkeypatch)
+    h, W, ids, logq = _head()
+    loss, _ = fused_lm_head_topk_distill(h, W, ids, logq, denom=40.0)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(loss, h, create_graph=True)
+
+
+def test_forward_mode_is_refused():
+    from torch.autograd import forward_ad
+
+    with forward_ad.dual_level():
+        x = forward_ad.make_dual(torch.randn(3, 20), torch.randn(3, 20))
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            token_logprobs(x, torch.tensor([1, 2, 3]))
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            topk_distill_loss(x, torch.tensor([[0, 4]] * 3), torch.full((3, 2), -1.5), denom=3.0)

@@ -158,3 +158,32 @@ def test_head_unannounced_loss_scale_in_fp16(main, temp):
     got = W.main_grad if main else W.grad
     assert float((h.grad - dh).abs().max()) <= 2.0 ** -6 * float(dh.abs().max())
     assert float((got - dw).abs().max()) <= 2.0 ** -6 * float(dw.abs().max())
+
+
+# -------------------------------------------------------------------------------- no second derivative
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_second_derivatives_and_forward_mode_are_refused(dtype):
+    from torch.autograd import forward_ad
+
+    ops = _ops()
+    x = _logits(3, 50, dtype).requires_grad_()
+    tokens = torch.tensor([1, 2, 3], device=DEV)
+    ids, logq = _teacher(3, 50, 4)
+    r = ops.token_logprobs(x, tokens)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(r.logp.sum() + r.entropy.sum(), x, create_graph=True)
+    loss, _ = ops.topk_distill_loss(x, ids, logq, denom=3.0)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(loss, x, create_graph=True, retain_graph=True)
+    assert bool(torch.autograd.grad(loss, x)[0].any())          # (the refusal took nothing away)
+    h, W, ids, logq, _ = _head()
+    loss, _ = ops.fused_lm_head_topk_distill(h.requires_grad_(), W, ids, logq, denom=200.0)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(loss, h, create_graph=True)
+    with forward_ad.dual_level():
+        for grad in (False, True):
+            y = forward_ad.make_dual(x.detach().requires_grad_(grad), torch.randn_like(x))
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                ops.token_logprobs(y, tokens)
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                ops.topk_distill_loss(y, ids[:3] % 50, logq[:3], denom=3.0)
