@@ -1091,6 +1091,11 @@ __device__ __forceinline__ Teacher join_blocks(Teacher t) {
   return t;
 }
 
+// What FP32 log-probs can leave of 1 by rounding (theirs are right to 2e-6, and q to as much of itself).  Where the
+// student has nothing outside the entries, as when both are under a mask that leaves fewer tokens than there are
+// entries, a remainder of this size is no probability without a home: it would make the divergence infinite.
+constexpr double kResidue = 3.814697265625e-6;      // 2^-18
+
 // `some`: the row has entries that count.  `scale` includes the row's weight and 1 / T.
 __device__ __forceinline__ Finished finish_row(const Teacher& t, Stat rest, bool some, bool tail, double scale) {
   // (written with selects: the long FP64 chains are independent and overlap)
@@ -1100,7 +1105,7 @@ __device__ __forceinline__ Finished finish_row(const Teacher& t, Stat rest, bool
   const bool lost = m == -INFINITY;                     // none anywhere
   const double m0 = lost ? 0.0 : m;
   const double s = out ? (double)rest.s : 1.0;
-  const double q_rest = tail ? fmax(0.0, 1.0 - t.q) : 0.0, total = tail ? t.q + q_rest : 1.0;
+  const double left = tail ? fmax(0.0, 1.0 - t.q) : 0.0, q_rest = out || left > kResidue ? left : 0.0, total = tail ? t.q + q_rest : 1.0;
   const double q_norm = tail ? 1.0 : t.q;
   const double log_s = log2_d(s), log_qr = log2_d(q_rest), log_norm = log2_d(q_norm);
   const double inv_s = rcp_d(s), norm = rcp_d(q_norm);

@@ -20,7 +20,9 @@ scale would lose it).  Vocabularies in shards write theirs in the backward.
 followed by a backward, changes no gradient.
 
 Rows of weight 0 and rows without an entry have divergence 0 and gradient 0 whatever their logits hold.
-A given token (``q_j > 0``) without student probability makes the divergence infinite.
+A given token (``q_j > 0``) without student probability makes the divergence infinite, and so does a
+tail without any; but a ``q_r`` of at most ``2^-18`` is then taken for the rounding of FP32 log-probs and
+dropped (a teacher's alternatives under a mask that leaves no more than ``K`` tokens).
 """
 
 from __future__ import annotations
@@ -35,6 +37,9 @@ from ._ext import kernels, on_gpu
 from .gemm import gemm
 from .token_logprob import (MAX_TOP, _LN2, _MASKED, check_ids, check_logits, first_order, join_shards, log2_scale, picked,
                             row_floats, shard_sums, split_temperature, tp_world, unit_columns)
+
+
+_RESIDUE = 2.0 ** -18      # of a teacher's probability that FP32 log-probs may leave by rounding
 
 
 # ------------------------------------------------------------------------- PyTorch form (CPU, oracle)
@@ -81,6 +86,7 @@ def _finish_reference(stats, xc, ids, logq, weights, temp, temp1, scale, tail, t
     logp = _LN2 * (xc - m[:, None] - log2z[:, None])
     kl = torch.where(q == 0, torch.zeros_like(q), q * (logq - logp)).sum(dim=1)
     q_rest = (1.0 - q.sum(dim=1)).clamp(min=0.0) if tail else torch.zeros_like(m)
+    q_rest = torch.where((rest == 0) & (q_rest <= _RESIDUE), torch.zeros_like(m), q_rest)
     total_q = q.sum(dim=1) + q_rest
     p_rest = rest / z
     kl = kl + torch.where(q_rest > 0, q_rest * (torch.log(q_rest) - torch.log(p_rest)), torch.zeros_like(m))

@@ -184,3 +184,34 @@ def test_forward_mode_is_refused():
             token_logprobs(x, torch.tensor([1, 2, 3]))
         with pytest.raises((RuntimeError, NotImplementedError)):
             topk_distill_loss(x, torch.tensor([[0, 4]] * 3), torch.full((3, 2), -1.5), denom=3.0)
+
+
+# --------------------------------------------------------------------------- teachers that cover all that lives
+def _covered(rows=16, vocab=120, live=40, device="cpu", seed=0):
+    """Teacher and student under the same mask, which leaves fewer tokens than the teacher gives alternatives."""
+    g = torch.Generator().manual_seed(seed)
+    t, x = (3.0 * torch.randn(rows, vocab, generator=g) for _ in range(2))
+    for u in range(rows):
+        gone = torch.randperm(vocab, generator=g)[live:]
+        t[u, gone] = x[u, gone] = -math.inf
+    return t.to(device), x.to(device)
+
+
+def _kl_of_live(t, x, temp=1.0):
+    lq, lp = torch.log_softmax(t.double() / temp, 1), torch.log_softmax(x.double() / temp, 1)
+    q, p = lq.exp(), lp.exp()
+    return torch.where(q > 0, q * (lq - lp), torch.zeros_like(q)).sum(1), (p - q) / temp
+
+
+def test_teacher_of_all_live_tokens_is_finite():
+    """What FP32 log-probs leave of 1 is no probability where the student has none either: the KL of the live tokens."""
+    t, x = _covered()
+    teacher = token_logprobs(t, top_k=64)
+    x.requires_grad_()
+    loss, rows = topk_distill_loss(x, teacher.top_ids, teacher.top_logp, denom=16.0)
+    want, grad = _kl_of_live(t, x.detach())
+    assert torch.allclose(rows.double(), want, atol=1e-5) and bool(torch.isfinite(loss))
+    assert torch.allclose(torch.autograd.grad(loss, x)[0].double(), grad / 16.0, atol=1e-6)
+    # while mass that is really missing has nowhere to go
+    _, rows = topk_distill_loss(x.detach(), teacher.top_ids, teacher.top_logp - 1e-3, denom=16.0)
+    assert bool((rows == math.inf).all())

@@ -187,3 +187,39 @@ def test_second_derivatives_and_forward_mode_are_refused(dtype):
                 ops.token_logprobs(y, tokens)
             with pytest.raises((RuntimeError, NotImplementedError)):
                 ops.topk_distill_loss(y, ids[:3] % 50, logq[:3], denom=3.0)
+
+
+# --------------------------------------------------------------------------- teachers that cover all that lives
+@pytest.mark.parametrize("vocab", [120, 2000, 70001])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_teacher_of_all_live_tokens_is_finite(vocab, dtype):
+    """The operator's own alternatives of masked rows, to a student under the same mask: the KL of the live tokens."""
+    from tests.test_vocab_rows_edges_cpu import _covered, _kl_of_live
+
+    t, x = (v.to(dtype) for v in _covered(rows=32, vocab=vocab, device=DEV))
+    ops = _ops()
+    for temp in (1.0, 0.6):
+        teacher = ops.token_logprobs(t, None, temp, top_k=64)
+        xg = x.detach().requires_grad_()
+        loss, rows = ops.topk_distill_loss(xg, teacher.top_ids, teacher.top_logp, denom=1.0, temperature=temp)
+        want, grad = _kl_of_live(t, x, temp)
+        _close(rows, want, 8e-6, 1e-6, "rows")                # (2e-6 of every log-prob of the teacher besides)
+        assert bool(torch.isfinite(loss))
+        _check_grad(torch.autograd.grad(loss, xg)[0], grad, torch.full((32, 1), 2.0 / temp, device=DEV).double(), dtype)
+        _, rows = ops.topk_distill_loss(x, teacher.top_ids, teacher.top_logp - 1e-3, denom=1.0, temperature=temp)
+        assert bool((rows == math.inf).all())
+
+
+def test_teacher_of_all_live_tokens_in_shards():
+    from bridge_b200.ops._ext import kernels
+    from tests.test_vocab_rows_edges_cpu import _covered, _kl_of_live
+
+    m = kernels()
+    t, x = _covered(rows=32, vocab=900, device=DEV)
+    teacher = _ops().token_logprobs(t, top_k=64)
+    stats, xc = m.distill_open(x, teacher.top_ids, teacher.top_logp, None, None, 1.0, 0, 900)
+    rows, coef, fix = m.distill_finish(stats, xc, teacher.top_ids, teacher.top_logp, None, None, 1.0, 1.0, True, 900)
+    want, grad = _kl_of_live(t, x)
+    _close(rows, want, 1e-5, 2e-6, "rows")
+    got = m.distill_grad(x, teacher.top_ids, coef, fix, None, 1.0, 0, 900, False)
+    _check_grad(got, grad, torch.full((32, 1), 4.0, device=DEV).double(), torch.float32)
