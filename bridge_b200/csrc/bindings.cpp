@@ -69,7 +69,6 @@ torch::Tensor distill_grad(torch::Tensor logits, torch::Tensor ids, torch::Tenso
                            c10::optional<torch::Tensor> temp, double temp1, int64_t vocab_start, int64_t vocab_total,
                            bool inplace);
 torch::Tensor weighted_rows_sum(torch::Tensor rows, c10::optional<torch::Tensor> weights, double denom);
-void scale_unless_one(torch::Tensor x, torch::Tensor num, double den);
 void adamw_step(torch::Tensor master, torch::Tensor param, torch::Tensor grad, torch::Tensor m, torch::Tensor v,
                 torch::Tensor clip, double lr, double b1, double b2, double eps, double wd, double bc1, double bc2);
 std::vector<torch::Tensor> tree_attn_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor pk,
@@ -178,7 +177,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("distill_finish", &distill_finish, "... rows and gradient factors from the joined sums");
   m.def("distill_grad", &distill_grad, "... the shard's gradient");
   m.def("weighted_rows_sum", &weighted_rows_sum, "sum(w * rows) / denom, fixed order");
-  m.def("scale_unless_one", &scale_unless_one, "x *= num / den in place, skipped on the device when that is 1");
   m.def("adamw_step", &adamw_step);
   m.def("tree_attn_fwd", &tree_attn_fwd);
   m.def("tree_attn_bwd", &tree_attn_bwd);

@@ -1555,11 +1555,12 @@ __global__ void weighted_sum_kernel(const float* __restrict__ rows, const float*
   }
 }
 
-// x *= num / den unless that is 1 (the factor is on the device; the usual 1 costs one read per block).
+// x *= num / den unless that is 1 (the factor is on the device; the usual 1 costs one read per block).  The two are
+// compared and not their quotient, which is a product with a reciprocal in this build and misses 1 for many equals.
 template <typename T>
 __global__ void scale_unless_one_kernel(T* __restrict__ x, long n, const float* __restrict__ num, float den) {
-  const float f = num[0] / den;
-  if (f == 1.f) return;
+  if (num[0] == den) return;
+  const float f = __fdiv_rn(num[0], den);
   for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long)gridDim.x * blockDim.x)
     x[i] = from_f<T>(to_f(x[i]) * f);
 }

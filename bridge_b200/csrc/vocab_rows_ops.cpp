@@ -413,11 +413,3 @@ torch::Tensor weighted_rows_sum(torch::Tensor rows, OptTensor weights, double de
   check_vec(weights, rows.numel(), at::kFloat, rows, "weights must be float32 [U]");
   return sum_rows(rows, weights, denom);
 }
-
-void scale_unless_one(torch::Tensor x, torch::Tensor num, double den) {
-  TORCH_CHECK(x.is_cuda() && x.is_contiguous() && num.device() == x.device() && num.scalar_type() == at::kFloat &&
-                  num.numel() == 1,
-              "scale: contiguous CUDA tensor and one float32 factor");
-  const c10::cuda::CUDAGuard guard(x.device());
-  scale_grad(x, num, den);
-}

@@ -223,3 +223,19 @@ def test_teacher_of_all_live_tokens_in_shards():
     _close(rows, want, 1e-5, 2e-6, "rows")
     got = m.distill_grad(x, teacher.top_ids, coef, fix, None, 1.0, 0, 900, False)
     _check_grad(got, grad, torch.full((32, 1), 4.0, device=DEV).double(), torch.float32)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_announced_scales_leave_the_gradient_alone(dtype):
+    """The gradient of a loss scaled as announced is the forward's own, bit for bit and without a write, whatever the
+    announced number: also where a reciprocal's product would not give exactly 1."""
+    x = _logits(4, 600, dtype).requires_grad_()
+    ids, logq = _teacher(4, 600, 5)
+    from bridge_b200.ops._ext import kernels
+
+    for scale in [*range(1, 200), 1.1, 3e-3, 12345.678]:
+        own = x.detach().clone()
+        kernels().distill_rows_inplace(own, ids, logq, None, None, 1.0, scale / 7.0, True, True)
+        loss, _ = _ops().topk_distill_loss(x, ids, logq, denom=7.0, grad_scale=scale)
+        (got,) = torch.autograd.grad(loss, x, torch.tensor(scale, device=DEV))
+        assert torch.equal(got, own), scale
