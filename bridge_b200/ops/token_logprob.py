@@ -104,6 +104,12 @@ def log2_scale(temp: Tensor | None, temp1: float, logits: Tensor) -> Tensor:
     return (_LOG2E / temp.to(dt))[:, None]
 
 
+def _exact_scale(temp: Tensor | None, temp1: float, device, own: bool) -> Tensor:
+    """:func:`log2_scale` in 64 bits; of the kernels, the FP32 number that they multiply by."""
+    c = _LOG2E / (torch.full((1,), temp1, dtype=torch.float64, device=device) if temp is None else temp.double())
+    return (c.float().double() if own else c)[:, None]
+
+
 def shard_sums(xc: Tensor) -> tuple[Tensor, Tensor, Tensor]:
     """``(R, s, sum e t)`` of log2-domain rows: ``t = xc - R``, ``e = 2^t``; masked columns count nothing."""
     r = xc.amax(dim=1).clamp(min=_MASKED)
@@ -158,17 +164,20 @@ class _TokenLogprobFn(torch.autograd.Function):
         k = min(top_k, logits.shape[1])
         ctx.set_materialize_grads(False)
         ctx.vocab_start, ctx.total, ctx.temp1, ctx.own = vocab_start, total, temp1, own
+        # Logits and sums travel as they are; what they make is worked out in 64 bits, like the kernel's own rows: a
+        # log-prob is the small difference of x c and a log-sum that are as large as the logits.
+        c = _exact_scale(temp, temp1, logits.device, own)
+        out = torch.promote_types(logits.dtype, torch.float32)
+        xt = picked(logits, tokens, vocab_start).to(out) if tokens is not None else None
         if own:
-            xt, sums, ids, top = kernels().token_logprob_open(logits, tokens, temp, temp1, k, with_entropy, vocab_start)
-            r, s, et = sums.unbind(1)
+            _, sums, ids, top = kernels().token_logprob_open(logits, None, temp, temp1, k, with_entropy, vocab_start)
+            r, s, et = sums.double().unbind(1)
         else:
-            xc = logits.to(torch.promote_types(logits.dtype, torch.float32)) * log2_scale(temp, temp1, logits)
-            r, s, et = shard_sums(xc)
-            xt = picked(xc, tokens, vocab_start) if tokens is not None else None
+            r, s, et = shard_sums(logits.double() * c)
             ids = top = None
             if k:
                 ids = top_rows(logits, k)
-                top = logits.gather(1, ids).to(xc.dtype)
+                top = logits.gather(1, ids).to(out)
                 ids = ids + vocab_start
         if world > 1:
             r, s, et = join_shards(r, s, et, group)
@@ -180,14 +189,18 @@ class _TokenLogprobFn(torch.autograd.Function):
         full = r + log2s
         logp = None
         if tokens is not None:
-            logp = _finish(xt, full, s)
+            logp = _finish(xt.double() * c, full, s).to(out)
             logp = torch.where((tokens >= 0) & (tokens < total), logp, torch.zeros_like(logp))
         empty = s == 0
         one = torch.where(empty, torch.ones_like(s), s)
         ent = torch.where(empty, torch.zeros_like(s), _LN2 * (log2s - et / one)) if with_entropy else None
         stats = torch.stack((r, torch.where(empty, torch.zeros_like(s), 1.0 / one), et / one), dim=1)
+        if own:
+            stats = stats.float()
+        if with_entropy:
+            ent = ent.to(out)
         if top_k:
-            top = _finish(top * log2_scale(temp, temp1, top), full, s)
+            top = _finish(top.double() * c, full, s).to(out)
             ctx.mark_non_differentiable(ids, top)
         ctx.save_for_backward(logits, tokens, temp, stats)
         return logp, ent, ids, top
@@ -230,9 +243,9 @@ def _join_tops(ids: Tensor, top: Tensor, k: int, world: int, group) -> tuple[Ten
 
 
 def _grad_reference(logits, tokens, temp, temp1, stats, d_logp, d_ent, vocab_start, total):
-    c = log2_scale(temp, temp1, logits)
+    c = _exact_scale(temp, temp1, logits.device, False)
     r, inv, mean = (v[:, None] for v in stats.unbind(1))
-    t = logits.to(c.dtype) * c - r
+    t = logits.double() * c - r
     p = torch.exp2(t) * inv
     g = torch.zeros_like(p)
     if d_logp is not None:

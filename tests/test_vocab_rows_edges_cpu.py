@@ -215,3 +215,18 @@ def test_teacher_of_all_live_tokens_is_finite():
     # while mass that is really missing has nowhere to go
     _, rows = topk_distill_loss(x.detach(), teacher.top_ids, teacher.top_logp - 1e-3, denom=16.0)
     assert bool((rows == math.inf).all())
+
+
+# ------------------------------------------------------------------------------------------- precision
+def test_log_probs_keep_their_digits_far_from_zero():
+    """FP32 logits around 60: a log-prob is right to 2e-6 and 2^-21 of its size, not to the logits' last place."""
+    g = torch.Generator().manual_seed(2)
+    x = 60.0 + torch.randn(50, 300, generator=g)
+    tokens = torch.randint(0, 300, (50, 2), generator=g)
+    r = token_logprobs(x, tokens, 0.7, top_k=5)
+    want, ent = oracle.token_logprobs(x, tokens, 0.7)
+    assert r.logp.dtype == r.entropy.dtype == r.top_logp.dtype == torch.float32
+    assert bool(((r.logp.double() - want).abs() <= 2e-6 + 5e-7 * want.abs()).all())
+    top, _ = oracle.token_logprobs(x, r.top_ids, 0.7)
+    assert bool(((r.top_logp.double() - top).abs() <= 2e-6 + 5e-7 * top.abs()).all())
+    assert bool(((r.entropy.double() - ent).abs() <= 4e-5).all())

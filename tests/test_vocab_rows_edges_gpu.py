@@ -239,3 +239,147 @@ def test_announced_scales_leave_the_gradient_alone(dtype):
         loss, _ = _ops().topk_distill_loss(x, ids, logq, denom=7.0, grad_scale=scale)
         (got,) = torch.autograd.grad(loss, x, torch.tensor(scale, device=DEV))
         assert torch.equal(got, own), scale
+
+
+# ------------------------------------------------------------------------------------ vocabularies in shards
+def _ranks(monkeypatch, n, work):
+    """``work(rank, group)`` on ``n`` threads of this process, with collectives between the threads on the host."""
+    import threading
+
+    from bridge_b200.ops import distill, token_logprob
+
+    barrier, slots, me = threading.Barrier(n, timeout=60), [None] * n, threading.local()
+
+    def everyone(t):
+        slots[me.rank] = t.clone()
+        barrier.wait()
+        got = list(slots)
+        barrier.wait()
+        return got
+
+    class Dist:
+        ReduceOp = torch.distributed.ReduceOp
+
+        @staticmethod
+        def get_world_size(group):
+            return n
+
+        @staticmethod
+        def all_reduce(t, op=torch.distributed.ReduceOp.SUM, group=None):
+            got = torch.stack(everyone(t))
+            t.copy_(got.amax(0) if op == torch.distributed.ReduceOp.MAX else got.sum(0))
+
+        @staticmethod
+        def all_gather(out, t, group=None):
+            for o, v in zip(out, everyone(t)):
+                o.copy_(v)
+
+    for module in (distill, token_logprob):
+        monkeypatch.setattr(module, "dist", Dist)
+    out, failed = [None] * n, []
+
+    def run(rank):
+        me.rank = rank
+        try:
+            out[rank] = work(rank, "threads")
+        except BaseException as exc:  # noqa: BLE001 - raised again below
+            failed.append(exc)
+            barrier.abort()
+
+    threads = [threading.Thread(target=run, args=(r,)) for r in range(n)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    if failed:
+        raise failed[0]
+    return out
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("temp", [0.9, "rows"])
+def test_scores_in_shards(monkeypatch, dtype, temp):
+    """The whole call on every rank, at the whole row's tolerance, with logits far from 0."""
+    rows, part, n = 40, 1501, 3
+    vocab = n * part
+    x = _logits(rows, vocab, dtype) + 60.0
+    x[4, part:2 * part] = -math.inf
+    x[5] = -math.inf
+    tokens = torch.randint(0, vocab, (rows, 2), device=DEV)
+    tokens[0, 1] = -1
+    t = 0.5 + torch.rand(rows, device=DEV) if temp == "rows" else temp
+    d, dh = torch.randn(rows, 2, device=DEV), torch.randn(rows, device=DEV)
+
+    def work(rank, group):
+        mine = x[:, rank * part:(rank + 1) * part].clone().requires_grad_()
+        r = _ops().token_logprobs(mine, tokens, t, top_k=20, vocab_start=rank * part, tp_group=group)
+        return r, torch.autograd.grad((r.logp, r.entropy), mine, (d, dh))[0]
+
+    got = _ranks(monkeypatch, n, work)
+    for r, _ in got:
+        _check_logp(r, x, tokens, t)
+        _check_top(r, x, t, 20)
+        assert r.logp.dtype == r.entropy.dtype == r.top_logp.dtype == torch.float32
+    size = ((d.abs().sum(1) + 32 * dh.abs()) / t)[:, None].double()
+    _check_grad(torch.cat([g for _, g in got], 1), oracle.token_grad(x, tokens, t, d, dh), size, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tail", [True, False])
+def test_distillation_in_shards(monkeypatch, dtype, tail):
+    """Loss and gradient on every rank, under a loss scale that was not announced; tolerances of the open form's test."""
+    rows, part, n = 20, 1001, 3
+    x = _logits(rows, n * part, dtype)
+    ids, logq = _teacher(rows, n * part, 9)
+    ids[1, 4:] = -1
+    w = torch.rand(rows, device=DEV) + 0.1
+
+    def work(rank, group):
+        mine = x[:, rank * part:(rank + 1) * part].clone().requires_grad_()
+        loss, kl = _ops().topk_distill_loss(mine, ids, logq, denom=4096.0, weights=w, temperature=0.9, tail=tail,
+                                            vocab_start=rank * part, tp_group=group)
+        return loss.detach(), kl, torch.autograd.grad(loss * 16384.0, mine)[0]
+
+    got = _ranks(monkeypatch, n, work)
+    kl_want, g_want = oracle.distill(x, ids, logq, 0.9, tail)
+    for loss, kl, _ in got:
+        _close(kl, kl_want, 1e-5, 2e-6, "rows")
+        _close(loss, (kl_want * w.double()).sum() / 4096.0, 1e-5, 2e-6, "loss")
+    f = (w.double() * 4.0)[:, None]
+    _check_grad(torch.cat([g for *_, g in got], 1), g_want * f, 4 * f, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_heads_in_shards(monkeypatch, dtype):
+    """Teacher alternatives and the student's loss through heads in shards against the whole head on one rank."""
+    ops = _ops()
+    h, W, *_ = _head(V=1200, dtype=dtype)
+    w = 0.2 + torch.rand(200, device=DEV)
+    whole = ops.fused_lm_head_token_logprobs(h, W, top_k=8, chunk_rows=64)
+
+    def student(Wr, group=None, start=0):
+        hr = h.clone().requires_grad_()
+        Wr = Wr.clone().requires_grad_()
+        Wr.main_grad = torch.zeros(Wr.shape, device=DEV)
+        loss, kl = ops.fused_lm_head_topk_distill(hr, Wr, whole.top_ids, whole.top_logp, denom=200.0, weights=w,
+                                                  chunk_rows=64, vocab_start=start, tp_group=group)
+        (loss * 0.5).backward()
+        return loss.detach(), kl, hr.grad, Wr.main_grad
+
+    Ws = (W.float() + 0.05 * torch.randn(W.shape, device=DEV)).to(dtype)
+    loss, kl, dh, dw = student(Ws)
+
+    def work(rank, group):
+        at = slice(rank * 400, (rank + 1) * 400)
+        r = ops.fused_lm_head_token_logprobs(h, W[at], top_k=8, chunk_rows=64, vocab_start=rank * 400, tp_group=group)
+        return r, student(Ws[at], group, rank * 400)
+
+    got = _ranks(monkeypatch, 3, work)
+    for r, s in got:
+        assert torch.equal(r.top_ids, whole.top_ids)
+        _close(r.top_logp, whole.top_logp, 4e-6, 1e-6, "teacher")
+        _close(s[0], loss, 1e-5, 4e-6, "loss")
+        _close(s[1], kl, 1e-5, 4e-6, "rows")
+    # (gradients in the logits' 16-bit type: a rounding each side of another sum)
+    _close(sum(s[2].float() for _, s in got), dh, 2.0 ** -6 * float(dh.abs().max()), 0.0, "dh")
+    _close(torch.cat([s[3] for _, s in got]), dw, 2.0 ** -6 * float(dw.abs().max()), 0.0, "dW")
