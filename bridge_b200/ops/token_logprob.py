@@ -309,11 +309,15 @@ def fused_lm_head_token_logprobs(h: Tensor, weight: Tensor, tokens: Tensor | Non
                                  vocab_start: int = 0, tp_group=None, chunk_rows: int = 4096) -> TokenLogprobs:
     """:func:`token_logprobs` of hidden rows ``h [U, H]`` under the head ``weight [V_local, H]``, scoring only
     (no gradient): the logits exist for ``chunk_rows`` rows at a time."""
+    name = "fused_lm_head_token_logprobs"
     if h.ndim != 2 or weight.ndim != 2 or h.shape[1] != weight.shape[1]:
-        raise ValueError(f"fused_lm_head_token_logprobs: h {tuple(h.shape)} does not fit the head "
-                         f"{tuple(weight.shape)}")
+        raise ValueError(f"{name}: h {tuple(h.shape)} does not fit the head {tuple(weight.shape)}")
     if chunk_rows < 1:
-        raise ValueError("fused_lm_head_token_logprobs: chunk_rows must be positive")
+        raise ValueError(f"{name}: chunk_rows must be positive")
+    if tokens is not None:
+        tokens = check_ids(name, "tokens", tokens, h.shape[0], h.device)
+    if isinstance(temperature, Tensor):
+        temperature = row_floats(name, "temperature", temperature, h.shape[0], h.device)
     parts = []
     for a in range(0, max(h.shape[0], 1), chunk_rows):
         at = slice(a, min(a + chunk_rows, h.shape[0]))

@@ -5,7 +5,8 @@ import math
 import pytest
 import torch
 
-from bridge_b200.ops import fused_lm_head_topk_distill, token_logprobs, topk_distill_loss
+from bridge_b200.ops import (fused_lm_head_token_logprobs, fused_lm_head_topk_distill, token_logprobs,
+                             topk_distill_loss)
 from tests import vocab_oracle as oracle
 from tests.test_vocab_rows_cpu import _case
 
@@ -230,3 +231,19 @@ def test_log_probs_keep_their_digits_far_from_zero():
     top, _ = oracle.token_logprobs(x, r.top_ids, 0.7)
     assert bool(((r.top_logp.double() - top).abs() <= 2e-6 + 5e-7 * top.abs()).all())
     assert bool(((r.entropy.double() - ent).abs() <= 4e-5).all())
+
+
+# -------------------------------------------------------------------------------------------- refusals
+def test_scoring_hidden_rows_checks_its_rows():
+    """One token and one temperature a row; more of them were cut off in silence."""
+    h, W = torch.randn(5, 16), torch.randn(30, 16)
+    for bad in (dict(tokens=torch.zeros(6, dtype=torch.long)), dict(tokens=torch.zeros(4, dtype=torch.long)),
+                dict(temperature=torch.ones(6)), dict(temperature=torch.ones(5, 1)),
+                dict(tokens=torch.zeros(5, 2, 2, dtype=torch.long))):
+        for chunk in (2, 3, 4096):
+            with pytest.raises(ValueError):
+                fused_lm_head_token_logprobs(h, W, chunk_rows=chunk, **bad)
+    with pytest.raises(TypeError):
+        fused_lm_head_token_logprobs(h, W, torch.zeros(5))
+    r = fused_lm_head_token_logprobs(h, W, torch.zeros(5, dtype=torch.long), torch.ones(5), chunk_rows=2)
+    assert r.logp.shape == (5,)
