@@ -35,8 +35,8 @@ from torch import Tensor
 
 from ._ext import kernels, on_gpu
 from .gemm import gemm
-from .token_logprob import (MAX_TOP, _LN2, _MASKED, check_ids, check_logits, first_order, join_shards, log2_scale, picked,
-                            row_floats, shard_sums, split_temperature, tp_world, unit_columns)
+from .token_logprob import (MAX_TOP, _LN2, _MASKED, check_ids, check_logits, check_shard, first_order, join_shards,
+                            log2_scale, picked, row_floats, shard_sums, split_temperature, tp_world, unit_columns)
 
 
 _RESIDUE = 2.0 ** -18      # of a teacher's probability that FP32 log-probs may leave by rounding
@@ -285,12 +285,13 @@ def topk_distill_loss(logits: Tensor, teacher_ids: Tensor, teacher_logp: Tensor,
     can be called once.  With ``tp_group``, ``logits`` is this rank's
     equal shard of the vocabulary and ``vocab_start`` its first token.
     """
-    if tp_group is None and on_gpu(logits):
+    if tp_group is None and not vocab_start and on_gpu(logits):
         got = _own(logits, teacher_ids, teacher_logp, weights, temperature, tail, denom, grad_scale)
         if got:                                   # arguments that the kernels take as they are
             return got[0], got[1]
     name = "topk_distill_loss"
     check_logits(name, logits)
+    check_shard(name, vocab_start, tp_group)
     args = _arguments(name, logits.shape[0], logits.device, teacher_ids, teacher_logp, weights, temperature, denom,
                       grad_scale)
     logits = unit_columns(logits)
@@ -326,6 +327,7 @@ def fused_lm_head_topk_distill(h: Tensor, weight: Tensor, teacher_ids: Tensor, t
         raise ValueError(f"{name}: h {tuple(h.shape)} does not fit the head {tuple(weight.shape)}")
     if chunk_rows < 1:
         raise ValueError(f"{name}: chunk_rows must be positive")
+    check_shard(name, vocab_start, tp_group)
     args = _arguments(name, h.shape[0], h.device, teacher_ids, teacher_logp, weights, temperature, denom, grad_scale)
     if on_gpu(h):
         return _FusedHeadDistillFn.apply(h.contiguous(), weight, *args, bool(tail), float(denom), float(grad_scale),

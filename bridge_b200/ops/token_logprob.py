@@ -53,6 +53,12 @@ def tp_world(group) -> int:
     return 1 if group is None else dist.get_world_size(group)
 
 
+def check_shard(name: str, vocab_start: int, group) -> None:
+    if vocab_start and tp_world(group) == 1:
+        raise ValueError(f"{name}: vocab_start {vocab_start} says that this is a shard of the vocabulary, which needs "
+                         "tp_group")
+
+
 def check_logits(name: str, logits: Tensor) -> None:
     if logits.ndim != 2 or logits.shape[1] < 1:
         raise ValueError(f"{name}: logits must be [U, V] with V >= 1, got {tuple(logits.shape)}")
@@ -266,14 +272,15 @@ def token_logprobs(logits: Tensor, tokens: Tensor | None = None, temperature: Te
 
     ``temperature`` is one positive number or ``[U]``; ``top_k`` (at most 256) also returns the likeliest
     tokens.  With ``tp_group``, ``logits`` is this rank's equal shard of the vocabulary, whose first token
-    is ``vocab_start``; every rank gets the whole result and its shard's gradient.
+    is ``vocab_start`` (0 without a group); every rank gets the whole result and its shard's gradient.
     """
-    if tp_group is None and on_gpu(logits):
+    if tp_group is None and not vocab_start and on_gpu(logits):
         got = _own(logits, tokens, temperature, top_k, with_entropy)
         if got:                                   # arguments that the kernels take as they are
             return TokenLogprobs(*got)
     name = "token_logprobs"
     check_logits(name, logits)
+    check_shard(name, vocab_start, tp_group)
     rows, device = logits.shape[0], logits.device
     world = tp_world(tp_group)
     total = logits.shape[1] * world

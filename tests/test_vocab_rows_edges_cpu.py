@@ -247,3 +247,15 @@ def test_scoring_hidden_rows_checks_its_rows():
         fused_lm_head_token_logprobs(h, W, torch.zeros(5))
     r = fused_lm_head_token_logprobs(h, W, torch.zeros(5, dtype=torch.long), torch.ones(5), chunk_rows=2)
     assert r.logp.shape == (5,)
+
+
+def test_a_shard_needs_its_group():
+    """A first token other than 0 says that the logits are a shard, whose rows mean nothing alone."""
+    x, tokens, ids = torch.randn(3, 20), torch.tensor([21, 22, 23]), torch.tensor([[21, 24]] * 3)
+    logq, h, W = torch.full((3, 2), -1.5), torch.randn(3, 16), torch.randn(20, 16)
+    for call in (lambda: token_logprobs(x, tokens, vocab_start=20),
+                 lambda: topk_distill_loss(x, ids, logq, denom=3.0, vocab_start=20),
+                 lambda: fused_lm_head_token_logprobs(h, W, tokens, vocab_start=20),
+                 lambda: fused_lm_head_topk_distill(h, W, ids, logq, denom=3.0, vocab_start=20)):
+        with pytest.raises(ValueError, match="vocab_start"):
+            call()

@@ -383,3 +383,16 @@ def test_heads_in_shards(monkeypatch, dtype):
     # (gradients in the logits' 16-bit type: a rounding each side of another sum)
     _close(sum(s[2].float() for _, s in got), dh, 2.0 ** -6 * float(dh.abs().max()), 0.0, "dh")
     _close(torch.cat([s[3] for _, s in got]), dw, 2.0 ** -6 * float(dw.abs().max()), 0.0, "dW")
+
+
+def test_a_shard_needs_its_group():
+    ops = _ops()
+    x, tokens = torch.randn(3, 64, device=DEV).bfloat16(), torch.tensor([71, 72, 73], device=DEV)
+    ids, logq = _teacher(3, 64, 2)
+    h, W = torch.randn(3, 64, device=DEV).bfloat16(), torch.randn(64, 64, device=DEV).bfloat16()
+    for call in (lambda: ops.token_logprobs(x, tokens, vocab_start=64),
+                 lambda: ops.topk_distill_loss(x, ids, logq, denom=3.0, vocab_start=64),
+                 lambda: ops.fused_lm_head_token_logprobs(h, W, tokens, vocab_start=64),
+                 lambda: ops.fused_lm_head_topk_distill(h, W, ids, logq, denom=3.0, vocab_start=64)):
+        with pytest.raises(ValueError, match="vocab_start"):
+            call()
