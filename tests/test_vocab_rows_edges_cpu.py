@@ -8,7 +8,7 @@ import torch
 from bridge_b200.ops import (fused_lm_head_token_logprobs, fused_lm_head_topk_distill, token_logprobs,
                              topk_distill_loss)
 from tests import vocab_oracle as oracle
-from tests.test_vocab_rows_cpu import _case
+from tests.dist_utils import run_ranks
 
 
 def test_rows_of_finite_masks_carry_nothing():
@@ -259,3 +259,37 @@ def test_a_shard_needs_its_group():
                  lambda: fused_lm_head_topk_distill(h, W, ids, logq, denom=3.0, vocab_start=20)):
         with pytest.raises(ValueError, match="vocab_start"):
             call()
+
+
+# ------------------------------------------------------------------------------- tensor-parallel models
+def _model_worker(rank, world):
+    import torch.distributed as dist
+
+    from bridge_b200.models import build_model, get_config
+    from bridge_b200.rl import distill_loss, teacher_alternatives
+
+    cfg = get_config("tiny")
+    teacher, student = (build_model(cfg, seed=s, tp_group=dist.group.WORLD, dtype=torch.float32) for s in (1, 2))
+    g = torch.Generator().manual_seed(0)
+    h = torch.randn(9, cfg.hidden_size, generator=g).requires_grad_()
+    ids, logp = teacher_alternatives(teacher, h.detach(), top_k=12, temperature=0.8)
+    loss, rows = distill_loss(student, h, ids, logp, denom=9.0, temperature=0.8)
+    (3.0 * loss).backward()
+    return [v.detach().tolist() for v in (teacher.head_weight, student.head_weight, h, ids, logp, loss, rows, h.grad,
+                                          student.head_weight.grad)]
+
+
+def test_distillation_of_tensor_parallel_models():
+    """Every rank of two vocabulary-parallel models gets the whole alternatives, loss and ``dh``, and its head's part."""
+    ranks = [[torch.tensor(v) for v in r] for r in run_ranks(2, _model_worker)]
+    wt, ws = (torch.cat([r[i] for r in ranks]).double() for i in (0, 1))
+    h = ranks[0][2].double()
+    ids = oracle.top(h @ wt.t(), 12)
+    logq = oracle.token_logprobs(h @ wt.t(), ids, 0.8)[0]
+    kl, gx = oracle.distill(h @ ws.t(), ids, logq, 0.8, True)
+    gx = gx * 3.0 / 9.0
+    for r in ranks:
+        assert torch.equal(r[3], ids) and torch.allclose(r[4].double(), logq, atol=1e-5)
+        assert torch.allclose(r[5].double(), kl.mean(), atol=1e-5) and torch.allclose(r[6].double(), kl, atol=1e-5)
+        assert torch.allclose(r[7].double(), gx @ ws, atol=1e-5)
+    assert torch.allclose(torch.cat([r[8] for r in ranks]).double(), gx.t() @ h, atol=1e-5)

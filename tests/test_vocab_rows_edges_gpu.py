@@ -396,3 +396,71 @@ def test_a_shard_needs_its_group():
                  lambda: ops.fused_lm_head_topk_distill(h, W, ids, logq, denom=3.0, vocab_start=64)):
         with pytest.raises(ValueError, match="vocab_start"):
             call()
+
+
+# ------------------------------------------------------------------------------------- every column's gradient
+def _check_columns(got, want, bound, dtype):
+    """`bound` of every element, before the rounding to the type."""
+    limit = bound + 1.01 * ROUND[dtype] * want.abs() + TINY[dtype]
+    off = (got.double() - want).abs()
+    assert bool((off <= limit).all()), (float((off / limit).max()), torch.nonzero(off > limit)[0].tolist())
+    assert float(((got == 0) & (want.abs() > 4 * TINY[dtype])).double().mean()) == 0.0
+
+
+def _long_rows(rows, vocab, dtype, kind, view):
+    x = _logits(rows, vocab + 9, dtype, seed=vocab + rows, spread=3.0 if kind == "spread" else 0.05)
+    if kind == "flat":
+        x = (x.float() * 0.1).to(dtype)
+    return x[:, 9:] if view == "offset" else x[:, :vocab].contiguous()
+
+
+COLUMNS = [(3, 151936), (40, 60013), (260, 50021), (700, 20011), (5, 1003)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind,view", [("flat", "whole"), ("spread", "whole"), ("flat", "offset")])
+@pytest.mark.parametrize("rows,vocab", COLUMNS)
+def test_every_column_of_the_scores_gradient(rows, vocab, dtype, kind, view):
+    """An element is p times factors: t = x c - R to 2 x 2^-24 |t|, |t| <= 60, makes e right to 5e-6; the exponential, 1 / s
+    and four products add 3e-6.  The entropy's factor ln p + H is right to that of its two terms and 4e-5."""
+    x = _long_rows(rows, vocab, dtype, kind, view).requires_grad_()
+    g = torch.Generator(device=DEV).manual_seed(4)
+    tokens = torch.randint(0, vocab, (rows, 2), device=DEV, generator=g)
+    up = 4096.0 if dtype == torch.float16 else 1.0
+    d, dh = (up * torch.randn(rows, 2, device=DEV, generator=g), up * torch.randn(rows, device=DEV, generator=g))
+    r = _ops().token_logprobs(x, tokens, 0.9)
+    (got,) = torch.autograd.grad((r.logp, r.entropy), x, (d, dh))
+    want = oracle.token_grad(x.detach(), tokens, 0.9, d, dh)
+    logp = oracle.log_softmax(oracle.scaled(x.detach(), 0.9))
+    p, D, H = logp.exp(), d.double().abs(), dh.double().abs()[:, None]
+    terms = 8e-6 * (D.sum(1, keepdim=True) + H * (logp.abs() - (p * logp).sum(1, keepdim=True))) + 4e-5 * H
+    bound = (p * terms).scatter_add_(1, tokens, D * 2.0 ** -22) / 0.9
+    _check_columns(got, want, bound, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind,view", [("flat", "whole"), ("spread", "whole"), ("flat", "offset")])
+@pytest.mark.parametrize("rows,vocab", COLUMNS)
+@pytest.mark.parametrize("tail", [True, False])
+def test_every_column_of_the_distillation_gradient(rows, vocab, dtype, kind, view, tail):
+    """Outside the entries (Q - q_r / p_r) p, its parts as right as those of the scores' gradient; on them Q p - q."""
+    x = _long_rows(rows, vocab, dtype, kind, view).requires_grad_()
+    ids, logq = _teacher(rows, vocab, 24)
+    up = 4096.0 if dtype == torch.float16 else 1.0
+    loss, _ = _ops().topk_distill_loss(x, ids, logq, denom=1.0, temperature=0.9, tail=tail, grad_scale=up)
+    (got,) = torch.autograd.grad(loss, x, torch.tensor(up, device=DEV))
+    _, want = oracle.distill(x.detach(), ids, logq, 0.9, tail)
+    p = oracle.log_softmax(oracle.scaled(x.detach(), 0.9)).exp()
+    q = torch.zeros_like(p).scatter_(1, ids, logq.double().exp())
+    if tail:
+        rest = p.scatter(1, ids, 0.0).sum(1, keepdim=True)
+        factor = 1.0 + (1.0 - q.sum(1, keepdim=True)) / rest
+    else:
+        q, factor = q / q.sum(1, keepdim=True), 1.0
+    _check_columns(got, want * up, 8e-6 * up * (p * factor + q) / 0.9, dtype)
+    if view == "whole" and dtype != torch.float16:
+        from bridge_b200.ops._ext import kernels
+
+        own = x.detach().clone()
+        kernels().distill_rows_inplace(own, ids, logq, None, None, 0.9, 1.0, tail, True)
+        assert torch.equal(own, got)
