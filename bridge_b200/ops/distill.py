@@ -15,9 +15,9 @@ The gradient of every row is known as soon as its statistics are, so the forward
 backward only checks that the loss was scaled by ``grad_scale`` as announced, and rescales otherwise (FP16
 gradients are written again from the logits, which they keep for that: scaling what was rounded at another
 scale would lose it).  Vocabularies in shards write theirs in the backward.
-:func:`fused_lm_head_topk_distill` goes on to the LM head's own backward inside the forward and keeps
-``dh`` and, in FP32, ``dW`` for a factor that only the backward knows: a forward that is run again, or never
-followed by a backward, changes no gradient.
+:func:`fused_lm_head_topk_distill` goes on to the LM head's own backward inside the forward and keeps what a
+factor that only the backward knows is still to come to: a forward that is run again, or never followed by a
+backward, changes no gradient.
 
 Rows of weight 0 and rows without an entry have divergence 0 and gradient 0 whatever their logits hold.
 A given token (``q_j > 0``) without student probability makes the divergence infinite, and so does a
@@ -173,10 +173,14 @@ class _TopkDistillFn(torch.autograd.Function):
 
 
 class _FusedHeadDistillFn(torch.autograd.Function):
-    """LM head + divergence with the head's backward inside the forward (see the module docstring).
+    """LM head + divergence with the head's backward as far inside the forward as the loss's factor allows.
 
-    FP16 heads run it in the backward, on the chunks' logits computed again: there only the loss's own factor
-    says at which scale a gradient may be rounded."""
+    ``dh`` is made in the forward and scaled in the backward.  For ``dW`` few rows keep their chunks'
+    gradients, whose product with ``h`` the backward adds to ``main_grad`` itself; where these would be larger
+    than an FP32 ``dW``, that is summed in the forward and added with the factor (4096 rows, H 2560, vocabulary
+    151936, BF16, forward and backward: 8.6 to 8.8 ms kept as chunks, 9.7 to 10.7 ms summed).  FP16 heads do
+    all of it in the backward, on the chunks' logits computed again: there only the loss's own factor says at
+    which scale a gradient may be rounded."""
 
     @staticmethod
     def forward(ctx, h, weight, ids, logq, weights, temp, temp1, tail, denom, grad_scale, vocab_start, group,
@@ -185,8 +189,9 @@ class _FusedHeadDistillFn(torch.autograd.Function):
         want_dh, want_dw = (differentiable and n for n in ctx.needs_input_grad[:2])
         late = h.dtype == torch.float16 and (want_dh or want_dw)
         want = not late and (want_dh or want_dw)
-        dh, dw = _head_gradients(h, weight, want and want_dh, want and want_dw)
-        parts = []
+        keep = want and want_dw and h.shape[0] * h.element_size() <= 4 * h.shape[1]
+        dh, dw = _head_gradients(h, weight, want and want_dh, want and want_dw and not keep)
+        parts, kept = [], []
         for at in _chunks(h, chunk_rows):
             lg = gemm(h[at], weight)
             teacher = (ids[at], logq[at], None if weights is None else weights[at], None if temp is None else temp[at],
@@ -199,15 +204,17 @@ class _FusedHeadDistillFn(torch.autograd.Function):
                 if want:
                     dlg = _grad(lg, ids[at], *parts[-1][1:], *teacher[3:5], vocab_start, group, inplace=True)
             if want:
-                _head_backward(dlg, h, weight, at, dh, dw)
+                _head_backward(dlg, h[at], weight, None if dh is None else dh[at], dw)
+            if keep:
+                kept.append(dlg)
         rows = torch.cat([p[0] for p in parts]) if parts else torch.zeros(0, dtype=torch.float32, device=h.device)
-        if late and parts:
+        ctx.late = (temp1, vocab_start, group) if late and parts else None
+        if ctx.late:
             coef, fix = (torch.cat([p[i] for p in parts]) for i in (1, 2))
             ctx.save_for_backward(h, weight, ids, coef, fix, temp)
         else:
-            ctx.save_for_backward(dh, dw)
-        ctx.late = (temp1, vocab_start, group, chunk_rows) if late and parts else None
-        ctx.grad_scale, ctx.dtype = grad_scale, weight.dtype
+            ctx.save_for_backward(dh, dw, h if kept else None, *kept)
+        ctx.grad_scale, ctx.chunk_rows, ctx.weight = grad_scale, chunk_rows, (weight.shape, weight.dtype)
         ctx.main_grad = getattr(weight, "main_grad", None)
         ctx.mark_non_differentiable(rows)
         return _weighted_sum(rows, weights, denom), rows
@@ -215,25 +222,34 @@ class _FusedHeadDistillFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dloss, _drows):
         first_order("fused_lm_head_topk_distill")
-        f = dloss.float() / ctx.grad_scale
-        if ctx.late is None:
-            dh, dw = ctx.saved_tensors
-            if dh is not None:
-                dh = (dh.float() * f).to(dh.dtype)
-        else:
+        f, main, (shape, dtype) = dloss.float() / ctx.grad_scale, ctx.main_grad, ctx.weight
+        direct = main is not None and main.dtype == torch.float32      # a sum that products can be added to
+        if ctx.late:
             h, weight, ids, coef, fix, temp = ctx.saved_tensors
-            temp1, vocab_start, group, chunk_rows = ctx.late
-            dh, dw = _head_gradients(h, weight, *ctx.needs_input_grad[:2])
-            for at in _chunks(h, chunk_rows):
+            temp1, vocab_start, group = ctx.late
+            dh, dw = _head_gradients(h, weight, ctx.needs_input_grad[0], ctx.needs_input_grad[1] and not direct)
+            for at in _chunks(h, ctx.chunk_rows):
                 dlg = _grad(gemm(h[at], weight), ids[at], coef[at], fix[at], None if temp is None else temp[at], temp1,
                             vocab_start, group, factor=f, inplace=True)
-                _head_backward(dlg, h, weight, at, dh, dw)
+                _head_backward(dlg, h[at], weight, None if dh is None else dh[at],
+                               main if direct and ctx.needs_input_grad[1] else dw)
             f = torch.ones_like(f)
-        if dw is not None and ctx.main_grad is not None:
-            ctx.main_grad.addcmul_(dw.to(ctx.main_grad.dtype), f.to(ctx.main_grad.dtype))
+        else:
+            dh, dw, h, *kept = ctx.saved_tensors
+            if dh is not None:
+                dh = (dh.float() * f).to(dh.dtype)
+            if kept:
+                if not direct:
+                    dw = torch.zeros(shape, dtype=torch.float32, device=h.device)
+                hf = (h.float() * f).to(h.dtype)       # (rounded as dh is; exact for the announced factor)
+                for at, dlg in zip(_chunks(h, ctx.chunk_rows), kept):
+                    _head_backward(dlg, hf[at], None, None, main if direct else dw)
+                f = torch.ones_like(f)
+        if dw is not None and main is not None:
+            main.addcmul_(dw.to(main.dtype), f.to(main.dtype))
             dw = None
         elif dw is not None:
-            dw = (dw * f).to(ctx.dtype)
+            dw = (dw * f).to(dtype)
         return (dh, dw) + (None,) * 12
 
 
@@ -246,11 +262,11 @@ def _head_gradients(h, weight, want_dh, want_dw):
             torch.zeros(weight.shape, dtype=torch.float32, device=weight.device) if want_dw else None)
 
 
-def _head_backward(dlg, h, weight, at, dh, dw):
+def _head_backward(dlg, h, weight, dh, dw):
     if dh is not None:
-        dh[at] = gemm(dlg, weight, b_mn=True)                          # dlogits @ W
+        dh.copy_(gemm(dlg, weight, b_mn=True))                         # dlogits @ W
     if dw is not None:
-        gemm(dlg, h[at], a_mn=True, b_mn=True, out=dw, accumulate=True)      # += dlogits^T h
+        gemm(dlg, h, a_mn=True, b_mn=True, out=dw, accumulate=True)    # += dlogits^T h
 
 
 # ------------------------------------------------------------------------------------------------- API
@@ -318,9 +334,10 @@ def fused_lm_head_topk_distill(h: Tensor, weight: Tensor, teacher_ids: Tensor, t
                                chunk_rows: int = 4096) -> tuple[Tensor, Tensor]:
     """:func:`topk_distill_loss` of hidden rows ``h [U, H]`` under the head ``weight [V_local, H]``.
 
-    The logits exist for ``chunk_rows`` rows at a time and become their own gradient in place.  ``dW`` is summed
-    in FP32 and kept for the backward, which adds it to ``weight.main_grad`` where there is one.  FP16 heads compute
-    the logits once more in the backward instead, so that only scaled gradients are rounded.
+    The logits exist for ``chunk_rows`` rows at a time and become their own gradient in place.  Until the
+    backward, which adds ``dW`` to ``weight.main_grad`` where there is one, these chunks are kept, or their sum
+    ``dW`` in FP32, whichever is smaller; a ``grad_scale`` other than the loss's own factor costs ``dh`` and ``dW``
+    one more rounding.  FP16 heads compute the logits once more in the backward instead.
     """
     name = "fused_lm_head_topk_distill"
     if h.ndim != 2 or weight.ndim != 2 or h.shape[1] != weight.shape[1]:

@@ -293,3 +293,21 @@ def test_distillation_of_tensor_parallel_models():
         assert torch.allclose(r[5].double(), kl.mean(), atol=1e-5) and torch.allclose(r[6].double(), kl, atol=1e-5)
         assert torch.allclose(r[7].double(), gx @ ws, atol=1e-5)
     assert torch.allclose(torch.cat([r[8] for r in ranks]).double(), gx.t() @ h, atol=1e-5)
+
+
+@pytest.mark.parametrize("main", [True, False])
+@pytest.mark.parametrize("rows", [1, 16, 17, 40])
+@pytest.mark.parametrize("chunk", [7, 64])
+def test_head_gradients_kept_either_way(monkeypatch, main, rows, chunk):
+    """Few rows keep the chunks' gradients for the backward (up to 16 of FP32 here), many the weight's."""
+    _stand_in(monkeypatch)
+    h, W, ids, logq = _head(U=rows)
+    if main:
+        W.main_grad = torch.full(W.shape, 2.0)
+    loss, _ = fused_lm_head_topk_distill(h, W, ids, logq, denom=float(rows), chunk_rows=chunk)
+    assert not main or bool((W.main_grad == 2.0).all())
+    (loss * 0.3).backward()
+    dh, dw = _head_gradients(h, W, ids, logq, 0.3)
+    got = W.main_grad - 2.0 if main else W.grad
+    assert torch.allclose(h.grad.double(), dh, atol=1e-5, rtol=1e-4)
+    assert torch.allclose(got.double(), dw, atol=1e-5, rtol=1e-4)

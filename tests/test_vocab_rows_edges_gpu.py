@@ -464,3 +464,25 @@ def test_every_column_of_the_distillation_gradient(rows, vocab, dtype, kind, vie
         own = x.detach().clone()
         kernels().distill_rows_inplace(own, ids, logq, None, None, 0.9, 1.0, tail, True)
         assert torch.equal(own, got)
+
+
+@pytest.mark.parametrize("main", [True, False])
+@pytest.mark.parametrize("rows", [1, 200, 256, 257, 700])
+def test_head_gradients_kept_either_way(main, rows):
+    """Up to 2 H = 256 rows of BF16 keep the chunks' gradients for the backward, more of them the weight's."""
+    h, W, ids, logq, w = _head(U=rows)
+    h.requires_grad_()
+    W.requires_grad_()
+    if main:
+        W.main_grad = torch.full(W.shape, 2.0, device=DEV)
+    loss, _ = _ops().fused_lm_head_topk_distill(h, W, ids, logq, denom=float(rows), weights=w, chunk_rows=96)
+    assert not main or bool((W.main_grad == 2.0).all())
+    (loss * 0.3).backward(retain_graph=True)
+    loss.backward()
+    hd, Wd = h.detach().double(), W.detach().double()
+    _, gx = oracle.distill(hd @ Wd.t(), ids, logq, 1.0, True)
+    gx = gx * w.double()[:, None] * 1.3 / rows
+    dh, dw = gx @ Wd, gx.t() @ hd
+    got = W.main_grad - 2.0 if main else W.grad
+    _close(h.grad, dh, 2e-2 * float(dh.abs().max()), 5e-2, "dh")
+    _close(got, dw, 2e-2 * float(dw.abs().max()), 5e-2, "dW")
