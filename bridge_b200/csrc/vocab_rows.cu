@@ -20,10 +20,10 @@
 // What bounds them: reading the row.  8 BF16 logits cost 16 bytes, 8 exponentials (half a cycle of an SM) and about
 // 40 instructions a pass, which at 6.4 TB/s is two thirds of what the SMs can issue, so the loops are kept lean (paired
 // FP32 instructions, no checks inside a row) and everything that is per row overlaps other blocks' streaming.  B200,
-// vocabulary 151936, BF16, device time: scoring 4096 rows with entropy 0.20 ms (6.2 TB/s; 0.22 ms, 5.7 TB/s, under a
-// sustained power cap), 1024 rows with 64 alternatives 0.079 ms; gradient of the scores 0.21 ms for 2048 rows (6.0 TB/s);
-// distillation loss 0.061 ms for 1024 rows, loss and gradient 0.48 ms for 4096 (5.2 TB/s of one read and one write);
-// one row with 20 alternatives 9 us, 8 rows of distillation with gradient 12 us.
+// vocabulary 151936, BF16, device time: scoring 4096 rows with entropy 0.20 ms (6.1 TB/s at full clocks; 0.23 ms, 5.4 TB/s,
+// among other calls under a sustained power cap), 1024 rows with 64 alternatives 0.076 ms; gradient of the scores 0.21 ms
+// for 2048 rows (6.0 TB/s); distillation loss 0.059 ms for 1024 rows, loss and gradient 0.48 ms for 4096 (5.2 TB/s of one
+// read and one write); one row with 20 alternatives 9 us, 8 rows of distillation with gradient 15 us in three launches.
 #include "vocab_rows.h"
 
 #include <c10/util/Exception.h>
@@ -300,9 +300,9 @@ __device__ __forceinline__ double warp_max_d(double v) {
 // what was read late is the likeliest to be in L2.  A warp barrier orders the reads of a batch's slots before the copies
 // that refill them.
 //
-// 3 groups of 8 KB for 8 warps are 48 KB a block, 4 blocks an SM.  Scoring 4096 x 151936 BF16: 194 us against 267 us for
-// plain loads, one unit in flight per thread.  Second pass of distillation, 4096 rows: 593 us in reverse order with the
-// stores and last reads marked evict-first, 627 us in the order of the first pass without hints.
+// 3 groups of 16 KB for 8 warps are 48 KB a block, 4 blocks an SM.  Distillation with gradient of 4096 x 151936 BF16, each
+// step alone: 627 us with plain loads, the second pass in the order of the first; 593 us in reverse order with the stores
+// and last reads marked evict-first; 533 us with the copies.
 constexpr int kBatch = 4, kGroups = 3, kSpan = 32 * kBatch;
 static_assert(kBatch == 4, "a batch is written out unit by unit");
 

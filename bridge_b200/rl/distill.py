@@ -28,8 +28,8 @@ def teacher_alternatives(model, hidden_rows: Tensor, *, top_k: int, temperature:
 def distill_loss(model, hidden_rows: Tensor, teacher_ids: Tensor, teacher_logp: Tensor, *, denom: float,
                  weights: Tensor | None = None, temperature: Tensor | float = 1.0, tail: bool = True,
                  grad_scale: float = 1.0, chunk_rows: int = 4096) -> tuple[Tensor, Tensor]:
-    """``(sum_u w_u KL_u / denom, KL [U])`` of the student at ``hidden_rows``; ``grad_scale`` announces the factor
-    by which the caller multiplies the loss before ``backward``."""
+    """``(sum_u w_u KL_u / denom, KL [U])`` of the student at ``hidden_rows``; any factor on the loss is
+    right; one that ``grad_scale`` announces saves a rounding of the gradients."""
     return fused_lm_head_topk_distill(model.head_input(hidden_rows), model.head_weight, teacher_ids, teacher_logp,
                                       denom=denom, weights=weights, temperature=temperature, tail=tail,
                                       grad_scale=grad_scale, vocab_start=model.vocab_start, tp_group=model.tp_group,
