@@ -8,7 +8,8 @@
 // given tokens' shares) are FP64.
 //
 // A logit with x c <= -2^31 (-inf, the type's lowest value, any customary finite mask from -1e10 down) carries no
-// probability; a row without any other has log-probs -inf, entropy 0 and gradient 0.  The bound is where FP32 ends: R is
+// probability; a row without any other has log-probs -inf, entropy 0 and gradient 0.  (In a row with others its own
+// log-prob is what the fill makes it, and -inf from x c = -1e30 down.)  The bound is where FP32 ends: R is
 // rounded, so t at the largest logit can be off 0 by half a unit of R's last place, 64 for |R| < 2^31 (2^64 V is still a
 // number) and hundreds above, where a thread that sees nothing but a mask of -1e10 would sum to infinity.  A row with
 // x c > 2^31 is NaN, as with an infinite logit.
@@ -47,7 +48,8 @@ constexpr int kThreads = 512;   // at most, per block that holds its slice
 constexpr int kStream = 256;    // per block that streams it
 constexpr int kMaxCluster = 8;
 constexpr int kCand = 2048;     // candidates of the selection kept in shared memory
-constexpr float kMasked = -2147483648.f;      // -2^31, of x c
+constexpr float kFloor = -2147483648.f;       // -2^31, of x c: least reference of a sum
+constexpr float kMasked = -1e30f;             // of x c: as good as -inf
 constexpr float kOverflow = -1e29f;           // x c below this may be -inf
 constexpr float kSlack = 8.f;
 constexpr double kLn2 = 0.69314718055994530942;
@@ -213,7 +215,7 @@ struct Slice {
 struct Stat {
   float R, s, et;
 
-  static __device__ __forceinline__ Stat none() { return {kMasked, 0.f, 0.f}; }
+  static __device__ __forceinline__ Stat none() { return {kFloor, 0.f, 0.f}; }
   __device__ __forceinline__ void raise(float to) {
     const float d = R - to, k = ex2(d);
     et = k * (et + d * s);
@@ -223,14 +225,14 @@ struct Stat {
 };
 
 // The reference for a largest x c of `top`.
-__device__ __forceinline__ float reference(float top) { return top > -kMasked ? NAN : fmaxf(top, kMasked); }
+__device__ __forceinline__ float reference(float top) { return top > -kFloor ? NAN : fmaxf(top, kFloor); }
 
 // A thread's running sums, two FP32 lanes to an instruction.
 struct Sums {
   float R;
   float2 s, et;
 
-  __device__ __forceinline__ Sums() : R(kMasked), s(both(0.f)), et(both(0.f)) {}
+  __device__ __forceinline__ Sums() : R(kFloor), s(both(0.f)), et(both(0.f)) {}
   __device__ __forceinline__ void raise(float to) {
     const float d = R - to, k = ex2(d);
     et = __fmul2_rn(both(k), __ffma2_rn(both(d), s, et));
@@ -1102,7 +1104,7 @@ __device__ __forceinline__ Finished finish_row(const Teacher& t, Stat rest, bool
   const bool out = rest.s != 0.f, in = t.z != 0.0;      // student probability outside and on the entries
   const double Rd = out ? (double)rest.R : -INFINITY, md = in ? t.m : -INFINITY;
   const double m = fmax(Rd, md);
-  const bool lost = m == -INFINITY;                     // none anywhere
+  const bool lost = m <= (double)kFloor;                // none anywhere
   const double m0 = lost ? 0.0 : m;
   const double s = out ? (double)rest.s : 1.0;
   const double left = tail ? fmax(0.0, 1.0 - t.q) : 0.0, q_rest = out || left > kResidue ? left : 0.0, total = tail ? t.q + q_rest : 1.0;

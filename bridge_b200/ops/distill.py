@@ -35,8 +35,8 @@ from torch import Tensor
 
 from ._ext import kernels, on_gpu
 from .gemm import gemm
-from .token_logprob import (MAX_TOP, _LN2, _MASKED, check_ids, check_logits, check_shard, first_order, join_shards,
-                            log2_scale, picked, row_floats, shard_sums, split_temperature, tp_world, unit_columns)
+from .token_logprob import (MAX_TOP, _FLOOR, _LN2, _MASKED, check_ids, check_logits, check_shard, first_order,
+                            join_shards, log2_scale, picked, row_floats, shard_sums, split_temperature, tp_world, unit_columns)
 
 
 _RESIDUE = 2.0 ** -18      # of a teacher's probability that FP32 log-probs may leave by rounding
@@ -78,7 +78,7 @@ def _finish_reference(stats, xc, ids, logq, weights, temp, temp1, scale, tail, t
     xc = torch.where(xc <= _MASKED, none, xc)
     r = torch.where(stats[:, 1] == 0, none[:, 0], stats[:, 0]) if logq.shape[1] else stats[:, 0]
     m = torch.maximum(r, torch.where(first, xc, none).amax(dim=1))
-    lost = m == -math.inf                                        # no student probability anywhere
+    lost = m <= _FLOOR                                           # no student probability anywhere
     m = torch.where(lost, torch.zeros_like(m), m)
     rest = torch.where(stats[:, 1] == 0, torch.zeros_like(m), stats[:, 1] * torch.exp2(r - m))
     z = torch.where(first, torch.exp2(xc - m[:, None]), torch.zeros_like(xc)).sum(dim=1) + rest

@@ -15,7 +15,7 @@ as a teacher.
 Edge cases: a token outside the vocabulary (a padded position) has log-prob 0 and no gradient.  A logit
 of ``-inf``, or one with ``x / T`` at or below ``-2^31 ln 2`` (-1.49e9: FP32's lowest value, finite masks
 from -1e10 down), carries no probability; where a row holds nothing else its log-probs are ``-inf``, its
-entropy 0 and its gradient 0.  NaN, ``+inf`` or ``x / T`` above 1.49e9 in a row makes its log-probs and
+entropy 0 and its gradient 0 (in other rows a finite fill has its own log-prob).  NaN, ``+inf`` or ``x / T`` above 1.49e9 in a row makes its log-probs and
 entropy NaN (among the alternatives NaN counts as ``-inf``).  Subnormal logits count as 0.  There is a first derivative
 only: a backward with ``create_graph=True`` and forward-mode inputs are refused.
 """
@@ -35,7 +35,8 @@ from .gemm import gemm
 MAX_TOP = 256
 _LN2 = math.log(2.0)
 _LOG2E = 1.0 / _LN2
-_MASKED = -2.0 ** 31       # log2-domain logits at or below this carry no probability
+_FLOOR = -2.0 ** 31        # log2-domain logits at or below this carry no probability
+_MASKED = -1e30            # ... and at or below this are as good as -inf
 _FLOAT_TYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
@@ -118,9 +119,9 @@ def _exact_scale(temp: Tensor | None, temp1: float, device, own: bool) -> Tensor
 
 def shard_sums(xc: Tensor) -> tuple[Tensor, Tensor, Tensor]:
     """``(R, s, sum e t)`` of log2-domain rows: ``t = xc - R``, ``e = 2^t``; masked columns count nothing."""
-    r = xc.amax(dim=1).clamp(min=_MASKED)
-    r = torch.where(r > -_MASKED, torch.full_like(r, math.nan), r)
-    t = torch.where(xc > _MASKED, xc - r[:, None], torch.full_like(xc, -math.inf))
+    r = xc.amax(dim=1).clamp(min=_FLOOR)
+    r = torch.where(r > -_FLOOR, torch.full_like(r, math.nan), r)
+    t = torch.where(xc > _FLOOR, xc - r[:, None], torch.full_like(xc, -math.inf))
     t = torch.where(torch.isnan(xc), xc, t)
     e = torch.exp2(t)
     et = torch.where(e == 0, torch.zeros_like(e), e * t).sum(dim=1)

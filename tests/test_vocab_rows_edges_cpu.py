@@ -311,3 +311,19 @@ def test_head_gradients_kept_either_way(monkeypatch, main, rows, chunk):
     got = W.main_grad - 2.0 if main else W.grad
     assert torch.allclose(h.grad.double(), dh, atol=1e-5, rtol=1e-4)
     assert torch.allclose(got.double(), dw, atol=1e-5, rtol=1e-4)
+
+
+def test_tokens_under_a_finite_mask_keep_their_log_probs():
+    x = torch.randn(4, 60)
+    x[:, 7:40] = -1e10
+    tokens = torch.tensor([[7, 3], [8, 9], [39, 40], [30, 0]])
+    r = token_logprobs(x, tokens, 0.8)
+    want, _ = oracle.token_logprobs(x, tokens, 0.8)
+    assert bool(((r.logp.double() - want).abs() <= 2e-6 + 5e-7 * want.abs()).all())
+    logq = torch.full((4, 2), -1.0)
+    for tail in (True, False):
+        _, rows = topk_distill_loss(x, tokens, logq, denom=1.0, tail=tail)
+        kl, _ = oracle.distill(x, tokens, logq, 1.0, tail)
+        assert bool(((rows.double() - kl).abs() <= 1e-5 + 2e-6 * kl.abs()).all())
+    _, rows = topk_distill_loss(torch.full((4, 60), -1e10), tokens, logq, denom=1.0)
+    assert rows.tolist() == [math.inf] * 4

@@ -486,3 +486,41 @@ def test_head_gradients_kept_either_way(main, rows):
     got = W.main_grad - 2.0 if main else W.grad
     _close(h.grad, dh, 2e-2 * float(dh.abs().max()), 5e-2, "dh")
     _close(got, dw, 2e-2 * float(dw.abs().max()), 5e-2, "dW")
+
+
+@pytest.mark.parametrize("vocab", [300, 70001])
+@pytest.mark.parametrize("fill", [-1e10, -1e20])
+def test_tokens_under_a_finite_mask_keep_their_log_probs(vocab, fill):
+    """In a row with live logits a filled token has the log-prob of its fill, and a teacher's entry there costs as much."""
+    x = _logits(4, vocab, torch.float32)
+    x[:, 7:60] = fill
+    tokens = torch.tensor([[7, 3], [8, 9], [59, 60], [30, 0]], device=DEV)
+    r = _ops().token_logprobs(x, tokens, 0.8)
+    _check_logp(r, x, tokens, 0.8)
+    assert bool(torch.isfinite(r.logp).all())
+    y = torch.full((4, vocab), fill, device=DEV)
+    y[:, 5] = 1.0
+    r = _ops().token_logprobs(y, None, 0.8, top_k=3)
+    _check_top(r, y, 0.8, 3)
+    assert bool(torch.isfinite(r.top_logp).all())
+    logq = torch.full((4, 2), -1.0, device=DEV)
+    for tail in (True, False):
+        _check_distill(x, tokens, logq, tail=tail, temp=0.8)
+
+
+def test_tokens_under_a_finite_mask_in_shards(monkeypatch):
+    x = _logits(4, 900, torch.float32)
+    x[:, 250:800] = -1e10
+    tokens = torch.tensor([[7, 300], [8, 799], [59, 250], [899, 0]], device=DEV)
+    logq = torch.full((4, 2), -1.0, device=DEV)
+
+    def work(rank, group):
+        mine = x[:, rank * 300:(rank + 1) * 300].contiguous()
+        at = dict(vocab_start=rank * 300, tp_group=group)
+        return (_ops().token_logprobs(mine, tokens, 0.8, **at),
+                _ops().topk_distill_loss(mine, tokens, logq, denom=1.0, temperature=0.8, **at)[1])
+
+    kl, _ = oracle.distill(x, tokens, logq, 0.8, True)
+    for r, rows in _ranks(monkeypatch, 3, work):
+        _check_logp(r, x, tokens, 0.8)
+        _close(rows, kl, 1e-5, 2e-6, "rows")
