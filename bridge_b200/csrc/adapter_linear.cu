@@ -1,0 +1,744 @@
+// Low-rank adapters beside a shared projection:  y_t = W x_t + c_s B_s A_s x_t,  s the slot of row t's request.
+//
+//   shrink   u = c_s A_s x  (and, with B's transpose, du = c_s B_s^T dy):  a skinny product, bound by the read of x.
+//   joint    y = W x + B_s u (and dx = W^T dy + A_s^T du): the projection's own GEMM whose K loop goes on over u and
+//            the adapters of the slots that its tile of rows meets.  Adding the low-rank part afterwards would read
+//            and write y once more; here it costs R / K of the products.
+//   grads    dB_s = dy^T u and dA_s = du^T x over the rows of one slot: bound by the reads of dy and x.
+//
+// Rows of several requests share tiles.  Where a tile holds rows of several slots, each slot's products go into the
+// same accumulator under the matrix instruction's lane mask: a row takes nothing from another request's adapter, not
+// even a product with zero (which would carry that adapter's infinities over).  The gradients' sums run over rows, so
+// there the blocks of rows end where a slot's rows end, and the rows behind are cleared in both operands.
+//
+// u and du are rounded to the operands' 16 bits once (they feed matrix instructions); every sum is FP32.
+#include "adapter_linear.h"
+
+#include <c10/util/Exception.h>
+#include <cuda.h>
+#include <cudaTypedefs.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "common.cuh"
+#include "sm100_common.cuh"
+
+namespace bb {
+namespace {
+
+constexpr int BM = 128, BK = 64;
+constexpr int kThreads = 192;          // warp 0: TMA, warp 1: TMEM and MMA, warps 2-5: epilogue
+constexpr int kXBytes = BM * BK * 2;   // one block of x: 128 rows x 64, 16 KB
+constexpr int kPairInts = 12;
+
+__device__ int g_error;                // first wait that gave up (per device)
+
+__device__ __forceinline__ uint32_t pack2(float a, float b, bool half) {
+  if (half) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ uint16_t pack1(float a, bool half) {
+  if (half) return __half_as_ushort(__float2half_rn(a));
+  return __bfloat16_as_ushort(__float2bfloat16_rn(a));
+}
+
+// The pairs (slot, lanes) of a tile of 128 rows: half of what the plan notes for 256.
+struct TilePairs {
+  const int* at;
+  int p, end, half;
+  __device__ TilePairs(const AdapterPlan& plan, int tile128) {
+    const int t = tile128 >> 1;
+    half = tile128 & 1;
+    p = __ldg(plan.tile_start + t) - 1;
+    end = __ldg(plan.tile_start + t + 1);
+    at = plan.pairs;
+  }
+  // the next slot with a row in the tile; its lanes' mask
+  __device__ bool next(int& slot, uint32_t (&off)[4]) {
+    while (++p < end) {
+      const int4 m = __ldg(reinterpret_cast<const int4*>(at + (size_t)p * kPairInts) + 1 + half);
+      off[0] = m.x, off[1] = m.y, off[2] = m.z, off[3] = m.w;
+      if ((off[0] & off[1] & off[2] & off[3]) != 0xffffffffu) {
+        slot = __ldg(at + (size_t)p * kPairInts);
+        return true;
+      }
+    }
+    return false;
+  }
+};
+
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// A block of rows' accumulator (TMEM, `cols` columns) into this block's shared memory, row stride cols + 4 floats
+// (rows 16 bytes apart in the banks: neither these stores nor the sums' loads collide).  Warps 2-5.
+__device__ __forceinline__ void spill(uint32_t tmem, float* part, int cols, bool any) {
+  const int quarter = (threadIdx.x >> 5) & 3, row = quarter * 32 + (threadIdx.x & 31);
+  for (int c = 0; c < cols; c += 32) {
+    uint32_t r[32];
+    if (any) {
+      sm100::tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + c, r);
+      sm100::tmem_ld_wait();
+      sm100::tmem_regs_ready(r);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) r[i] = 0;
+    }
+#pragma unroll
+    for (int i = 0; i < 32; i += 4)
+      if (c + i < cols)
+        *reinterpret_cast<uint4*>(part + row * (cols + 4) + c + i) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
+  }
+}
+
+// The sum over the cluster's partial accumulators of four columns, in rank order.
+__device__ __forceinline__ float4 joined(uint32_t part, int at, int ranks) {
+  float4 s = ld_cluster4(sm100::mapa(part + at * 4, 0));
+  for (int j = 1; j < ranks; ++j) {
+    const float4 v = ld_cluster4(sm100::mapa(part + at * 4, j));
+    s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+  }
+  return s;
+}
+
+// ------------------------------------------------------------------------------------------------ shrink
+struct ShrinkParams {
+  AdapterPlan plan;
+  uint16_t* u;
+  const float* scales;
+  float scale;
+  int T, R, cols, op_bytes, stages, nk, ranks;
+  uint32_t idesc;
+  bool half;
+};
+
+// A cluster of `ranks` blocks takes 128 rows, each block a stretch of K; the partial sums meet in shared memory.
+template <bool OP_MN>
+__global__ void __launch_bounds__(kThreads)
+    adapter_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_op,
+                          const ShrinkParams p) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int stage_bytes = kXBytes + p.op_bytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + p.stages * stage_bytes);
+  uint64_t* empty = full + p.stages;
+  uint64_t* done = empty + p.stages;
+  uint32_t* slot_word = reinterpret_cast<uint32_t*>(done + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)sm100::cluster_ctarank(), tile = blockIdx.x / p.ranks;
+  const int kb0 = (int)((long)p.nk * rank / p.ranks), kb1 = (int)((long)p.nk * (rank + 1) / p.ranks);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      sm100::mbar_init(&full[s], 1);
+      sm100::mbar_init(&empty[s], 1);
+    }
+    sm100::mbar_init(done, 1);
+    sm100::fence_mbar_init();
+  }
+  if (warp == 1) sm100::tmem_alloc(slot_word, 128);
+  sm100::tc_fence_before();
+  __syncthreads();
+  sm100::tc_fence_after();
+  const uint32_t tmem = *slot_word;
+
+  bool any = false;
+  {
+    TilePairs it(p.plan, tile);
+    int slot;
+    uint32_t off[4];
+    any = kb1 > kb0 && it.next(slot, off);
+  }
+  if (warp == 0 && lane == 0 && any) {
+    TilePairs it(p.plan, tile);
+    int slot, stage = 0;
+    uint32_t off[4], phase = 0;
+    bool ok = true;
+    while (ok && it.next(slot, off)) {
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!sm100::mbar_wait(&empty[stage], phase ^ 1, &g_error, 31)) {
+          ok = false;
+          break;
+        }
+        unsigned char* dst = smem + stage * stage_bytes;
+        sm100::mbar_expect_tx(&full[stage], stage_bytes);
+        sm100::tma_load_2d(dst, &map_x, &full[stage], kb * BK, tile * BM);
+        if (OP_MN) {
+          for (int i = 0; i < p.cols / 64; ++i)
+            sm100::tma_load_3d(dst + kXBytes + i * 8192, &map_op, &full[stage], 64 * i, kb * BK, slot);
+        } else {
+          sm100::tma_load_3d(dst + kXBytes, &map_op, &full[stage], kb * BK, 0, slot);
+        }
+        if (++stage == p.stages) stage = 0, phase ^= 1;
+      }
+    }
+  } else if (warp == 1 && lane == 0 && any) {
+    TilePairs it(p.plan, tile);
+    int slot, stage = 0;
+    uint32_t off[4], phase = 0;
+    bool ok = true;
+    while (ok && it.next(slot, off)) {
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!sm100::mbar_wait(&full[stage], phase, &g_error, 32)) {
+          ok = false;
+          break;
+        }
+        sm100::tc_fence_after();
+        const uint32_t a = sm100::smem_addr(smem + stage * stage_bytes), b = a + kXBytes;
+#pragma unroll
+        for (int kk = 0; kk < BK / 16; ++kk)
+          sm100::umma_masked(tmem, sm100::umma_desc_sw128(a + kk * 32, 16, 1024),
+                             OP_MN ? sm100::umma_desc_sw128(b + kk * 2048, 8192, 1024)
+                                   : sm100::umma_desc_sw128(b + kk * 32, 16, 1024),
+                             p.idesc, kb > kb0 || kk > 0, off);
+        sm100::umma_commit(&empty[stage]);
+        if (++stage == p.stages) stage = 0, phase ^= 1;
+      }
+    }
+    sm100::umma_commit(done);
+  }
+  __syncwarp();
+  float* part = reinterpret_cast<float*>(smem);
+  if (warp >= 2) {
+    if (any) sm100::mbar_wait(done, 0, &g_error, 33);
+    __syncwarp();
+    sm100::tc_fence_after();
+    spill(tmem, part, p.cols, any);
+    sm100::tc_fence_before();
+  }
+  __syncthreads();
+  sm100::cluster_sync();
+  // this block's share of the rows: 8 columns a step, the finished values 16 bytes at a time
+  const int rows = BM / p.ranks, groups = p.R / 8;
+  const uint32_t base = sm100::smem_addr(part);
+  for (int i = threadIdx.x; i < rows * groups; i += kThreads) {
+    const int r = rank * rows + i / groups, c = (i % groups) * 8, row = tile * BM + r;
+    if (row >= p.T) continue;
+    const int slot = __ldg(p.plan.row_slot + row);
+    uint4 out = make_uint4(0, 0, 0, 0);
+    if (slot >= 0) {
+      const float f = p.scales ? __ldg(p.scales + slot) : p.scale;
+      const float4 v = joined(base, r * (p.cols + 4) + c, p.ranks), w = joined(base, r * (p.cols + 4) + c + 4, p.ranks);
+      out = make_uint4(pack2(f * v.x, f * v.y, p.half), pack2(f * v.z, f * v.w, p.half),
+                       pack2(f * w.x, f * w.y, p.half), pack2(f * w.z, f * w.w, p.half));
+    }
+    *reinterpret_cast<uint4*>(p.u + (size_t)row * p.R + c) = out;
+  }
+  sm100::cluster_sync();   // the peers' sums stay until all have read them
+  if (warp == 1) {
+    sm100::tc_fence_after();
+    sm100::tmem_dealloc(tmem, 128);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ joint
+constexpr int kJointStages = 4;
+
+template <int BN>
+struct JointSmem {
+  static constexpr int W_BYTES = BN * BK * 2;
+  static constexpr int STAGE = kXBytes + W_BYTES;
+  static constexpr int BAR_OFF = kJointStages * STAGE;
+  static constexpr int TOTAL = BAR_OFF + 256 + 1024;
+};
+
+struct JointParams {
+  AdapterPlan plan;
+  uint16_t* y;
+  int T, N, R, nk;
+  uint32_t idesc;
+  bool half;
+};
+
+// Tiles of 128 x BN; accumulators double-buffered in TMEM, so that a tile's stores overlap the next one's products.
+template <bool MN, int BN>
+__global__ void __launch_bounds__(kThreads, 1)
+    adapter_joint_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                         const __grid_constant__ CUtensorMap map_u, const __grid_constant__ CUtensorMap map_low,
+                         const JointParams p) {
+  using L = JointSmem<BN>;
+  constexpr int kCols = 2 * BN < 32 ? 32 : 2 * BN;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);
+  uint64_t* empty = full + kJointStages;
+  uint64_t* tfull = empty + kJointStages;
+  uint64_t* tempty = tfull + 2;
+  uint32_t* slot_word = reinterpret_cast<uint32_t*>(tempty + 2);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int m_tiles = (p.T + BM - 1) / BM, n_tiles = (p.N + BN - 1) / BN, num_tiles = m_tiles * n_tiles;
+  const int rank_blocks = (p.R + BK - 1) / BK;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kJointStages; ++s) {
+      sm100::mbar_init(&full[s], 1);
+      sm100::mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      sm100::mbar_init(&tfull[a], 1);
+      sm100::mbar_init(&tempty[a], 128);
+    }
+    sm100::fence_mbar_init();
+  }
+  if (warp == 1) sm100::tmem_alloc(slot_word, kCols);
+  sm100::tc_fence_before();
+  __syncthreads();
+  sm100::tc_fence_after();
+  const uint32_t tmem = *slot_word;
+
+  auto tile_at = [&](int t, int& mt, int& nt) {   // groups of 8 tiles of rows, so that a tile of W serves 8 from L2
+    const int per_group = 8 * n_tiles, first = t / per_group * 8, gm = min(8, m_tiles - first), r = t % per_group;
+    mt = first + r % gm;
+    nt = r / gm;
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      auto claim = [&]() {
+        ok = ok && sm100::mbar_wait(&empty[stage], phase ^ 1, &g_error, 41);
+        if (ok) sm100::mbar_expect_tx(&full[stage], L::STAGE);
+        return ok;
+      };
+      auto step = [&]() {
+        if (++stage == kJointStages) stage = 0, phase ^= 1;
+      };
+      for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
+        int mt, nt;
+        tile_at(t, mt, nt);
+        for (int kb = 0; kb < p.nk; ++kb) {
+          if (!claim()) break;
+          unsigned char* dst = smem + stage * L::STAGE;
+          sm100::tma_load_2d(dst, &map_x, &full[stage], kb * BK, mt * BM);
+          if (MN) {
+#pragma unroll
+            for (int i = 0; i < BN / 64; ++i)
+              sm100::tma_load_2d(dst + kXBytes + i * 8192, &map_w, &full[stage], nt * BN + 64 * i, kb * BK);
+          } else {
+            sm100::tma_load_2d(dst + kXBytes, &map_w, &full[stage], kb * BK, nt * BN);
+          }
+          step();
+        }
+        TilePairs it(p.plan, mt);
+        int slot;
+        uint32_t off[4];
+        while (ok && it.next(slot, off)) {
+          for (int rb = 0; rb < rank_blocks; ++rb) {
+            if (!claim()) break;
+            unsigned char* dst = smem + stage * L::STAGE;
+            sm100::tma_load_2d(dst, &map_u, &full[stage], rb * BK, mt * BM);
+            if (MN) {
+#pragma unroll
+              for (int i = 0; i < BN / 64; ++i)
+                sm100::tma_load_3d(dst + kXBytes + i * 8192, &map_low, &full[stage], nt * BN + 64 * i, rb * BK, slot);
+            } else {
+              sm100::tma_load_3d(dst + kXBytes, &map_low, &full[stage], rb * BK, nt * BN, slot);
+            }
+            step();
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      auto products = [&](uint32_t d, int steps, bool first, const uint32_t (&off)[4]) {
+        ok = ok && sm100::mbar_wait(&full[stage], phase, &g_error, 43);
+        if (!ok) return;
+        sm100::tc_fence_after();
+        const uint32_t a = sm100::smem_addr(smem + stage * L::STAGE), b = a + kXBytes;
+        for (int kk = 0; kk < steps; ++kk)
+          sm100::umma_masked(d, sm100::umma_desc_sw128(a + kk * 32, 16, 1024),
+                             MN ? sm100::umma_desc_sw128(b + kk * 2048, 8192, 1024)
+                                : sm100::umma_desc_sw128(b + kk * 32, 16, 1024),
+                             p.idesc, !first || kk > 0, off);
+        sm100::umma_commit(&empty[stage]);
+        if (++stage == kJointStages) stage = 0, phase ^= 1;
+      };
+      for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
+        if (!sm100::mbar_wait(&tempty[acc], acc_phase ^ 1, &g_error, 42)) break;
+        sm100::tc_fence_after();
+        const uint32_t d = tmem + acc * BN;
+        int mt, nt;
+        tile_at(t, mt, nt);
+        const uint32_t all[4] = {0, 0, 0, 0};
+        for (int kb = 0; kb < p.nk && ok; ++kb) products(d, BK / 16, kb == 0, all);
+        TilePairs it(p.plan, mt);
+        int slot;
+        uint32_t off[4];
+        while (ok && it.next(slot, off))
+          for (int rb = 0; rb < rank_blocks; ++rb) products(d, min(BK / 16, (p.R - rb * BK + 15) / 16), false, off);
+        if (!ok) break;
+        sm100::umma_commit(&tfull[acc]);
+        if (++acc == 2) acc = 0, acc_phase ^= 1;
+      }
+    }
+  } else {
+    const int quarter = warp & 3;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int t = blockIdx.x; t < num_tiles; t += gridDim.x) {
+      int mt, nt;
+      tile_at(t, mt, nt);
+      const bool got = sm100::mbar_wait(&tfull[acc], acc_phase, &g_error, 44);
+      if (!__all_sync(0xffffffffu, got)) break;
+      sm100::tc_fence_after();
+      const int row = mt * BM + quarter * 32 + lane;
+      const uint32_t src = tmem + ((uint32_t)(quarter * 32) << 16) + acc * BN;
+#pragma unroll 1
+      for (int c = 0; c < BN; c += 32) {
+        uint32_t r[32];
+        sm100::tmem_ld32(src + c, r);
+        sm100::tmem_ld_wait();
+        sm100::tmem_regs_ready(r);
+        const int col = nt * BN + c;
+        if (row < p.T) {
+          uint16_t* dst = p.y + (size_t)row * p.N + col;
+#pragma unroll
+          for (int j = 0; j < 32; j += 8)
+            if (col + j < p.N)     // N is a multiple of 8
+              *reinterpret_cast<uint4*>(dst + j) =
+                  make_uint4(pack2(__uint_as_float(r[j]), __uint_as_float(r[j + 1]), p.half),
+                             pack2(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]), p.half),
+                             pack2(__uint_as_float(r[j + 4]), __uint_as_float(r[j + 5]), p.half),
+                             pack2(__uint_as_float(r[j + 6]), __uint_as_float(r[j + 7]), p.half));
+        }
+      }
+      sm100::tc_fence_before();
+      sm100::mbar_arrive(&tempty[acc]);
+      if (++acc == 2) acc = 0, acc_phase ^= 1;
+    }
+  }
+  __syncwarp();
+  sm100::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    sm100::tc_fence_after();
+    sm100::tmem_dealloc(tmem, kCols);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ grads
+constexpr int kGradStages = 4;
+
+struct GradParams {
+  AdapterPlan plan;
+  void *da, *db;
+  int K, N, S, R, cols, tiles_a, tiles_b, ranks;
+  uint32_t idesc;
+  bool add_a, add_b, half;
+};
+
+// One cluster takes 128 columns of dy (or x) of one slot, each of its blocks a stretch of the slot's rows:
+// D [128, R] = sum over rows of dy^T u (x^T du); the partial sums meet in shared memory, in rank order.
+__global__ void __launch_bounds__(kThreads)
+    adapter_grads_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_dy,
+                         const __grid_constant__ CUtensorMap map_u, const __grid_constant__ CUtensorMap map_du,
+                         const GradParams p) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int low_bytes = p.cols / 64 * 8192, stage_bytes = kXBytes + low_bytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kGradStages * stage_bytes);
+  uint64_t* empty = full + kGradStages;
+  uint64_t* done = empty + kGradStages;
+  uint32_t* slot_word = reinterpret_cast<uint32_t*>(done + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)sm100::cluster_ctarank();
+  const int item = blockIdx.x / p.ranks, tiles = p.tiles_a + p.tiles_b, slot = item / tiles;
+  const bool is_b = item % tiles < p.tiles_b;
+  const int m0 = (is_b ? item % tiles : item % tiles - p.tiles_b) * BM;
+  const CUtensorMap* map_wide = is_b ? &map_dy : &map_x;
+  const CUtensorMap* map_thin = is_b ? &map_u : &map_du;
+  int first = 0, count = 0;
+  if (slot < p.plan.slots) {
+    first = __ldg(p.plan.block_start + slot);
+    count = __ldg(p.plan.block_start + slot + 1) - first;
+  }
+  const int b0 = first + (int)((long)count * rank / p.ranks), b1 = first + (int)((long)count * (rank + 1) / p.ranks);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kGradStages; ++s) {
+      sm100::mbar_init(&full[s], 1);
+      sm100::mbar_init(&empty[s], 1);
+    }
+    sm100::mbar_init(done, 1);
+    sm100::fence_mbar_init();
+  }
+  if (warp == 1) sm100::tmem_alloc(slot_word, 128);
+  sm100::tc_fence_before();
+  __syncthreads();
+  sm100::tc_fence_after();
+  const uint32_t tmem = *slot_word;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int b = b0; b < b1; ++b) {
+        if (!sm100::mbar_wait(&empty[stage], phase ^ 1, &g_error, 51)) break;
+        unsigned char* dst = smem + stage * stage_bytes;
+        const int row = __ldg(p.plan.blocks + 2 * b);
+        sm100::mbar_expect_tx(&full[stage], stage_bytes);
+        sm100::tma_load_2d(dst, map_wide, &full[stage], m0, row);
+        sm100::tma_load_2d(dst + 8192, map_wide, &full[stage], m0 + 64, row);
+        for (int i = 0; i < p.cols / 64; ++i)
+          sm100::tma_load_2d(dst + kXBytes + i * 8192, map_thin, &full[stage], 64 * i, row);
+        if (++stage == kGradStages) stage = 0, phase ^= 1;
+      }
+    }
+  } else if (warp == 1 && b1 > b0) {
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int b = b0; b < b1; ++b) {
+      const bool got = sm100::mbar_wait(&full[stage], phase, &g_error, 52);
+      if (!__all_sync(0xffffffffu, got)) break;
+      unsigned char* at = smem + stage * stage_bytes;
+      const int n = __ldg(p.plan.blocks + 2 * b + 1), steps = (n + 15) / 16;
+      if (n < steps * 16) {
+        // rows of other requests behind the block: a row is 128 bytes of every 64 columns, in whatever order
+        const int lines = (steps * 16 - n) * 8;
+        for (int i = lane; i < lines * (2 + p.cols / 64); i += 32)
+          *reinterpret_cast<uint4*>(at + i / lines * 8192 + n * 128 + i % lines * 16) = make_uint4(0, 0, 0, 0);
+        sm100::fence_proxy_async_smem();
+      }
+      __syncwarp();
+      if (lane == 0) {
+        sm100::tc_fence_after();
+        const uint32_t a = sm100::smem_addr(at), w = a + kXBytes;
+        for (int kk = 0; kk < steps; ++kk)
+          sm100::umma_bf16(tmem, sm100::umma_desc_sw128(a + kk * 2048, 8192, 1024),
+                           sm100::umma_desc_sw128(w + kk * 2048, 8192, 1024), p.idesc, b > b0 || kk > 0);
+        sm100::umma_commit(&empty[stage]);
+      }
+      __syncwarp();
+      if (++stage == kGradStages) stage = 0, phase ^= 1;
+    }
+    if (lane == 0) sm100::umma_commit(done);
+  }
+  __syncwarp();
+  float* part = reinterpret_cast<float*>(smem);
+  if (warp >= 2) {
+    if (b1 > b0) sm100::mbar_wait(done, 0, &g_error, 53);
+    __syncwarp();
+    sm100::tc_fence_after();
+    spill(tmem, part, p.cols, b1 > b0);
+    sm100::tc_fence_before();
+  }
+  __syncthreads();
+  sm100::cluster_sync();
+  const int rows = BM / p.ranks;
+  const uint32_t base = sm100::smem_addr(part);
+  const int limit = is_b ? p.N : p.K;
+  const bool add = is_b ? p.add_b : p.add_a;
+  if (!(add && count == 0)) {
+    for (int i = threadIdx.x; i < rows * (p.R / 4); i += kThreads) {
+      // dB: neighbours take neighbouring columns of a row; dA, whose rows are these columns: neighbouring rows
+      const int r = rank * rows + (is_b ? i / (p.R / 4) : i % rows), c = (is_b ? i % (p.R / 4) : i / rows) * 4;
+      if (m0 + r >= limit) continue;
+      const float4 v = joined(base, r * (p.cols + 4) + c, p.ranks);
+      if (is_b) {
+        const size_t to = ((size_t)slot * p.N + m0 + r) * p.R + c;
+        if (add) {
+          float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.db) + to);
+          const float4 o = *dst;
+          *dst = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
+        } else {
+          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.db) + to) =
+              make_uint2(pack2(v.x, v.y, p.half), pack2(v.z, v.w, p.half));
+        }
+      } else {
+        const size_t to = ((size_t)slot * p.R + c) * p.K + m0 + r;
+        const float q[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (add) static_cast<float*>(p.da)[to + (size_t)j * p.K] += q[j];
+          else static_cast<uint16_t*>(p.da)[to + (size_t)j * p.K] = pack1(q[j], p.half);
+        }
+      }
+    }
+  }
+  sm100::cluster_sync();
+  if (warp == 1) {
+    sm100::tc_fence_after();
+    sm100::tmem_dealloc(tmem, 128);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    cudaDriverEntryPointQueryResult q;
+    void* f = nullptr;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  }();
+  return fn;
+}
+
+// Row-major [batch][rows, cols] of 16-bit values, boxes of 64 columns x `box` rows, 128-byte swizzle.  Reads outside
+// give zeros, in each of the three dimensions: a box never reaches into the next slot.
+bool encode(CUtensorMap* m, const void* base, long cols, long rows, long ld, long batch, int box, bool half) {
+  const auto fn = encoder();
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)std::max(1l, batch)};
+  const cuuint64_t strides[2] = {(cuuint64_t)(ld * 2), (cuuint64_t)(ld * 2 * rows)};
+  const cuuint32_t boxes[3] = {64, (cuuint32_t)box, 1}, ones[3] = {1, 1, 1};
+  return fn(m, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, batch ? 3 : 2,
+            const_cast<void*>(base), dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// The encoder works in the calling thread's context, which a thread of autograd's may not have yet.
+cudaError_t have_context() {
+  CUcontext cur = nullptr;
+  if (cuCtxGetCurrent(&cur) == CUDA_SUCCESS && cur != nullptr) return cudaSuccess;
+  return cudaFree(nullptr);
+}
+
+int sm_count() {
+  int dev = 0, n = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  return n;
+}
+
+template <typename Kernel>
+cudaError_t allow_smem(Kernel kernel, int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || ((done.load() >> (dev & 63)) & 1)) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(1ull << (dev & 63));
+  return e;
+}
+
+template <typename... P, typename... A>
+cudaError_t launch(void (*kernel)(P...), int grid, int smem, int cluster, cudaStream_t stream, const A&... args) {
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e == cudaSuccess) launch_counter().fetch_add(1);
+  return e;
+}
+
+constexpr int kMaxSmem = 227 * 1024;
+
+template <bool OP_MN>
+cudaError_t run_shrink(const AdapterShrink& a, cudaStream_t stream) {
+  alignas(64) CUtensorMap x, op;
+  const int cols = OP_MN ? (a.R + 63) / 64 * 64 : (a.R + 15) / 16 * 16;
+  if (!encode(&x, a.x, a.K, a.T, a.ldx, 0, BM, a.half)) return cudaErrorInvalidValue;
+  if (!(OP_MN ? encode(&op, a.op, a.R, a.K, a.R, a.S, 64, a.half) : encode(&op, a.op, a.K, a.R, a.K, a.S, cols, a.half)))
+    return cudaErrorInvalidValue;
+  ShrinkParams p{};
+  p.plan = a.plan;
+  p.u = static_cast<uint16_t*>(a.u);
+  p.scales = a.scales, p.scale = a.scale;
+  p.T = a.T, p.R = a.R, p.cols = cols;
+  p.op_bytes = cols * 128;
+  p.nk = (a.K + BK - 1) / BK;
+  p.stages = 4;
+  p.ranks = 1;
+  p.idesc = sm100::umma_idesc_bf16(BM, cols, false, OP_MN) & ~(a.half ? sm100::kIdescBf16 : 0u);
+  p.half = a.half;
+  const int smem = std::max(p.stages * (kXBytes + p.op_bytes), BM * (cols + 4) * 4) + 256 + 1024;
+  static std::atomic<unsigned long long> done{0};
+  const cudaError_t e = allow_smem(adapter_shrink_kernel<OP_MN>, kMaxSmem, done);
+  if (e != cudaSuccess) return e;
+  return launch(adapter_shrink_kernel<OP_MN>, (a.T + BM - 1) / BM * p.ranks, smem, p.ranks, stream, x, op, p);
+}
+
+template <bool MN, int BN>
+cudaError_t run_joint(const AdapterJoint& a, cudaStream_t stream) {
+  alignas(64) CUtensorMap x, w, u, low;
+  bool ok = encode(&x, a.x, a.K, a.T, a.ldx, 0, BM, a.half) && encode(&u, a.u, a.R, a.T, a.R, 0, BM, a.half);
+  if (MN) ok = ok && encode(&w, a.w, a.N, a.K, a.ldw, 0, 64, a.half) && encode(&low, a.low, a.N, a.R, a.N, a.S, 64, a.half);
+  else ok = ok && encode(&w, a.w, a.K, a.N, a.ldw, 0, BN, a.half) && encode(&low, a.low, a.R, a.N, a.R, a.S, BN, a.half);
+  if (!ok) return cudaErrorInvalidValue;
+  JointParams p{};
+  p.plan = a.plan;
+  p.y = static_cast<uint16_t*>(a.y);
+  p.T = a.T, p.N = a.N, p.R = a.R;
+  p.nk = (a.K + BK - 1) / BK;
+  p.idesc = sm100::umma_idesc_bf16(BM, BN, false, MN) & ~(a.half ? sm100::kIdescBf16 : 0u);
+  p.half = a.half;
+  static std::atomic<unsigned long long> done{0};
+  const cudaError_t e = allow_smem(adapter_joint_kernel<MN, BN>, JointSmem<BN>::TOTAL, done);
+  if (e != cudaSuccess) return e;
+  const long tiles = (long)((a.T + BM - 1) / BM) * ((a.N + BN - 1) / BN);
+  return launch(adapter_joint_kernel<MN, BN>, (int)std::min<long>(tiles, sm_count()), JointSmem<BN>::TOTAL, 1, stream, x, w,
+                u, low, p);
+}
+
+}  // namespace
+
+cudaError_t launch_adapter_shrink(const AdapterShrink& a, cudaStream_t stream) {
+  const cudaError_t e = have_context();
+  if (e != cudaSuccess) return e;
+  return a.op_mn ? run_shrink<true>(a, stream) : run_shrink<false>(a, stream);
+}
+
+cudaError_t launch_adapter_joint(const AdapterJoint& a, cudaStream_t stream) {
+  const cudaError_t e = have_context();
+  if (e != cudaSuccess) return e;
+  return a.mn ? run_joint<true, 256>(a, stream) : run_joint<false, 256>(a, stream);
+}
+
+cudaError_t launch_adapter_grads(const AdapterGrads& a, cudaStream_t stream) {
+  cudaError_t e = have_context();
+  if (e != cudaSuccess) return e;
+  alignas(64) CUtensorMap x, dy, u, du;
+  // (an operand that is not asked for has no pointer: any valid map stands in for its own)
+  const bool ok = encode(&x, a.da ? a.x : a.dy, a.da ? a.K : a.N, a.T, a.da ? a.ldx : a.lddy, 0, 64, a.half) &&
+                  encode(&dy, a.db ? a.dy : a.x, a.db ? a.N : a.K, a.T, a.db ? a.lddy : a.ldx, 0, 64, a.half) &&
+                  encode(&u, a.db ? a.u : a.du, a.R, a.T, a.R, 0, 64, a.half) &&
+                  encode(&du, a.da ? a.du : a.u, a.R, a.T, a.R, 0, 64, a.half);
+  if (!ok) return cudaErrorInvalidValue;
+  GradParams p{};
+  p.plan = a.plan;
+  p.da = a.da, p.db = a.db;
+  p.K = a.K, p.N = a.N, p.S = a.S, p.R = a.R;
+  p.cols = (a.R + 63) / 64 * 64;
+  p.tiles_a = a.da ? (a.K + BM - 1) / BM : 0;
+  p.tiles_b = a.db ? (a.N + BM - 1) / BM : 0;
+  p.ranks = 1;
+  p.idesc = sm100::umma_idesc_bf16(BM, p.cols, true, true) & ~(a.half ? sm100::kIdescBf16 : 0u);
+  p.add_a = a.add_a, p.add_b = a.add_b, p.half = a.half;
+  const int smem = std::max(kGradStages * (kXBytes + p.cols * 128), BM * (p.cols + 4) * 4) + 256 + 1024;
+  static std::atomic<unsigned long long> done{0};
+  e = allow_smem(adapter_grads_kernel, kMaxSmem, done);
+  if (e != cudaSuccess) return e;
+  return launch(adapter_grads_kernel, a.S * (p.tiles_a + p.tiles_b) * p.ranks, smem, p.ranks, stream, x, dy, u, du, p);
+}
+
+int adapter_error_code() {
+  int v = -1;
+  return cudaMemcpyFromSymbol(&v, g_error, sizeof v) == cudaSuccess ? v : -1;
+}
+
+}  // namespace bb

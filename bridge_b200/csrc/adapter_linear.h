@@ -1,0 +1,64 @@
+// Launchers of the adapter kernels (adapter_linear.cu); checked and called by adapter_ops.cpp.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace bb {
+
+constexpr int kMaxAdapterRank = 128;
+
+// Where the rows of a batch find their adapter: device pointers into one int32 buffer that adapter_rows() lays out.
+struct AdapterPlan {
+  const int* row_slot;     // [T] slot, or -1
+  const int* tile_start;   // [ceil(T / 256) + 1] first pair of each tile of 256 rows
+  const int* pairs;        // [P][12] (slot, 0, 0, 0, 256 bits: set where a row of the tile is NOT the slot's)
+  const int* block_start;  // [slots + 1] first block of each slot
+  const int* blocks;       // [.][2] (first row, rows <= 64) of one slot, in row order
+  int slots;               // slots the plan speaks of: the largest one + 1
+};
+
+// u[t, r] = scale_s sum_k x[t, k] op_s[r, k] for the row's slot s, 0 without one
+struct AdapterShrink {
+  const void* x;           // [T, K], row stride ldx
+  const void* op;          // [S, R, K], or [S, K, R] with `op_mn`
+  void* u;                 // [T, R]
+  const float* scales;     // [S], or null: `scale`
+  float scale;
+  long ldx;
+  int T, K, S, R;
+  bool op_mn, half;        // half: FP16, else BF16
+  AdapterPlan plan;
+};
+
+// y[t, n] = sum_k x[t, k] w[n, k] + sum_r u[t, r] low_s[n, r]
+struct AdapterJoint {
+  const void* x;           // [T, K], row stride ldx
+  const void* w;           // [N, K], or [K, N] with `mn`; row stride ldw
+  const void* u;           // [T, R]
+  const void* low;         // [S, N, R], or [S, R, N] with `mn`
+  void* y;                 // [T, N]
+  long ldx, ldw;
+  int T, K, N, S, R;
+  bool mn, half;
+  AdapterPlan plan;
+};
+
+// db[s, n, r] = sum_t dy[t, n] u[t, r],  da[s, r, k] = sum_t du[t, r] x[t, k] over the rows of slot s
+struct AdapterGrads {
+  const void *x, *dy;      // [T, K], [T, N]
+  const void *u, *du;      // [T, R]
+  void *da, *db;           // null: not asked for
+  bool add_a, add_b;       // FP32, added to; else the inputs' type, written
+  long ldx, lddy;
+  int T, K, N, S, R;
+  bool half;
+  AdapterPlan plan;
+};
+
+cudaError_t launch_adapter_shrink(const AdapterShrink& a, cudaStream_t stream);
+cudaError_t launch_adapter_joint(const AdapterJoint& a, cudaStream_t stream);
+cudaError_t launch_adapter_grads(const AdapterGrads& a, cudaStream_t stream);
+int adapter_error_code();
+
+}  // namespace bb

@@ -1,0 +1,198 @@
+// Torch entry points of the adapter kernels (adapter_linear.cu): argument checks, allocation, autograd.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include "adapter_linear.h"
+
+torch::Tensor gemm(torch::Tensor a, torch::Tensor b, bool a_mn, bool b_mn, c10::optional<torch::Tensor> out,
+                   bool accumulate);
+
+namespace {
+
+using OptTensor = c10::optional<torch::Tensor>;
+using Meta = std::vector<int64_t>;   // rows, slots, then where the plan's parts begin in its buffer
+
+void check(cudaError_t e) { TORCH_CHECK(e == cudaSuccess, "CUDA error ", cudaGetErrorString(e)); }
+
+bool aligned(const torch::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+// Rows that a tensor map can describe: unit columns, rows 16 bytes apart or a multiple of it, not on top of each other.
+bool plain_rows(const torch::Tensor& t) {
+  return t.dim() == 2 && t.stride(1) == 1 && aligned(t) &&
+         (t.size(0) <= 1 || (t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1)));
+}
+long row_stride(const torch::Tensor& t) { return t.size(0) <= 1 ? t.size(1) : t.stride(0); }
+torch::Tensor as_rows(const torch::Tensor& t) {
+  return plain_rows(t) ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+bb::AdapterPlan plan_of(const torch::Tensor& buf, const Meta& meta) {
+  const int* p = buf.data_ptr<int>();
+  return {p + meta[2], p + meta[3], p + meta[4], p + meta[5], p + meta[6], (int)meta[1]};
+}
+
+struct Sizes {
+  int T, K, N, S, R;
+  bool half;
+  explicit Sizes(const torch::Tensor& x, const torch::Tensor& a, const torch::Tensor& b)
+      : T((int)x.size(0)), K((int)a.size(2)), N((int)b.size(1)), S((int)a.size(0)), R((int)a.size(1)),
+        half(a.scalar_type() == at::kHalf) {}
+};
+
+// u = scale A x, or du = scale B^T dy with `mn` (op [S, K, R] then)
+torch::Tensor shrink(const torch::Tensor& x, const torch::Tensor& op, bool mn, const torch::Tensor& buf,
+                     const Meta& meta, double scale, const OptTensor& scales) {
+  bb::AdapterShrink s{};
+  s.op_mn = mn;
+  s.S = (int)op.size(0), s.R = (int)op.size(mn ? 2 : 1), s.K = (int)op.size(mn ? 1 : 2), s.T = (int)x.size(0);
+  s.half = op.scalar_type() == at::kHalf;
+  auto u = at::empty({s.T, s.R}, op.options().requires_grad(false));
+  s.x = x.data_ptr(), s.op = op.data_ptr(), s.u = u.data_ptr();
+  s.ldx = row_stride(x);
+  s.scale = (float)scale;
+  s.scales = scales.has_value() ? scales->data_ptr<float>() : nullptr;
+  s.plan = plan_of(buf, meta);
+  check(bb::launch_adapter_shrink(s, at::cuda::getCurrentCUDAStream()));
+  return u;
+}
+
+torch::Tensor joint(const torch::Tensor& x, const torch::Tensor& w, const torch::Tensor& u, const torch::Tensor& low,
+                    bool mn, const torch::Tensor& buf, const Meta& meta) {
+  bb::AdapterJoint j{};
+  j.mn = mn;
+  j.T = (int)x.size(0), j.K = (int)x.size(1), j.N = (int)w.size(mn ? 1 : 0), j.S = (int)low.size(0), j.R = (int)u.size(1);
+  j.half = low.scalar_type() == at::kHalf;
+  auto y = at::empty({j.T, j.N}, low.options().requires_grad(false));
+  j.x = x.data_ptr(), j.w = w.data_ptr(), j.u = u.data_ptr(), j.low = low.data_ptr(), j.y = y.data_ptr();
+  j.ldx = row_stride(x), j.ldw = row_stride(w);
+  j.plan = plan_of(buf, meta);
+  check(bb::launch_adapter_joint(j, at::cuda::getCurrentCUDAStream()));
+  return y;
+}
+
+void first_order() {
+  TORCH_CHECK(!at::GradMode::is_enabled(),
+              "adapter_linear has no second derivative (backward was called with create_graph=True)");
+}
+
+class AdapterLinear : public torch::autograd::Function<AdapterLinear> {
+ public:
+  static torch::Tensor forward(torch::autograd::AutogradContext* ctx, const torch::Tensor& x, const torch::Tensor& w,
+                               const torch::Tensor& a, const torch::Tensor& b, const torch::Tensor& buf,
+                               const Meta& meta, double scale, const OptTensor& scales, const OptTensor& a_main,
+                               const OptTensor& b_main, const OptTensor& w_main) {
+    const c10::cuda::CUDAGuard guard(x.device());
+    torch::Tensor u, y;
+    if (x.size(0)) {
+      u = shrink(x, a, false, buf, meta, scale, scales);
+      y = joint(x, w, u, b, false, buf, meta);
+    } else {
+      u = at::empty({0, a.size(1)}, a.options().requires_grad(false));
+      y = at::empty({0, w.size(0)}, a.options().requires_grad(false));
+    }
+    const torch::Tensor none;
+    ctx->save_for_backward({x, w, a, b, u, buf, scales.value_or(none)});
+    ctx->saved_data["meta"] = meta;
+    ctx->saved_data["scale"] = scale;
+    if (a_main.has_value()) ctx->saved_data["a_main"] = *a_main;
+    if (b_main.has_value()) ctx->saved_data["b_main"] = *b_main;
+    if (w_main.has_value()) ctx->saved_data["w_main"] = *w_main;
+    return y;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    first_order();
+    const auto saved = ctx->get_saved_variables();
+    const torch::Tensor &x = saved[0], &w = saved[1], &a = saved[2], &b = saved[3], &u = saved[4], &buf = saved[5];
+    const OptTensor scales = saved[6].defined() ? OptTensor(saved[6]) : OptTensor();
+    const Meta meta = ctx->saved_data["meta"].toIntVector();
+    const double scale = ctx->saved_data["scale"].toDouble();
+    const auto main = [&](const char* name) {
+      const auto at = ctx->saved_data.find(name);
+      return at == ctx->saved_data.end() ? OptTensor() : OptTensor(at->second.toTensor());
+    };
+    const OptTensor a_main = main("a_main"), b_main = main("b_main"), w_main = main("w_main");
+    const c10::cuda::CUDAGuard guard(x.device());
+    const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1), want_a = ctx->needs_input_grad(2),
+               want_b = ctx->needs_input_grad(3);
+    const torch::Tensor none;
+    torch::Tensor dx, dw, da, db;
+    if (x.size(0) == 0) {
+      if (want_x) dx = at::empty(x.sizes(), a.options().requires_grad(false));
+      if (want_w && !w_main.has_value()) dw = at::zeros(w.sizes(), a.options().requires_grad(false));
+      if (want_a && !a_main.has_value()) da = at::zeros(a.sizes(), a.options().requires_grad(false));
+      if (want_b && !b_main.has_value()) db = at::zeros(b.sizes(), a.options().requires_grad(false));
+      return {dx, dw, da, db, none, none, none, none, none, none, none};
+    }
+    const auto dy = as_rows(grads[0]);
+    torch::Tensor du;
+    if (want_x || want_a) du = shrink(dy, b, true, buf, meta, scale, scales);
+    if (want_x) dx = joint(dy, w, du, a, true, buf, meta);
+    if (want_w) {
+      const auto rows = [](const torch::Tensor& t) { return t.as_strided(t.sizes(), {row_stride(t), 1}); };
+      if (w_main.has_value()) gemm(rows(dy), rows(x), true, true, w_main, true);
+      else dw = gemm(rows(dy), rows(x), true, true, c10::nullopt, false);
+    }
+    if (want_a || want_b) {
+      const Sizes n(x, a, b);
+      bb::AdapterGrads g{};
+      if (want_a) {
+        if (!a_main.has_value()) da = at::empty(a.sizes(), a.options().requires_grad(false));
+        g.da = a_main.has_value() ? a_main->data_ptr() : da.data_ptr();
+        g.add_a = a_main.has_value();
+        g.du = du.data_ptr();
+      }
+      if (want_b) {
+        if (!b_main.has_value()) db = at::empty(b.sizes(), b.options().requires_grad(false));
+        g.db = b_main.has_value() ? b_main->data_ptr() : db.data_ptr();
+        g.add_b = b_main.has_value();
+        g.u = u.data_ptr();
+      }
+      g.x = x.data_ptr(), g.dy = dy.data_ptr();
+      g.ldx = row_stride(x), g.lddy = row_stride(dy);
+      g.T = n.T, g.K = n.K, g.N = n.N, g.S = n.S, g.R = n.R, g.half = n.half;
+      g.plan = plan_of(buf, meta);
+      check(bb::launch_adapter_grads(g, at::cuda::getCurrentCUDAStream()));
+    }
+    return {dx, dw, da, db, none, none, none, none, none, none, none};
+  }
+};
+
+bool main_fits(const OptTensor& m, const torch::Tensor& p) {
+  return !m.has_value() || (m->scalar_type() == at::kFloat && m->is_contiguous() && m->numel() == p.numel() &&
+                            m->device() == p.device() && aligned(*m));
+}
+
+}  // namespace
+
+// y [T, N]; undefined where the arguments are not in the form that the kernels take.
+torch::Tensor adapter_linear(torch::Tensor x, torch::Tensor w, torch::Tensor a, torch::Tensor b, torch::Tensor buf,
+                             Meta meta, double scale, OptTensor scales, OptTensor a_main, OptTensor b_main,
+                             OptTensor w_main) {
+  const auto type = x.scalar_type();
+  const auto like_x = [&](const torch::Tensor& t) { return t.scalar_type() == type && t.device() == x.device(); };
+  const bool fits =
+      x.is_cuda() && (type == at::kBFloat16 || type == at::kHalf) && x.dim() == 2 && w.dim() == 2 && a.dim() == 3 &&
+      b.dim() == 3 && like_x(w) && like_x(a) && like_x(b) && x.size(1) == w.size(1) && a.size(2) == x.size(1) &&
+      b.size(1) == w.size(0) && a.size(0) == b.size(0) && a.size(1) == b.size(2) && a.size(0) >= 1 && x.size(1) >= 8 &&
+      w.size(0) >= 8 && a.size(1) >= 8 && x.size(1) % 8 == 0 && w.size(0) % 8 == 0 && a.size(1) % 8 == 0 &&
+      a.size(1) <= bb::kMaxAdapterRank && x.size(0) < (1l << 30) && x.size(1) < (1l << 30) && w.size(0) < (1l << 30) &&
+      a.size(0) < (1l << 16) && plain_rows(x) && plain_rows(w) && a.is_contiguous() && aligned(a) &&
+      b.is_contiguous() && aligned(b) && meta.size() == 7 && meta[0] == x.size(0) && meta[1] <= a.size(0) &&
+      buf.device() == x.device() && buf.scalar_type() == at::kInt && buf.is_contiguous() &&
+      (!scales.has_value() || (scales->dim() == 1 && scales->size(0) == a.size(0) && scales->is_contiguous() &&
+                               scales->scalar_type() == at::kFloat && scales->device() == x.device() &&
+                               !scales->requires_grad())) &&
+      !(w.requires_grad() && type == at::kHalf) && main_fits(a_main, a) && main_fits(b_main, b) && main_fits(w_main, w);
+  if (!fits) return {};
+  for (const auto& t : {x, w, a, b})
+    TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), "adapter_linear has no forward-mode derivative");
+  if (at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || a.requires_grad() || b.requires_grad()))
+    return AdapterLinear::apply(x, w, a, b, buf, meta, scale, scales, a_main, b_main, w_main);
+  const c10::cuda::CUDAGuard guard(x.device());
+  if (x.size(0) == 0) return at::empty({0, w.size(0)}, x.options().requires_grad(false));
+  return joint(x, w, shrink(x, a, false, buf, meta, scale, scales), b, false, buf, meta);
+}
+
+int64_t adapter_error_code() { return bb::adapter_error_code(); }

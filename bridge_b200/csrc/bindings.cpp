@@ -139,6 +139,12 @@ void tp_gemm_rs(torch::Tensor a, torch::Tensor b, bool b_mn, std::vector<int64_t
 torch::Tensor tp_sum_slots(torch::Tensor recv, int64_t n, int64_t ms, int64_t N);
 void symm_clear_error();
 
+torch::Tensor adapter_linear(torch::Tensor x, torch::Tensor w, torch::Tensor a, torch::Tensor b, torch::Tensor buf,
+                             std::vector<int64_t> meta, double scale, c10::optional<torch::Tensor> scales,
+                             c10::optional<torch::Tensor> a_main, c10::optional<torch::Tensor> b_main,
+                             c10::optional<torch::Tensor> w_main);
+int64_t adapter_error_code();
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "bridge_b200 sm_100a kernels";
   m.def("rmsnorm_fwd", &rmsnorm_fwd);
@@ -212,6 +218,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gemm_error_code", &gemm_error_code);
   m.def("grouped_gemm", &grouped_gemm, "MoE grouped tcgen05 GEMM (device expert offsets)");
   m.def("grouped_gemm_wgrad", &grouped_gemm_wgrad, "MoE grouped weight gradient, FP32 accumulate");
+  m.def("adapter_linear", &adapter_linear, "shared projection beside the low-rank adapters of the rows' requests");
+  m.def("adapter_error_code", &adapter_error_code);
   m.def("launch_count", &bb_launch_count,
         "kernels launched by this extension so far");
 }

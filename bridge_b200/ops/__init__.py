@@ -1,6 +1,7 @@
 """Hot ops: sm_100a CUDA kernels on CUDA tensors, PyTorch formulations on CPU."""
 
 from .activation import swiglu
+from .adapter import AdapterRows, adapter_linear, adapter_rows
 from .attention import rectangular_causal_attention, tree_attention
 from .distill import fused_lm_head_topk_distill, topk_distill_loss
 from .gdn import causal_conv1d, chunk_gated_delta_rule
