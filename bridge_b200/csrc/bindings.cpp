@@ -144,6 +144,8 @@ torch::Tensor adapter_linear(torch::Tensor x, torch::Tensor w, torch::Tensor a, 
                              c10::optional<torch::Tensor> a_main, c10::optional<torch::Tensor> b_main,
                              c10::optional<torch::Tensor> w_main);
 int64_t adapter_error_code();
+torch::Tensor clip_grad_norm(std::vector<torch::Tensor> grads, bool per_slot, double grad_scale, double max_norm,
+                             c10::optional<torch::Tensor> max_norms, c10::optional<std::vector<torch::Tensor>> out);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "bridge_b200 sm_100a kernels";
@@ -220,6 +222,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("grouped_gemm_wgrad", &grouped_gemm_wgrad, "MoE grouped weight gradient, FP32 accumulate");
   m.def("adapter_linear", &adapter_linear, "shared projection beside the low-rank adapters of the rows' requests");
   m.def("adapter_error_code", &adapter_error_code);
+  m.def("clip_grad_norm", &clip_grad_norm, "norm over many gradients, of all or by slot, and the scaling to a bound");
   m.def("launch_count", &bb_launch_count,
         "kernels launched by this extension so far");
 }

@@ -1,0 +1,369 @@
+// The 2-norm over many gradient tensors, of all or slot by slot, and the gradients scaled down to a bound.
+//
+//   sums     one block per chunk of a tensor (of one slot of it): the chunk's sum of squares, in 64 bits
+//   finish   one block per slot: the sum over the slot's chunks in a fixed order, norm = sqrt(sum) / grad_scale and the
+//            factor min(1, max_norm / (norm + eps)) / grad_scale
+//   scale    one block per chunk: out = factor x, rounded once
+//
+// What bounds it: reading every value once for the norm, and once more, above the L2's 126 MB, to scale it.  The second
+// pass goes through the chunks backwards, so that what the first one read last is still there.  A list's pointers travel
+// in the kernels' parameters: no table is uploaded, and a captured graph keeps its own.
+//
+// Squares are FP32 in sums of eight, which are added up in 64 bits; sums outside [1e-25, 1e37] (infinite or vanishing
+// squares, and zeros) are taken again value by value in 64 bits, so that no finite gradient overflows or disappears.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <cuda_fp16.h>
+#include <torch/extension.h>
+
+#include <algorithm>
+#include <string>
+#include <vector>
+
+#include "common.cuh"
+
+namespace {
+
+using OptTensor = c10::optional<torch::Tensor>;
+constexpr int kThreads = 256;
+constexpr int kUnroll = 4;      // 16-byte loads in flight per thread
+
+enum Kind : int { kF32 = 0, kBF16 = 1, kF16 = 2 };
+
+struct Entry {
+  const void* in;
+  void* out;
+  long n;            // values of one slot
+  int first;         // the tensor's first chunk among all of the launch
+  int chunks;        // per slot
+  int at;            // the tensor's first chunk among a slot's
+  short kind, out_kind;
+};
+
+template <int N>
+struct Table {
+  Entry e[N];
+  int count, slots, total, per_slot;   // total: chunks of the launch; per_slot: chunks of a slot, of all launches
+  long chunk;                          // values
+};
+
+template <typename T>
+struct Io;
+template <>
+struct Io<float> {
+  static __device__ __forceinline__ float get(float v) { return v; }
+  static __device__ __forceinline__ float put(float v) { return v; }
+};
+template <>
+struct Io<__nv_bfloat16> {
+  static __device__ __forceinline__ float get(__nv_bfloat16 v) { return __bfloat162float(v); }
+  static __device__ __forceinline__ __nv_bfloat16 put(float v) { return __float2bfloat16_rn(v); }
+};
+template <>
+struct Io<__half> {
+  static __device__ __forceinline__ float get(__half v) { return __half2float(v); }
+  static __device__ __forceinline__ __half put(float v) { return __float2half_rn(v); }
+};
+
+template <typename T>
+struct alignas(16) Vec {
+  T v[16 / sizeof(T)];
+};
+
+struct Chunk {
+  int entry, slot, part;   // part: the chunk among its slot's, of all tensors
+  long begin, n;           // values from the tensor's base
+};
+
+template <int N>
+__device__ __forceinline__ Chunk locate(const Table<N>& t, int id) {
+  int lo = 0, hi = t.count - 1;
+  while (lo < hi) {        // the last tensor that begins at or before the chunk
+    const int mid = (lo + hi + 1) >> 1;
+    if (t.e[mid].first <= id) lo = mid;
+    else hi = mid - 1;
+  }
+  const Entry& e = t.e[lo];
+  const int local = id - e.first, slot = local / e.chunks, j = local - slot * e.chunks;
+  const long at = (long)j * t.chunk;
+  return {lo, slot, e.at + j, (long)slot * e.n + at, min(t.chunk, e.n - at)};
+}
+
+// Values before the first 16-byte boundary.
+template <typename T>
+__device__ __forceinline__ long lead(const T* p, long n) {
+  const long k = (long)((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / (long)sizeof(T);
+  return k < n ? k : n;
+}
+
+template <typename T>
+__device__ double chunk_sum(const T* x, long n) {
+  constexpr int V = 16 / sizeof(T);
+  const long head = lead(x, n), vecs = (n - head) / V;
+  const Vec<T>* body = reinterpret_cast<const Vec<T>*>(x + head);
+  double sum = 0.0;
+  const auto one = [&](float v) { sum += (double)v * (double)v; };
+  const auto add = [&](const Vec<T>& a) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) s = fmaf(Io<T>::get(a.v[i]), Io<T>::get(a.v[i]), s);
+    if (s >= 1e-25f && s <= 1e37f) {
+      sum += (double)s;
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) one(Io<T>::get(a.v[i]));
+    }
+  };
+  long i = threadIdx.x;
+  for (; i + (kUnroll - 1) * kThreads < vecs; i += kUnroll * kThreads) {
+    Vec<T> a[kUnroll];
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k) a[k] = body[i + k * kThreads];
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k) add(a[k]);
+  }
+  for (; i < vecs; i += kThreads) add(body[i]);
+  if (threadIdx.x < head) one(Io<T>::get(x[threadIdx.x]));
+  const long tail = head + vecs * V + threadIdx.x;
+  if (tail < n) one(Io<T>::get(x[tail]));
+  return sum;
+}
+
+__device__ __forceinline__ double block_sum_f64(double v, double* scratch) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+  __syncthreads();
+  double s = 0.0;
+  for (int i = 0; i < (int)(blockDim.x >> 5); ++i) s += scratch[i];
+  return s;
+}
+
+template <int N>
+__global__ void __launch_bounds__(kThreads) sums_kernel(const __grid_constant__ Table<N> t, double* parts) {
+  __shared__ double scratch[kThreads / 32];
+  const Chunk c = locate(t, blockIdx.x);
+  const Entry& e = t.e[c.entry];
+  double s;
+  if (e.kind == kF32) s = chunk_sum(static_cast<const float*>(e.in) + c.begin, c.n);
+  else if (e.kind == kBF16) s = chunk_sum(static_cast<const __nv_bfloat16*>(e.in) + c.begin, c.n);
+  else s = chunk_sum(static_cast<const __half*>(e.in) + c.begin, c.n);
+  s = block_sum_f64(s, scratch);
+  if (threadIdx.x == 0) parts[(long)c.slot * t.per_slot + c.part] = s;
+}
+
+__global__ void __launch_bounds__(1024) finish_kernel(const double* parts, int per_slot, double grad_scale,
+                                                      double max_norm, const float* max_norms, float* norm,
+                                                      float* factor) {
+  __shared__ double scratch[32];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < per_slot; i += 1024) s += parts[(long)blockIdx.x * per_slot + i];
+  s = block_sum_f64(s, scratch);
+  if (threadIdx.x) return;
+  const double n = sqrt(s) / grad_scale;
+  norm[blockIdx.x] = (float)n;
+  if (!factor) return;
+  const double bound = max_norms ? (double)max_norms[blockIdx.x] : max_norm;
+  // (a NaN norm makes the factor NaN)
+  factor[blockIdx.x] = (float)((n + 1e-6 <= bound ? 1.0 : bound / (n + 1e-6)) / grad_scale);
+}
+
+template <typename T, typename O>
+__device__ void chunk_scale(const T* x, O* y, long n, float f) {
+  constexpr int V = 16 / sizeof(T);
+  const long head = lead(x, n), vecs = (n - head) / V;
+  const Vec<T>* body = reinterpret_cast<const Vec<T>*>(x + head);
+  O* to = y + head;
+  const bool wide = reinterpret_cast<uintptr_t>(to) % 16 == 0;
+  const auto put = [&](const Vec<T>& a, long i) {
+    alignas(16) O r[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) r[k] = Io<O>::put(f * Io<T>::get(a.v[k]));
+    if (wide) {
+#pragma unroll
+      for (int k = 0; k < (int)(V * sizeof(O) / 16); ++k)
+        reinterpret_cast<uint4*>(to + i * V)[k] = reinterpret_cast<const uint4*>(r)[k];
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k) to[i * V + k] = r[k];
+    }
+  };
+  long i = threadIdx.x;
+  for (; i + (kUnroll - 1) * kThreads < vecs; i += kUnroll * kThreads) {
+    Vec<T> a[kUnroll];
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k) a[k] = body[i + k * kThreads];
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k) put(a[k], i + k * kThreads);
+  }
+  for (; i < vecs; i += kThreads) put(body[i], i);
+  if (threadIdx.x < head) y[threadIdx.x] = Io<O>::put(f * Io<T>::get(x[threadIdx.x]));
+  const long tail = head + vecs * V + threadIdx.x;
+  if (tail < n) y[tail] = Io<O>::put(f * Io<T>::get(x[tail]));
+}
+
+template <int N>
+__global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ Table<N> t, const float* factor) {
+  const Chunk c = locate(t, t.total - 1 - blockIdx.x);
+  const Entry& e = t.e[c.entry];
+  const float f = factor[c.slot];
+  if (f == 1.f && e.in == e.out) return;
+  if (e.kind == kF32) {
+    chunk_scale(static_cast<const float*>(e.in) + c.begin, static_cast<float*>(e.out) + c.begin, c.n, f);
+  } else if (e.kind == kBF16) {
+    const auto* x = static_cast<const __nv_bfloat16*>(e.in) + c.begin;
+    if (e.out_kind == kF32) chunk_scale(x, static_cast<float*>(e.out) + c.begin, c.n, f);
+    else chunk_scale(x, static_cast<__nv_bfloat16*>(e.out) + c.begin, c.n, f);
+  } else {
+    const auto* x = static_cast<const __half*>(e.in) + c.begin;
+    if (e.out_kind == kF32) chunk_scale(x, static_cast<float*>(e.out) + c.begin, c.n, f);
+    else chunk_scale(x, static_cast<__half*>(e.out) + c.begin, c.n, f);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+short kind_of(const torch::Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return kF32;
+    case at::kBFloat16: return kBF16;
+    case at::kHalf: return kF16;
+    default: TORCH_CHECK_TYPE(false, "clip_grad_norm: gradients are float32, bfloat16 or float16, got ", t.scalar_type());
+  }
+}
+
+struct Span {
+  uintptr_t lo, hi;
+  int i;
+  bool out;
+};
+
+// Every value is scaled once, from a gradient that nothing else writes.
+void check_apart(const std::vector<Entry>& e, int slots, const std::vector<torch::Tensor>& grads,
+                 const std::vector<torch::Tensor>& out) {
+  std::vector<Span> s;
+  bool rising = true;
+  for (size_t i = 0; i < grads.size(); ++i) {
+    const auto lo = reinterpret_cast<uintptr_t>(grads[i].data_ptr()), to = reinterpret_cast<uintptr_t>(out[i].data_ptr());
+    const size_t bytes = grads[i].numel() * grads[i].element_size(), out_bytes = out[i].numel() * out[i].element_size();
+    if (!bytes) continue;
+    const bool same = lo == to && bytes == out_bytes;
+    if (!s.empty() && s.back().hi > to) rising = false;
+    s.push_back({to, to + out_bytes, (int)i, true});
+    if (!same) {
+      rising = false;
+      s.push_back({lo, lo + bytes, (int)i, false});
+    }
+  }
+  if (rising) return;
+  std::sort(s.begin(), s.end(), [](const Span& a, const Span& b) { return a.lo < b.lo; });
+  uintptr_t out_end = 0, any_end = 0;     // where the outputs, and all, that began so far end
+  for (const Span& v : s) {
+    TORCH_CHECK_VALUE(v.lo >= (v.out ? any_end : out_end),
+                      "clip_grad_norm: an output shares memory with another output or with a gradient that is not its own");
+    any_end = std::max(any_end, v.hi);
+    if (v.out) out_end = std::max(out_end, v.hi);
+  }
+}
+
+constexpr int kFew = 48, kMany = 640;   // tensors of a launch: parameters of 2 KB, or of 30 KB
+
+template <int N>
+void fill(Table<N>& t, const std::vector<Entry>& all, size_t from, int slots, int per_slot, long chunk) {
+  t.count = (int)std::min<size_t>(N, all.size() - from);
+  t.slots = slots, t.per_slot = per_slot, t.chunk = chunk, t.total = 0;
+  for (int i = 0; i < t.count; ++i) {
+    t.e[i] = all[from + i];
+    t.e[i].first = t.total;
+    t.total += slots * t.e[i].chunks;
+  }
+}
+
+template <int N>
+void run(const std::vector<Entry>& all, int slots, int per_slot, long chunk, double* parts, const float* factor,
+         cudaStream_t stream) {
+  // (the scaling takes the lists backwards too)
+  const size_t lists = (all.size() + N - 1) / N;
+  for (size_t l = 0; l < lists; ++l) {
+    Table<N> t;
+    fill(t, all, (factor ? lists - 1 - l : l) * N, slots, per_slot, chunk);
+    if (factor) scale_kernel<N><<<t.total, kThreads, 0, stream>>>(t, factor);
+    else sums_kernel<N><<<t.total, kThreads, 0, stream>>>(t, parts);
+    BB_POST_LAUNCH();
+  }
+}
+
+}  // namespace
+
+// Norms [slots] ([] without `per_slot`) of the gradients over `grad_scale`; with `out` (the gradients themselves, or
+// tensors like them), out = gradient * min(1, max_norm / (norm + 1e-6)) / grad_scale.
+torch::Tensor clip_grad_norm(std::vector<torch::Tensor> grads, bool per_slot, double grad_scale, double max_norm,
+                             OptTensor max_norms, c10::optional<std::vector<torch::Tensor>> out) {
+  TORCH_CHECK_VALUE(!grads.empty(), "clip_grad_norm: no gradients");
+  const auto device = grads[0].device();
+  TORCH_CHECK(device.is_cuda(), "clip_grad_norm: CUDA tensors");
+  const int64_t slots = per_slot ? (grads[0].dim() ? grads[0].size(0) : 0) : 1;
+  TORCH_CHECK_VALUE(!per_slot || (slots >= 1 && slots < (1 << 16)), "clip_grad_norm: per_slot needs gradients stacked by slot");
+  TORCH_CHECK_VALUE(!out.has_value() || out->size() == grads.size(), "clip_grad_norm: one output per gradient");
+  const c10::cuda::CUDAGuard guard(device);
+  // chunks of 64 KB of FP32; of 8 KB where all together are too few for the SMs
+  int64_t total = 0;
+  for (const auto& g : grads) total += g.numel();
+  const long chunk = total > (1 << 24) ? 16384 : 2048;
+  std::vector<Entry> all;
+  all.reserve(grads.size());
+  int64_t per = 0, blocks = 0;
+  for (size_t i = 0; i < grads.size(); ++i) {
+    const auto& g = grads[i];
+    TORCH_CHECK_TYPE(g.device() == device, "clip_grad_norm: gradients are on ", device, " and ", g.device());
+    Entry e{};
+    e.kind = kind_of(g);
+    const bool dense = per_slot ? g.is_contiguous() : g.is_non_overlapping_and_dense();
+    TORCH_CHECK_VALUE(dense, "clip_grad_norm: a gradient has to be dense (and contiguous where norms go by slot)");
+    TORCH_CHECK_VALUE(!per_slot || (g.dim() && g.size(0) == slots), "clip_grad_norm: gradients are stacks of ",
+                      std::to_string(slots), " slots, got one of ", g.dim() ? std::to_string(g.size(0)) : "none");
+    if (out.has_value()) {
+      const auto& o = (*out)[i];
+      TORCH_CHECK_TYPE(o.device() == device && (o.scalar_type() == g.scalar_type() || o.scalar_type() == at::kFloat),
+                       "clip_grad_norm: an output is float32 or its gradient's type, on its device");
+      TORCH_CHECK_VALUE(o.sizes() == g.sizes() && (o.strides() == g.strides() || (o.is_contiguous() && g.is_contiguous())),
+                        "clip_grad_norm: an output has its gradient's sizes and strides");
+      e.out = o.data_ptr();
+      e.out_kind = kind_of(o);
+    }
+    if (g.numel() == 0) continue;
+    e.in = g.data_ptr();
+    e.n = g.numel() / slots;
+    e.chunks = (int)((e.n + chunk - 1) / chunk);
+    e.at = (int)per;
+    per += e.chunks;
+    blocks += slots * e.chunks;
+    all.push_back(e);
+  }
+  TORCH_CHECK_VALUE(blocks < (1ll << 31), "clip_grad_norm: too many values");
+  if (out.has_value()) check_apart(all, (int)slots, grads, *out);
+  TORCH_CHECK_VALUE(!max_norms.has_value() ||
+                        (max_norms->device() == device && max_norms->scalar_type() == at::kFloat &&
+                         max_norms->is_contiguous() && max_norms->numel() == slots),
+                    "clip_grad_norm: max_norm is a number or float32, one per slot, on the gradients' device");
+  const auto f32 = at::TensorOptions().device(device).dtype(at::kFloat);
+  auto norm = per_slot ? at::empty({slots}, f32) : at::empty({}, f32);
+  auto parts = at::empty({slots * per + slots}, f32.dtype(at::kDouble));     // sums, then factors
+  double* sums = parts.data_ptr<double>();
+  float* factor = reinterpret_cast<float*>(sums + slots * per);
+  const auto stream = at::cuda::getCurrentCUDAStream();
+  const bool few = all.size() <= kFew;
+  if (!all.empty()) {
+    if (few) run<kFew>(all, (int)slots, (int)per, chunk, sums, nullptr, stream);
+    else run<kMany>(all, (int)slots, (int)per, chunk, sums, nullptr, stream);
+  }
+  finish_kernel<<<(int)slots, 1024, 0, stream>>>(sums, (int)per, grad_scale, max_norm,
+                                                 max_norms.has_value() ? max_norms->data_ptr<float>() : nullptr,
+                                                 norm.data_ptr<float>(), out.has_value() ? factor : nullptr);
+  BB_POST_LAUNCH();
+  if (out.has_value() && !all.empty()) {
+    if (few) run<kFew>(all, (int)slots, (int)per, chunk, nullptr, factor, stream);
+    else run<kMany>(all, (int)slots, (int)per, chunk, nullptr, factor, stream);
+    for (const auto& o : *out) o.unsafeGetTensorImpl()->bump_version();
+  }
+  return norm;
+}
