@@ -114,6 +114,12 @@ def _init(weight: Tensor, std: float, seed_offset: int) -> None:
         weight.normal_(0.0, std)
 
 
+def _product(x: Tensor, layer: nn.Module) -> Tensor:
+    """The layer's own product, with its adapters beside it where it has any in use."""
+    y = layer.adapter(x, layer.weight) if layer.adapter is not None else None
+    return linear(x, layer.weight) if y is None else y
+
+
 class ColumnParallelLinear(nn.Module):
     """``out_features`` sharded over the TP group; ``sequence_parallel`` all-gathers tokens first."""
 
@@ -124,6 +130,7 @@ class ColumnParallelLinear(nn.Module):
         if out_features % n:
             raise ValueError(f"out_features {out_features} not divisible by TP size {n}")
         self.group, self.sp = group, sequence_parallel
+        self.adapter = None       # set by models.adapters.AdapterSet (unsharded layers)
         self.in_features, self.out_features = in_features, out_features
         self.weight = nn.Parameter(torch.empty(out_features // n, in_features, dtype=dtype, device=device))
         _init(self.weight, std, 0)
@@ -137,7 +144,7 @@ class ColumnParallelLinear(nn.Module):
             if comm is not None:
                 return ag_linear(x, self.weight, comm)      # all-gather fused into the GEMM
         x = gather_from_sp(x, self.group) if self.sp else copy_to_tp(x, self.group)
-        return linear(x, self.weight)
+        return _product(x, self)
 
 
 class RowParallelLinear(nn.Module):
@@ -150,6 +157,7 @@ class RowParallelLinear(nn.Module):
         if in_features % n:
             raise ValueError(f"in_features {in_features} not divisible by TP size {n}")
         self.group, self.sp = group, sequence_parallel
+        self.adapter = None       # set by models.adapters.AdapterSet (unsharded layers)
         self.weight = nn.Parameter(torch.empty(out_features, in_features // n, dtype=dtype, device=device))
         _init(self.weight, std, 1)
         self.weight.tp_split_dim = 1  # type: ignore[attr-defined]
@@ -161,7 +169,7 @@ class RowParallelLinear(nn.Module):
             comm = fused_comm(self.group, x)
             if comm is not None:
                 return linear_rs(x, self.weight, comm)      # reduce-scatter fused into the GEMM epilogue
-        y = linear(x, self.weight)
+        y = _product(x, self)
         return reduce_scatter_to_sp(y, self.group) if self.sp else reduce_from_tp(y, self.group)
 
 
