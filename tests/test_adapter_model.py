@@ -67,11 +67,14 @@ def _train(device, dtype=None):
     g = torch.Generator().manual_seed(0)
     ids = torch.randint(0, cfg.vocab_size, (cu[-1],), generator=g).to(device)
     pos = torch.arange(cu[-1], device=device)
+    way = torch.randn(cu[-1], cfg.hidden_size, generator=g).to(device)
     records = []
     for _ in range(2):
         with adapters.use(rows):
             hidden = model(ids, pos, cu[-1])
-        hidden.float().square().mean().backward()
+        # (a linear functional: the mean square of what the last RMSNorm gives is 1 whatever the adapters are, so its
+        # gradient would be nothing but rounding)
+        (hidden.float() * way).mean().backward()
         raw = [x.clone() for x in adapters.gradients()]
         norms = adapters.clip_grad_norm_(1e-4)
         records.append((raw, norms, [x.clone() for x in adapters.gradients()]))
@@ -102,7 +105,8 @@ def test_training_run_on_gpu(monkeypatch):
     _check(adapters, records)
     monkeypatch.setenv("BRIDGE_B200_IMPL", "reference")
     _, plain = _train("cuda")
-    # BF16 activations rounded in other places: gradients of the first step agree to a few per cent as vectors
+    # some 20 BF16 roundings (half a step: 2^-8) of activations and their gradients on the way through two layers, in
+    # other places: sqrt(20) 2^-8 = 1.7 % of a vector's length, allowed three times
     for got, want in zip(records[0][0], plain[0][0]):
         assert (got - want).norm() <= 0.05 * want.norm() + 1e-8
 
