@@ -80,6 +80,11 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
   return v;
 }
 
+// Programmatic dependent launch: the next kernel of the stream may begin (its blocks find room as this grid's end); and
+// what a kernel that began so waits for before it reads what the one before it wrote.
+__device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // A block of rows' accumulator (TMEM, `cols` columns) into this block's shared memory, row stride cols + 4 floats
 // (rows 16 bytes apart in the banks: neither these stores nor the sums' loads collide).  Warps 2-5.
 __device__ __forceinline__ void spill(uint32_t tmem, float* part, int cols, bool any) {
@@ -99,6 +104,12 @@ __device__ __forceinline__ void spill(uint32_t tmem, float* part, int cols, bool
       if (c + i < cols)
         *reinterpret_cast<uint4*>(part + row * (cols + 4) + c + i) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
   }
+}
+
+__device__ __forceinline__ float ld_cluster1(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
 }
 
 // The sum over the cluster's partial accumulators of four columns, in rank order.
@@ -122,7 +133,8 @@ struct ShrinkParams {
   bool half;
 };
 
-// A cluster of `ranks` blocks takes 128 rows, each block a stretch of K; the partial sums meet in shared memory.
+// A cluster of `ranks` blocks takes one slot's rows of a tile of 128, each block a stretch of K; the partial sums meet in
+// shared memory.  Rows without an adapter are not written: nothing reads them.
 template <bool OP_MN>
 __global__ void __launch_bounds__(kThreads)
     adapter_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_op,
@@ -133,9 +145,11 @@ __global__ void __launch_bounds__(kThreads)
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + p.stages * stage_bytes);
   uint64_t* empty = full + p.stages;
   uint64_t* done = empty + p.stages;
-  uint32_t* slot_word = reinterpret_cast<uint32_t*>(done + 1);
+  uint32_t* tmem_word = reinterpret_cast<uint32_t*>(done + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = (int)sm100::cluster_ctarank(), tile = blockIdx.x / p.ranks;
+  const int rank = (int)sm100::cluster_ctarank();
+  const int* unit = p.plan.units + (size_t)(blockIdx.x / p.ranks) * 8;
+  const int tile = __ldg(unit), slot = __ldg(unit + 1);
   const int kb0 = (int)((long)p.nk * rank / p.ranks), kb1 = (int)((long)p.nk * (rank + 1) / p.ranks);
 
   if (threadIdx.x == 0) {
@@ -146,74 +160,54 @@ __global__ void __launch_bounds__(kThreads)
     sm100::mbar_init(done, 1);
     sm100::fence_mbar_init();
   }
-  if (warp == 1) sm100::tmem_alloc(slot_word, 128);
+  if (warp == 1) sm100::tmem_alloc(tmem_word, 128);
   sm100::tc_fence_before();
   __syncthreads();
   sm100::tc_fence_after();
-  const uint32_t tmem = *slot_word;
+  const uint32_t tmem = *tmem_word;
+  let_next_begin();        // (not before: a block that waits for TMEM must not wait for one that waits for this grid)
 
-  bool any = false;
-  {
-    TilePairs it(p.plan, tile);
-    int slot;
-    uint32_t off[4];
-    any = kb1 > kb0 && it.next(slot, off);
-  }
-  if (warp == 0 && lane == 0 && any) {
-    TilePairs it(p.plan, tile);
-    int slot, stage = 0;
-    uint32_t off[4], phase = 0;
-    bool ok = true;
-    while (ok && it.next(slot, off)) {
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!sm100::mbar_wait(&empty[stage], phase ^ 1, &g_error, 31)) {
-          ok = false;
-          break;
-        }
-        unsigned char* dst = smem + stage * stage_bytes;
-        sm100::mbar_expect_tx(&full[stage], stage_bytes);
-        sm100::tma_load_2d(dst, &map_x, &full[stage], kb * BK, tile * BM);
-        if (OP_MN) {
-          for (int i = 0; i < p.cols / 64; ++i)
-            sm100::tma_load_3d(dst + kXBytes + i * 8192, &map_op, &full[stage], 64 * i, kb * BK, slot);
-        } else {
-          sm100::tma_load_3d(dst + kXBytes, &map_op, &full[stage], kb * BK, 0, slot);
-        }
-        if (++stage == p.stages) stage = 0, phase ^= 1;
+  if (warp == 0 && lane == 0) {
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!sm100::mbar_wait(&empty[stage], phase ^ 1, &g_error, 31)) break;
+      unsigned char* dst = smem + stage * stage_bytes;
+      sm100::mbar_expect_tx(&full[stage], stage_bytes);
+      sm100::tma_load_2d(dst, &map_x, &full[stage], kb * BK, tile * BM);
+      if (OP_MN) {
+        for (int i = 0; i < p.cols / 64; ++i)
+          sm100::tma_load_3d(dst + kXBytes + i * 8192, &map_op, &full[stage], 64 * i, kb * BK, slot);
+      } else {
+        sm100::tma_load_3d(dst + kXBytes, &map_op, &full[stage], kb * BK, 0, slot);
       }
+      if (++stage == p.stages) stage = 0, phase ^= 1;
     }
-  } else if (warp == 1 && lane == 0 && any) {
-    TilePairs it(p.plan, tile);
-    int slot, stage = 0;
-    uint32_t off[4], phase = 0;
-    bool ok = true;
-    while (ok && it.next(slot, off)) {
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!sm100::mbar_wait(&full[stage], phase, &g_error, 32)) {
-          ok = false;
-          break;
-        }
-        sm100::tc_fence_after();
-        const uint32_t a = sm100::smem_addr(smem + stage * stage_bytes), b = a + kXBytes;
+  } else if (warp == 1 && lane == 0 && kb1 > kb0) {
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!sm100::mbar_wait(&full[stage], phase, &g_error, 32)) break;
+      sm100::tc_fence_after();
+      const uint32_t a = sm100::smem_addr(smem + stage * stage_bytes), b = a + kXBytes;
 #pragma unroll
-        for (int kk = 0; kk < BK / 16; ++kk)
-          sm100::umma_masked(tmem, sm100::umma_desc_sw128(a + kk * 32, 16, 1024),
-                             OP_MN ? sm100::umma_desc_sw128(b + kk * 2048, 8192, 1024)
-                                   : sm100::umma_desc_sw128(b + kk * 32, 16, 1024),
-                             p.idesc, kb > kb0 || kk > 0, off);
-        sm100::umma_commit(&empty[stage]);
-        if (++stage == p.stages) stage = 0, phase ^= 1;
-      }
+      for (int kk = 0; kk < BK / 16; ++kk)
+        sm100::umma_bf16(tmem, sm100::umma_desc_sw128(a + kk * 32, 16, 1024),
+                         OP_MN ? sm100::umma_desc_sw128(b + kk * 2048, 8192, 1024)
+                               : sm100::umma_desc_sw128(b + kk * 32, 16, 1024),
+                         p.idesc, kb > kb0 || kk > 0);
+      sm100::umma_commit(&empty[stage]);
+      if (++stage == p.stages) stage = 0, phase ^= 1;
     }
     sm100::umma_commit(done);
   }
   __syncwarp();
   float* part = reinterpret_cast<float*>(smem);
   if (warp >= 2) {
-    if (any) sm100::mbar_wait(done, 0, &g_error, 33);
+    if (kb1 > kb0) sm100::mbar_wait(done, 0, &g_error, 33);
     __syncwarp();
     sm100::tc_fence_after();
-    spill(tmem, part, p.cols, any);
+    spill(tmem, part, p.cols, kb1 > kb0);
     sm100::tc_fence_before();
   }
   __syncthreads();
@@ -221,18 +215,146 @@ __global__ void __launch_bounds__(kThreads)
   // this block's share of the rows: 8 columns a step, the finished values 16 bytes at a time
   const int rows = BM / p.ranks, groups = p.R / 8;
   const uint32_t base = sm100::smem_addr(part);
+  const float f = p.scales ? __ldg(p.scales + slot) : p.scale;
   for (int i = threadIdx.x; i < rows * groups; i += kThreads) {
-    const int r = rank * rows + i / groups, c = (i % groups) * 8, row = tile * BM + r;
-    if (row >= p.T) continue;
-    const int slot = __ldg(p.plan.row_slot + row);
-    uint4 out = make_uint4(0, 0, 0, 0);
-    if (slot >= 0) {
-      const float f = p.scales ? __ldg(p.scales + slot) : p.scale;
-      const float4 v = joined(base, r * (p.cols + 4) + c, p.ranks), w = joined(base, r * (p.cols + 4) + c + 4, p.ranks);
-      out = make_uint4(pack2(f * v.x, f * v.y, p.half), pack2(f * v.z, f * v.w, p.half),
-                       pack2(f * w.x, f * w.y, p.half), pack2(f * w.z, f * w.w, p.half));
+    const int r = rank * rows + i / groups, c = (i % groups) * 8;
+    if (__ldg(unit + 4 + r / 32) >> (r % 32) & 1) continue;      // another request's row
+    const float4 v = joined(base, r * (p.cols + 4) + c, p.ranks), w = joined(base, r * (p.cols + 4) + c + 4, p.ranks);
+    *reinterpret_cast<uint4*>(p.u + (size_t)(tile * BM + r) * p.R + c) =
+        make_uint4(pack2(f * v.x, f * v.y, p.half), pack2(f * v.z, f * v.w, p.half),
+                   pack2(f * w.x, f * w.y, p.half), pack2(f * w.z, f * w.w, p.half));
+  }
+  sm100::cluster_sync();   // the peers' sums stay until all have read them
+  if (warp == 1) {
+    sm100::tc_fence_after();
+    sm100::tmem_dealloc(tmem, 128);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ few rows
+struct FewParams {
+  AdapterPlan plan;
+  const uint16_t *u, *low;
+  uint16_t* y;
+  int T, N, R, cols, stages, nk, ranks;
+  uint32_t idesc;
+  bool half;
+};
+
+__device__ __forceinline__ float2 unpack2(uint32_t v, bool half) {
+  if (half) return __half22float2(*reinterpret_cast<const __half2*>(&v));
+  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+}
+__device__ __forceinline__ float unpack1(uint16_t v, bool half) {
+  return half ? __half2float(__ushort_as_half(v)) : __bfloat162float(__ushort_as_bfloat16(v));
+}
+
+// At most 128 rows: bound by the read of W, so W takes the matrix instructions' wide side.  A cluster of `ranks` blocks
+// streams 128 rows (with MN: columns) of W, each block a stretch of K, for all rows of x: y^T = W x^T.  The low-rank part
+// is a few products per value, made with ordinary FP32 arithmetic where the partial sums meet.  u is waited for there,
+// so that this kernel streams W while the one before it still makes u.
+template <bool MN>
+__global__ void __launch_bounds__(kThreads)
+    adapter_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+                       const FewParams p) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int stage_bytes = kXBytes + p.cols * 128;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + p.stages * stage_bytes);
+  uint64_t* empty = full + p.stages;
+  uint64_t* done = empty + p.stages;
+  uint32_t* tmem_word = reinterpret_cast<uint32_t*>(done + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)sm100::cluster_ctarank(), n0 = blockIdx.x / p.ranks * BM;
+  const int kb0 = (int)((long)p.nk * rank / p.ranks), kb1 = (int)((long)p.nk * (rank + 1) / p.ranks);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      sm100::mbar_init(&full[s], 1);
+      sm100::mbar_init(&empty[s], 1);
     }
-    *reinterpret_cast<uint4*>(p.u + (size_t)row * p.R + c) = out;
+    sm100::mbar_init(done, 1);
+    sm100::fence_mbar_init();
+  }
+  if (warp == 1) sm100::tmem_alloc(tmem_word, 128);
+  sm100::tc_fence_before();
+  __syncthreads();
+  sm100::tc_fence_after();
+  const uint32_t tmem = *tmem_word;
+
+  if (warp == 0 && lane == 0) {
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!sm100::mbar_wait(&empty[stage], phase ^ 1, &g_error, 61)) break;
+      unsigned char* dst = smem + stage * stage_bytes;
+      sm100::mbar_expect_tx(&full[stage], stage_bytes);
+      if (MN) {
+        sm100::tma_load_2d(dst, &map_w, &full[stage], n0, kb * BK);
+        sm100::tma_load_2d(dst + 8192, &map_w, &full[stage], n0 + 64, kb * BK);
+      } else {
+        sm100::tma_load_2d(dst, &map_w, &full[stage], kb * BK, n0);
+      }
+      sm100::tma_load_2d(dst + kXBytes, &map_x, &full[stage], kb * BK, 0);
+      if (++stage == p.stages) stage = 0, phase ^= 1;
+    }
+  } else if (warp == 1 && lane == 0 && kb1 > kb0) {
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!sm100::mbar_wait(&full[stage], phase, &g_error, 62)) break;
+      sm100::tc_fence_after();
+      const uint32_t a = sm100::smem_addr(smem + stage * stage_bytes), b = a + kXBytes;
+#pragma unroll
+      for (int kk = 0; kk < BK / 16; ++kk)
+        sm100::umma_bf16(tmem, MN ? sm100::umma_desc_sw128(a + kk * 2048, 8192, 1024)
+                                  : sm100::umma_desc_sw128(a + kk * 32, 16, 1024),
+                         sm100::umma_desc_sw128(b + kk * 32, 16, 1024), p.idesc, kb > kb0 || kk > 0);
+      sm100::umma_commit(&empty[stage]);
+      if (++stage == p.stages) stage = 0, phase ^= 1;
+    }
+    sm100::umma_commit(done);
+  }
+  __syncwarp();
+  float* part = reinterpret_cast<float*>(smem);
+  if (warp >= 2) {
+    if (kb1 > kb0) sm100::mbar_wait(done, 0, &g_error, 63);
+    __syncwarp();
+    sm100::tc_fence_after();
+    spill(tmem, part, p.cols, kb1 > kb0);
+    sm100::tc_fence_before();
+  }
+  __syncthreads();
+  sm100::cluster_sync();
+  wait_for_previous();
+  // this block's share of W's rows; neighbours take neighbouring columns of y
+  const int rows = BM / p.ranks;
+  const uint32_t base = sm100::smem_addr(part);
+  for (int i = threadIdx.x; i < rows * p.T; i += kThreads) {
+    const int r = rank * rows + i % rows, t = i / rows, n = n0 + r;
+    if (n >= p.N) continue;
+    float v = 0.f;
+    for (int j = 0; j < p.ranks; ++j) v += ld_cluster1(sm100::mapa(base + (r * (p.cols + 4) + t) * 4, j));
+    const int slot = __ldg(p.plan.row_slot + t);
+    if (slot >= 0) {
+      const uint16_t* u = p.u + (size_t)t * p.R;
+      for (int c = 0; c < p.R; c += 8) {
+        const uint4 a = *reinterpret_cast<const uint4*>(u + c);
+        const float2 a0 = unpack2(a.x, p.half), a1 = unpack2(a.y, p.half), a2 = unpack2(a.z, p.half), a3 = unpack2(a.w, p.half);
+        if (MN) {
+          const uint16_t* b = p.low + ((size_t)slot * p.R + c) * p.N + n;
+          const float q[8] = {a0.x, a0.y, a1.x, a1.y, a2.x, a2.y, a3.x, a3.y};
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v = fmaf(q[j], unpack1(__ldg(b + (size_t)j * p.N), p.half), v);
+        } else {
+          const uint4 b = __ldg(reinterpret_cast<const uint4*>(p.low + ((size_t)slot * p.N + n) * p.R + c));
+          const float2 b0 = unpack2(b.x, p.half), b1 = unpack2(b.y, p.half), b2 = unpack2(b.z, p.half), b3 = unpack2(b.w, p.half);
+          v = fmaf(a0.x, b0.x, v), v = fmaf(a0.y, b0.y, v), v = fmaf(a1.x, b1.x, v), v = fmaf(a1.y, b1.y, v);
+          v = fmaf(a2.x, b2.x, v), v = fmaf(a2.y, b2.y, v), v = fmaf(a3.x, b3.x, v), v = fmaf(a3.y, b3.y, v);
+        }
+      }
+    }
+    p.y[(size_t)t * p.N + n] = pack1(v, p.half);
   }
   sm100::cluster_sync();   // the peers' sums stay until all have read them
   if (warp == 1) {
@@ -334,6 +456,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         TilePairs it(p.plan, mt);
         int slot;
         uint32_t off[4];
+        if (t == blockIdx.x) {
+          wait_for_previous();       // u, which TMA reads from here on
+          asm volatile("fence.proxy.async.global;" ::: "memory");
+        }
         while (ok && it.next(slot, off)) {
           for (int rb = 0; rb < rank_blocks; ++rb) {
             if (!claim()) break;
@@ -629,21 +755,31 @@ cudaError_t allow_smem(Kernel kernel, int bytes, std::atomic<unsigned long long>
   return e;
 }
 
+// `early`: the kernel may begin while the one before it in the stream ends (it waits by itself for what that one wrote).
 template <typename... P, typename... A>
-cudaError_t launch(void (*kernel)(P...), int grid, int smem, int cluster, cudaStream_t stream, const A&... args) {
+cudaError_t launch(void (*kernel)(P...), int grid, int smem, int cluster, bool early, cudaStream_t stream, const A&... args) {
   cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = cluster, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = early ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
   if (e == cudaSuccess) launch_counter().fetch_add(1);
   return e;
+}
+
+// Blocks of a cluster: as many (1, 2, 4, 8) as it takes to have two per SM, while each still has two blocks of the sum.
+int split(long clusters, int nk) {
+  int ranks = 1;
+  while (ranks < 8 && clusters * ranks < 2 * sm_count() && nk >= 4 * ranks) ranks *= 2;
+  return ranks;
 }
 
 constexpr int kMaxSmem = 227 * 1024;
@@ -663,14 +799,41 @@ cudaError_t run_shrink(const AdapterShrink& a, cudaStream_t stream) {
   p.op_bytes = cols * 128;
   p.nk = (a.K + BK - 1) / BK;
   p.stages = 4;
-  p.ranks = 1;
+  p.ranks = split(a.plan.num_units, p.nk);
   p.idesc = sm100::umma_idesc_bf16(BM, cols, false, OP_MN) & ~(a.half ? sm100::kIdescBf16 : 0u);
   p.half = a.half;
   const int smem = std::max(p.stages * (kXBytes + p.op_bytes), BM * (cols + 4) * 4) + 256 + 1024;
   static std::atomic<unsigned long long> done{0};
   const cudaError_t e = allow_smem(adapter_shrink_kernel<OP_MN>, kMaxSmem, done);
   if (e != cudaSuccess) return e;
-  return launch(adapter_shrink_kernel<OP_MN>, (a.T + BM - 1) / BM * p.ranks, smem, p.ranks, stream, x, op, p);
+  return launch(adapter_shrink_kernel<OP_MN>, a.plan.num_units * p.ranks, smem, p.ranks, false, stream, x, op, p);
+}
+
+constexpr int kFewRows = 128;
+
+template <bool MN>
+cudaError_t run_few(const AdapterJoint& a, cudaStream_t stream) {
+  alignas(64) CUtensorMap w, x;
+  const int cols = (a.T + 15) / 16 * 16;
+  if (!(MN ? encode(&w, a.w, a.N, a.K, a.ldw, 0, 64, a.half) : encode(&w, a.w, a.K, a.N, a.ldw, 0, BM, a.half)) ||
+      !encode(&x, a.x, a.K, a.T, a.ldx, 0, cols, a.half))
+    return cudaErrorInvalidValue;
+  FewParams p{};
+  p.plan = a.plan;
+  p.u = static_cast<const uint16_t*>(a.u), p.low = static_cast<const uint16_t*>(a.low);
+  p.y = static_cast<uint16_t*>(a.y);
+  p.T = a.T, p.N = a.N, p.R = a.R, p.cols = cols;
+  p.nk = (a.K + BK - 1) / BK;
+  p.stages = 4;
+  const int tiles = (a.N + BM - 1) / BM;
+  p.ranks = split(tiles, p.nk);
+  p.idesc = sm100::umma_idesc_bf16(BM, cols, MN, false) & ~(a.half ? sm100::kIdescBf16 : 0u);
+  p.half = a.half;
+  const int smem = std::max(p.stages * (kXBytes + cols * 128), BM * (cols + 4) * 4) + 256 + 1024;
+  static std::atomic<unsigned long long> done{0};
+  const cudaError_t e = allow_smem(adapter_few_kernel<MN>, kMaxSmem, done);
+  if (e != cudaSuccess) return e;
+  return launch(adapter_few_kernel<MN>, tiles * p.ranks, smem, p.ranks, a.plan.num_units > 0, stream, w, x, p);
 }
 
 template <bool MN, int BN>
@@ -691,21 +854,22 @@ cudaError_t run_joint(const AdapterJoint& a, cudaStream_t stream) {
   const cudaError_t e = allow_smem(adapter_joint_kernel<MN, BN>, JointSmem<BN>::TOTAL, done);
   if (e != cudaSuccess) return e;
   const long tiles = (long)((a.T + BM - 1) / BM) * ((a.N + BN - 1) / BN);
-  return launch(adapter_joint_kernel<MN, BN>, (int)std::min<long>(tiles, sm_count()), JointSmem<BN>::TOTAL, 1, stream, x, w,
-                u, low, p);
+  return launch(adapter_joint_kernel<MN, BN>, (int)std::min<long>(tiles, sm_count()), JointSmem<BN>::TOTAL, 1,
+                a.plan.num_units > 0, stream, x, w, u, low, p);
 }
 
 }  // namespace
 
 cudaError_t launch_adapter_shrink(const AdapterShrink& a, cudaStream_t stream) {
   const cudaError_t e = have_context();
-  if (e != cudaSuccess) return e;
+  if (e != cudaSuccess || a.plan.num_units == 0) return e;
   return a.op_mn ? run_shrink<true>(a, stream) : run_shrink<false>(a, stream);
 }
 
 cudaError_t launch_adapter_joint(const AdapterJoint& a, cudaStream_t stream) {
   const cudaError_t e = have_context();
   if (e != cudaSuccess) return e;
+  if (a.T <= kFewRows) return a.mn ? run_few<true>(a, stream) : run_few<false>(a, stream);
   return a.mn ? run_joint<true, 256>(a, stream) : run_joint<false, 256>(a, stream);
 }
 
@@ -733,7 +897,7 @@ cudaError_t launch_adapter_grads(const AdapterGrads& a, cudaStream_t stream) {
   static std::atomic<unsigned long long> done{0};
   e = allow_smem(adapter_grads_kernel, kMaxSmem, done);
   if (e != cudaSuccess) return e;
-  return launch(adapter_grads_kernel, a.S * (p.tiles_a + p.tiles_b) * p.ranks, smem, p.ranks, stream, x, dy, u, du, p);
+  return launch(adapter_grads_kernel, a.S * (p.tiles_a + p.tiles_b) * p.ranks, smem, p.ranks, false, stream, x, dy, u, du, p);
 }
 
 int adapter_error_code() {

@@ -13,12 +13,14 @@ struct AdapterPlan {
   const int* row_slot;     // [T] slot, or -1
   const int* tile_start;   // [ceil(T / 256) + 1] first pair of each tile of 256 rows
   const int* pairs;        // [P][12] (slot, 0, 0, 0, 256 bits: set where a row of the tile is NOT the slot's)
+  const int* units;        // [.][8] (tile of 128 rows, slot, 0, 0, 128 bits as above): every pair by itself
   const int* block_start;  // [slots + 1] first block of each slot
   const int* blocks;       // [.][2] (first row, rows <= 64) of one slot, in row order
+  int num_units;
   int slots;               // slots the plan speaks of: the largest one + 1
 };
 
-// u[t, r] = scale_s sum_k x[t, k] op_s[r, k] for the row's slot s, 0 without one
+// u[t, r] = scale_s sum_k x[t, k] op_s[r, k] for the row's slot s; rows without one are left as they are
 struct AdapterShrink {
   const void* x;           // [T, K], row stride ldx
   const void* op;          // [S, R, K], or [S, K, R] with `op_mn`

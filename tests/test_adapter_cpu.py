@@ -51,11 +51,11 @@ def test_plan(seed):
     for n in lengths:
         cu.append(cu[-1] + n)
     rows = adapter_rows(cu, slots, device="cpu")
-    total, top, o_row, o_tile, o_pair, o_start, o_block = rows.meta
+    total, top, units, o_row, o_tile, o_pair, o_unit, o_start, o_block = rows.meta
     table = rows.table.tolist()
     want = row_slots(cu, slots, "cpu").tolist()
     assert total == cu[-1] and top == max(slots) + 1 and table[o_row:o_row + total] == want
-    assert all(o % 4 == 0 for o in (o_row, o_tile, o_pair, o_start, o_block))
+    assert all(o % 4 == 0 for o in (o_row, o_tile, o_pair, o_unit, o_start, o_block))
     seen = [-1] * total
     for t in range(-(-total // 256)):
         for p in range(table[o_tile + t], table[o_tile + t + 1]):
@@ -64,6 +64,15 @@ def test_plan(seed):
                 if not pair[4 + i // 32] >> (i % 32) & 1:
                     assert seen[256 * t + i] == -1
                     seen[256 * t + i] = pair[0]
+    assert seen == want
+    seen = [-1] * total
+    for u in range(units):
+        unit = table[o_unit + 8 * u:o_unit + 8 * u + 8]
+        here = [i for i in range(128) if not unit[4 + i // 32] >> (i % 32) & 1]
+        assert here
+        for i in here:
+            assert seen[128 * unit[0] + i] == -1
+            seen[128 * unit[0] + i] = unit[1]
     assert seen == want
     seen = [-1] * total
     for s in range(top):
