@@ -49,31 +49,6 @@ __device__ __forceinline__ uint16_t pack1(float a, bool half) {
   return __bfloat16_as_ushort(__float2bfloat16_rn(a));
 }
 
-// The pairs (slot, lanes) of a tile of 128 rows: half of what the plan notes for 256.
-struct TilePairs {
-  const int* at;
-  int p, end, half;
-  __device__ TilePairs(const AdapterPlan& plan, int tile128) {
-    const int t = tile128 >> 1;
-    half = tile128 & 1;
-    p = __ldg(plan.tile_start + t) - 1;
-    end = __ldg(plan.tile_start + t + 1);
-    at = plan.pairs;
-  }
-  // the next slot with a row in the tile; its lanes' mask
-  __device__ bool next(int& slot, uint32_t (&off)[4]) {
-    while (++p < end) {
-      const int4 m = __ldg(reinterpret_cast<const int4*>(at + (size_t)p * kPairInts) + 1 + half);
-      off[0] = m.x, off[1] = m.y, off[2] = m.z, off[3] = m.w;
-      if ((off[0] & off[1] & off[2] & off[3]) != 0xffffffffu) {
-        slot = __ldg(at + (size_t)p * kPairInts);
-        return true;
-      }
-    }
-    return false;
-  }
-};
-
 __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
@@ -364,152 +339,189 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // ------------------------------------------------------------------------------------------------ joint
-constexpr int kJointStages = 4;
-
-template <int BN>
-struct JointSmem {
-  static constexpr int W_BYTES = BN * BK * 2;
-  static constexpr int STAGE = kXBytes + W_BYTES;
-  static constexpr int BAR_OFF = kJointStages * STAGE;
-  static constexpr int TOTAL = BAR_OFF + 256 + 1024;
-};
+// A pair of blocks (two SMs) computes tiles of 256 x 256: each holds its 128 rows of x and its half of W's 256, so that
+// every block of K costs an SM 32 KB for 2 x 128 x 256 x 64 products.  Accumulators are double-buffered in TMEM: a tile's
+// stores overlap the next one's products.
+//
+// Tiles go round the pairs; those of a last round that would leave most pairs idle are cut along K into `slices`, whose
+// FP32 sums adapter_join_kernel adds up in slice order.
+constexpr int kPairStages = 6;
+constexpr int kPairHalf = 128 * BK * 2;
+constexpr int kPairStage = 2 * kPairHalf;
+constexpr int kPairSmem = kPairStages * kPairStage + 256 + 1024;
+constexpr int kPairTile = 256 * 256;
 
 struct JointParams {
   AdapterPlan plan;
   uint16_t* y;
+  float* sums;             // [units of cut tiles][256 / 4 columns][256 rows][4]
   int T, N, R, nk;
+  int whole, slices, units;   // tiles that are not cut, cuts of each other one, pieces of work in all
   uint32_t idesc;
   bool half;
 };
 
-// Tiles of 128 x BN; accumulators double-buffered in TMEM, so that a tile's stores overlap the next one's products.
-template <bool MN, int BN>
-__global__ void __launch_bounds__(kThreads, 1)
+struct Piece {
+  int mt, nt, kb0, kb1, sum;   // sum: which partial sum, or -1
+  bool last;                   // takes the low-rank part
+};
+
+__device__ __forceinline__ Piece piece_at(const JointParams& p, int q) {
+  const int m_tiles = (p.T + 255) / 256, n_tiles = (p.N + 255) / 256;
+  Piece w;
+  int tile = q;
+  w.kb0 = 0, w.kb1 = p.nk, w.sum = -1, w.last = true;
+  if (q >= p.whole) {
+    const int j = q - p.whole, slice = j % p.slices;
+    tile = p.whole + j / p.slices;
+    if (p.slices > 1) {
+      w.kb0 = (int)((long)p.nk * slice / p.slices), w.kb1 = (int)((long)p.nk * (slice + 1) / p.slices);
+      w.sum = j, w.last = slice == p.slices - 1;
+    }
+  }
+  // groups of 8 tiles of rows, so that a tile of W serves 8 from L2
+  const int per_group = 8 * n_tiles, first = tile / per_group * 8, gm = min(8, m_tiles - first), r = tile % per_group;
+  w.mt = first + r % gm;
+  w.nt = r / gm;
+  return w;
+}
+
+template <bool MN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     adapter_joint_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                          const __grid_constant__ CUtensorMap map_u, const __grid_constant__ CUtensorMap map_low,
-                         const JointParams p) {
-  using L = JointSmem<BN>;
-  constexpr int kCols = 2 * BN < 32 ? 32 : 2 * BN;
+                         const __grid_constant__ JointParams p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);
-  uint64_t* empty = full + kJointStages;
-  uint64_t* tfull = empty + kJointStages;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kPairStages * kPairStage);
+  uint64_t* empty = full + kPairStages;
+  uint64_t* tfull = empty + kPairStages;
   uint64_t* tempty = tfull + 2;
-  uint32_t* slot_word = reinterpret_cast<uint32_t*>(tempty + 2);
+  uint32_t* tmem_word = reinterpret_cast<uint32_t*>(tempty + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int m_tiles = (p.T + BM - 1) / BM, n_tiles = (p.N + BN - 1) / BN, num_tiles = m_tiles * n_tiles;
+  const int rank = (int)sm100::cluster_ctarank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int rank_blocks = (p.R + BK - 1) / BK;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kJointStages; ++s) {
+    for (int s = 0; s < kPairStages; ++s) {
       sm100::mbar_init(&full[s], 1);
       sm100::mbar_init(&empty[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
       sm100::mbar_init(&tfull[a], 1);
-      sm100::mbar_init(&tempty[a], 128);
+      sm100::mbar_init(&tempty[a], 256);
     }
     sm100::fence_mbar_init();
+    sm100::prefetch_tmap(&map_x);
+    sm100::prefetch_tmap(&map_w);
   }
-  if (warp == 1) sm100::tmem_alloc(slot_word, kCols);
+  if (warp == 1) sm100::tmem_alloc_pair(tmem_word, 512);
   sm100::tc_fence_before();
   __syncthreads();
+  sm100::cluster_sync();
   sm100::tc_fence_after();
-  const uint32_t tmem = *slot_word;
-
-  auto tile_at = [&](int t, int& mt, int& nt) {   // groups of 8 tiles of rows, so that a tile of W serves 8 from L2
-    const int per_group = 8 * n_tiles, first = t / per_group * 8, gm = min(8, m_tiles - first), r = t % per_group;
-    mt = first + r % gm;
-    nt = r / gm;
-  };
+  const uint32_t tmem = *tmem_word;
+  let_next_begin();
 
   if (warp == 0) {
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
+      uint32_t bar = 0;
+      unsigned char *x_dst = nullptr, *w_dst = nullptr;
       auto claim = [&]() {
-        ok = ok && sm100::mbar_wait(&empty[stage], phase ^ 1, &g_error, 41);
-        if (ok) sm100::mbar_expect_tx(&full[stage], L::STAGE);
-        return ok;
+        ok = ok && sm100::mbar_wait_cluster(&empty[stage], phase ^ 1, &g_error, 41);
+        if (!ok) return false;
+        if (rank == 0) sm100::mbar_expect_tx(&full[stage], 2 * kPairStage);
+        bar = sm100::mapa(sm100::smem_addr(&full[stage]), 0);      // both blocks' loads count on the leader's barrier
+        x_dst = smem + stage * kPairStage, w_dst = x_dst + kPairHalf;
+        if (++stage == kPairStages) stage = 0, phase ^= 1;
+        return true;
       };
-      auto step = [&]() {
-        if (++stage == kJointStages) stage = 0, phase ^= 1;
-      };
-      for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
-        int mt, nt;
-        tile_at(t, mt, nt);
-        for (int kb = 0; kb < p.nk; ++kb) {
+      for (int q = pair; q < p.units && ok; q += pairs) {
+        const Piece w = piece_at(p, q);
+        const int m0 = w.mt * 256 + 128 * rank, n0 = w.nt * 256 + 128 * rank;
+        for (int kb = w.kb0; kb < w.kb1; ++kb) {
           if (!claim()) break;
-          unsigned char* dst = smem + stage * L::STAGE;
-          sm100::tma_load_2d(dst, &map_x, &full[stage], kb * BK, mt * BM);
+          sm100::tma_load_2d_pair(x_dst, &map_x, bar, kb * BK, m0);
           if (MN) {
-#pragma unroll
-            for (int i = 0; i < BN / 64; ++i)
-              sm100::tma_load_2d(dst + kXBytes + i * 8192, &map_w, &full[stage], nt * BN + 64 * i, kb * BK);
+            sm100::tma_load_2d_pair(w_dst, &map_w, bar, n0, kb * BK);
+            sm100::tma_load_2d_pair(w_dst + 8192, &map_w, bar, n0 + 64, kb * BK);
           } else {
-            sm100::tma_load_2d(dst + kXBytes, &map_w, &full[stage], kb * BK, nt * BN);
+            sm100::tma_load_2d_pair(w_dst, &map_w, bar, kb * BK, n0);
           }
-          step();
         }
-        TilePairs it(p.plan, mt);
-        int slot;
-        uint32_t off[4];
-        if (t == blockIdx.x) {
+        if (q == pair) {
           wait_for_previous();       // u, which TMA reads from here on
           asm volatile("fence.proxy.async.global;" ::: "memory");
         }
-        while (ok && it.next(slot, off)) {
+        if (!w.last) continue;
+        const int end = __ldg(p.plan.tile_start + w.mt + 1);
+        for (int i = __ldg(p.plan.tile_start + w.mt); i < end && ok; ++i) {
+          const int slot = __ldg(p.plan.pairs + (size_t)i * kPairInts);
           for (int rb = 0; rb < rank_blocks; ++rb) {
             if (!claim()) break;
-            unsigned char* dst = smem + stage * L::STAGE;
-            sm100::tma_load_2d(dst, &map_u, &full[stage], rb * BK, mt * BM);
+            sm100::tma_load_2d_pair(x_dst, &map_u, bar, rb * BK, m0);
             if (MN) {
-#pragma unroll
-              for (int i = 0; i < BN / 64; ++i)
-                sm100::tma_load_3d(dst + kXBytes + i * 8192, &map_low, &full[stage], nt * BN + 64 * i, rb * BK, slot);
+              sm100::tma_load_3d_pair(w_dst, &map_low, bar, n0, rb * BK, slot);
+              sm100::tma_load_3d_pair(w_dst + 8192, &map_low, bar, n0 + 64, rb * BK, slot);
             } else {
-              sm100::tma_load_3d(dst + kXBytes, &map_low, &full[stage], rb * BK, nt * BN, slot);
+              sm100::tma_load_3d_pair(w_dst, &map_low, bar, rb * BK, n0, slot);
             }
-            step();
           }
         }
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (rank == 0 && lane == 0) {
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
-      auto products = [&](uint32_t d, int steps, bool first, const uint32_t (&off)[4]) {
-        ok = ok && sm100::mbar_wait(&full[stage], phase, &g_error, 43);
-        if (!ok) return;
+      for (int q = pair; q < p.units && ok; q += pairs) {
+        if (!sm100::mbar_wait_cluster(&tempty[acc], acc_phase ^ 1, &g_error, 42)) break;
         sm100::tc_fence_after();
-        const uint32_t a = sm100::smem_addr(smem + stage * L::STAGE), b = a + kXBytes;
-        for (int kk = 0; kk < steps; ++kk)
-          sm100::umma_masked(d, sm100::umma_desc_sw128(a + kk * 32, 16, 1024),
-                             MN ? sm100::umma_desc_sw128(b + kk * 2048, 8192, 1024)
-                                : sm100::umma_desc_sw128(b + kk * 32, 16, 1024),
-                             p.idesc, !first || kk > 0, off);
-        sm100::umma_commit(&empty[stage]);
-        if (++stage == kJointStages) stage = 0, phase ^= 1;
-      };
-      for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
-        if (!sm100::mbar_wait(&tempty[acc], acc_phase ^ 1, &g_error, 42)) break;
-        sm100::tc_fence_after();
-        const uint32_t d = tmem + acc * BN;
-        int mt, nt;
-        tile_at(t, mt, nt);
-        const uint32_t all[4] = {0, 0, 0, 0};
-        for (int kb = 0; kb < p.nk && ok; ++kb) products(d, BK / 16, kb == 0, all);
-        TilePairs it(p.plan, mt);
-        int slot;
-        uint32_t off[4];
-        while (ok && it.next(slot, off))
-          for (int rb = 0; rb < rank_blocks; ++rb) products(d, min(BK / 16, (p.R - rb * BK + 15) / 16), false, off);
+        const uint32_t d = tmem + acc * 256;
+        const Piece w = piece_at(p, q);
+        for (int kb = w.kb0; kb < w.kb1; ++kb) {
+          ok = sm100::mbar_wait_cluster(&full[stage], phase, &g_error, 43);
+          if (!ok) break;
+          sm100::tc_fence_after();
+          const uint32_t a = sm100::smem_addr(smem + stage * kPairStage), b = a + kPairHalf;
+#pragma unroll
+          for (int kk = 0; kk < BK / 16; ++kk)
+            sm100::umma_bf16_pair(d, sm100::umma_desc_sw128(a + kk * 32, 16, 1024),
+                                  MN ? sm100::umma_desc_sw128(b + kk * 2048, 8192, 1024)
+                                     : sm100::umma_desc_sw128(b + kk * 32, 16, 1024),
+                                  p.idesc, kb > w.kb0 || kk > 0);
+          sm100::umma_commit_pair_mc(&empty[stage], 0x3);
+          if (++stage == kPairStages) stage = 0, phase ^= 1;
+        }
+        if (w.last) {
+          const int end = __ldg(p.plan.tile_start + w.mt + 1);
+          for (int i = __ldg(p.plan.tile_start + w.mt); i < end && ok; ++i) {
+            const int4* m = reinterpret_cast<const int4*>(p.plan.pairs + (size_t)i * kPairInts);
+            const int4 lo = __ldg(m + 1), hi = __ldg(m + 2);
+            const uint32_t off[8] = {(uint32_t)lo.x, (uint32_t)lo.y, (uint32_t)lo.z, (uint32_t)lo.w,
+                                     (uint32_t)hi.x, (uint32_t)hi.y, (uint32_t)hi.z, (uint32_t)hi.w};
+            for (int rb = 0; rb < rank_blocks; ++rb) {
+              ok = sm100::mbar_wait_cluster(&full[stage], phase, &g_error, 45);
+              if (!ok) break;
+              sm100::tc_fence_after();
+              const uint32_t a = sm100::smem_addr(smem + stage * kPairStage), b = a + kPairHalf;
+              const int steps = min(BK / 16, (p.R - rb * BK + 15) / 16);
+              for (int kk = 0; kk < steps; ++kk)
+                sm100::umma_pair_masked(d, sm100::umma_desc_sw128(a + kk * 32, 16, 1024),
+                                        MN ? sm100::umma_desc_sw128(b + kk * 2048, 8192, 1024)
+                                           : sm100::umma_desc_sw128(b + kk * 32, 16, 1024),
+                                        p.idesc, 1, off);
+              sm100::umma_commit_pair_mc(&empty[stage], 0x3);
+              if (++stage == kPairStages) stage = 0, phase ^= 1;
+            }
+          }
+        }
         if (!ok) break;
-        sm100::umma_commit(&tfull[acc]);
+        sm100::umma_commit_pair_mc(&tfull[acc], 0x3);
         if (++acc == 2) acc = 0, acc_phase ^= 1;
       }
     }
@@ -517,22 +529,27 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int quarter = warp & 3;
     int acc = 0;
     uint32_t acc_phase = 0;
-    for (int t = blockIdx.x; t < num_tiles; t += gridDim.x) {
-      int mt, nt;
-      tile_at(t, mt, nt);
-      const bool got = sm100::mbar_wait(&tfull[acc], acc_phase, &g_error, 44);
+    for (int q = pair; q < p.units; q += pairs) {
+      const bool got = sm100::mbar_wait_cluster(&tfull[acc], acc_phase, &g_error, 44);
       if (!__all_sync(0xffffffffu, got)) break;
       sm100::tc_fence_after();
-      const int row = mt * BM + quarter * 32 + lane;
-      const uint32_t src = tmem + ((uint32_t)(quarter * 32) << 16) + acc * BN;
+      const Piece w = piece_at(p, q);
+      const int at = 128 * rank + quarter * 32 + lane, row = w.mt * 256 + at;
+      const uint32_t src = tmem + ((uint32_t)(quarter * 32) << 16) + acc * 256;
 #pragma unroll 1
-      for (int c = 0; c < BN; c += 32) {
+      for (int c = 0; c < 256; c += 32) {
         uint32_t r[32];
         sm100::tmem_ld32(src + c, r);
         sm100::tmem_ld_wait();
         sm100::tmem_regs_ready(r);
-        const int col = nt * BN + c;
-        if (row < p.T) {
+        if (w.sum >= 0) {
+          float4* dst = reinterpret_cast<float4*>(p.sums + (size_t)w.sum * kPairTile) + (size_t)(c / 4) * 256 + at;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            dst[j * 256] = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]),
+                                       __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
+        } else if (row < p.T) {
+          const int col = w.nt * 256 + c;
           uint16_t* dst = p.y + (size_t)row * p.N + col;
 #pragma unroll
           for (int j = 0; j < 32; j += 8)
@@ -545,17 +562,44 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       sm100::tc_fence_before();
-      sm100::mbar_arrive(&tempty[acc]);
+      sm100::mbar_arrive_cluster(sm100::mapa(sm100::smem_addr(&tempty[acc]), 0));
       if (++acc == 2) acc = 0, acc_phase ^= 1;
     }
   }
   __syncwarp();
   sm100::tc_fence_before();
   __syncthreads();
+  sm100::cluster_sync();   // the peer's barriers and operands stay until both are done
   if (warp == 1) {
     sm100::tc_fence_after();
-    sm100::tmem_dealloc(tmem, kCols);
+    sm100::tmem_dealloc_pair(tmem, 512);
   }
+}
+
+// The cut tiles: y = the sum over a tile's slices, in their order.  One block: 16 columns of the 256 rows.
+__global__ void __launch_bounds__(256) adapter_join_kernel(const __grid_constant__ JointParams p) {
+  const int tile = blockIdx.x / 16, c = blockIdx.x % 16 * 16;
+  const Piece w = piece_at(p, p.whole + tile * p.slices);
+  const int row = w.mt * 256 + threadIdx.x, col = w.nt * 256 + c;
+  wait_for_previous();
+  if (row >= p.T || col >= p.N) return;
+  float4 v[4] = {};
+  for (int s = 0; s < p.slices; ++s) {
+    const float4* src = reinterpret_cast<const float4*>(p.sums + (size_t)(tile * p.slices + s) * kPairTile) +
+                        (size_t)(c / 4) * 256 + threadIdx.x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float4 a = __ldcs(src + j * 256);
+      v[j].x += a.x, v[j].y += a.y, v[j].z += a.z, v[j].w += a.w;
+    }
+  }
+  uint16_t* dst = p.y + (size_t)row * p.N + col;
+#pragma unroll
+  for (int j = 0; j < 4; j += 2)
+    if (col + j * 4 < p.N)
+      *reinterpret_cast<uint4*>(dst + j * 4) =
+          make_uint4(pack2(v[j].x, v[j].y, p.half), pack2(v[j].z, v[j].w, p.half),
+                     pack2(v[j + 1].x, v[j + 1].y, p.half), pack2(v[j + 1].z, v[j + 1].w, p.half));
 }
 
 // ------------------------------------------------------------------------------------------------ grads
@@ -756,20 +800,29 @@ cudaError_t allow_smem(Kernel kernel, int bytes, std::atomic<unsigned long long>
 }
 
 // `early`: the kernel may begin while the one before it in the stream ends (it waits by itself for what that one wrote).
+// `cluster`: blocks of one, 0 where the kernel says it itself.
 template <typename... P, typename... A>
-cudaError_t launch(void (*kernel)(P...), int grid, int smem, int cluster, bool early, cudaStream_t stream, const A&... args) {
+cudaError_t launch(void (*kernel)(P...), int grid, int threads, int smem, int cluster, bool early, cudaStream_t stream,
+                   const A&... args) {
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[2];
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cluster, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  int n = 0;
+  if (cluster) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = cluster, attr[n].val.clusterDim.y = 1, attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (early) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = early ? 2 : 1;
+  cfg.numAttrs = n;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
   if (e == cudaSuccess) launch_counter().fetch_add(1);
   return e;
@@ -806,7 +859,7 @@ cudaError_t run_shrink(const AdapterShrink& a, cudaStream_t stream) {
   static std::atomic<unsigned long long> done{0};
   const cudaError_t e = allow_smem(adapter_shrink_kernel<OP_MN>, kMaxSmem, done);
   if (e != cudaSuccess) return e;
-  return launch(adapter_shrink_kernel<OP_MN>, a.plan.num_units * p.ranks, smem, p.ranks, false, stream, x, op, p);
+  return launch(adapter_shrink_kernel<OP_MN>, a.plan.num_units * p.ranks, kThreads, smem, p.ranks, false, stream, x, op, p);
 }
 
 constexpr int kFewRows = 128;
@@ -833,29 +886,53 @@ cudaError_t run_few(const AdapterJoint& a, cudaStream_t stream) {
   static std::atomic<unsigned long long> done{0};
   const cudaError_t e = allow_smem(adapter_few_kernel<MN>, kMaxSmem, done);
   if (e != cudaSuccess) return e;
-  return launch(adapter_few_kernel<MN>, tiles * p.ranks, smem, p.ranks, a.plan.num_units > 0, stream, w, x, p);
+  return launch(adapter_few_kernel<MN>, tiles * p.ranks, kThreads, smem, p.ranks, a.plan.num_units > 0, stream, w, x, p);
 }
 
-template <bool MN, int BN>
+// How the tiles of 256 x 256 go to the pairs of SMs.
+struct Cut {
+  int pairs, whole, slices, units;
+};
+
+// A last round of `rest` tiles takes a whole tile's time of nk blocks of K; cut into slices nk / slices, the slices' sums
+// (256 KB each, through L2) and another launch, together about 16 blocks' time.
+Cut cut_tiles(int T, int K, int N) {
+  const int tiles = (T + 255) / 256 * ((N + 255) / 256), nk = (K + BK - 1) / BK, pairs = std::max(1, sm_count() / 2);
+  Cut c{pairs, tiles, 1, tiles};
+  const int rest = tiles % pairs;
+  const int slices = rest ? std::min({8, pairs / rest, nk / 4}) : 1;
+  if (slices >= 2 && nk - nk / slices > 16) {
+    c.whole = tiles - rest;
+    c.slices = slices;
+    c.units = c.whole + rest * slices;
+  }
+  c.pairs = std::min(pairs, c.units);
+  return c;
+}
+
+template <bool MN>
 cudaError_t run_joint(const AdapterJoint& a, cudaStream_t stream) {
   alignas(64) CUtensorMap x, w, u, low;
   bool ok = encode(&x, a.x, a.K, a.T, a.ldx, 0, BM, a.half) && encode(&u, a.u, a.R, a.T, a.R, 0, BM, a.half);
   if (MN) ok = ok && encode(&w, a.w, a.N, a.K, a.ldw, 0, 64, a.half) && encode(&low, a.low, a.N, a.R, a.N, a.S, 64, a.half);
-  else ok = ok && encode(&w, a.w, a.K, a.N, a.ldw, 0, BN, a.half) && encode(&low, a.low, a.R, a.N, a.R, a.S, BN, a.half);
+  else ok = ok && encode(&w, a.w, a.K, a.N, a.ldw, 0, BM, a.half) && encode(&low, a.low, a.R, a.N, a.R, a.S, BM, a.half);
   if (!ok) return cudaErrorInvalidValue;
+  const Cut c = cut_tiles(a.T, a.K, a.N);
   JointParams p{};
   p.plan = a.plan;
   p.y = static_cast<uint16_t*>(a.y);
+  p.sums = static_cast<float*>(a.workspace);
   p.T = a.T, p.N = a.N, p.R = a.R;
   p.nk = (a.K + BK - 1) / BK;
-  p.idesc = sm100::umma_idesc_bf16(BM, BN, false, MN) & ~(a.half ? sm100::kIdescBf16 : 0u);
+  p.whole = c.whole, p.slices = c.slices, p.units = c.units;
+  p.idesc = sm100::umma_idesc_bf16(256, 256, false, MN) & ~(a.half ? sm100::kIdescBf16 : 0u);
   p.half = a.half;
   static std::atomic<unsigned long long> done{0};
-  const cudaError_t e = allow_smem(adapter_joint_kernel<MN, BN>, JointSmem<BN>::TOTAL, done);
+  cudaError_t e = allow_smem(adapter_joint_kernel<MN>, kPairSmem, done);
   if (e != cudaSuccess) return e;
-  const long tiles = (long)((a.T + BM - 1) / BM) * ((a.N + BN - 1) / BN);
-  return launch(adapter_joint_kernel<MN, BN>, (int)std::min<long>(tiles, sm_count()), JointSmem<BN>::TOTAL, 1,
-                a.plan.num_units > 0, stream, x, w, u, low, p);
+  e = launch(adapter_joint_kernel<MN>, 2 * c.pairs, kThreads, kPairSmem, 0, a.plan.num_units > 0, stream, x, w, u, low, p);
+  if (e != cudaSuccess || c.units == c.whole) return e;
+  return launch(adapter_join_kernel, (c.units - c.whole) / c.slices * 16, 256, 0, 0, true, stream, p);
 }
 
 }  // namespace
@@ -870,7 +947,13 @@ cudaError_t launch_adapter_joint(const AdapterJoint& a, cudaStream_t stream) {
   const cudaError_t e = have_context();
   if (e != cudaSuccess) return e;
   if (a.T <= kFewRows) return a.mn ? run_few<true>(a, stream) : run_few<false>(a, stream);
-  return a.mn ? run_joint<true, 256>(a, stream) : run_joint<false, 256>(a, stream);
+  return a.mn ? run_joint<true>(a, stream) : run_joint<false>(a, stream);
+}
+
+size_t adapter_joint_workspace(int T, int K, int N) {
+  if (T <= kFewRows) return 0;
+  const Cut c = cut_tiles(T, K, N);
+  return (size_t)(c.units - c.whole) * kPairTile * sizeof(float);
 }
 
 cudaError_t launch_adapter_grads(const AdapterGrads& a, cudaStream_t stream) {
@@ -897,7 +980,7 @@ cudaError_t launch_adapter_grads(const AdapterGrads& a, cudaStream_t stream) {
   static std::atomic<unsigned long long> done{0};
   e = allow_smem(adapter_grads_kernel, kMaxSmem, done);
   if (e != cudaSuccess) return e;
-  return launch(adapter_grads_kernel, a.S * (p.tiles_a + p.tiles_b) * p.ranks, smem, p.ranks, false, stream, x, dy, u, du, p);
+  return launch(adapter_grads_kernel, a.S * (p.tiles_a + p.tiles_b) * p.ranks, kThreads, smem, p.ranks, false, stream, x, dy, u, du, p);
 }
 
 int adapter_error_code() {

@@ -40,6 +40,7 @@ struct AdapterJoint {
   const void* u;           // [T, R]
   const void* low;         // [S, N, R], or [S, R, N] with `mn`
   void* y;                 // [T, N]
+  void* workspace;         // adapter_joint_workspace() bytes
   long ldx, ldw;
   int T, K, N, S, R;
   bool mn, half;
@@ -59,6 +60,7 @@ struct AdapterGrads {
 };
 
 cudaError_t launch_adapter_shrink(const AdapterShrink& a, cudaStream_t stream);
+size_t adapter_joint_workspace(int T, int K, int N);
 cudaError_t launch_adapter_joint(const AdapterJoint& a, cudaStream_t stream);
 cudaError_t launch_adapter_grads(const AdapterGrads& a, cudaStream_t stream);
 int adapter_error_code();

@@ -65,6 +65,11 @@ torch::Tensor joint(const torch::Tensor& x, const torch::Tensor& w, const torch:
   auto y = at::empty({j.T, j.N}, low.options().requires_grad(false));
   j.x = x.data_ptr(), j.w = w.data_ptr(), j.u = u.data_ptr(), j.low = low.data_ptr(), j.y = y.data_ptr();
   j.ldx = row_stride(x), j.ldw = row_stride(w);
+  torch::Tensor sums;      // the call's own: two of them may run at once
+  if (const size_t bytes = bb::adapter_joint_workspace(j.T, j.K, j.N)) {
+    sums = at::empty({(int64_t)bytes}, low.options().dtype(at::kByte).requires_grad(false));
+    j.workspace = sums.data_ptr();
+  }
   j.plan = plan_of(buf, meta);
   check(bb::launch_adapter_joint(j, at::cuda::getCurrentCUDAStream()));
   return y;
