@@ -348,7 +348,8 @@ __global__ void __launch_bounds__(kThreads)
 constexpr int kPairStages = 6;
 constexpr int kPairHalf = 128 * BK * 2;
 constexpr int kPairStage = 2 * kPairHalf;
-constexpr int kPairSmem = kPairStages * kPairStage + 256 + 1024;
+constexpr int kStoreBytes = 32 * 64 * 2;       // what a warp of the epilogue stores at a time: 32 rows x 64 columns
+constexpr int kPairSmem = kPairStages * kPairStage + 4 * 2 * kStoreBytes + 256 + 1024;
 constexpr int kPairTile = 256 * 256;
 
 struct JointParams {
@@ -390,10 +391,11 @@ template <bool MN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     adapter_joint_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                          const __grid_constant__ CUtensorMap map_u, const __grid_constant__ CUtensorMap map_low,
-                         const __grid_constant__ JointParams p) {
+                         const __grid_constant__ CUtensorMap map_y, const __grid_constant__ JointParams p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kPairStages * kPairStage);
+  unsigned char* store = smem + kPairStages * kPairStage;
+  uint64_t* full = reinterpret_cast<uint64_t*>(store + 4 * 2 * kStoreBytes);
   uint64_t* empty = full + kPairStages;
   uint64_t* tfull = empty + kPairStages;
   uint64_t* tempty = tfull + 2;
@@ -534,37 +536,66 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (!__all_sync(0xffffffffu, got)) break;
       sm100::tc_fence_after();
       const Piece w = piece_at(p, q);
-      const int at = 128 * rank + quarter * 32 + lane, row = w.mt * 256 + at;
+      const int at = 128 * rank + quarter * 32 + lane;
       const uint32_t src = tmem + ((uint32_t)(quarter * 32) << 16) + acc * 256;
+      if (w.sum >= 0) {
 #pragma unroll 1
-      for (int c = 0; c < 256; c += 32) {
-        uint32_t r[32];
-        sm100::tmem_ld32(src + c, r);
-        sm100::tmem_ld_wait();
-        sm100::tmem_regs_ready(r);
-        if (w.sum >= 0) {
+        for (int c = 0; c < 256; c += 32) {
+          uint32_t r[32];
+          sm100::tmem_ld32(src + c, r);
+          sm100::tmem_ld_wait();
+          sm100::tmem_regs_ready(r);
           float4* dst = reinterpret_cast<float4*>(p.sums + (size_t)w.sum * kPairTile) + (size_t)(c / 4) * 256 + at;
 #pragma unroll
           for (int j = 0; j < 8; ++j)
             dst[j * 256] = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]),
                                        __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
-        } else if (row < p.T) {
+        }
+      } else {
+        // 32 rows x 64 columns at a time through shared memory (128-byte swizzle: 16-byte piece j of row i lies at
+        // j ^ i % 8), so that y is written in whole lines; straight from the registers its sectors went out in halves
+        const int row0 = w.mt * 256 + 128 * rank + quarter * 32;
+#pragma unroll 1
+        for (int c = 0; c < 256; c += 64) {
           const int col = w.nt * 256 + c;
-          uint16_t* dst = p.y + (size_t)row * p.N + col;
+          if (row0 >= p.T || col >= p.N) break;
+          uint32_t r[32], r2[32];
+          sm100::tmem_ld32(src + c, r);
+          sm100::tmem_ld32(src + c + 32, r2);
+          sm100::tmem_ld_wait();
+          sm100::tmem_regs_ready(r);
+          sm100::tmem_regs_ready(r2);
+          unsigned char* buf = store + (quarter * 2 + (c / 64 & 1)) * kStoreBytes;
+          if (lane == 0) sm100::tma_store_wait_read<1>();      // the store before the last one has left this buffer
+          __syncwarp();
 #pragma unroll
-          for (int j = 0; j < 32; j += 8)
-            if (col + j < p.N)     // N is a multiple of 8
-              *reinterpret_cast<uint4*>(dst + j) =
-                  make_uint4(pack2(__uint_as_float(r[j]), __uint_as_float(r[j + 1]), p.half),
-                             pack2(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]), p.half),
-                             pack2(__uint_as_float(r[j + 4]), __uint_as_float(r[j + 5]), p.half),
-                             pack2(__uint_as_float(r[j + 6]), __uint_as_float(r[j + 7]), p.half));
+          for (int j = 0; j < 8; ++j) {
+            uint4 v;
+            if (j < 4)
+              v = make_uint4(pack2(__uint_as_float(r[8 * j]), __uint_as_float(r[8 * j + 1]), p.half),
+                             pack2(__uint_as_float(r[8 * j + 2]), __uint_as_float(r[8 * j + 3]), p.half),
+                             pack2(__uint_as_float(r[8 * j + 4]), __uint_as_float(r[8 * j + 5]), p.half),
+                             pack2(__uint_as_float(r[8 * j + 6]), __uint_as_float(r[8 * j + 7]), p.half));
+            else
+              v = make_uint4(pack2(__uint_as_float(r2[8 * j - 32]), __uint_as_float(r2[8 * j - 31]), p.half),
+                             pack2(__uint_as_float(r2[8 * j - 30]), __uint_as_float(r2[8 * j - 29]), p.half),
+                             pack2(__uint_as_float(r2[8 * j - 28]), __uint_as_float(r2[8 * j - 27]), p.half),
+                             pack2(__uint_as_float(r2[8 * j - 26]), __uint_as_float(r2[8 * j - 25]), p.half));
+            *reinterpret_cast<uint4*>(buf + lane * 128 + ((j ^ (lane & 7)) * 16)) = v;
+          }
+          sm100::fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            sm100::tma_store_2d(&map_y, buf, col, row0);
+            sm100::tma_store_commit();
+          }
         }
       }
       sm100::tc_fence_before();
       sm100::mbar_arrive_cluster(sm100::mapa(sm100::smem_addr(&tempty[acc]), 0));
       if (++acc == 2) acc = 0, acc_phase ^= 1;
     }
+    if (lane == 0) sm100::tma_store_wait_all();
   }
   __syncwarp();
   sm100::tc_fence_before();
@@ -912,8 +943,9 @@ Cut cut_tiles(int T, int K, int N) {
 
 template <bool MN>
 cudaError_t run_joint(const AdapterJoint& a, cudaStream_t stream) {
-  alignas(64) CUtensorMap x, w, u, low;
-  bool ok = encode(&x, a.x, a.K, a.T, a.ldx, 0, BM, a.half) && encode(&u, a.u, a.R, a.T, a.R, 0, BM, a.half);
+  alignas(64) CUtensorMap x, w, u, low, y;
+  bool ok = encode(&x, a.x, a.K, a.T, a.ldx, 0, BM, a.half) && encode(&u, a.u, a.R, a.T, a.R, 0, BM, a.half) &&
+            encode(&y, a.y, a.N, a.T, a.N, 0, 32, a.half);
   if (MN) ok = ok && encode(&w, a.w, a.N, a.K, a.ldw, 0, 64, a.half) && encode(&low, a.low, a.N, a.R, a.N, a.S, 64, a.half);
   else ok = ok && encode(&w, a.w, a.K, a.N, a.ldw, 0, BM, a.half) && encode(&low, a.low, a.R, a.N, a.R, a.S, BM, a.half);
   if (!ok) return cudaErrorInvalidValue;
@@ -930,7 +962,7 @@ cudaError_t run_joint(const AdapterJoint& a, cudaStream_t stream) {
   static std::atomic<unsigned long long> done{0};
   cudaError_t e = allow_smem(adapter_joint_kernel<MN>, kPairSmem, done);
   if (e != cudaSuccess) return e;
-  e = launch(adapter_joint_kernel<MN>, 2 * c.pairs, kThreads, kPairSmem, 0, a.plan.num_units > 0, stream, x, w, u, low, p);
+  e = launch(adapter_joint_kernel<MN>, 2 * c.pairs, kThreads, kPairSmem, 0, a.plan.num_units > 0, stream, x, w, u, low, y, p);
   if (e != cudaSuccess || c.units == c.whole) return e;
   return launch(adapter_join_kernel, (c.units - c.whole) / c.slices * 16, 256, 0, 0, true, stream, p);
 }
