@@ -21,6 +21,8 @@
 
 #include <algorithm>
 #include <atomic>
+#include <mutex>
+#include <vector>
 
 #include "common.cuh"
 #include "sm100_common.cuh"
@@ -188,11 +190,11 @@ __global__ void __launch_bounds__(kThreads)
   __syncthreads();
   sm100::cluster_sync();
   // this block's share of the rows: 8 columns a step, the finished values 16 bytes at a time
-  const int rows = BM / p.ranks, groups = p.R / 8;
+  const int lo = BM * rank / p.ranks, rows = BM * (rank + 1) / p.ranks - lo, groups = p.R / 8;
   const uint32_t base = sm100::smem_addr(part);
   const float f = p.scales ? __ldg(p.scales + slot) : p.scale;
   for (int i = threadIdx.x; i < rows * groups; i += kThreads) {
-    const int r = rank * rows + i / groups, c = (i % groups) * 8;
+    const int r = lo + i / groups, c = (i % groups) * 8;
     if (__ldg(unit + 4 + r / 32) >> (r % 32) & 1) continue;      // another request's row
     const float4 v = joined(base, r * (p.cols + 4) + c, p.ranks), w = joined(base, r * (p.cols + 4) + c + 4, p.ranks);
     *reinterpret_cast<uint4*>(p.u + (size_t)(tile * BM + r) * p.R + c) =
@@ -303,10 +305,10 @@ __global__ void __launch_bounds__(kThreads)
   sm100::cluster_sync();
   wait_for_previous();
   // this block's share of W's rows; neighbours take neighbouring columns of y
-  const int rows = BM / p.ranks;
+  const int lo = BM * rank / p.ranks, rows = BM * (rank + 1) / p.ranks - lo;
   const uint32_t base = sm100::smem_addr(part);
   for (int i = threadIdx.x; i < rows * p.T; i += kThreads) {
-    const int r = rank * rows + i % rows, t = i / rows, n = n0 + r;
+    const int r = lo + i % rows, t = i / rows, n = n0 + r;
     if (n >= p.N) continue;
     float v = 0.f;
     for (int j = 0; j < p.ranks; ++j) v += ld_cluster1(sm100::mapa(base + (r * (p.cols + 4) + t) * 4, j));
@@ -644,8 +646,45 @@ struct GradParams {
   bool add_a, add_b, half;
 };
 
-// One cluster takes 128 columns of dy (or x) of one slot, each of its blocks a stretch of the slot's rows:
-// D [128, R] = sum over rows of dy^T u (x^T du); the partial sums meet in shared memory, in rank order.
+// What a block writes of the gradients: 128 columns of dy (rows of dB) or of x (columns of dA).
+struct GradTile {
+  void* out;
+  int m0, limit, R;
+  bool is_b, add, half;
+
+  // four values of row m0 + r, columns c to c + 3
+  __device__ __forceinline__ void put(int slot, int r, int c, float4 v) const {
+    if (m0 + r >= limit) return;
+    if (is_b) {
+      const size_t to = ((size_t)slot * limit + m0 + r) * R + c;
+      if (add) {
+        float4* dst = reinterpret_cast<float4*>(static_cast<float*>(out) + to);
+        const float4 o = *dst;
+        *dst = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
+      } else {
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + to) = make_uint2(pack2(v.x, v.y, half), pack2(v.z, v.w, half));
+      }
+    } else {
+      const size_t to = ((size_t)slot * R + c) * limit + m0 + r;
+      const float q[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (add) static_cast<float*>(out)[to + (size_t)j * limit] += q[j];
+        else static_cast<uint16_t*>(out)[to + (size_t)j * limit] = pack1(q[j], half);
+      }
+    }
+  }
+  // i-th piece of four of `rows` rows from `lo`: dB has neighbours in a row of R, dA in a column
+  __device__ __forceinline__ void place(int i, int lo, int rows, int& r, int& c) const {
+    r = lo + (is_b ? i / (R / 4) : i % rows);
+    c = (is_b ? i % (R / 4) : i / rows) * 4;
+  }
+};
+
+// A cluster takes 128 columns of dy (or x) and the rows of all slots, cut evenly over its blocks whatever the slots'
+// shares: D_s [128, R] = sum over slot s's rows of dy^T u (x^T du).  A slot whose rows all fall to one block is written
+// by it at once, from the accumulator, while the next slot's products go into another one; of the slots that begin or end
+// in another block (at most two a block) the partial sums meet in shared memory at the end, in the blocks' order.
 __global__ void __launch_bounds__(kThreads)
     adapter_grads_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_dy,
                          const __grid_constant__ CUtensorMap map_u, const __grid_constant__ CUtensorMap map_du,
@@ -653,62 +692,78 @@ __global__ void __launch_bounds__(kThreads)
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int low_bytes = p.cols / 64 * 8192, stage_bytes = kXBytes + low_bytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kGradStages * stage_bytes);
+  const int part_floats = BM * (p.cols + 4), tmem_cols = p.cols == 64 ? 256 : 512;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + max(kGradStages * stage_bytes, 2 * part_floats * 4));
   uint64_t* empty = full + kGradStages;
-  uint64_t* done = empty + kGradStages;
-  uint32_t* slot_word = reinterpret_cast<uint32_t*>(done + 1);
+  uint64_t* tfull = empty + kGradStages;     // of the three accumulators
+  uint64_t* tempty = tfull + 3;
+  uint32_t* tmem_word = reinterpret_cast<uint32_t*>(tempty + 3);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = (int)sm100::cluster_ctarank();
-  const int item = blockIdx.x / p.ranks, tiles = p.tiles_a + p.tiles_b, slot = item / tiles;
-  const bool is_b = item % tiles < p.tiles_b;
-  const int m0 = (is_b ? item % tiles : item % tiles - p.tiles_b) * BM;
+  const int rank = (int)sm100::cluster_ctarank(), tile = blockIdx.x / p.ranks;
+  const bool is_b = tile < p.tiles_b;
+  const GradTile g{is_b ? p.db : p.da, (is_b ? tile : tile - p.tiles_b) * BM, is_b ? p.N : p.K, p.R, is_b,
+                   is_b ? p.add_b : p.add_a, p.half};
   const CUtensorMap* map_wide = is_b ? &map_dy : &map_x;
   const CUtensorMap* map_thin = is_b ? &map_u : &map_du;
-  int first = 0, count = 0;
-  if (slot < p.plan.slots) {
-    first = __ldg(p.plan.block_start + slot);
-    count = __ldg(p.plan.block_start + slot + 1) - first;
-  }
-  const int b0 = first + (int)((long)count * rank / p.ranks), b1 = first + (int)((long)count * (rank + 1) / p.ranks);
+  const int4* blocks = reinterpret_cast<const int4*>(p.plan.blocks);
+  const auto cut = [&](int r) { return (int)((long)p.plan.num_blocks * r / p.ranks); };
+  const int b0 = cut(rank), b1 = cut(rank + 1);
+  // the first slot's rows began in an earlier block: its sum stays in accumulator 0 to the end
+  const bool began = b1 > b0 && __ldg(p.plan.block_start + __ldg(&blocks[b0]).z) < b0;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kGradStages; ++s) {
       sm100::mbar_init(&full[s], 1);
       sm100::mbar_init(&empty[s], 1);
     }
-    sm100::mbar_init(done, 1);
+    for (int i = 0; i < 3; ++i) {
+      sm100::mbar_init(&tfull[i], 1);
+      sm100::mbar_init(&tempty[i], 128);
+    }
     sm100::fence_mbar_init();
   }
-  if (warp == 1) sm100::tmem_alloc(slot_word, 128);
+  if (warp == 1) sm100::tmem_alloc(tmem_word, tmem_cols);
   sm100::tc_fence_before();
   __syncthreads();
   sm100::tc_fence_after();
-  const uint32_t tmem = *slot_word;
+  const uint32_t tmem = *tmem_word;
+  float* part = reinterpret_cast<float*>(smem);
 
   if (warp == 0) {
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
       for (int b = b0; b < b1; ++b) {
+        const int row = __ldg(&blocks[b]).x;
         if (!sm100::mbar_wait(&empty[stage], phase ^ 1, &g_error, 51)) break;
         unsigned char* dst = smem + stage * stage_bytes;
-        const int row = __ldg(p.plan.blocks + 2 * b);
         sm100::mbar_expect_tx(&full[stage], stage_bytes);
-        sm100::tma_load_2d(dst, map_wide, &full[stage], m0, row);
-        sm100::tma_load_2d(dst + 8192, map_wide, &full[stage], m0 + 64, row);
+        sm100::tma_load_2d(dst, map_wide, &full[stage], g.m0, row);
+        sm100::tma_load_2d(dst + 8192, map_wide, &full[stage], g.m0 + 64, row);
         for (int i = 0; i < p.cols / 64; ++i)
           sm100::tma_load_2d(dst + kXBytes + i * 8192, map_thin, &full[stage], 64 * i, row);
         if (++stage == kGradStages) stage = 0, phase ^= 1;
       }
     }
-  } else if (warp == 1 && b1 > b0) {
-    int stage = 0;
-    uint32_t phase = 0;
-    for (int b = b0; b < b1; ++b) {
-      const bool got = sm100::mbar_wait(&full[stage], phase, &g_error, 52);
-      if (!__all_sync(0xffffffffu, got)) break;
+  } else if (warp == 1) {
+    int stage = 0, slot = -1, acc = 2;
+    uint32_t phase = 0, acc_phase[3] = {0, 0, 0};
+    bool ok = true;
+    for (int b = b0; b < b1 && ok; ++b) {
+      const int4 block = __ldg(&blocks[b]);
+      const bool fresh = block.z != slot;
+      if (fresh) {
+        if (slot >= 0 && lane == 0) sm100::umma_commit(&tfull[acc]);
+        acc = slot < 0 && began ? 0 : acc == 1 ? 2 : 1;
+        slot = block.z;
+        ok = sm100::mbar_wait(&tempty[acc], acc_phase[acc] ^ 1, &g_error, 54);
+        acc_phase[acc] ^= 1;
+      }
+      ok = ok && sm100::mbar_wait(&full[stage], phase, &g_error, 52);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
       unsigned char* at = smem + stage * stage_bytes;
-      const int n = __ldg(p.plan.blocks + 2 * b + 1), steps = (n + 15) / 16;
+      const int n = block.y, steps = (n + 15) / 16;
       if (n < steps * 16) {
         // rows of other requests behind the block: a row is 128 bytes of every 64 columns, in whatever order
         const int lines = (steps * 16 - n) * 8;
@@ -721,61 +776,90 @@ __global__ void __launch_bounds__(kThreads)
         sm100::tc_fence_after();
         const uint32_t a = sm100::smem_addr(at), w = a + kXBytes;
         for (int kk = 0; kk < steps; ++kk)
-          sm100::umma_bf16(tmem, sm100::umma_desc_sw128(a + kk * 2048, 8192, 1024),
-                           sm100::umma_desc_sw128(w + kk * 2048, 8192, 1024), p.idesc, b > b0 || kk > 0);
+          sm100::umma_bf16(tmem + acc * p.cols, sm100::umma_desc_sw128(a + kk * 2048, 8192, 1024),
+                           sm100::umma_desc_sw128(w + kk * 2048, 8192, 1024), p.idesc, !fresh || kk > 0);
         sm100::umma_commit(&empty[stage]);
       }
       __syncwarp();
       if (++stage == kGradStages) stage = 0, phase ^= 1;
     }
-    if (lane == 0) sm100::umma_commit(done);
-  }
-  __syncwarp();
-  float* part = reinterpret_cast<float*>(smem);
-  if (warp >= 2) {
-    if (b1 > b0) sm100::mbar_wait(done, 0, &g_error, 53);
-    __syncwarp();
-    sm100::tc_fence_after();
-    spill(tmem, part, p.cols, b1 > b0);
-    sm100::tc_fence_before();
-  }
-  __syncthreads();
-  sm100::cluster_sync();
-  const int rows = BM / p.ranks;
-  const uint32_t base = sm100::smem_addr(part);
-  const int limit = is_b ? p.N : p.K;
-  const bool add = is_b ? p.add_b : p.add_a;
-  if (!(add && count == 0)) {
-    for (int i = threadIdx.x; i < rows * (p.R / 4); i += kThreads) {
-      // dB: neighbours take neighbouring columns of a row; dA, whose rows are these columns: neighbouring rows
-      const int r = rank * rows + (is_b ? i / (p.R / 4) : i % rows), c = (is_b ? i % (p.R / 4) : i / rows) * 4;
-      if (m0 + r >= limit) continue;
-      const float4 v = joined(base, r * (p.cols + 4) + c, p.ranks);
-      if (is_b) {
-        const size_t to = ((size_t)slot * p.N + m0 + r) * p.R + c;
-        if (add) {
-          float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.db) + to);
-          const float4 o = *dst;
-          *dst = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
-        } else {
-          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.db) + to) =
-              make_uint2(pack2(v.x, v.y, p.half), pack2(v.z, v.w, p.half));
-        }
-      } else {
-        const size_t to = ((size_t)slot * p.R + c) * p.K + m0 + r;
-        const float q[4] = {v.x, v.y, v.z, v.w};
+    if (slot >= 0 && lane == 0) sm100::umma_commit(&tfull[acc]);
+  } else {
+    const int quarter = warp & 3;
+    int acc = 2, slot = -1;
+    uint32_t acc_phase[3] = {0, 0, 0};
+    for (int b = b0; b < b1;) {
+      acc = slot < 0 && began ? 0 : acc == 1 ? 2 : 1;
+      slot = __ldg(&blocks[b]).z;
+      const int end = __ldg(p.plan.block_start + slot + 1);
+      const bool got = sm100::mbar_wait(&tfull[acc], acc_phase[acc], &g_error, 53);
+      acc_phase[acc] ^= 1;
+      if (!__all_sync(0xffffffffu, got)) break;
+      sm100::tc_fence_after();
+      if (!(began && acc == 0) && end <= b1) {       // all of the slot's rows were this block's
+        for (int c = 0; c < p.R; c += 32) {
+          uint32_t r[32];
+          sm100::tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + acc * p.cols + c, r);
+          sm100::tmem_ld_wait();
+          sm100::tmem_regs_ready(r);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (add) static_cast<float*>(p.da)[to + (size_t)j * p.K] += q[j];
-          else static_cast<uint16_t*>(p.da)[to + (size_t)j * p.K] = pack1(q[j], p.half);
+          for (int j = 0; j < 32; j += 4)
+            if (c + j < p.R)
+              g.put(slot, quarter * 32 + lane, c + j, make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]),
+                                                                  __uint_as_float(r[j + 2]), __uint_as_float(r[j + 3])));
         }
       }
+      sm100::tc_fence_before();
+      if (acc) sm100::mbar_arrive(&tempty[acc]);
+      b = end;
+    }
+    // every product is done, so the operands' memory is free: the sums that are others' too
+    sm100::tc_fence_after();
+    if (began) spill(tmem, part, p.cols, true);
+    if (b1 > b0 && __ldg(p.plan.block_start + slot + 1) > b1 && !(began && acc == 0))
+      spill(tmem + acc * p.cols, part + part_floats, p.cols, true);
+    sm100::tc_fence_before();
+  }
+  __syncwarp();
+  __syncthreads();
+  sm100::cluster_sync();
+  // slots that share this block's first or last rows with other blocks: each of those takes a share of the 128 rows
+  const uint32_t base = sm100::smem_addr(part);
+  for (int k = 0; k < 2 && b1 > b0; ++k) {
+    const int slot = __ldg(&blocks[k ? b1 - 1 : b0]).z;
+    const int first = __ldg(p.plan.block_start + slot), end = __ldg(p.plan.block_start + slot + 1);
+    if (k ? (end <= b1 || (began && slot == __ldg(&blocks[b0]).z)) : !began) continue;
+    int lo = 0, hi = p.ranks - 1;
+    while (cut(lo + 1) <= first) ++lo;
+    while (cut(hi) >= end) --hi;
+    const int r0 = BM * (rank - lo) / (hi - lo + 1), rows = BM * (rank - lo + 1) / (hi - lo + 1) - r0;
+    for (int i = threadIdx.x; i < rows * (p.R / 4); i += kThreads) {
+      int r, c;
+      g.place(i, r0, rows, r, c);
+      // (the block where the slot begins keeps it as its last, the others as their first)
+      const uint32_t at = base + (r * (p.cols + 4) + c) * 4;
+      float4 v = ld_cluster4(sm100::mapa(at + part_floats * 4, lo));
+      for (int j = lo + 1; j <= hi; ++j) {
+        if (cut(j) == cut(j + 1)) continue;
+        const float4 o = ld_cluster4(sm100::mapa(at, j));
+        v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+      }
+      g.put(slot, r, c, v);
     }
   }
+  if (!g.add)        // slots without rows
+    for (int s = rank; s < p.S; s += p.ranks) {
+      if (s < p.plan.slots && __ldg(p.plan.block_start + s + 1) > __ldg(p.plan.block_start + s)) continue;
+      for (int i = threadIdx.x; i < BM * (p.R / 4); i += kThreads) {
+        int r, c;
+        g.place(i, 0, BM, r, c);
+        g.put(s, r, c, make_float4(0.f, 0.f, 0.f, 0.f));
+      }
+    }
   sm100::cluster_sync();
   if (warp == 1) {
     sm100::tc_fence_after();
-    sm100::tmem_dealloc(tmem, 128);
+    sm100::tmem_dealloc(tmem, tmem_cols);
   }
 }
 
@@ -820,6 +904,8 @@ int sm_count() {
   return n;
 }
 
+constexpr int kMaxSmem = 227 * 1024;
+
 template <typename Kernel>
 cudaError_t allow_smem(Kernel kernel, int bytes, std::atomic<unsigned long long>& done) {
   int dev = 0;
@@ -859,14 +945,48 @@ cudaError_t launch(void (*kernel)(P...), int grid, int threads, int smem, int cl
   return e;
 }
 
-// Blocks of a cluster: as many (1, 2, 4, 8) as it takes to have two per SM, while each still has two blocks of the sum.
-int split(long clusters, int nk) {
-  int ranks = 1;
-  while (ranks < 8 && clusters * ranks < 2 * sm_count() && nk >= 4 * ranks) ranks *= 2;
+// Blocks of a cluster: as many (at most 8, each with two blocks of the sum or more) as let all clusters run at once.
+// More blocks mean more loads in flight; a cluster that has to wait for room, a second round.  (Clusters lie within a
+// GPC, so how many fit is less than blocks over SMs: 15 of 8 with a block to an SM, not 18.  The runtime counts one block
+// of a kernel with TMEM to an SM; there are as many as its shared memory and its `columns` of TMEM leave room for.)
+template <typename... P>
+int split(void (*kernel)(P...), int smem, int columns, int clusters, int nk) {
+  struct Fit {
+    const void* kernel;
+    int device, smem, fits[9];
+  };
+  static std::mutex lock;
+  static std::vector<Fit> known;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const std::lock_guard<std::mutex> hold(lock);
+  const void* key = reinterpret_cast<const void*>(kernel);
+  const Fit* fit = nullptr;
+  for (const Fit& f : known)
+    if (f.kernel == key && f.device == dev && f.smem == smem) fit = &f;
+  if (!fit) {
+    Fit f{key, dev, smem, {}};
+    for (int r = 2; r <= 8; ++r) {
+      cudaLaunchConfig_t cfg{};
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = r, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+      cfg.gridDim = dim3(r), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = smem;
+      cfg.attrs = attr, cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&f.fits[r], kernel, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        f.fits[r] = 0;
+      }
+    }
+    known.push_back(f);
+    fit = &known.back();
+  }
+  const int per_sm = std::max(1, std::min(kMaxSmem / (smem + 1024), 512 / columns));
+  int ranks = 8;
+  while (ranks > 1 && (clusters > per_sm * fit->fits[ranks] || nk < 2 * ranks)) --ranks;
   return ranks;
 }
 
-constexpr int kMaxSmem = 227 * 1024;
 
 template <bool OP_MN>
 cudaError_t run_shrink(const AdapterShrink& a, cudaStream_t stream) {
@@ -883,13 +1003,13 @@ cudaError_t run_shrink(const AdapterShrink& a, cudaStream_t stream) {
   p.op_bytes = cols * 128;
   p.nk = (a.K + BK - 1) / BK;
   p.stages = 4;
-  p.ranks = split(a.plan.num_units, p.nk);
   p.idesc = sm100::umma_idesc_bf16(BM, cols, false, OP_MN) & ~(a.half ? sm100::kIdescBf16 : 0u);
   p.half = a.half;
   const int smem = std::max(p.stages * (kXBytes + p.op_bytes), BM * (cols + 4) * 4) + 256 + 1024;
   static std::atomic<unsigned long long> done{0};
   const cudaError_t e = allow_smem(adapter_shrink_kernel<OP_MN>, kMaxSmem, done);
   if (e != cudaSuccess) return e;
+  p.ranks = split(adapter_shrink_kernel<OP_MN>, smem, 128, a.plan.num_units, p.nk);
   return launch(adapter_shrink_kernel<OP_MN>, a.plan.num_units * p.ranks, kThreads, smem, p.ranks, false, stream, x, op, p);
 }
 
@@ -910,13 +1030,13 @@ cudaError_t run_few(const AdapterJoint& a, cudaStream_t stream) {
   p.nk = (a.K + BK - 1) / BK;
   p.stages = 4;
   const int tiles = (a.N + BM - 1) / BM;
-  p.ranks = split(tiles, p.nk);
   p.idesc = sm100::umma_idesc_bf16(BM, cols, MN, false) & ~(a.half ? sm100::kIdescBf16 : 0u);
   p.half = a.half;
   const int smem = std::max(p.stages * (kXBytes + cols * 128), BM * (cols + 4) * 4) + 256 + 1024;
   static std::atomic<unsigned long long> done{0};
   const cudaError_t e = allow_smem(adapter_few_kernel<MN>, kMaxSmem, done);
   if (e != cudaSuccess) return e;
+  p.ranks = split(adapter_few_kernel<MN>, smem, 128, tiles, p.nk);
   return launch(adapter_few_kernel<MN>, tiles * p.ranks, kThreads, smem, p.ranks, a.plan.num_units > 0, stream, w, x, p);
 }
 
@@ -1005,14 +1125,18 @@ cudaError_t launch_adapter_grads(const AdapterGrads& a, cudaStream_t stream) {
   p.cols = (a.R + 63) / 64 * 64;
   p.tiles_a = a.da ? (a.K + BM - 1) / BM : 0;
   p.tiles_b = a.db ? (a.N + BM - 1) / BM : 0;
-  p.ranks = 1;
   p.idesc = sm100::umma_idesc_bf16(BM, p.cols, true, true) & ~(a.half ? sm100::kIdescBf16 : 0u);
   p.add_a = a.add_a, p.add_b = a.add_b, p.half = a.half;
-  const int smem = std::max(kGradStages * (kXBytes + p.cols * 128), BM * (p.cols + 4) * 4) + 256 + 1024;
+  int smem = std::max(kGradStages * (kXBytes + p.cols * 128), 2 * BM * (p.cols + 4) * 4) + 256 + 1024;
+  // Blocks that hold all of an SM's TMEM have the SM for themselves: of two clusters that wait for each other's, each in
+  // another SM, neither would end.  (All other blocks here take 72 KB of shared memory or more, and at most 256 columns.)
+  if (p.cols > 64) smem = std::max(smem, 160 * 1024);
   static std::atomic<unsigned long long> done{0};
   e = allow_smem(adapter_grads_kernel, kMaxSmem, done);
   if (e != cudaSuccess) return e;
-  return launch(adapter_grads_kernel, a.S * (p.tiles_a + p.tiles_b) * p.ranks, kThreads, smem, p.ranks, false, stream, x, dy, u, du, p);
+  const int tiles = p.tiles_a + p.tiles_b;
+  p.ranks = split(adapter_grads_kernel, smem, p.cols == 64 ? 256 : 512, tiles, std::max(1, a.plan.num_blocks));
+  return launch(adapter_grads_kernel, tiles * p.ranks, kThreads, smem, p.ranks, false, stream, x, dy, u, du, p);
 }
 
 int adapter_error_code() {

@@ -15,8 +15,8 @@ struct AdapterPlan {
   const int* pairs;        // [P][12] (slot, 0, 0, 0, 256 bits: set where a row of the tile is NOT the slot's)
   const int* units;        // [.][8] (tile of 128 rows, slot, 0, 0, 128 bits as above): every pair by itself
   const int* block_start;  // [slots + 1] first block of each slot
-  const int* blocks;       // [.][2] (first row, rows <= 64) of one slot, in row order
-  int num_units;
+  const int* blocks;       // [.][4] (first row, rows <= 64, slot, 0), slot by slot and in row order
+  int num_units, num_blocks;
   int slots;               // slots the plan speaks of: the largest one + 1
 };
 

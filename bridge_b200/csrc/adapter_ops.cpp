@@ -11,7 +11,7 @@ torch::Tensor gemm(torch::Tensor a, torch::Tensor b, bool a_mn, bool b_mn, c10::
 namespace {
 
 using OptTensor = c10::optional<torch::Tensor>;
-using Meta = std::vector<int64_t>;   // rows, slots, units, then where the plan's parts begin in its buffer
+using Meta = std::vector<int64_t>;   // rows, slots, units, blocks, then where the plan's parts begin in its buffer
 
 void check(cudaError_t e) { TORCH_CHECK(e == cudaSuccess, "CUDA error ", cudaGetErrorString(e)); }
 
@@ -28,7 +28,8 @@ torch::Tensor as_rows(const torch::Tensor& t) {
 
 bb::AdapterPlan plan_of(const torch::Tensor& buf, const Meta& meta) {
   const int* p = buf.data_ptr<int>();
-  return {p + meta[3], p + meta[4], p + meta[5], p + meta[6], p + meta[7], p + meta[8], (int)meta[2], (int)meta[1]};
+  return {p + meta[4], p + meta[5], p + meta[6], p + meta[7], p + meta[8], p + meta[9],
+          (int)meta[2], (int)meta[3], (int)meta[1]};
 }
 
 struct Sizes {
@@ -184,7 +185,7 @@ torch::Tensor adapter_linear(torch::Tensor x, torch::Tensor w, torch::Tensor a, 
       w.size(0) >= 8 && a.size(1) >= 8 && x.size(1) % 8 == 0 && w.size(0) % 8 == 0 && a.size(1) % 8 == 0 &&
       a.size(1) <= bb::kMaxAdapterRank && x.size(0) < (1l << 30) && x.size(1) < (1l << 30) && w.size(0) < (1l << 30) &&
       a.size(0) < (1l << 16) && plain_rows(x) && plain_rows(w) && a.is_contiguous() && aligned(a) &&
-      b.is_contiguous() && aligned(b) && meta.size() == 9 && meta[0] == x.size(0) && meta[1] <= a.size(0) &&
+      b.is_contiguous() && aligned(b) && meta.size() == 10 && meta[0] == x.size(0) && meta[1] <= a.size(0) &&
       buf.device() == x.device() && buf.scalar_type() == at::kInt && buf.is_contiguous() &&
       (!scales.has_value() || (scales->dim() == 1 && scales->size(0) == a.size(0) && scales->is_contiguous() &&
                                scales->scalar_type() == at::kFloat && scales->device() == x.device() &&

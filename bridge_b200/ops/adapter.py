@@ -54,14 +54,14 @@ class AdapterRows:
 
 
 def _lay_out(cu: list[int], slots: list[int]) -> tuple[np.ndarray, list[int]]:
-    """The plan as the kernels read it, one int32 buffer, and ``[rows, slots, units, where its parts begin]``.
+    """The plan as the kernels read it, one int32 buffer, and ``[rows, slots, units, blocks, where its parts begin]``.
 
     * ``row_slot [T]``;
     * per tile of 256 rows, the slots that it meets: ``tile_start [tiles + 1]`` into ``pairs [., 12]`` =
       (slot, 0, 0, 0, 8 words with the bits of the rows that are NOT the slot's);
     * the same by tiles of 128 rows, each pair by itself: ``units [., 8]`` = (tile, slot, 0, 0, 4 words);
-    * per slot, its rows in blocks of at most 64: ``block_start [slots + 1]`` into ``blocks [., 2]`` = (first
-      row, rows).  A block ends where the slot's rows end, so that it holds no other request's row.
+    * per slot, its rows in blocks of at most 64: ``block_start [slots + 1]`` into ``blocks [., 4]`` = (first
+      row, rows, slot, 0).  A block ends where the slot's rows end, so that it holds no other request's row.
     """
     rows, top = cu[-1], max(slots, default=-1) + 1
     row_slot = np.repeat(np.asarray(slots, np.int64), np.diff(np.asarray(cu, np.int64)))
@@ -85,8 +85,9 @@ def _lay_out(cu: list[int], slots: list[int]) -> tuple[np.ndarray, list[int]]:
     count = -(-length // _BLOCK)
     run = np.repeat(np.arange(len(first)), count)
     step = np.arange(len(run)) - np.repeat(np.cumsum(count) - count, count)
-    blocks = np.stack((first[run] + _BLOCK * step, np.minimum(_BLOCK, length[run] - _BLOCK * step)), axis=1)
-    owner = row_slot[blocks[:, 0]] if len(blocks) else np.zeros(0, np.int64)
+    row = first[run] + _BLOCK * step
+    owner = row_slot[row]
+    blocks = np.stack((row, np.minimum(_BLOCK, length[run] - _BLOCK * step), owner, 0 * row), axis=1)
     order = np.argsort(owner, kind="stable")
     block_start = np.searchsorted(owner[order], np.arange(top + 1))
 
@@ -96,7 +97,7 @@ def _lay_out(cu: list[int], slots: list[int]) -> tuple[np.ndarray, list[int]]:
         where.append(total)
         parts.append(np.concatenate((flat, np.zeros(-len(flat) % 4, np.int32))))      # each begins at 16 bytes
         total += len(parts[-1])
-    return np.concatenate(parts), [rows, top, len(units), *where]
+    return np.concatenate(parts), [rows, top, len(units), len(blocks), *where]
 
 
 def adapter_rows(cu_seqlens: Sequence[int], slots: Sequence[int], device=None) -> AdapterRows:

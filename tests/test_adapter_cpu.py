@@ -51,7 +51,7 @@ def test_plan(seed):
     for n in lengths:
         cu.append(cu[-1] + n)
     rows = adapter_rows(cu, slots, device="cpu")
-    total, top, units, o_row, o_tile, o_pair, o_unit, o_start, o_block = rows.meta
+    total, top, units, blocks, o_row, o_tile, o_pair, o_unit, o_start, o_block = rows.meta
     table = rows.table.tolist()
     want = row_slots(cu, slots, "cpu").tolist()
     assert total == cu[-1] and top == max(slots) + 1 and table[o_row:o_row + total] == want
@@ -75,11 +75,12 @@ def test_plan(seed):
             seen[128 * unit[0] + i] = unit[1]
     assert seen == want
     seen = [-1] * total
+    assert table[o_start] == 0 and table[o_start + top] == blocks
     for s in range(top):
         last = -1
         for at in range(table[o_start + s], table[o_start + s + 1]):
-            row, n = table[o_block + 2 * at:o_block + 2 * at + 2]
-            assert 1 <= n <= 64 and row > last
+            row, n, slot, _ = table[o_block + 4 * at:o_block + 4 * at + 4]
+            assert 1 <= n <= 64 and row > last and slot == s
             last = row + n - 1
             assert seen[row:row + n] == [-1] * n
             seen[row:row + n] = [s] * n
