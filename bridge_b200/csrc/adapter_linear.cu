@@ -83,12 +83,6 @@ __device__ __forceinline__ void spill(uint32_t tmem, float* part, int cols, bool
   }
 }
 
-__device__ __forceinline__ float ld_cluster1(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
-}
-
 // The sum over the cluster's partial accumulators of four columns, in rank order.
 __device__ __forceinline__ float4 joined(uint32_t part, int at, int ranks) {
   float4 s = ld_cluster4(sm100::mapa(part + at * 4, 0));
@@ -211,32 +205,24 @@ __global__ void __launch_bounds__(kThreads)
 // ------------------------------------------------------------------------------------------------ few rows
 struct FewParams {
   AdapterPlan plan;
-  const uint16_t *u, *low;
   uint16_t* y;
-  int T, N, R, cols, stages, nk, ranks;
+  int T, N, R, rows, stages, nk, ranks;   // rows: T up to the next 8
   uint32_t idesc;
   bool half;
 };
 
-__device__ __forceinline__ float2 unpack2(uint32_t v, bool half) {
-  if (half) return __half22float2(*reinterpret_cast<const __half2*>(&v));
-  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
-}
-__device__ __forceinline__ float unpack1(uint16_t v, bool half) {
-  return half ? __half2float(__ushort_as_half(v)) : __bfloat162float(__ushort_as_bfloat16(v));
-}
-
-// At most 128 rows: bound by the read of W, so W takes the matrix instructions' wide side.  A cluster of `ranks` blocks
-// streams 128 rows (with MN: columns) of W, each block a stretch of K, for all rows of x: y^T = W x^T.  The low-rank part
-// is a few products per value, made with ordinary FP32 arithmetic where the partial sums meet.  u is waited for there,
-// so that this kernel streams W while the one before it still makes u.
+// At most 128 rows: bound by the read of W.  A cluster of `ranks` blocks takes 128 columns of y, each block a stretch of K
+// (and some of the slots' low-rank products); the partial sums meet in shared memory.  Only the rows that there are get
+// loaded: the matrix instruction's other rows read whatever lies behind, and nobody reads what becomes of them.  u is
+// waited for when W has been asked for, so that this kernel streams W while the one before it still makes u.
 template <bool MN>
 __global__ void __launch_bounds__(kThreads)
-    adapter_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+    adapter_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                       const __grid_constant__ CUtensorMap map_u, const __grid_constant__ CUtensorMap map_low,
                        const FewParams p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int stage_bytes = kXBytes + p.cols * 128;
+  const int x_bytes = p.rows * 128, stage_bytes = x_bytes + kXBytes;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + p.stages * stage_bytes);
   uint64_t* empty = full + p.stages;
   uint64_t* done = empty + p.stages;
@@ -244,6 +230,7 @@ __global__ void __launch_bounds__(kThreads)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)sm100::cluster_ctarank(), n0 = blockIdx.x / p.ranks * BM;
   const int kb0 = (int)((long)p.nk * rank / p.ranks), kb1 = (int)((long)p.nk * (rank + 1) / p.ranks);
+  const int rank_blocks = (p.R + BK - 1) / BK;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
@@ -262,76 +249,99 @@ __global__ void __launch_bounds__(kThreads)
   if (warp == 0 && lane == 0) {
     int stage = 0;
     uint32_t phase = 0;
-    for (int kb = kb0; kb < kb1; ++kb) {
-      if (!sm100::mbar_wait(&empty[stage], phase ^ 1, &g_error, 61)) break;
-      unsigned char* dst = smem + stage * stage_bytes;
-      sm100::mbar_expect_tx(&full[stage], stage_bytes);
-      if (MN) {
-        sm100::tma_load_2d(dst, &map_w, &full[stage], n0, kb * BK);
-        sm100::tma_load_2d(dst + 8192, &map_w, &full[stage], n0 + 64, kb * BK);
-      } else {
-        sm100::tma_load_2d(dst, &map_w, &full[stage], kb * BK, n0);
-      }
-      sm100::tma_load_2d(dst + kXBytes, &map_x, &full[stage], kb * BK, 0);
+    bool ok = true;
+    unsigned char *x_dst = nullptr, *w_dst = nullptr;
+    uint64_t* bar = nullptr;
+    auto claim = [&]() {
+      ok = ok && sm100::mbar_wait(&empty[stage], phase ^ 1, &g_error, 61);
+      if (!ok) return false;
+      bar = &full[stage];
+      x_dst = smem + stage * stage_bytes, w_dst = x_dst + x_bytes;
+      sm100::mbar_expect_tx(bar, stage_bytes);
       if (++stage == p.stages) stage = 0, phase ^= 1;
+      return true;
+    };
+    for (int kb = kb0; kb < kb1 && claim(); ++kb) {
+      if (MN) {
+        sm100::tma_load_2d(w_dst, &map_w, bar, n0, kb * BK);
+        sm100::tma_load_2d(w_dst + 8192, &map_w, bar, n0 + 64, kb * BK);
+      } else {
+        sm100::tma_load_2d(w_dst, &map_w, bar, kb * BK, n0);
+      }
+      sm100::tma_load_2d(x_dst, &map_x, bar, kb * BK, 0);
     }
-  } else if (warp == 1 && lane == 0 && kb1 > kb0) {
+    wait_for_previous();       // u, which TMA reads from here on
+    asm volatile("fence.proxy.async.global;" ::: "memory");
+    for (int i = rank; i < p.plan.num_units; i += p.ranks) {
+      const int slot = __ldg(p.plan.units + (size_t)i * 8 + 1);
+      for (int rb = 0; rb < rank_blocks && claim(); ++rb) {
+        sm100::tma_load_2d(x_dst, &map_u, bar, rb * BK, 0);
+        if (MN) {
+          sm100::tma_load_3d(w_dst, &map_low, bar, n0, rb * BK, slot);
+          sm100::tma_load_3d(w_dst + 8192, &map_low, bar, n0 + 64, rb * BK, slot);
+        } else {
+          sm100::tma_load_3d(w_dst, &map_low, bar, rb * BK, n0, slot);
+        }
+      }
+    }
+  } else if (warp == 1 && lane == 0) {
     int stage = 0;
     uint32_t phase = 0;
-    for (int kb = kb0; kb < kb1; ++kb) {
-      if (!sm100::mbar_wait(&full[stage], phase, &g_error, 62)) break;
+    bool ok = true;
+    auto products = [&](int steps, bool first, const uint32_t (&off)[4]) {
+      ok = ok && sm100::mbar_wait(&full[stage], phase, &g_error, 62);
+      if (!ok) return;
       sm100::tc_fence_after();
-      const uint32_t a = sm100::smem_addr(smem + stage * stage_bytes), b = a + kXBytes;
-#pragma unroll
-      for (int kk = 0; kk < BK / 16; ++kk)
-        sm100::umma_bf16(tmem, MN ? sm100::umma_desc_sw128(a + kk * 2048, 8192, 1024)
-                                  : sm100::umma_desc_sw128(a + kk * 32, 16, 1024),
-                         sm100::umma_desc_sw128(b + kk * 32, 16, 1024), p.idesc, kb > kb0 || kk > 0);
+      const uint32_t a = sm100::smem_addr(smem + stage * stage_bytes), b = a + x_bytes;
+      for (int kk = 0; kk < steps; ++kk)
+        sm100::umma_masked(tmem, sm100::umma_desc_sw128(a + kk * 32, 16, 1024),
+                           MN ? sm100::umma_desc_sw128(b + kk * 2048, 8192, 1024)
+                              : sm100::umma_desc_sw128(b + kk * 32, 16, 1024),
+                           p.idesc, !first || kk > 0, off);
       sm100::umma_commit(&empty[stage]);
       if (++stage == p.stages) stage = 0, phase ^= 1;
+    };
+    const uint32_t all[4] = {0, 0, 0, 0};
+    for (int kb = kb0; kb < kb1; ++kb) products(BK / 16, kb == kb0, all);
+    for (int i = rank; i < p.plan.num_units; i += p.ranks) {
+      const int4 m = __ldg(reinterpret_cast<const int4*>(p.plan.units + (size_t)i * 8) + 1);
+      const uint32_t off[4] = {(uint32_t)m.x, (uint32_t)m.y, (uint32_t)m.z, (uint32_t)m.w};
+      for (int rb = 0; rb < rank_blocks; ++rb) products(min(BK / 16, (p.R - rb * BK + 15) / 16), false, off);
     }
     sm100::umma_commit(done);
   }
   __syncwarp();
+  constexpr int kRow = BM + 4;     // floats: rows 16 bytes apart in the banks
   float* part = reinterpret_cast<float*>(smem);
   if (warp >= 2) {
-    if (kb1 > kb0) sm100::mbar_wait(done, 0, &g_error, 63);
+    const int quarter = warp & 3, row = quarter * 32 + lane;
+    sm100::mbar_wait(done, 0, &g_error, 63);
     __syncwarp();
     sm100::tc_fence_after();
-    spill(tmem, part, p.cols, kb1 > kb0);
+    if (quarter * 32 < p.T)
+      for (int c = 0; c < BM; c += 32) {
+        uint32_t r[32];
+        sm100::tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + c, r);
+        sm100::tmem_ld_wait();
+        sm100::tmem_regs_ready(r);
+        if (row < p.T)
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<uint4*>(part + row * kRow + c + i) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
+      }
     sm100::tc_fence_before();
   }
   __syncthreads();
   sm100::cluster_sync();
-  wait_for_previous();
-  // this block's share of W's rows; neighbours take neighbouring columns of y
-  const int lo = BM * rank / p.ranks, rows = BM * (rank + 1) / p.ranks - lo;
+  // this block's share of the 16 groups of 8 columns
+  const int lo = 16 * rank / p.ranks, groups = 16 * (rank + 1) / p.ranks - lo;
   const uint32_t base = sm100::smem_addr(part);
-  for (int i = threadIdx.x; i < rows * p.T; i += kThreads) {
-    const int r = lo + i % rows, t = i / rows, n = n0 + r;
-    if (n >= p.N) continue;
-    float v = 0.f;
-    for (int j = 0; j < p.ranks; ++j) v += ld_cluster1(sm100::mapa(base + (r * (p.cols + 4) + t) * 4, j));
-    const int slot = __ldg(p.plan.row_slot + t);
-    if (slot >= 0) {
-      const uint16_t* u = p.u + (size_t)t * p.R;
-      for (int c = 0; c < p.R; c += 8) {
-        const uint4 a = *reinterpret_cast<const uint4*>(u + c);
-        const float2 a0 = unpack2(a.x, p.half), a1 = unpack2(a.y, p.half), a2 = unpack2(a.z, p.half), a3 = unpack2(a.w, p.half);
-        if (MN) {
-          const uint16_t* b = p.low + ((size_t)slot * p.R + c) * p.N + n;
-          const float q[8] = {a0.x, a0.y, a1.x, a1.y, a2.x, a2.y, a3.x, a3.y};
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v = fmaf(q[j], unpack1(__ldg(b + (size_t)j * p.N), p.half), v);
-        } else {
-          const uint4 b = __ldg(reinterpret_cast<const uint4*>(p.low + ((size_t)slot * p.N + n) * p.R + c));
-          const float2 b0 = unpack2(b.x, p.half), b1 = unpack2(b.y, p.half), b2 = unpack2(b.z, p.half), b3 = unpack2(b.w, p.half);
-          v = fmaf(a0.x, b0.x, v), v = fmaf(a0.y, b0.y, v), v = fmaf(a1.x, b1.x, v), v = fmaf(a1.y, b1.y, v);
-          v = fmaf(a2.x, b2.x, v), v = fmaf(a2.y, b2.y, v), v = fmaf(a3.x, b3.x, v), v = fmaf(a3.y, b3.y, v);
-        }
-      }
-    }
-    p.y[(size_t)t * p.N + n] = pack1(v, p.half);
+  for (int i = threadIdx.x; i < groups * p.T; i += kThreads) {
+    const int c = (lo + i % groups) * 8, t = i / groups;
+    if (n0 + c >= p.N) continue;
+    const float4 v = joined(base, t * kRow + c, p.ranks), w = joined(base, t * kRow + c + 4, p.ranks);
+    *reinterpret_cast<uint4*>(p.y + (size_t)t * p.N + n0 + c) =
+        make_uint4(pack2(v.x, v.y, p.half), pack2(v.z, v.w, p.half), pack2(w.x, w.y, p.half), pack2(w.z, w.w, p.half));
   }
   sm100::cluster_sync();   // the peers' sums stay until all have read them
   if (warp == 1) {
@@ -1017,27 +1027,28 @@ constexpr int kFewRows = 128;
 
 template <bool MN>
 cudaError_t run_few(const AdapterJoint& a, cudaStream_t stream) {
-  alignas(64) CUtensorMap w, x;
-  const int cols = (a.T + 15) / 16 * 16;
-  if (!(MN ? encode(&w, a.w, a.N, a.K, a.ldw, 0, 64, a.half) : encode(&w, a.w, a.K, a.N, a.ldw, 0, BM, a.half)) ||
-      !encode(&x, a.x, a.K, a.T, a.ldx, 0, cols, a.half))
-    return cudaErrorInvalidValue;
+  alignas(64) CUtensorMap x, w, u, low;
+  const int rows = (a.T + 7) / 8 * 8;
+  bool ok = encode(&x, a.x, a.K, a.T, a.ldx, 0, rows, a.half) && encode(&u, a.u, a.R, a.T, a.R, 0, rows, a.half);
+  if (MN) ok = ok && encode(&w, a.w, a.N, a.K, a.ldw, 0, 64, a.half) && encode(&low, a.low, a.N, a.R, a.N, a.S, 64, a.half);
+  else ok = ok && encode(&w, a.w, a.K, a.N, a.ldw, 0, BM, a.half) && encode(&low, a.low, a.R, a.N, a.R, a.S, BM, a.half);
+  if (!ok) return cudaErrorInvalidValue;
   FewParams p{};
   p.plan = a.plan;
-  p.u = static_cast<const uint16_t*>(a.u), p.low = static_cast<const uint16_t*>(a.low);
   p.y = static_cast<uint16_t*>(a.y);
-  p.T = a.T, p.N = a.N, p.R = a.R, p.cols = cols;
+  p.T = a.T, p.N = a.N, p.R = a.R, p.rows = rows;
   p.nk = (a.K + BK - 1) / BK;
   p.stages = 4;
   const int tiles = (a.N + BM - 1) / BM;
-  p.idesc = sm100::umma_idesc_bf16(BM, cols, MN, false) & ~(a.half ? sm100::kIdescBf16 : 0u);
+  p.idesc = sm100::umma_idesc_bf16(BM, BM, false, MN) & ~(a.half ? sm100::kIdescBf16 : 0u);
   p.half = a.half;
-  const int smem = std::max(p.stages * (kXBytes + cols * 128), BM * (cols + 4) * 4) + 256 + 1024;
+  const int smem = std::max(p.stages * (kXBytes + rows * 128), a.T * (BM + 4) * 4) + 256 + 1024;
   static std::atomic<unsigned long long> done{0};
   const cudaError_t e = allow_smem(adapter_few_kernel<MN>, kMaxSmem, done);
   if (e != cudaSuccess) return e;
   p.ranks = split(adapter_few_kernel<MN>, smem, 128, tiles, p.nk);
-  return launch(adapter_few_kernel<MN>, tiles * p.ranks, kThreads, smem, p.ranks, a.plan.num_units > 0, stream, w, x, p);
+  return launch(adapter_few_kernel<MN>, tiles * p.ranks, kThreads, smem, p.ranks, a.plan.num_units > 0, stream, x, w, u,
+                low, p);
 }
 
 // How the tiles of 256 x 256 go to the pairs of SMs.
