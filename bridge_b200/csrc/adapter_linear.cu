@@ -58,7 +58,10 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
 }
 
 // Programmatic dependent launch: the next kernel of the stream may begin (its blocks find room as this grid's end); and
-// what a kernel that began so waits for before it reads what the one before it wrote.
+// the wait, until the kernel before this one is complete, of one that began so.  Every kernel here begins early, prepares
+// itself and waits before it touches anything that another one makes (the plan was complete before any launch).  The
+// joint products go further: behind a shrink they take x and W without a wait, and wait for u only; so a shrink lets
+// them begin only when its own wait, for x and W among others, is over.
 __device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
@@ -136,7 +139,8 @@ __global__ void __launch_bounds__(kThreads)
   __syncthreads();
   sm100::tc_fence_after();
   const uint32_t tmem = *tmem_word;
-  let_next_begin();        // (not before: a block that waits for TMEM must not wait for one that waits for this grid)
+  wait_for_previous();
+  let_next_begin();        // (not before: see there; nor before this block has its TMEM, which one that waits may take)
 
   if (warp == 0 && lane == 0) {
     int stage = 0;
@@ -245,6 +249,9 @@ __global__ void __launch_bounds__(kThreads)
   __syncthreads();
   sm100::tc_fence_after();
   const uint32_t tmem = *tmem_word;
+
+  if (p.plan.num_units == 0) wait_for_previous();
+  let_next_begin();
 
   if (warp == 0 && lane == 0) {
     int stage = 0;
@@ -435,6 +442,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   sm100::cluster_sync();
   sm100::tc_fence_after();
   const uint32_t tmem = *tmem_word;
+  if (p.plan.num_units == 0) wait_for_previous();
   let_next_begin();
 
   if (warp == 0) {
@@ -624,6 +632,7 @@ __global__ void __launch_bounds__(256) adapter_join_kernel(const __grid_constant
   const int tile = blockIdx.x / 16, c = blockIdx.x % 16 * 16;
   const Piece w = piece_at(p, p.whole + tile * p.slices);
   const int row = w.mt * 256 + threadIdx.x, col = w.nt * 256 + c;
+  let_next_begin();
   wait_for_previous();
   if (row >= p.T || col >= p.N) return;
   float4 v[4] = {};
@@ -737,6 +746,8 @@ __global__ void __launch_bounds__(kThreads)
   __syncthreads();
   sm100::tc_fence_after();
   const uint32_t tmem = *tmem_word;
+  let_next_begin();
+  wait_for_previous();
   float* part = reinterpret_cast<float*>(smem);
 
   if (warp == 0) {
@@ -926,10 +937,10 @@ cudaError_t allow_smem(Kernel kernel, int bytes, std::atomic<unsigned long long>
   return e;
 }
 
-// `early`: the kernel may begin while the one before it in the stream ends (it waits by itself for what that one wrote).
+// The kernel may begin while the one before it in the stream ends (it waits by itself for what that one wrote).
 // `cluster`: blocks of one, 0 where the kernel says it itself.
 template <typename... P, typename... A>
-cudaError_t launch(void (*kernel)(P...), int grid, int threads, int smem, int cluster, bool early, cudaStream_t stream,
+cudaError_t launch(void (*kernel)(P...), int grid, int threads, int smem, int cluster, cudaStream_t stream,
                    const A&... args) {
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[2];
@@ -943,11 +954,9 @@ cudaError_t launch(void (*kernel)(P...), int grid, int threads, int smem, int cl
     attr[n].val.clusterDim.x = cluster, attr[n].val.clusterDim.y = 1, attr[n].val.clusterDim.z = 1;
     ++n;
   }
-  if (early) {
-    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[n].val.programmaticStreamSerializationAllowed = 1;
-    ++n;
-  }
+  attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[n].val.programmaticStreamSerializationAllowed = 1;
+  ++n;
   cfg.attrs = attr;
   cfg.numAttrs = n;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
@@ -1020,7 +1029,7 @@ cudaError_t run_shrink(const AdapterShrink& a, cudaStream_t stream) {
   const cudaError_t e = allow_smem(adapter_shrink_kernel<OP_MN>, kMaxSmem, done);
   if (e != cudaSuccess) return e;
   p.ranks = split(adapter_shrink_kernel<OP_MN>, smem, 128, a.plan.num_units, p.nk);
-  return launch(adapter_shrink_kernel<OP_MN>, a.plan.num_units * p.ranks, kThreads, smem, p.ranks, false, stream, x, op, p);
+  return launch(adapter_shrink_kernel<OP_MN>, a.plan.num_units * p.ranks, kThreads, smem, p.ranks, stream, x, op, p);
 }
 
 constexpr int kFewRows = 128;
@@ -1038,7 +1047,8 @@ cudaError_t run_few(const AdapterJoint& a, cudaStream_t stream) {
   p.y = static_cast<uint16_t*>(a.y);
   p.T = a.T, p.N = a.N, p.R = a.R, p.rows = rows;
   p.nk = (a.K + BK - 1) / BK;
-  p.stages = 4;
+  // two blocks to an SM: 3 stages (of 32 KB, 128 rows) to 6 (of 17 KB, 8 rows)
+  p.stages = std::min(6, 110 * 1024 / (kXBytes + rows * 128));
   const int tiles = (a.N + BM - 1) / BM;
   p.idesc = sm100::umma_idesc_bf16(BM, BM, false, MN) & ~(a.half ? sm100::kIdescBf16 : 0u);
   p.half = a.half;
@@ -1047,7 +1057,7 @@ cudaError_t run_few(const AdapterJoint& a, cudaStream_t stream) {
   const cudaError_t e = allow_smem(adapter_few_kernel<MN>, kMaxSmem, done);
   if (e != cudaSuccess) return e;
   p.ranks = split(adapter_few_kernel<MN>, smem, 128, tiles, p.nk);
-  return launch(adapter_few_kernel<MN>, tiles * p.ranks, kThreads, smem, p.ranks, a.plan.num_units > 0, stream, x, w, u,
+  return launch(adapter_few_kernel<MN>, tiles * p.ranks, kThreads, smem, p.ranks, stream, x, w, u,
                 low, p);
 }
 
@@ -1093,9 +1103,9 @@ cudaError_t run_joint(const AdapterJoint& a, cudaStream_t stream) {
   static std::atomic<unsigned long long> done{0};
   cudaError_t e = allow_smem(adapter_joint_kernel<MN>, kPairSmem, done);
   if (e != cudaSuccess) return e;
-  e = launch(adapter_joint_kernel<MN>, 2 * c.pairs, kThreads, kPairSmem, 0, a.plan.num_units > 0, stream, x, w, u, low, y, p);
+  e = launch(adapter_joint_kernel<MN>, 2 * c.pairs, kThreads, kPairSmem, 0, stream, x, w, u, low, y, p);
   if (e != cudaSuccess || c.units == c.whole) return e;
-  return launch(adapter_join_kernel, (c.units - c.whole) / c.slices * 16, 256, 0, 0, true, stream, p);
+  return launch(adapter_join_kernel, (c.units - c.whole) / c.slices * 16, 256, 0, 0, stream, p);
 }
 
 }  // namespace
@@ -1147,7 +1157,7 @@ cudaError_t launch_adapter_grads(const AdapterGrads& a, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   const int tiles = p.tiles_a + p.tiles_b;
   p.ranks = split(adapter_grads_kernel, smem, p.cols == 64 ? 256 : 512, tiles, std::max(1, a.plan.num_blocks));
-  return launch(adapter_grads_kernel, tiles * p.ranks, kThreads, smem, p.ranks, false, stream, x, dy, u, du, p);
+  return launch(adapter_grads_kernel, tiles * p.ranks, kThreads, smem, p.ranks, stream, x, dy, u, du, p);
 }
 
 int adapter_error_code() {

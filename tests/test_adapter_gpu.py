@@ -215,6 +215,45 @@ def test_same_results_again_on_another_stream_and_captured(t):
         assert all(torch.equal(out[n], v) for n, v in want.items())
 
 
+@pytest.mark.parametrize("t", [17, 400])
+@pytest.mark.parametrize("slot", [-1, 1])
+def test_inputs_made_just_before(t, slot):
+    """Every kernel begins while the one before it ends: inputs that the stream has only just filled, by copies, memsets
+    and kernels, eagerly and captured, are those that count."""
+    x, w, a, b, dy = _inputs(t, 1024, 768, 2, 16, torch.bfloat16)
+    rows = adapter_rows([0, t], [slot], device=DEV)
+    want = _train(x, w, a, b, rows, 1.0, dy)
+    live = [torch.empty_like(v) for v in (x, w, a, b, dy)]
+    big = torch.randn(64, 1 << 20, device=DEV)
+
+    def fill_and_run():
+        for v in live:
+            v.zero_()
+        big.mul_(1.0)
+        for v, of in zip(live, (x, w, a, b, dy)):
+            v.copy_(of)
+        out = _train(*live[:4], rows, 1.0, live[4])
+        for v in live:               # ... and are read before the stream's next work overwrites them
+            v.fill_(math.nan)
+        return out
+
+    for _ in range(5):
+        got = fill_and_run()
+        assert all(torch.equal(got[n], v) for n, v in want.items())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = fill_and_run()
+    for _ in range(5):
+        g.replay()
+        assert all(torch.equal(got[n], v) for n, v in want.items())
+    w2, a2 = w[:, :768].contiguous(), a[:, :, :768].contiguous()      # a projection of what another one made
+    chained = adapter_linear(adapter_linear(x, w, a, b, rows), w2, a2, b, rows)
+    torch.cuda.synchronize()
+    mid = adapter_linear(x, w, a, b, rows)
+    torch.cuda.synchronize()
+    assert torch.equal(chained, adapter_linear(mid, w2, a2, b, rows))
+
+
 def test_gradients_against_differences():
     """A direction's derivative of a weighted sum of y, from y alone."""
     x, w, a, b, dy = _inputs(150, 256, 256, 2, 8, torch.float16)
