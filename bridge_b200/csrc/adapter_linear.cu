@@ -964,10 +964,13 @@ cudaError_t launch(void (*kernel)(P...), int grid, int threads, int smem, int cl
   return e;
 }
 
-// Blocks of a cluster: as many (at most 8, each with two blocks of the sum or more) as let all clusters run at once.
-// More blocks mean more loads in flight; a cluster that has to wait for room, a second round.  (Clusters lie within a
-// GPC, so how many fit is less than blocks over SMs: 15 of 8 with a block to an SM, not 18.  The runtime counts one block
-// of a kernel with TMEM to an SM; there are as many as its shared memory and its `columns` of TMEM leave room for.)
+// Blocks of a cluster: as many, at most 8, as let all clusters run at once, each with two blocks of the sum; more than one
+// block per SM only if each has eight.  More blocks mean more loads in flight, but each costs its start and its part in
+// the joining of sums.  Measured: one row through 2560 -> 6144 (48 clusters) 16.9, 11.1, 9.3, 9.6 us with 1, 2, 4 and 6
+// blocks; the shrink of 71 tiles over K = 9728 68, 48, 44, 53 us with 1, 2, 4 and 6, of 30 over 2048 3 us more with 8 than
+// with 4.  (Clusters lie within a GPC, so how many fit is less than blocks over SMs: 15 of 8 with a block to an SM, not 18.
+// The runtime counts one block of a kernel with TMEM to an SM; there are as many as its shared memory and its `columns`
+// of TMEM leave room for.)
 template <typename... P>
 int split(void (*kernel)(P...), int smem, int columns, int clusters, int nk) {
   struct Fit {
@@ -1002,7 +1005,7 @@ int split(void (*kernel)(P...), int smem, int columns, int clusters, int nk) {
   }
   const int per_sm = std::max(1, std::min(kMaxSmem / (smem + 1024), 512 / columns));
   int ranks = 8;
-  while (ranks > 1 && (clusters > per_sm * fit->fits[ranks] || nk < 2 * ranks)) --ranks;
+  while (ranks > 1 && (clusters > per_sm * fit->fits[ranks] || nk < (clusters * ranks > sm_count() ? 8 : 2) * ranks)) --ranks;
   return ranks;
 }
 
@@ -1047,9 +1050,10 @@ cudaError_t run_few(const AdapterJoint& a, cudaStream_t stream) {
   p.y = static_cast<uint16_t*>(a.y);
   p.T = a.T, p.N = a.N, p.R = a.R, p.rows = rows;
   p.nk = (a.K + BK - 1) / BK;
-  // two blocks to an SM: 3 stages (of 32 KB, 128 rows) to 6 (of 17 KB, 8 rows)
-  p.stages = std::min(6, 110 * 1024 / (kXBytes + rows * 128));
   const int tiles = (a.N + BM - 1) / BM;
+  // 72 to 128 KB; where tiles outnumber the SMs, little enough for two blocks to an SM.  (128 rows, 4 stages: 14.7 us with
+  // 2 blocks a cluster and one to an SM, 18 with 3 stages and more of them; 152 tiles: 27 us with 3 stages, 42 with 4.)
+  p.stages = tiles > sm_count() ? std::min(4, 110 * 1024 / (kXBytes + rows * 128)) : 4;
   p.idesc = sm100::umma_idesc_bf16(BM, BM, false, MN) & ~(a.half ? sm100::kIdescBf16 : 0u);
   p.half = a.half;
   const int smem = std::max(p.stages * (kXBytes + rows * 128), a.T * (BM + 4) * 4) + 256 + 1024;
