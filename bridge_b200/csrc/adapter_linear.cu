@@ -210,13 +210,13 @@ __global__ void __launch_bounds__(kThreads)
 struct FewParams {
   AdapterPlan plan;
   uint16_t* y;
-  int T, N, R, rows, stages, nk, ranks;   // rows: T up to the next 8
+  int T, N, R, rows, stages, nk, ranks;   // rows of a tile: 128, or T up to the next 8
   uint32_t idesc;
   bool half;
 };
 
-// At most 128 rows: bound by the read of W.  A cluster of `ranks` blocks takes 128 columns of y, each block a stretch of K
-// (and some of the slots' low-rank products); the partial sums meet in shared memory.  Only the rows that there are get
+// Few rows: bound by the read of W.  A cluster of `ranks` blocks takes 128 columns of y (and 128 rows), each block a
+// stretch of K and some of the slots' low-rank products; the partial sums meet in shared memory.  Only the rows that there are get
 // loaded: the matrix instruction's other rows read whatever lies behind, and nobody reads what becomes of them.  u is
 // waited for when W has been asked for, so that this kernel streams W while the one before it still makes u.
 template <bool MN>
@@ -232,7 +232,9 @@ __global__ void __launch_bounds__(kThreads)
   uint64_t* done = empty + p.stages;
   uint32_t* tmem_word = reinterpret_cast<uint32_t*>(done + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = (int)sm100::cluster_ctarank(), n0 = blockIdx.x / p.ranks * BM;
+  const int tile = blockIdx.x / p.ranks, m_tiles = (p.T + BM - 1) / BM;    // neighbours share columns of W
+  const int rank = (int)sm100::cluster_ctarank(), mt = tile % m_tiles, m0 = mt * BM, n0 = tile / m_tiles * BM;
+  const int rows = min(BM, p.T - m0);
   const int kb0 = (int)((long)p.nk * rank / p.ranks), kb1 = (int)((long)p.nk * (rank + 1) / p.ranks);
   const int rank_blocks = (p.R + BK - 1) / BK;
 
@@ -275,14 +277,16 @@ __global__ void __launch_bounds__(kThreads)
       } else {
         sm100::tma_load_2d(w_dst, &map_w, bar, kb * BK, n0);
       }
-      sm100::tma_load_2d(x_dst, &map_x, bar, kb * BK, 0);
+      sm100::tma_load_2d(x_dst, &map_x, bar, kb * BK, m0);
     }
     wait_for_previous();       // u, which TMA reads from here on
     asm volatile("fence.proxy.async.global;" ::: "memory");
-    for (int i = rank; i < p.plan.num_units; i += p.ranks) {
-      const int slot = __ldg(p.plan.units + (size_t)i * 8 + 1);
+    for (int i = 0, mine = 0; i < p.plan.num_units; ++i) {
+      const int2 unit = __ldg(reinterpret_cast<const int2*>(p.plan.units + (size_t)i * 8));
+      if (unit.x != mt || mine++ % p.ranks != rank) continue;
+      const int slot = unit.y;
       for (int rb = 0; rb < rank_blocks && claim(); ++rb) {
-        sm100::tma_load_2d(x_dst, &map_u, bar, rb * BK, 0);
+        sm100::tma_load_2d(x_dst, &map_u, bar, rb * BK, m0);
         if (MN) {
           sm100::tma_load_3d(w_dst, &map_low, bar, n0, rb * BK, slot);
           sm100::tma_load_3d(w_dst + 8192, &map_low, bar, n0 + 64, rb * BK, slot);
@@ -310,7 +314,8 @@ __global__ void __launch_bounds__(kThreads)
     };
     const uint32_t all[4] = {0, 0, 0, 0};
     for (int kb = kb0; kb < kb1; ++kb) products(BK / 16, kb == kb0, all);
-    for (int i = rank; i < p.plan.num_units; i += p.ranks) {
+    for (int i = 0, mine = 0; i < p.plan.num_units; ++i) {
+      if (__ldg(p.plan.units + (size_t)i * 8) != mt || mine++ % p.ranks != rank) continue;
       const int4 m = __ldg(reinterpret_cast<const int4*>(p.plan.units + (size_t)i * 8) + 1);
       const uint32_t off[4] = {(uint32_t)m.x, (uint32_t)m.y, (uint32_t)m.z, (uint32_t)m.w};
       for (int rb = 0; rb < rank_blocks; ++rb) products(min(BK / 16, (p.R - rb * BK + 15) / 16), false, off);
@@ -325,13 +330,13 @@ __global__ void __launch_bounds__(kThreads)
     sm100::mbar_wait(done, 0, &g_error, 63);
     __syncwarp();
     sm100::tc_fence_after();
-    if (quarter * 32 < p.T)
+    if (quarter * 32 < rows)
       for (int c = 0; c < BM; c += 32) {
         uint32_t r[32];
         sm100::tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + c, r);
         sm100::tmem_ld_wait();
         sm100::tmem_regs_ready(r);
-        if (row < p.T)
+        if (row < rows)
 #pragma unroll
           for (int i = 0; i < 32; i += 4)
             *reinterpret_cast<uint4*>(part + row * kRow + c + i) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
@@ -343,11 +348,11 @@ __global__ void __launch_bounds__(kThreads)
   // this block's share of the 16 groups of 8 columns
   const int lo = 16 * rank / p.ranks, groups = 16 * (rank + 1) / p.ranks - lo;
   const uint32_t base = sm100::smem_addr(part);
-  for (int i = threadIdx.x; i < groups * p.T; i += kThreads) {
+  for (int i = threadIdx.x; i < groups * rows; i += kThreads) {
     const int c = (lo + i % groups) * 8, t = i / groups;
     if (n0 + c >= p.N) continue;
     const float4 v = joined(base, t * kRow + c, p.ranks), w = joined(base, t * kRow + c + 4, p.ranks);
-    *reinterpret_cast<uint4*>(p.y + (size_t)t * p.N + n0 + c) =
+    *reinterpret_cast<uint4*>(p.y + (size_t)(m0 + t) * p.N + n0 + c) =
         make_uint4(pack2(v.x, v.y, p.half), pack2(v.z, v.w, p.half), pack2(w.x, w.y, p.half), pack2(w.z, w.w, p.half));
   }
   sm100::cluster_sync();   // the peers' sums stay until all have read them
@@ -964,8 +969,8 @@ cudaError_t launch(void (*kernel)(P...), int grid, int threads, int smem, int cl
   return e;
 }
 
-// Blocks of a cluster: as many, at most 8, as let all clusters run at once, each with two blocks of the sum; more than one
-// block per SM only if each has eight.  More blocks mean more loads in flight, but each costs its start and its part in
+// Blocks of a cluster: as many, at most 8, as let all clusters run at once, each with four steps of 64 of the sum; more than
+// one per SM only if each has eight.  More blocks mean more loads in flight, but each costs its start and its part in
 // the joining of sums.  Measured: one row through 2560 -> 6144 (48 clusters) 16.9, 11.1, 9.3, 9.6 us with 1, 2, 4 and 6
 // blocks; the shrink of 71 tiles over K = 9728 68, 48, 44, 53 us with 1, 2, 4 and 6, of 30 over 2048 3 us more with 8 than
 // with 4.  (Clusters lie within a GPC, so how many fit is less than blocks over SMs: 15 of 8 with a block to an SM, not 18.
@@ -1005,7 +1010,7 @@ int split(void (*kernel)(P...), int smem, int columns, int clusters, int nk) {
   }
   const int per_sm = std::max(1, std::min(kMaxSmem / (smem + 1024), 512 / columns));
   int ranks = 8;
-  while (ranks > 1 && (clusters > per_sm * fit->fits[ranks] || nk < (clusters * ranks > sm_count() ? 8 : 2) * ranks)) --ranks;
+  while (ranks > 1 && (clusters > per_sm * fit->fits[ranks] || nk < (clusters * ranks > sm_count() ? 8 : 4) * ranks)) --ranks;
   return ranks;
 }
 
@@ -1035,12 +1040,19 @@ cudaError_t run_shrink(const AdapterShrink& a, cudaStream_t stream) {
   return launch(adapter_shrink_kernel<OP_MN>, a.plan.num_units * p.ranks, kThreads, smem, p.ranks, stream, x, op, p);
 }
 
-constexpr int kFewRows = 128;
+// Which kernel makes the joint product.  Up to 128 rows the read of W is all there is, and clusters that split K read it
+// fastest; further on as long as tiles of 128 x 128 are few (to a cluster of 3 blocks or more each) and K is long:
+// 4096 -> 2560, 256 rows (40 tiles): 18 us, on pairs of SMs 23; 2560 -> 6144, 256 rows (96 tiles): 22 and 18; 256 -> 512,
+// 256 rows: 11 and 8.5.
+bool few_rows(int T, int K, int N) {
+  const long tiles = (long)((T + BM - 1) / BM) * ((N + BM - 1) / BM);
+  return T <= BM || (tiles <= 48 && K >= 2048);
+}
 
 template <bool MN>
 cudaError_t run_few(const AdapterJoint& a, cudaStream_t stream) {
   alignas(64) CUtensorMap x, w, u, low;
-  const int rows = (a.T + 7) / 8 * 8;
+  const int rows = std::min(BM, (a.T + 7) / 8 * 8);
   bool ok = encode(&x, a.x, a.K, a.T, a.ldx, 0, rows, a.half) && encode(&u, a.u, a.R, a.T, a.R, 0, rows, a.half);
   if (MN) ok = ok && encode(&w, a.w, a.N, a.K, a.ldw, 0, 64, a.half) && encode(&low, a.low, a.N, a.R, a.N, a.S, 64, a.half);
   else ok = ok && encode(&w, a.w, a.K, a.N, a.ldw, 0, BM, a.half) && encode(&low, a.low, a.R, a.N, a.R, a.S, BM, a.half);
@@ -1050,13 +1062,13 @@ cudaError_t run_few(const AdapterJoint& a, cudaStream_t stream) {
   p.y = static_cast<uint16_t*>(a.y);
   p.T = a.T, p.N = a.N, p.R = a.R, p.rows = rows;
   p.nk = (a.K + BK - 1) / BK;
-  const int tiles = (a.N + BM - 1) / BM;
-  // 72 to 128 KB; where tiles outnumber the SMs, little enough for two blocks to an SM.  (128 rows, 4 stages: 14.7 us with
+  const int tiles = (a.T + BM - 1) / BM * ((a.N + BM - 1) / BM);
+  // 69 to 128 KB; where tiles outnumber the SMs, little enough for two blocks to an SM.  (128 rows, 4 stages: 14.7 us with
   // 2 blocks a cluster and one to an SM, 18 with 3 stages and more of them; 152 tiles: 27 us with 3 stages, 42 with 4.)
   p.stages = tiles > sm_count() ? std::min(4, 110 * 1024 / (kXBytes + rows * 128)) : 4;
   p.idesc = sm100::umma_idesc_bf16(BM, BM, false, MN) & ~(a.half ? sm100::kIdescBf16 : 0u);
   p.half = a.half;
-  const int smem = std::max(p.stages * (kXBytes + rows * 128), a.T * (BM + 4) * 4) + 256 + 1024;
+  const int smem = std::max(p.stages * (kXBytes + rows * 128), std::min(BM, a.T) * (BM + 4) * 4) + 256 + 1024;
   static std::atomic<unsigned long long> done{0};
   const cudaError_t e = allow_smem(adapter_few_kernel<MN>, kMaxSmem, done);
   if (e != cudaSuccess) return e;
@@ -1071,13 +1083,13 @@ struct Cut {
 };
 
 // A last round of `rest` tiles takes a whole tile's time of nk blocks of K; cut into slices nk / slices, the slices' sums
-// (256 KB each, through L2) and another launch, together about 16 blocks' time.
+// (256 KB each, through L2) and another launch, together about 10 us or 28 blocks' time.
 Cut cut_tiles(int T, int K, int N) {
   const int tiles = (T + 255) / 256 * ((N + 255) / 256), nk = (K + BK - 1) / BK, pairs = std::max(1, sm_count() / 2);
   Cut c{pairs, tiles, 1, tiles};
   const int rest = tiles % pairs;
   const int slices = rest ? std::min({8, pairs / rest, nk / 4}) : 1;
-  if (slices >= 2 && nk - nk / slices > 16) {
+  if (slices >= 2 && nk - nk / slices > 28) {
     c.whole = tiles - rest;
     c.slices = slices;
     c.units = c.whole + rest * slices;
@@ -1123,12 +1135,12 @@ cudaError_t launch_adapter_shrink(const AdapterShrink& a, cudaStream_t stream) {
 cudaError_t launch_adapter_joint(const AdapterJoint& a, cudaStream_t stream) {
   const cudaError_t e = have_context();
   if (e != cudaSuccess) return e;
-  if (a.T <= kFewRows) return a.mn ? run_few<true>(a, stream) : run_few<false>(a, stream);
+  if (few_rows(a.T, a.K, a.N)) return a.mn ? run_few<true>(a, stream) : run_few<false>(a, stream);
   return a.mn ? run_joint<true>(a, stream) : run_joint<false>(a, stream);
 }
 
 size_t adapter_joint_workspace(int T, int K, int N) {
-  if (T <= kFewRows) return 0;
+  if (few_rows(T, K, N)) return 0;
   const Cut c = cut_tiles(T, K, N);
   return (size_t)(c.units - c.whole) * kPairTile * sizeof(float);
 }
@@ -1154,7 +1166,7 @@ cudaError_t launch_adapter_grads(const AdapterGrads& a, cudaStream_t stream) {
   p.add_a = a.add_a, p.add_b = a.add_b, p.half = a.half;
   int smem = std::max(kGradStages * (kXBytes + p.cols * 128), 2 * BM * (p.cols + 4) * 4) + 256 + 1024;
   // Blocks that hold all of an SM's TMEM have the SM for themselves: of two clusters that wait for each other's, each in
-  // another SM, neither would end.  (All other blocks here take 72 KB of shared memory or more, and at most 256 columns.)
+  // another SM, neither would end.  (All other blocks here take 69 KB of shared memory or more, and at most 256 columns.)
   if (p.cols > 64) smem = std::max(smem, 160 * 1024);
   static std::atomic<unsigned long long> done{0};
   e = allow_smem(adapter_grads_kernel, kMaxSmem, done);
