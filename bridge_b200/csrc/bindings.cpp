@@ -144,8 +144,9 @@ torch::Tensor adapter_linear(torch::Tensor x, torch::Tensor w, torch::Tensor a, 
                              c10::optional<torch::Tensor> a_main, c10::optional<torch::Tensor> b_main,
                              c10::optional<torch::Tensor> w_main);
 int64_t adapter_error_code();
-torch::Tensor clip_grad_norm(std::vector<torch::Tensor> grads, bool per_slot, double grad_scale, double max_norm,
-                             c10::optional<torch::Tensor> max_norms, c10::optional<std::vector<torch::Tensor>> out);
+torch::Tensor clip_grad_norm(const std::vector<torch::Tensor>& grads, bool per_slot, double grad_scale, bool clip,
+                             double max_norm, c10::optional<torch::Tensor> max_norms,
+                             const std::vector<torch::Tensor>& out);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "bridge_b200 sm_100a kernels";

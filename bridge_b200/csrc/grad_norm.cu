@@ -5,6 +5,9 @@
 //            factor min(1, max_norm / (norm + eps)) / grad_scale
 //   scale    one block per chunk: out = factor x, rounded once
 //
+// Lists of at most 1 MB are one launch: a cluster of eight blocks whose warps sum their chunks, meet in shared memory and
+// scale them.
+//
 // What bounds it: reading every value once for the norm, and once more, above the L2's 126 MB, to scale it.  The second
 // pass goes through the chunks backwards, so that what the first one read last is still there.  A list's pointers travel
 // in the kernels' parameters: no table is uploaded, and a captured graph keeps its own.
@@ -13,6 +16,7 @@
 // squares, and zeros) are taken again value by value in 64 bits, so that no finite gradient overflows or disappears.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 #include <torch/extension.h>
 
@@ -24,6 +28,7 @@
 
 namespace {
 
+namespace cg = cooperative_groups;
 using OptTensor = c10::optional<torch::Tensor>;
 constexpr int kThreads = 256;
 constexpr int kUnroll = 4;      // 16-byte loads in flight per thread
@@ -96,8 +101,9 @@ __device__ __forceinline__ long lead(const T* p, long n) {
   return k < n ? k : n;
 }
 
-template <typename T>
-__device__ double chunk_sum(const T* x, long n) {
+// A chunk's sum of squares, of thread `tid` of NT.
+template <int NT, typename T>
+__device__ double chunk_sum(const T* x, long n, int tid) {
   constexpr int V = 16 / sizeof(T);
   const long head = lead(x, n), vecs = (n - head) / V;
   const Vec<T>* body = reinterpret_cast<const Vec<T>*>(x + head);
@@ -114,17 +120,17 @@ __device__ double chunk_sum(const T* x, long n) {
       for (int i = 0; i < V; ++i) one(Io<T>::get(a.v[i]));
     }
   };
-  long i = threadIdx.x;
-  for (; i + (kUnroll - 1) * kThreads < vecs; i += kUnroll * kThreads) {
+  long i = tid;
+  for (; i + (kUnroll - 1) * NT < vecs; i += kUnroll * NT) {
     Vec<T> a[kUnroll];
 #pragma unroll
-    for (int k = 0; k < kUnroll; ++k) a[k] = body[i + k * kThreads];
+    for (int k = 0; k < kUnroll; ++k) a[k] = body[i + k * NT];
 #pragma unroll
     for (int k = 0; k < kUnroll; ++k) add(a[k]);
   }
-  for (; i < vecs; i += kThreads) add(body[i]);
-  if (threadIdx.x < head) one(Io<T>::get(x[threadIdx.x]));
-  const long tail = head + vecs * V + threadIdx.x;
+  for (; i < vecs; i += NT) add(body[i]);
+  if (tid < head) one(Io<T>::get(x[tid]));
+  const long tail = head + vecs * V + tid;
   if (tail < n) one(Io<T>::get(x[tail]));
   return sum;
 }
@@ -139,37 +145,8 @@ __device__ __forceinline__ double block_sum_f64(double v, double* scratch) {
   return s;
 }
 
-template <int N>
-__global__ void __launch_bounds__(kThreads) sums_kernel(const __grid_constant__ Table<N> t, double* parts) {
-  __shared__ double scratch[kThreads / 32];
-  const Chunk c = locate(t, blockIdx.x);
-  const Entry& e = t.e[c.entry];
-  double s;
-  if (e.kind == kF32) s = chunk_sum(static_cast<const float*>(e.in) + c.begin, c.n);
-  else if (e.kind == kBF16) s = chunk_sum(static_cast<const __nv_bfloat16*>(e.in) + c.begin, c.n);
-  else s = chunk_sum(static_cast<const __half*>(e.in) + c.begin, c.n);
-  s = block_sum_f64(s, scratch);
-  if (threadIdx.x == 0) parts[(long)c.slot * t.per_slot + c.part] = s;
-}
-
-__global__ void __launch_bounds__(1024) finish_kernel(const double* parts, int per_slot, double grad_scale,
-                                                      double max_norm, const float* max_norms, float* norm,
-                                                      float* factor) {
-  __shared__ double scratch[32];
-  double s = 0.0;
-  for (int i = threadIdx.x; i < per_slot; i += 1024) s += parts[(long)blockIdx.x * per_slot + i];
-  s = block_sum_f64(s, scratch);
-  if (threadIdx.x) return;
-  const double n = sqrt(s) / grad_scale;
-  norm[blockIdx.x] = (float)n;
-  if (!factor) return;
-  const double bound = max_norms ? (double)max_norms[blockIdx.x] : max_norm;
-  // (a NaN norm makes the factor NaN)
-  factor[blockIdx.x] = (float)((n + 1e-6 <= bound ? 1.0 : bound / (n + 1e-6)) / grad_scale);
-}
-
-template <typename T, typename O>
-__device__ void chunk_scale(const T* x, O* y, long n, float f) {
+template <int NT, typename T, typename O>
+__device__ void chunk_scale(const T* x, O* y, long n, float f, int tid) {
   constexpr int V = 16 / sizeof(T);
   const long head = lead(x, n), vecs = (n - head) / V;
   const Vec<T>* body = reinterpret_cast<const Vec<T>*>(x + head);
@@ -188,36 +165,119 @@ __device__ void chunk_scale(const T* x, O* y, long n, float f) {
       for (int k = 0; k < V; ++k) to[i * V + k] = r[k];
     }
   };
-  long i = threadIdx.x;
-  for (; i + (kUnroll - 1) * kThreads < vecs; i += kUnroll * kThreads) {
+  long i = tid;
+  for (; i + (kUnroll - 1) * NT < vecs; i += kUnroll * NT) {
     Vec<T> a[kUnroll];
 #pragma unroll
-    for (int k = 0; k < kUnroll; ++k) a[k] = body[i + k * kThreads];
+    for (int k = 0; k < kUnroll; ++k) a[k] = body[i + k * NT];
 #pragma unroll
-    for (int k = 0; k < kUnroll; ++k) put(a[k], i + k * kThreads);
+    for (int k = 0; k < kUnroll; ++k) put(a[k], i + k * NT);
   }
-  for (; i < vecs; i += kThreads) put(body[i], i);
-  if (threadIdx.x < head) y[threadIdx.x] = Io<O>::put(f * Io<T>::get(x[threadIdx.x]));
-  const long tail = head + vecs * V + threadIdx.x;
+  for (; i < vecs; i += NT) put(body[i], i);
+  if (tid < head) y[tid] = Io<O>::put(f * Io<T>::get(x[tid]));
+  const long tail = head + vecs * V + tid;
   if (tail < n) y[tail] = Io<O>::put(f * Io<T>::get(x[tail]));
+}
+
+template <int NT>
+__device__ double sum_of(const Entry& e, const Chunk& c, int tid) {
+  if (e.kind == kF32) return chunk_sum<NT>(static_cast<const float*>(e.in) + c.begin, c.n, tid);
+  if (e.kind == kBF16) return chunk_sum<NT>(static_cast<const __nv_bfloat16*>(e.in) + c.begin, c.n, tid);
+  return chunk_sum<NT>(static_cast<const __half*>(e.in) + c.begin, c.n, tid);
+}
+
+template <int NT>
+__device__ void scale_of(const Entry& e, const Chunk& c, float f, int tid) {
+  if (f == 1.f && e.in == e.out) return;
+  if (e.kind == kF32) {
+    chunk_scale<NT>(static_cast<const float*>(e.in) + c.begin, static_cast<float*>(e.out) + c.begin, c.n, f, tid);
+  } else if (e.kind == kBF16) {
+    const auto* x = static_cast<const __nv_bfloat16*>(e.in) + c.begin;
+    if (e.out_kind == kF32) chunk_scale<NT>(x, static_cast<float*>(e.out) + c.begin, c.n, f, tid);
+    else chunk_scale<NT>(x, static_cast<__nv_bfloat16*>(e.out) + c.begin, c.n, f, tid);
+  } else {
+    const auto* x = static_cast<const __half*>(e.in) + c.begin;
+    if (e.out_kind == kF32) chunk_scale<NT>(x, static_cast<float*>(e.out) + c.begin, c.n, f, tid);
+    else chunk_scale<NT>(x, static_cast<__half*>(e.out) + c.begin, c.n, f, tid);
+  }
+}
+
+struct Bound {
+  double grad_scale, max_norm;
+  const float* max_norms;    // per slot, or null
+  float* norm;
+  bool scale;
+};
+
+__device__ __forceinline__ float finish(const Bound& b, int slot, double sum, bool write) {
+  const double n = sqrt(sum) / b.grad_scale;
+  if (write) b.norm[slot] = (float)n;
+  const double most = b.max_norms ? (double)b.max_norms[slot] : b.max_norm;
+  // (a NaN norm makes the factor NaN)
+  return (float)((n + 1e-6 <= most ? 1.0 : most / (n + 1e-6)) / b.grad_scale);
+}
+
+template <int N>
+__global__ void __launch_bounds__(kThreads) sums_kernel(const __grid_constant__ Table<N> t, double* parts) {
+  __shared__ double scratch[kThreads / 32];
+  const Chunk c = locate(t, blockIdx.x);
+  const double s = block_sum_f64(sum_of<kThreads>(t.e[c.entry], c, threadIdx.x), scratch);
+  if (threadIdx.x == 0) parts[(long)c.slot * t.per_slot + c.part] = s;
+}
+
+__global__ void __launch_bounds__(1024) finish_kernel(const double* parts, int per_slot, const Bound b, float* factor) {
+  __shared__ double scratch[32];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < per_slot; i += 1024) s += parts[(long)blockIdx.x * per_slot + i];
+  s = block_sum_f64(s, scratch);
+  if (threadIdx.x) return;
+  const float f = finish(b, blockIdx.x, s, true);
+  if (b.scale) factor[blockIdx.x] = f;
 }
 
 template <int N>
 __global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ Table<N> t, const float* factor) {
   const Chunk c = locate(t, t.total - 1 - blockIdx.x);
-  const Entry& e = t.e[c.entry];
-  const float f = factor[c.slot];
-  if (f == 1.f && e.in == e.out) return;
-  if (e.kind == kF32) {
-    chunk_scale(static_cast<const float*>(e.in) + c.begin, static_cast<float*>(e.out) + c.begin, c.n, f);
-  } else if (e.kind == kBF16) {
-    const auto* x = static_cast<const __nv_bfloat16*>(e.in) + c.begin;
-    if (e.out_kind == kF32) chunk_scale(x, static_cast<float*>(e.out) + c.begin, c.n, f);
-    else chunk_scale(x, static_cast<__nv_bfloat16*>(e.out) + c.begin, c.n, f);
-  } else {
-    const auto* x = static_cast<const __half*>(e.in) + c.begin;
-    if (e.out_kind == kF32) chunk_scale(x, static_cast<float*>(e.out) + c.begin, c.n, f);
-    else chunk_scale(x, static_cast<__half*>(e.out) + c.begin, c.n, f);
+  scale_of<kThreads>(t.e[c.entry], c, factor[c.slot], threadIdx.x);
+}
+
+// A short list: every warp of the cluster takes every 128th chunk; sums go warp by warp, in the blocks' and warps' order.
+constexpr int kSmallBlocks = 8, kSmallWarps = 16, kSmallSlots = 32;
+
+template <int N>
+__global__ void __cluster_dims__(kSmallBlocks, 1, 1) __launch_bounds__(32 * kSmallWarps)
+    small_kernel(const __grid_constant__ Table<N> t, const Bound b) {
+  __shared__ double sums[kSmallWarps][kSmallSlots];
+  __shared__ float factor[kSmallSlots];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int first = blockIdx.x * kSmallWarps + warp, step = kSmallBlocks * kSmallWarps;
+  if (lane < t.slots) sums[warp][lane] = 0.0;
+  __syncwarp();
+  for (int id = first; id < t.total; id += step) {
+    const Chunk c = locate(t, id);
+    double s = sum_of<32>(t.e[c.entry], c, lane);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0) sums[warp][c.slot] += s;
+  }
+  cluster.sync();
+  for (int slot = warp; slot < t.slots; slot += kSmallWarps) {
+    double s = 0.0;       // four of the 128 warps' sums a lane
+#pragma unroll
+    for (int k = 0; k < kSmallBlocks * kSmallWarps / 32; ++k) {
+      const int i = lane * (kSmallBlocks * kSmallWarps / 32) + k;
+      s += *cluster.map_shared_rank(&sums[i % kSmallWarps][slot], i / kSmallWarps);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0) factor[slot] = finish(b, slot, s, blockIdx.x == 0);
+  }
+  cluster.sync();         // (the peers' sums stay until all have read them)
+  if (!b.scale) return;
+  for (int id = first; id < t.total; id += step) {
+    const Chunk c = locate(t, id);
+    scale_of<32>(t.e[c.entry], c, factor[c.slot], lane);
   }
 }
 
@@ -233,26 +293,22 @@ short kind_of(const torch::Tensor& t) {
 
 struct Span {
   uintptr_t lo, hi;
-  int i;
   bool out;
 };
 
 // Every value is scaled once, from a gradient that nothing else writes.
-void check_apart(const std::vector<Entry>& e, int slots, const std::vector<torch::Tensor>& grads,
-                 const std::vector<torch::Tensor>& out) {
+void check_apart(const std::vector<Entry>& e, int slots) {
+  constexpr int kWidth[3] = {4, 2, 2};
   std::vector<Span> s;
-  bool rising = true;
-  for (size_t i = 0; i < grads.size(); ++i) {
-    const auto lo = reinterpret_cast<uintptr_t>(grads[i].data_ptr()), to = reinterpret_cast<uintptr_t>(out[i].data_ptr());
-    const size_t bytes = grads[i].numel() * grads[i].element_size(), out_bytes = out[i].numel() * out[i].element_size();
-    if (!bytes) continue;
-    const bool same = lo == to && bytes == out_bytes;
-    if (!s.empty() && s.back().hi > to) rising = false;
-    s.push_back({to, to + out_bytes, (int)i, true});
-    if (!same) {
-      rising = false;
-      s.push_back({lo, lo + bytes, (int)i, false});
-    }
+  s.reserve(2 * e.size());
+  bool rising = true;      // the outputs in the order of their addresses, and no other gradients: the usual list
+  for (size_t i = 0; i < e.size(); ++i) {
+    const auto lo = reinterpret_cast<uintptr_t>(e[i].in), to = reinterpret_cast<uintptr_t>(e[i].out);
+    const size_t n = e[i].n * (size_t)slots;
+    const bool same = lo == to && kWidth[e[i].kind] == kWidth[e[i].out_kind];
+    if (!same || (!s.empty() && s.back().hi > to)) rising = false;
+    s.push_back({to, to + n * kWidth[e[i].out_kind], true});
+    if (!same) s.push_back({lo, lo + n * kWidth[e[i].kind], false});
   }
   if (rising) return;
   std::sort(s.begin(), s.end(), [](const Span& a, const Span& b) { return a.lo < b.lo; });
@@ -279,6 +335,14 @@ void fill(Table<N>& t, const std::vector<Entry>& all, size_t from, int slots, in
 }
 
 template <int N>
+void run_small(const std::vector<Entry>& all, int slots, int per_slot, long chunk, const Bound& bound, cudaStream_t stream) {
+  Table<N> t;
+  fill(t, all, 0, slots, per_slot, chunk);
+  small_kernel<N><<<kSmallBlocks, 32 * kSmallWarps, 0, stream>>>(t, bound);
+  BB_POST_LAUNCH();
+}
+
+template <int N>
 void run(const std::vector<Entry>& all, int slots, int per_slot, long chunk, double* parts, const float* factor,
          cudaStream_t stream) {
   // (the scaling takes the lists backwards too)
@@ -294,44 +358,49 @@ void run(const std::vector<Entry>& all, int slots, int per_slot, long chunk, dou
 
 }  // namespace
 
-// Norms [slots] ([] without `per_slot`) of the gradients over `grad_scale`; with `out` (the gradients themselves, or
-// tensors like them), out = gradient * min(1, max_norm / (norm + 1e-6)) / grad_scale.
-torch::Tensor clip_grad_norm(std::vector<torch::Tensor> grads, bool per_slot, double grad_scale, double max_norm,
-                             OptTensor max_norms, c10::optional<std::vector<torch::Tensor>> out) {
+// Norms [slots] ([] without `per_slot`) of the gradients over `grad_scale`; with `clip`,
+// out (or the gradients themselves) = gradient * min(1, max_norm / (norm + 1e-6)) / grad_scale.
+torch::Tensor clip_grad_norm(const std::vector<torch::Tensor>& grads, bool per_slot, double grad_scale, bool clip,
+                             double max_norm, OptTensor max_norms, const std::vector<torch::Tensor>& out) {
   TORCH_CHECK_VALUE(!grads.empty(), "clip_grad_norm: no gradients");
   const auto device = grads[0].device();
   TORCH_CHECK(device.is_cuda(), "clip_grad_norm: CUDA tensors");
   const int64_t slots = per_slot ? (grads[0].dim() ? grads[0].size(0) : 0) : 1;
   TORCH_CHECK_VALUE(!per_slot || (slots >= 1 && slots < (1 << 16)), "clip_grad_norm: per_slot needs gradients stacked by slot");
-  TORCH_CHECK_VALUE(!out.has_value() || out->size() == grads.size(), "clip_grad_norm: one output per gradient");
+  const bool in_place = out.empty();
+  TORCH_CHECK_VALUE(in_place || out.size() == grads.size(), "clip_grad_norm: one output per gradient");
+  const bool watched = at::GradMode::is_enabled();
   const c10::cuda::CUDAGuard guard(device);
-  // chunks of 64 KB of FP32; of 8 KB where all together are too few for the SMs
-  int64_t total = 0;
-  for (const auto& g : grads) total += g.numel();
-  const long chunk = total > (1 << 24) ? 16384 : 2048;
+  int64_t total = 0, bytes = 0;
+  for (const auto& g : grads) total += g.numel(), bytes += g.numel() * g.element_size();
+  const bool small = bytes <= (1 << 20) && slots <= kSmallSlots && grads.size() <= kMany;
+  // chunks of 64 KB of FP32; of 8 KB where all together are too few for the SMs; of a warp's 4 KB
+  const long chunk = small ? 1024 : total > (1 << 24) ? 16384 : 2048;
   std::vector<Entry> all;
   all.reserve(grads.size());
   int64_t per = 0, blocks = 0;
   for (size_t i = 0; i < grads.size(); ++i) {
     const auto& g = grads[i];
+    const auto& o = in_place ? g : out[i];
     TORCH_CHECK_TYPE(g.device() == device, "clip_grad_norm: gradients are on ", device, " and ", g.device());
+    TORCH_CHECK(!watched || !(g.requires_grad() || (clip && o.requires_grad())),
+                "clip_grad_norm: norms and clipped gradients are not differentiable; detach the tensors");
     Entry e{};
     e.kind = kind_of(g);
-    const bool dense = per_slot ? g.is_contiguous() : g.is_non_overlapping_and_dense();
+    const bool dense = per_slot ? g.is_contiguous() : (g.is_contiguous() || g.is_non_overlapping_and_dense());
     TORCH_CHECK_VALUE(dense, "clip_grad_norm: a gradient has to be dense (and contiguous where norms go by slot)");
     TORCH_CHECK_VALUE(!per_slot || (g.dim() && g.size(0) == slots), "clip_grad_norm: gradients are stacks of ",
                       std::to_string(slots), " slots, got one of ", g.dim() ? std::to_string(g.size(0)) : "none");
-    if (out.has_value()) {
-      const auto& o = (*out)[i];
+    if (clip && !in_place) {
       TORCH_CHECK_TYPE(o.device() == device && (o.scalar_type() == g.scalar_type() || o.scalar_type() == at::kFloat),
                        "clip_grad_norm: an output is float32 or its gradient's type, on its device");
       TORCH_CHECK_VALUE(o.sizes() == g.sizes() && (o.strides() == g.strides() || (o.is_contiguous() && g.is_contiguous())),
                         "clip_grad_norm: an output has its gradient's sizes and strides");
-      e.out = o.data_ptr();
-      e.out_kind = kind_of(o);
     }
     if (g.numel() == 0) continue;
     e.in = g.data_ptr();
+    e.out = o.data_ptr();
+    e.out_kind = in_place ? e.kind : kind_of(o);
     e.n = g.numel() / slots;
     e.chunks = (int)((e.n + chunk - 1) / chunk);
     e.at = (int)per;
@@ -340,30 +409,34 @@ torch::Tensor clip_grad_norm(std::vector<torch::Tensor> grads, bool per_slot, do
     all.push_back(e);
   }
   TORCH_CHECK_VALUE(blocks < (1ll << 31), "clip_grad_norm: too many values");
-  if (out.has_value()) check_apart(all, (int)slots, grads, *out);
+  if (clip) check_apart(all, (int)slots);
   TORCH_CHECK_VALUE(!max_norms.has_value() ||
                         (max_norms->device() == device && max_norms->scalar_type() == at::kFloat &&
                          max_norms->is_contiguous() && max_norms->numel() == slots),
                     "clip_grad_norm: max_norm is a number or float32, one per slot, on the gradients' device");
   const auto f32 = at::TensorOptions().device(device).dtype(at::kFloat);
   auto norm = per_slot ? at::empty({slots}, f32) : at::empty({}, f32);
-  auto parts = at::empty({slots * per + slots}, f32.dtype(at::kDouble));     // sums, then factors
-  double* sums = parts.data_ptr<double>();
-  float* factor = reinterpret_cast<float*>(sums + slots * per);
   const auto stream = at::cuda::getCurrentCUDAStream();
   const bool few = all.size() <= kFew;
-  if (!all.empty()) {
+  const Bound bound{grad_scale, max_norm, max_norms.has_value() ? max_norms->data_ptr<float>() : nullptr,
+                    norm.data_ptr<float>(), clip};
+  if (small) {
+    if (few) run_small<kFew>(all, (int)slots, (int)per, chunk, bound, stream);
+    else run_small<kMany>(all, (int)slots, (int)per, chunk, bound, stream);
+  } else {
+    auto parts = at::empty({slots * per + slots}, f32.dtype(at::kDouble));     // sums, then factors
+    double* sums = parts.data_ptr<double>();
+    float* factor = reinterpret_cast<float*>(sums + slots * per);
     if (few) run<kFew>(all, (int)slots, (int)per, chunk, sums, nullptr, stream);
     else run<kMany>(all, (int)slots, (int)per, chunk, sums, nullptr, stream);
+    finish_kernel<<<(int)slots, 1024, 0, stream>>>(sums, (int)per, bound, factor);
+    BB_POST_LAUNCH();
+    if (clip) {
+      if (few) run<kFew>(all, (int)slots, (int)per, chunk, nullptr, factor, stream);
+      else run<kMany>(all, (int)slots, (int)per, chunk, nullptr, factor, stream);
+    }
   }
-  finish_kernel<<<(int)slots, 1024, 0, stream>>>(sums, (int)per, grad_scale, max_norm,
-                                                 max_norms.has_value() ? max_norms->data_ptr<float>() : nullptr,
-                                                 norm.data_ptr<float>(), out.has_value() ? factor : nullptr);
-  BB_POST_LAUNCH();
-  if (out.has_value() && !all.empty()) {
-    if (few) run<kFew>(all, (int)slots, (int)per, chunk, nullptr, factor, stream);
-    else run<kMany>(all, (int)slots, (int)per, chunk, nullptr, factor, stream);
-    for (const auto& o : *out) o.unsafeGetTensorImpl()->bump_version();
-  }
+  if (clip)
+    for (const auto& o : in_place ? grads : out) o.unsafeGetTensorImpl()->bump_version();
   return norm;
 }

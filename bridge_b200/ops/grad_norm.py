@@ -23,15 +23,18 @@ from torch import Tensor
 from ._ext import kernels, on_gpu
 
 
-def _check(grads, per_slot: bool, grad_scale: float) -> list[Tensor]:
+def _check(grads, grad_scale: float) -> list[Tensor]:
     grads = list(grads)
     if not grads or any(not isinstance(g, Tensor) for g in grads):
         raise ValueError("clip_grad_norm: needs a list of gradient tensors, without None")
     if not (grad_scale > 0 and math.isfinite(grad_scale)):
         raise ValueError(f"clip_grad_norm: grad_scale must be positive and finite, got {grad_scale}")
-    if torch.is_grad_enabled() and any(g.requires_grad for g in grads):
-        raise RuntimeError("clip_grad_norm: norms and clipped gradients are not differentiable; detach the gradients")
     return grads
+
+
+def _detached(tensors) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError("clip_grad_norm: norms and clipped gradients are not differentiable; detach the tensors")
 
 
 def _groups(g: Tensor, per_slot: bool, slots: int) -> Tensor:
@@ -54,8 +57,6 @@ def clip_grad_norm_reference(grads: list[Tensor], max_norm, per_slot: bool, grad
     if out is not None:
         bound = max_norm.double().reshape(-1) if isinstance(max_norm, Tensor) else torch.full_like(norm, max_norm)
         factor = (torch.where(norm + 1e-6 <= bound, torch.ones_like(norm), bound / (norm + 1e-6)) / grad_scale).float()
-        if len(out) != len(grads):
-            raise ValueError("clip_grad_norm: one output per gradient")
         for g, o in zip(grads, out):
             wide = torch.promote_types(g.dtype, torch.float32)
             o.copy_((_groups(g, per_slot, slots).to(wide) * factor[:, None].to(wide)).view(g.shape))
@@ -64,9 +65,10 @@ def clip_grad_norm_reference(grads: list[Tensor], max_norm, per_slot: bool, grad
 
 def global_grad_norm(grads: Sequence[Tensor], *, per_slot: bool = False, grad_scale: float = 1.0) -> Tensor:
     """2-norm over all tensors, FP32 ``[]``; with ``per_slot`` ``[S]``, each slot's own.  No host synchronisation."""
-    grads = _check(grads, per_slot, grad_scale)
+    grads = _check(grads, grad_scale)
     if on_gpu(grads[0]):
-        return kernels().clip_grad_norm(grads, per_slot, grad_scale, 0.0, None, None)
+        return kernels().clip_grad_norm(grads, per_slot, grad_scale, False, 0.0, None, [])
+    _detached(grads)
     with torch.no_grad():
         return clip_grad_norm_reference(grads, 0.0, per_slot, grad_scale, None)
 
@@ -77,15 +79,18 @@ def clip_grad_norm(grads: Sequence[Tensor], max_norm: Tensor | float, *, per_slo
 
     The gradients (dense FP32, BF16 or FP16 tensors of any mix, on one device) are overwritten, or left and written to
     ``out``, tensors like them that may be FP32.  ``max_norm`` is a number, or FP32 ``[S]`` with ``per_slot``."""
-    grads = _check(grads, per_slot, grad_scale)
-    out = grads if out is None else list(out)
+    grads = _check(grads, grad_scale)
+    if out is not None and len(out) != len(grads):
+        raise ValueError(f"clip_grad_norm: one output per gradient, got {len(out)} for {len(grads)}")
+    out = [] if out is None else list(out)
+    if any(not isinstance(o, Tensor) for o in out):
+        raise ValueError("clip_grad_norm: outputs are tensors")
     bounds = isinstance(max_norm, Tensor)
     if not bounds and not max_norm >= 0:
         raise ValueError(f"clip_grad_norm: max_norm must not be negative, got {max_norm}")
-    if torch.is_grad_enabled() and any(isinstance(o, Tensor) and o.requires_grad for o in out):
-        raise RuntimeError("clip_grad_norm: norms and clipped gradients are not differentiable; detach the outputs")
     if on_gpu(grads[0]):
-        return kernels().clip_grad_norm(grads, per_slot, grad_scale, 0.0 if bounds else max_norm,
+        return kernels().clip_grad_norm(grads, per_slot, grad_scale, True, 0.0 if bounds else max_norm,
                                         max_norm if bounds else None, out)
+    _detached(grads + out)
     with torch.no_grad():
-        return clip_grad_norm_reference(grads, max_norm, per_slot, grad_scale, out)
+        return clip_grad_norm_reference(grads, max_norm, per_slot, grad_scale, out or grads)

@@ -56,9 +56,11 @@ SHAPES = [(1,), (7,), (33, 5), (2048,), (2049,), (3, 1111), (256, 129), (0,), (6
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("bound", [1e-2, 5.0, math.inf])
-def test_types_and_sizes(dtype, bound):
+@pytest.mark.parametrize("more", [[], [(700, 1001)], [(3000, 2003), (5, 1 << 20), (7,)]])
+def test_types_and_sizes(dtype, bound, more):
+    """Lists below and above 1 MB, and beyond 2^24 values."""
     for out_type in (None, dtype, torch.float32):
-        _check(_grads(SHAPES, dtype), bound, out_type=out_type, grad_scale=1.0 if out_type is None else 64.0)
+        _check(_grads(SHAPES + more, dtype), bound, out_type=out_type, grad_scale=1.0 if out_type is None else 64.0)
 
 
 def test_mixed_types_in_one_list():
@@ -67,17 +69,17 @@ def test_mixed_types_in_one_list():
     _check(grads, 3.0)
 
 
-@pytest.mark.parametrize("slots", [1, 3, 17])
+@pytest.mark.parametrize("slots,more", [(1, 0), (3, 0), (17, 0), (32, 0), (33, 0), (5, 130001), (200, 3001)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_by_slot(slots, dtype):
+def test_by_slot(slots, more, dtype):
     """Odd sizes, so that the slots begin at any alignment; one slot is clipped, one is not, one is zero."""
-    grads = _grads([(slots, 3, 5), (slots, 8191), (slots, 1), (slots, 129, 65)], dtype)
+    grads = _grads([(slots, 3, 5), (slots, 2191), (slots, 1), (slots, 29, 65), (slots, more)], dtype)
     for g in grads:
         g[0] *= 0.01
         g[-1] = 0 if slots > 1 else g[-1]
     got = _check(grads, 20.0, per_slot=True)
-    if slots > 1:
-        assert got[-1] == 0 and got[0] < 20.0
+    if slots > 2:
+        assert got[-1] == 0 and got[0] < 20.0 < got[1]
     _check(grads, torch.linspace(0.5, 40.0, slots, device=DEV), per_slot=True, grad_scale=8.0, out_type=torch.float32)
 
 
