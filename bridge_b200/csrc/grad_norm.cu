@@ -151,15 +151,20 @@ __device__ void chunk_scale(const T* x, O* y, long n, float f, int tid) {
   const long head = lead(x, n), vecs = (n - head) / V;
   const Vec<T>* body = reinterpret_cast<const Vec<T>*>(x + head);
   O* to = y + head;
-  const bool wide = reinterpret_cast<uintptr_t>(to) % 16 == 0;
+  const bool wide = reinterpret_cast<uintptr_t>(to) % (V * sizeof(O)) == 0;
   const auto put = [&](const Vec<T>& a, long i) {
-    alignas(16) O r[V];
+    alignas(32) O r[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) r[k] = Io<O>::put(f * Io<T>::get(a.v[k]));
     if (wide) {
-#pragma unroll
-      for (int k = 0; k < (int)(V * sizeof(O) / 16); ++k)
-        reinterpret_cast<uint4*>(to + i * V)[k] = reinterpret_cast<const uint4*>(r)[k];
+      // (16-bit gradients into FP32: 32 bytes in one store, or every sector would be written in halves)
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(r);
+      if constexpr (V * sizeof(O) == 32)
+        asm volatile("st.global.cs.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to + i * V), "r"(w[0]), "r"(w[1]),
+                     "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                     : "memory");
+      else
+        __stcs(reinterpret_cast<uint4*>(to + i * V), *reinterpret_cast<const uint4*>(r));
     } else {
 #pragma unroll
       for (int k = 0; k < V; ++k) to[i * V + k] = r[k];
