@@ -86,14 +86,23 @@ __device__ __forceinline__ void spill(uint32_t tmem, float* part, int cols, bool
   }
 }
 
-// The sum over the cluster's partial accumulators of four columns, in rank order.
-__device__ __forceinline__ float4 joined(uint32_t part, int at, int ranks) {
-  float4 s = ld_cluster4(sm100::mapa(part + at * 4, 0));
-  for (int j = 1; j < ranks; ++j) {
-    const float4 v = ld_cluster4(sm100::mapa(part + at * 4, j));
-    s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
-  }
-  return s;
+// The sums over the cluster's partial accumulators of eight columns, in rank order; all loads are under way together.
+__device__ __forceinline__ void joined8(uint32_t part, int at, int ranks, float (&v)[8]) {
+  float4 a[8], b[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < ranks) {
+      const uint32_t from = sm100::mapa(part + at * 4, j);
+      a[j] = ld_cluster4(from);
+      b[j] = ld_cluster4(from + 16);
+    }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < ranks) {
+      const float q[8] = {a[j].x, a[j].y, a[j].z, a[j].w, b[j].x, b[j].y, b[j].z, b[j].w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = j ? v[i] + q[i] : q[i];
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ shrink
@@ -194,10 +203,11 @@ __global__ void __launch_bounds__(kThreads)
   for (int i = threadIdx.x; i < rows * groups; i += kThreads) {
     const int r = lo + i / groups, c = (i % groups) * 8;
     if (__ldg(unit + 4 + r / 32) >> (r % 32) & 1) continue;      // another request's row
-    const float4 v = joined(base, r * (p.cols + 4) + c, p.ranks), w = joined(base, r * (p.cols + 4) + c + 4, p.ranks);
+    float v[8];
+    joined8(base, r * (p.cols + 4) + c, p.ranks, v);
     *reinterpret_cast<uint4*>(p.u + (size_t)(tile * BM + r) * p.R + c) =
-        make_uint4(pack2(f * v.x, f * v.y, p.half), pack2(f * v.z, f * v.w, p.half),
-                   pack2(f * w.x, f * w.y, p.half), pack2(f * w.z, f * w.w, p.half));
+        make_uint4(pack2(f * v[0], f * v[1], p.half), pack2(f * v[2], f * v[3], p.half),
+                   pack2(f * v[4], f * v[5], p.half), pack2(f * v[6], f * v[7], p.half));
   }
   sm100::cluster_sync();   // the peers' sums stay until all have read them
   if (warp == 1) {
@@ -351,9 +361,10 @@ __global__ void __launch_bounds__(kThreads)
   for (int i = threadIdx.x; i < groups * rows; i += kThreads) {
     const int c = (lo + i % groups) * 8, t = i / groups;
     if (n0 + c >= p.N) continue;
-    const float4 v = joined(base, t * kRow + c, p.ranks), w = joined(base, t * kRow + c + 4, p.ranks);
+    float v[8];
+    joined8(base, t * kRow + c, p.ranks, v);
     *reinterpret_cast<uint4*>(p.y + (size_t)(m0 + t) * p.N + n0 + c) =
-        make_uint4(pack2(v.x, v.y, p.half), pack2(v.z, v.w, p.half), pack2(w.x, w.y, p.half), pack2(w.z, w.w, p.half));
+        make_uint4(pack2(v[0], v[1], p.half), pack2(v[2], v[3], p.half), pack2(v[4], v[5], p.half), pack2(v[6], v[7], p.half));
   }
   sm100::cluster_sync();   // the peers' sums stay until all have read them
   if (warp == 1) {
