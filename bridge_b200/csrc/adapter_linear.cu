@@ -142,8 +142,14 @@ __global__ void __launch_bounds__(kThreads)
     }
     sm100::mbar_init(done, 1);
     sm100::fence_mbar_init();
+    sm100::prefetch_tmap(&map_x);
+    sm100::prefetch_tmap(&map_op);
   }
   if (warp == 1) sm100::tmem_alloc(tmem_word, 128);
+  if (warp == 0 && lane < kb1 - kb0) {     // weights into L2 while the kernel before this one ends
+    if (OP_MN) sm100::tma_prefetch_3d(&map_op, 0, (kb0 + lane) * BK, slot);
+    else sm100::tma_prefetch_3d(&map_op, (kb0 + lane) * BK, 0, slot);
+  }
   sm100::tc_fence_before();
   __syncthreads();
   sm100::tc_fence_after();
@@ -199,7 +205,7 @@ __global__ void __launch_bounds__(kThreads)
   // this block's share of the rows: 8 columns a step, the finished values 16 bytes at a time
   const int lo = BM * rank / p.ranks, rows = BM * (rank + 1) / p.ranks - lo, groups = p.R / 8;
   const uint32_t base = sm100::smem_addr(part);
-  const float f = p.scales ? __ldg(p.scales + slot) : p.scale;
+  const float f = p.scales ? p.scales[slot] : p.scale;
   for (int i = threadIdx.x; i < rows * groups; i += kThreads) {
     const int r = lo + i / groups, c = (i % groups) * 8;
     if (__ldg(unit + 4 + r / 32) >> (r % 32) & 1) continue;      // another request's row
@@ -241,12 +247,16 @@ __global__ void __launch_bounds__(kThreads)
   uint64_t* empty = full + p.stages;
   uint64_t* done = empty + p.stages;
   uint32_t* tmem_word = reinterpret_cast<uint32_t*>(done + 1);
+  int4* my_mask = reinterpret_cast<int4*>(full + 32);      // this block's share of the tile's units (256 bytes on)
+  int* my_slot = reinterpret_cast<int*>(my_mask + BM);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tile = blockIdx.x / p.ranks, m_tiles = (p.T + BM - 1) / BM;    // neighbours share columns of W
   const int rank = (int)sm100::cluster_ctarank(), mt = tile % m_tiles, m0 = mt * BM, n0 = tile / m_tiles * BM;
   const int rows = min(BM, p.T - m0);
   const int kb0 = (int)((long)p.nk * rank / p.ranks), kb1 = (int)((long)p.nk * (rank + 1) / p.ranks);
   const int rank_blocks = (p.R + BK - 1) / BK;
+  const int unit0 = __ldg(p.plan.unit_start + mt) + rank;
+  const int units = max(0, (__ldg(p.plan.unit_start + mt + 1) - unit0 + p.ranks - 1) / p.ranks);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
@@ -255,8 +265,15 @@ __global__ void __launch_bounds__(kThreads)
     }
     sm100::mbar_init(done, 1);
     sm100::fence_mbar_init();
+    sm100::prefetch_tmap(&map_x);
+    sm100::prefetch_tmap(&map_w);
   }
   if (warp == 1) sm100::tmem_alloc(tmem_word, 128);
+  if (warp >= 2 && (int)threadIdx.x - 64 < units) {        // (one at a time in the loops below, each would be a wait)
+    const int4* unit = reinterpret_cast<const int4*>(p.plan.units) + 2 * (size_t)(unit0 + (threadIdx.x - 64) * p.ranks);
+    my_slot[threadIdx.x - 64] = __ldg(unit).y;
+    my_mask[threadIdx.x - 64] = __ldg(unit + 1);
+  }
   sm100::tc_fence_before();
   __syncthreads();
   sm100::tc_fence_after();
@@ -291,20 +308,16 @@ __global__ void __launch_bounds__(kThreads)
     }
     wait_for_previous();       // u, which TMA reads from here on
     asm volatile("fence.proxy.async.global;" ::: "memory");
-    for (int i = 0, mine = 0; i < p.plan.num_units; ++i) {
-      const int2 unit = __ldg(reinterpret_cast<const int2*>(p.plan.units + (size_t)i * 8));
-      if (unit.x != mt || mine++ % p.ranks != rank) continue;
-      const int slot = unit.y;
+    for (int i = 0; i < units; ++i)
       for (int rb = 0; rb < rank_blocks && claim(); ++rb) {
-        sm100::tma_load_2d(x_dst, &map_u, bar, rb * BK, m0);
         if (MN) {
-          sm100::tma_load_3d(w_dst, &map_low, bar, n0, rb * BK, slot);
-          sm100::tma_load_3d(w_dst + 8192, &map_low, bar, n0 + 64, rb * BK, slot);
+          sm100::tma_load_3d(w_dst, &map_low, bar, n0, rb * BK, my_slot[i]);
+          sm100::tma_load_3d(w_dst + 8192, &map_low, bar, n0 + 64, rb * BK, my_slot[i]);
         } else {
-          sm100::tma_load_3d(w_dst, &map_low, bar, rb * BK, n0, slot);
+          sm100::tma_load_3d(w_dst, &map_low, bar, rb * BK, n0, my_slot[i]);
         }
+        sm100::tma_load_2d(x_dst, &map_u, bar, rb * BK, m0);
       }
-    }
   } else if (warp == 1 && lane == 0) {
     int stage = 0;
     uint32_t phase = 0;
@@ -324,9 +337,8 @@ __global__ void __launch_bounds__(kThreads)
     };
     const uint32_t all[4] = {0, 0, 0, 0};
     for (int kb = kb0; kb < kb1; ++kb) products(BK / 16, kb == kb0, all);
-    for (int i = 0, mine = 0; i < p.plan.num_units; ++i) {
-      if (__ldg(p.plan.units + (size_t)i * 8) != mt || mine++ % p.ranks != rank) continue;
-      const int4 m = __ldg(reinterpret_cast<const int4*>(p.plan.units + (size_t)i * 8) + 1);
+    for (int i = 0; i < units; ++i) {
+      const int4 m = my_mask[i];
       const uint32_t off[4] = {(uint32_t)m.x, (uint32_t)m.y, (uint32_t)m.z, (uint32_t)m.w};
       for (int rb = 0; rb < rank_blocks; ++rb) products(min(BK / 16, (p.R - rb * BK + 15) / 16), false, off);
     }
@@ -370,6 +382,215 @@ __global__ void __launch_bounds__(kThreads)
   if (warp == 1) {
     sm100::tc_fence_after();
     sm100::tmem_dealloc(tmem, 128);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ tokens
+struct TokenParams {
+  AdapterPlan plan;
+  uint16_t *y, *u;
+  const uint16_t* low;
+  const float* scales;
+  float scale;
+  int T, N, R, rows, slot_cols, stages, nk, ranks, columns;   // slot_cols: of a slot in the accumulator; columns: of TMEM
+  uint32_t idesc;
+  bool half;
+};
+
+__device__ __forceinline__ float2 unpack2(uint32_t v, bool half) {
+  if (half) return __half22float2(*reinterpret_cast<const __half2*>(&v));
+  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+}
+__device__ __forceinline__ float unpack1(uint16_t v, bool half) {
+  return half ? __half2float(__ushort_as_half(v)) : __bfloat162float(__ushort_as_bfloat16(v));
+}
+__device__ __forceinline__ float ld_cluster1(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
+// A few rows of few slots, in one kernel: every cluster (128 columns of y, each of its blocks a stretch of K) makes
+// u for itself as it goes, from the slots' rows of A beside W's: more reading from L2, but no second kernel to start, to
+// end and to wait for.  The accumulator holds y's 128 columns and the products with every slot's A, of which a row takes
+// its own slot's.  Where the partial sums meet, each block adds up u, rounds it as the other kernels do, and makes its
+// share of the columns: a few FP32 products a value.  The first cluster keeps u if it is asked for.
+template <bool MN>
+__global__ void __launch_bounds__(kThreads)
+    adapter_token_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                         const __grid_constant__ CUtensorMap map_op, const TokenParams p) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int slots = p.plan.num_units, u_cols = slots * p.slot_cols;
+  const int x_bytes = p.rows * 128, stage_bytes = x_bytes + kXBytes + u_cols * 128;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + p.stages * stage_bytes);
+  uint64_t* empty = full + p.stages;
+  uint64_t* done = empty + p.stages;
+  uint32_t* tmem_word = reinterpret_cast<uint32_t*>(done + 1);
+  int* slot_of = reinterpret_cast<int*>(done + 2);       // of the units, at most 16
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)sm100::cluster_ctarank(), n0 = blockIdx.x / p.ranks * BM;
+  const int kb0 = (int)((long)p.nk * rank / p.ranks), kb1 = (int)((long)p.nk * (rank + 1) / p.ranks);
+  const int lo = BM * rank / p.ranks, cols = BM * (rank + 1) / p.ranks - lo;      // this block's columns
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      sm100::mbar_init(&full[s], 1);
+      sm100::mbar_init(&empty[s], 1);
+    }
+    sm100::mbar_init(done, 1);
+    sm100::fence_mbar_init();
+    sm100::prefetch_tmap(&map_x);
+    sm100::prefetch_tmap(&map_w);
+    sm100::prefetch_tmap(&map_op);
+  }
+  if (warp == 1) sm100::tmem_alloc(tmem_word, p.columns);
+  if (warp == 0 && lane < slots) slot_of[lane] = __ldg(p.plan.units + (size_t)lane * 8 + 1);
+  // weights into L2 while the kernel before this one ends (whatever it still writes there, L2 has)
+  if (warp == 0 && lane < kb1 - kb0) {
+    if (MN) {
+      sm100::tma_prefetch_2d(&map_w, n0, (kb0 + lane) * BK);
+      sm100::tma_prefetch_2d(&map_w, n0 + 64, (kb0 + lane) * BK);
+    } else {
+      sm100::tma_prefetch_2d(&map_w, (kb0 + lane) * BK, n0);
+    }
+  } else if (warp >= 2) {
+    const int lines = MN ? p.R * ((cols * 2 + 127) / 128) : (cols * p.R * 2 + 127) / 128;
+    for (int i = threadIdx.x - 64; i < lines * slots; i += kThreads - 64) {
+      const int slot = __ldg(p.plan.units + (size_t)(i / lines) * 8 + 1), l = i % lines;
+      const size_t at = MN ? ((size_t)slot * p.R + l % p.R) * p.N + n0 + lo + l / p.R * 64
+                           : ((size_t)slot * p.N + n0 + lo) * p.R + l * 64;
+      if (n0 + lo < p.N && at < (size_t)(slot + 1) * p.N * p.R) prefetch_l2(p.low + at);
+    }
+  }
+  sm100::tc_fence_before();
+  __syncthreads();
+  sm100::tc_fence_after();
+  const uint32_t tmem = *tmem_word;
+  let_next_begin();
+  wait_for_previous();
+
+  if (warp == 0 && lane == 0) {
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!sm100::mbar_wait(&empty[stage], phase ^ 1, &g_error, 71)) break;
+      unsigned char *x_dst = smem + stage * stage_bytes, *w_dst = x_dst + x_bytes, *op_dst = w_dst + kXBytes;
+      uint64_t* bar = &full[stage];
+      sm100::mbar_expect_tx(bar, stage_bytes);
+      if (MN) {
+        sm100::tma_load_2d(w_dst, &map_w, bar, n0, kb * BK);
+        sm100::tma_load_2d(w_dst + 8192, &map_w, bar, n0 + 64, kb * BK);
+      } else {
+        sm100::tma_load_2d(w_dst, &map_w, bar, kb * BK, n0);
+      }
+      sm100::tma_load_2d(x_dst, &map_x, bar, kb * BK, 0);
+      for (int i = 0; i < slots; ++i) {
+        const int slot = slot_of[i];
+        if (MN) {
+          for (int j = 0; j < p.slot_cols / 64; ++j)
+            sm100::tma_load_3d(op_dst + (i * (p.slot_cols / 64) + j) * 8192, &map_op, bar, 64 * j, kb * BK, slot);
+        } else {
+          sm100::tma_load_3d(op_dst + i * p.slot_cols * 128, &map_op, bar, kb * BK, 0, slot);
+        }
+      }
+      if (++stage == p.stages) stage = 0, phase ^= 1;
+    }
+  } else if (warp == 1 && lane == 0) {
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!sm100::mbar_wait(&full[stage], phase, &g_error, 72)) break;
+      sm100::tc_fence_after();
+      // the slots' rows of A lie behind W's: one instruction makes both
+      const uint32_t a = sm100::smem_addr(smem + stage * stage_bytes), b = a + x_bytes;
+#pragma unroll
+      for (int kk = 0; kk < BK / 16; ++kk)
+        sm100::umma_bf16(tmem, sm100::umma_desc_sw128(a + kk * 32, 16, 1024),
+                         MN ? sm100::umma_desc_sw128(b + kk * 2048, 8192, 1024)
+                            : sm100::umma_desc_sw128(b + kk * 32, 16, 1024), p.idesc, kb > kb0 || kk > 0);
+      sm100::umma_commit(&empty[stage]);
+      if (++stage == p.stages) stage = 0, phase ^= 1;
+    }
+    sm100::umma_commit(done);
+  }
+  __syncwarp();
+  const int row_floats = BM + u_cols + 4;       // rows 16 bytes apart in the banks
+  float* part = reinterpret_cast<float*>(smem);
+  if (warp >= 2) {
+    const int quarter = warp & 3, row = quarter * 32 + lane;
+    sm100::mbar_wait(done, 0, &g_error, 73);
+    __syncwarp();
+    sm100::tc_fence_after();
+    if (quarter * 32 < p.T)
+      for (int c = 0; c < BM + u_cols; c += 16) {
+        uint32_t r[16];
+        sm100::tmem_ld16(tmem + ((uint32_t)(quarter * 32) << 16) + c, r);
+        sm100::tmem_ld_wait();
+        sm100::tmem_regs_ready(r);
+        if (row < p.T)
+#pragma unroll
+          for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<uint4*>(part + row * row_floats + c + i) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
+      }
+    sm100::tc_fence_before();
+  }
+  __syncthreads();
+  sm100::cluster_sync();
+  const uint32_t base = sm100::smem_addr(part);
+  // u of every row, from its slot's columns
+  uint16_t* u = reinterpret_cast<uint16_t*>(part + p.T * row_floats);
+  for (int i = threadIdx.x; i < p.T * (p.R / 8); i += kThreads) {
+    const int t = i / (p.R / 8), c = i % (p.R / 8) * 8, slot = __ldg(p.plan.row_slot + t);
+    if (slot < 0) continue;
+    int at = 0;
+    while (slot_of[at] != slot) ++at;
+    float v[8];
+    joined8(base, t * row_floats + BM + at * p.slot_cols + c, p.ranks, v);
+    const float f = p.scales ? p.scales[slot] : p.scale;
+    const uint4 out = make_uint4(pack2(f * v[0], f * v[1], p.half), pack2(f * v[2], f * v[3], p.half),
+                                 pack2(f * v[4], f * v[5], p.half), pack2(f * v[6], f * v[7], p.half));
+    *reinterpret_cast<uint4*>(u + t * p.R + c) = out;
+    if (p.u && blockIdx.x == 0) *reinterpret_cast<uint4*>(p.u + (size_t)t * p.R + c) = out;
+  }
+  __syncthreads();
+  // this block's columns of y
+  for (int i = threadIdx.x; i < cols * p.T; i += kThreads) {
+    const int c = lo + i % cols, t = i / cols, n = n0 + c;
+    if (n >= p.N) continue;
+    float q[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < p.ranks) q[j] = ld_cluster1(sm100::mapa(base + (t * row_floats + c) * 4, j));
+    float v = q[0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j)
+      if (j < p.ranks) v += q[j];
+    const int slot = __ldg(p.plan.row_slot + t);
+    if (slot >= 0) {
+      for (int k = 0; k < p.R; k += 8) {
+        const uint4 a = *reinterpret_cast<const uint4*>(u + t * p.R + k);
+        const float2 a0 = unpack2(a.x, p.half), a1 = unpack2(a.y, p.half), a2 = unpack2(a.z, p.half), a3 = unpack2(a.w, p.half);
+        if (MN) {
+          const uint16_t* b = p.low + ((size_t)slot * p.R + k) * p.N + n;
+          const float w[8] = {a0.x, a0.y, a1.x, a1.y, a2.x, a2.y, a3.x, a3.y};
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v = fmaf(w[j], unpack1(b[(size_t)j * p.N], p.half), v);
+        } else {
+          const uint4 b = *reinterpret_cast<const uint4*>(p.low + ((size_t)slot * p.N + n) * p.R + k);
+          const float2 b0 = unpack2(b.x, p.half), b1 = unpack2(b.y, p.half), b2 = unpack2(b.z, p.half), b3 = unpack2(b.w, p.half);
+          v = fmaf(a0.x, b0.x, v), v = fmaf(a0.y, b0.y, v), v = fmaf(a1.x, b1.x, v), v = fmaf(a1.y, b1.y, v);
+          v = fmaf(a2.x, b2.x, v), v = fmaf(a2.y, b2.y, v), v = fmaf(a3.x, b3.x, v), v = fmaf(a3.y, b3.y, v);
+        }
+      }
+    }
+    p.y[(size_t)t * p.N + n] = pack1(v, p.half);
+  }
+  sm100::cluster_sync();   // the peers' sums stay until all have read them
+  if (warp == 1) {
+    sm100::tc_fence_after();
+    sm100::tmem_dealloc(tmem, p.columns);
   }
 }
 
@@ -480,6 +701,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       for (int q = pair; q < p.units && ok; q += pairs) {
         const Piece w = piece_at(p, q);
         const int m0 = w.mt * 256 + 128 * rank, n0 = w.nt * 256 + 128 * rank;
+        const int first = __ldg(p.plan.tile_start + w.mt), end = __ldg(p.plan.tile_start + w.mt + 1);
+        int next_slot = first < end ? __ldg(p.plan.pairs + (size_t)first * kPairInts) : 0;
         for (int kb = w.kb0; kb < w.kb1; ++kb) {
           if (!claim()) break;
           sm100::tma_load_2d_pair(x_dst, &map_x, bar, kb * BK, m0);
@@ -495,9 +718,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           asm volatile("fence.proxy.async.global;" ::: "memory");
         }
         if (!w.last) continue;
-        const int end = __ldg(p.plan.tile_start + w.mt + 1);
-        for (int i = __ldg(p.plan.tile_start + w.mt); i < end && ok; ++i) {
-          const int slot = __ldg(p.plan.pairs + (size_t)i * kPairInts);
+        for (int i = first; i < end && ok; ++i) {
+          const int slot = next_slot;        // (asked for a pair ahead: the answer takes longer than the pair's products)
+          if (i + 1 < end) next_slot = __ldg(p.plan.pairs + (size_t)(i + 1) * kPairInts);
           for (int rb = 0; rb < rank_blocks; ++rb) {
             if (!claim()) break;
             sm100::tma_load_2d_pair(x_dst, &map_u, bar, rb * BK, m0);
@@ -521,6 +744,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         sm100::tc_fence_after();
         const uint32_t d = tmem + acc * 256;
         const Piece w = piece_at(p, q);
+        const int4* masks = reinterpret_cast<const int4*>(p.plan.pairs);
+        const int first = __ldg(p.plan.tile_start + w.mt), end = __ldg(p.plan.tile_start + w.mt + 1);
+        int4 next_lo = {}, next_hi = {};
+        if (first < end) next_lo = __ldg(masks + 3 * (size_t)first + 1), next_hi = __ldg(masks + 3 * (size_t)first + 2);
         for (int kb = w.kb0; kb < w.kb1; ++kb) {
           ok = sm100::mbar_wait_cluster(&full[stage], phase, &g_error, 43);
           if (!ok) break;
@@ -536,10 +763,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           if (++stage == kPairStages) stage = 0, phase ^= 1;
         }
         if (w.last) {
-          const int end = __ldg(p.plan.tile_start + w.mt + 1);
-          for (int i = __ldg(p.plan.tile_start + w.mt); i < end && ok; ++i) {
-            const int4* m = reinterpret_cast<const int4*>(p.plan.pairs + (size_t)i * kPairInts);
-            const int4 lo = __ldg(m + 1), hi = __ldg(m + 2);
+          for (int i = first; i < end && ok; ++i) {
+            const int4 lo = next_lo, hi = next_hi;
+            if (i + 1 < end) next_lo = __ldg(masks + 3 * (size_t)i + 4), next_hi = __ldg(masks + 3 * (size_t)i + 5);
             const uint32_t off[8] = {(uint32_t)lo.x, (uint32_t)lo.y, (uint32_t)lo.z, (uint32_t)lo.w,
                                      (uint32_t)hi.x, (uint32_t)hi.y, (uint32_t)hi.z, (uint32_t)hi.w};
             for (int rb = 0; rb < rank_blocks; ++rb) {
@@ -756,6 +982,8 @@ __global__ void __launch_bounds__(kThreads)
       sm100::mbar_init(&tempty[i], 128);
     }
     sm100::fence_mbar_init();
+    sm100::prefetch_tmap(map_wide);
+    sm100::prefetch_tmap(map_thin);
   }
   if (warp == 1) sm100::tmem_alloc(tmem_word, tmem_cols);
   sm100::tc_fence_before();
@@ -1027,7 +1255,7 @@ int split(void (*kernel)(P...), int smem, int columns, int clusters, int nk) {
 
 
 template <bool OP_MN>
-cudaError_t run_shrink(const AdapterShrink& a, cudaStream_t stream) {
+cudaError_t run_shrink(const AdapterProduct& a, cudaStream_t stream) {
   alignas(64) CUtensorMap x, op;
   const int cols = OP_MN ? (a.R + 63) / 64 * 64 : (a.R + 15) / 16 * 16;
   if (!encode(&x, a.x, a.K, a.T, a.ldx, 0, BM, a.half)) return cudaErrorInvalidValue;
@@ -1061,7 +1289,7 @@ bool few_rows(int T, int K, int N) {
 }
 
 template <bool MN>
-cudaError_t run_few(const AdapterJoint& a, cudaStream_t stream) {
+cudaError_t run_few(const AdapterProduct& a, cudaStream_t stream) {
   alignas(64) CUtensorMap x, w, u, low;
   const int rows = std::min(BM, (a.T + 7) / 8 * 8);
   bool ok = encode(&x, a.x, a.K, a.T, a.ldx, 0, rows, a.half) && encode(&u, a.u, a.R, a.T, a.R, 0, rows, a.half);
@@ -1079,13 +1307,52 @@ cudaError_t run_few(const AdapterJoint& a, cudaStream_t stream) {
   p.stages = tiles > sm_count() ? std::min(4, 110 * 1024 / (kXBytes + rows * 128)) : 4;
   p.idesc = sm100::umma_idesc_bf16(BM, BM, false, MN) & ~(a.half ? sm100::kIdescBf16 : 0u);
   p.half = a.half;
-  const int smem = std::max(p.stages * (kXBytes + rows * 128), std::min(BM, a.T) * (BM + 4) * 4) + 256 + 1024;
+  const int smem = std::max(p.stages * (kXBytes + rows * 128), std::min(BM, a.T) * (BM + 4) * 4) + 256 + BM * 20 + 1024;
   static std::atomic<unsigned long long> done{0};
   const cudaError_t e = allow_smem(adapter_few_kernel<MN>, kMaxSmem, done);
   if (e != cudaSuccess) return e;
   p.ranks = split(adapter_few_kernel<MN>, smem, 128, tiles, p.nk);
   return launch(adapter_few_kernel<MN>, tiles * p.ranks, kThreads, smem, p.ranks, stream, x, w, u,
                 low, p);
+}
+
+// Columns of the accumulator that a batch's slots take beside y's 128 in the one-kernel form, or 0 where it does not apply.
+// Its low-rank part goes by rows x rank, its reading by the slots: 2560 -> 6144, one and two kernels: 1 row of rank 16
+// 10.8 and 11.9 us, 16 rows 12.5 and 13.4, 32 rows 14.5 and 14.2 (and a launch less), 16 rows of rank 64 19 and 15; 4 slots
+// 11.8 and 13.2, 8 slots 20 and 15.
+int token_columns(const AdapterProduct& a) {
+  const int each = a.mn ? (a.R + 63) / 64 * 64 : (a.R + 15) / 16 * 16, all = a.plan.num_units * each;
+  return a.T * a.R <= 512 && all <= 64 ? all : 0;
+}
+
+template <bool MN>
+cudaError_t run_token(const AdapterProduct& a, int u_cols, cudaStream_t stream) {
+  alignas(64) CUtensorMap x, w, op;
+  const int rows = (a.T + 7) / 8 * 8, each = u_cols / a.plan.num_units;
+  bool ok = encode(&x, a.x, a.K, a.T, a.ldx, 0, rows, a.half);
+  if (MN) ok = ok && encode(&w, a.w, a.N, a.K, a.ldw, 0, 64, a.half) && encode(&op, a.op, a.R, a.K, a.R, a.S, 64, a.half);
+  else ok = ok && encode(&w, a.w, a.K, a.N, a.ldw, 0, BM, a.half) && encode(&op, a.op, a.K, a.R, a.K, a.S, each, a.half);
+  if (!ok) return cudaErrorInvalidValue;
+  TokenParams p{};
+  p.plan = a.plan;
+  p.y = static_cast<uint16_t*>(a.y), p.u = a.keep_u ? static_cast<uint16_t*>(a.u) : nullptr;
+  p.low = static_cast<const uint16_t*>(a.low);
+  p.scales = a.scales, p.scale = a.scale;
+  p.T = a.T, p.N = a.N, p.R = a.R, p.rows = rows, p.slot_cols = each;
+  p.nk = (a.K + BK - 1) / BK;
+  p.columns = 256;
+  const int stage = rows * 128 + kXBytes + u_cols * 128, tiles = (a.N + BM - 1) / BM;
+  p.stages = std::min(4, 220 * 1024 / stage);
+  p.idesc = sm100::umma_idesc_bf16(BM, BM + u_cols, false, MN) & ~(a.half ? sm100::kIdescBf16 : 0u);
+  p.half = a.half;
+  int smem = std::max(p.stages * stage, a.T * (BM + u_cols + 4) * 4 + a.T * a.R * 2) + 256 + 1024;
+  // (three blocks of 256 columns must not meet on an SM: see the gradients)
+  smem = std::max(smem, 80 * 1024);
+  static std::atomic<unsigned long long> done{0};
+  const cudaError_t e = allow_smem(adapter_token_kernel<MN>, kMaxSmem, done);
+  if (e != cudaSuccess) return e;
+  p.ranks = split(adapter_token_kernel<MN>, smem, p.columns, tiles, p.nk);
+  return launch(adapter_token_kernel<MN>, tiles * p.ranks, kThreads, smem, p.ranks, stream, x, w, op, p);
 }
 
 // How the tiles of 256 x 256 go to the pairs of SMs.
@@ -1110,7 +1377,7 @@ Cut cut_tiles(int T, int K, int N) {
 }
 
 template <bool MN>
-cudaError_t run_joint(const AdapterJoint& a, cudaStream_t stream) {
+cudaError_t run_joint(const AdapterProduct& a, cudaStream_t stream) {
   alignas(64) CUtensorMap x, w, u, low, y;
   bool ok = encode(&x, a.x, a.K, a.T, a.ldx, 0, BM, a.half) && encode(&u, a.u, a.R, a.T, a.R, 0, BM, a.half) &&
             encode(&y, a.y, a.N, a.T, a.N, 0, 32, a.half);
@@ -1137,23 +1404,29 @@ cudaError_t run_joint(const AdapterJoint& a, cudaStream_t stream) {
 
 }  // namespace
 
-cudaError_t launch_adapter_shrink(const AdapterShrink& a, cudaStream_t stream) {
+cudaError_t launch_adapter_shrink(const AdapterProduct& a, cudaStream_t stream) {
   const cudaError_t e = have_context();
   if (e != cudaSuccess || a.plan.num_units == 0) return e;
-  return a.op_mn ? run_shrink<true>(a, stream) : run_shrink<false>(a, stream);
+  return a.mn ? run_shrink<true>(a, stream) : run_shrink<false>(a, stream);
 }
 
-cudaError_t launch_adapter_joint(const AdapterJoint& a, cudaStream_t stream) {
-  const cudaError_t e = have_context();
+AdapterNeeds adapter_product_needs(const AdapterProduct& a) {
+  if (a.plan.num_units && token_columns(a)) return {a.keep_u, 0};
+  if (few_rows(a.T, a.K, a.N)) return {true, 0};
+  const Cut c = cut_tiles(a.T, a.K, a.N);
+  return {true, (size_t)(c.units - c.whole) * kPairTile * sizeof(float)};
+}
+
+cudaError_t launch_adapter_product(const AdapterProduct& a, cudaStream_t stream) {
+  cudaError_t e = have_context();
+  if (e != cudaSuccess) return e;
+  if (a.plan.num_units)
+    if (const int columns = token_columns(a))
+      return a.mn ? run_token<true>(a, columns, stream) : run_token<false>(a, columns, stream);
+  e = launch_adapter_shrink(a, stream);
   if (e != cudaSuccess) return e;
   if (few_rows(a.T, a.K, a.N)) return a.mn ? run_few<true>(a, stream) : run_few<false>(a, stream);
   return a.mn ? run_joint<true>(a, stream) : run_joint<false>(a, stream);
-}
-
-size_t adapter_joint_workspace(int T, int K, int N) {
-  if (few_rows(T, K, N)) return 0;
-  const Cut c = cut_tiles(T, K, N);
-  return (size_t)(c.units - c.whole) * kPairTile * sizeof(float);
 }
 
 cudaError_t launch_adapter_grads(const AdapterGrads& a, cudaStream_t stream) {
@@ -1177,7 +1450,8 @@ cudaError_t launch_adapter_grads(const AdapterGrads& a, cudaStream_t stream) {
   p.add_a = a.add_a, p.add_b = a.add_b, p.half = a.half;
   int smem = std::max(kGradStages * (kXBytes + p.cols * 128), 2 * BM * (p.cols + 4) * 4) + 256 + 1024;
   // Blocks that hold all of an SM's TMEM have the SM for themselves: of two clusters that wait for each other's, each in
-  // another SM, neither would end.  (All other blocks here take 69 KB of shared memory or more, and at most 256 columns.)
+  // another SM, neither would end.  (All other blocks here take 69 KB of shared memory
+  // or more, 80 with 256 columns: what room there is for blocks is room for their columns.)
   if (p.cols > 64) smem = std::max(smem, 160 * 1024);
   static std::atomic<unsigned long long> done{0};
   e = allow_smem(adapter_grads_kernel, kMaxSmem, done);

@@ -28,7 +28,7 @@ torch::Tensor as_rows(const torch::Tensor& t) {
 
 bb::AdapterPlan plan_of(const torch::Tensor& buf, const Meta& meta) {
   const int* p = buf.data_ptr<int>();
-  return {p + meta[4], p + meta[5], p + meta[6], p + meta[7], p + meta[8], p + meta[9],
+  return {p + meta[4], p + meta[5], p + meta[6], p + meta[7], p + meta[8], p + meta[9], p + meta[10],
           (int)meta[2], (int)meta[3], (int)meta[1]};
 }
 
@@ -40,40 +40,45 @@ struct Sizes {
         half(a.scalar_type() == at::kHalf) {}
 };
 
-// u = scale A x, or du = scale B^T dy with `mn` (op [S, K, R] then)
-torch::Tensor shrink(const torch::Tensor& x, const torch::Tensor& op, bool mn, const torch::Tensor& buf,
-                     const Meta& meta, double scale, const OptTensor& scales) {
-  bb::AdapterShrink s{};
-  s.op_mn = mn;
-  s.S = (int)op.size(0), s.R = (int)op.size(mn ? 2 : 1), s.K = (int)op.size(mn ? 1 : 2), s.T = (int)x.size(0);
-  s.half = op.scalar_type() == at::kHalf;
-  auto u = at::empty({s.T, s.R}, op.options().requires_grad(false));
-  s.x = x.data_ptr(), s.op = op.data_ptr(), s.u = u.data_ptr();
-  s.ldx = row_stride(x);
-  s.scale = (float)scale;
-  s.scales = scales.has_value() ? scales->data_ptr<float>() : nullptr;
-  s.plan = plan_of(buf, meta);
-  check(bb::launch_adapter_shrink(s, at::cuda::getCurrentCUDAStream()));
-  return u;
-}
+struct Products {
+  torch::Tensor u, y;      // undefined where not asked for
+};
 
-torch::Tensor joint(const torch::Tensor& x, const torch::Tensor& w, const torch::Tensor& u, const torch::Tensor& low,
-                    bool mn, const torch::Tensor& buf, const Meta& meta) {
-  bb::AdapterJoint j{};
-  j.mn = mn;
-  j.T = (int)x.size(0), j.K = (int)x.size(1), j.N = (int)w.size(mn ? 1 : 0), j.S = (int)low.size(0), j.R = (int)u.size(1);
-  j.half = low.scalar_type() == at::kHalf;
-  auto y = at::empty({j.T, j.N}, low.options().requires_grad(false));
-  j.x = x.data_ptr(), j.w = w.data_ptr(), j.u = u.data_ptr(), j.low = low.data_ptr(), j.y = y.data_ptr();
-  j.ldx = row_stride(x), j.ldw = row_stride(w);
-  torch::Tensor sums;      // the call's own: two of them may run at once
-  if (const size_t bytes = bb::adapter_joint_workspace(j.T, j.K, j.N)) {
-    sums = at::empty({(int64_t)bytes}, low.options().dtype(at::kByte).requires_grad(false));
-    j.workspace = sums.data_ptr();
+// u = scale A x and y = W x + B u from (x, W, A, B); du = scale B^T dy and dx = W^T dy + A^T du from (dy, W, B, A) with `mn`.
+Products products(const torch::Tensor& x, const torch::Tensor& w, const torch::Tensor& op, const torch::Tensor& low, bool mn,
+                  bool want_u, bool want_y, const torch::Tensor& buf, const Meta& meta, double scale,
+                  const OptTensor& scales) {
+  bb::AdapterProduct a{};
+  a.mn = mn, a.keep_u = want_u;
+  a.T = (int)x.size(0), a.K = (int)x.size(1), a.N = (int)w.size(mn ? 1 : 0);
+  a.S = (int)op.size(0), a.R = (int)op.size(mn ? 2 : 1);
+  a.half = op.scalar_type() == at::kHalf;
+  a.x = x.data_ptr(), a.op = op.data_ptr(), a.w = w.data_ptr(), a.low = low.data_ptr();
+  a.ldx = row_stride(x), a.ldw = row_stride(w);
+  a.scale = (float)scale;
+  a.scales = scales.has_value() ? scales->data_ptr<float>() : nullptr;
+  a.plan = plan_of(buf, meta);
+  const auto opts = op.options().requires_grad(false);
+  const auto stream = at::cuda::getCurrentCUDAStream();
+  const bb::AdapterNeeds needs = want_y ? bb::adapter_product_needs(a) : bb::AdapterNeeds{true, 0};
+  Products out;
+  if (needs.u) {
+    out.u = at::empty({a.T, a.R}, opts);
+    a.u = out.u.data_ptr();
   }
-  j.plan = plan_of(buf, meta);
-  check(bb::launch_adapter_joint(j, at::cuda::getCurrentCUDAStream()));
-  return y;
+  if (!want_y) {
+    check(bb::launch_adapter_shrink(a, stream));
+    return out;
+  }
+  out.y = at::empty({a.T, a.N}, opts);
+  a.y = out.y.data_ptr();
+  torch::Tensor sums;      // the call's own: two of them may run at once
+  if (needs.workspace) {
+    sums = at::empty({(int64_t)needs.workspace}, opts.dtype(at::kByte));
+    a.workspace = sums.data_ptr();
+  }
+  check(bb::launch_adapter_product(a, stream));
+  return out;
 }
 
 void first_order() {
@@ -90,8 +95,8 @@ class AdapterLinear : public torch::autograd::Function<AdapterLinear> {
     const c10::cuda::CUDAGuard guard(x.device());
     torch::Tensor u, y;
     if (x.size(0)) {
-      u = shrink(x, a, false, buf, meta, scale, scales);
-      y = joint(x, w, u, b, false, buf, meta);
+      const Products out = products(x, w, a, b, false, true, true, buf, meta, scale, scales);
+      u = out.u, y = out.y;
     } else {
       u = at::empty({0, a.size(1)}, a.options().requires_grad(false));
       y = at::empty({0, w.size(0)}, a.options().requires_grad(false));
@@ -133,8 +138,10 @@ class AdapterLinear : public torch::autograd::Function<AdapterLinear> {
     }
     const auto dy = as_rows(grads[0]);
     torch::Tensor du;
-    if (want_x || want_a) du = shrink(dy, b, true, buf, meta, scale, scales);
-    if (want_x) dx = joint(dy, w, du, a, true, buf, meta);
+    if (want_x || want_a) {
+      const Products out = products(dy, w, b, a, true, want_a, want_x, buf, meta, scale, scales);
+      du = out.u, dx = out.y;
+    }
     if (want_w) {
       const auto rows = [](const torch::Tensor& t) { return t.as_strided(t.sizes(), {row_stride(t), 1}); };
       if (w_main.has_value()) gemm(rows(dy), rows(x), true, true, w_main, true);
@@ -185,7 +192,7 @@ torch::Tensor adapter_linear(torch::Tensor x, torch::Tensor w, torch::Tensor a, 
       w.size(0) >= 8 && a.size(1) >= 8 && x.size(1) % 8 == 0 && w.size(0) % 8 == 0 && a.size(1) % 8 == 0 &&
       a.size(1) <= bb::kMaxAdapterRank && x.size(0) < (1l << 30) && x.size(1) < (1l << 30) && w.size(0) < (1l << 30) &&
       a.size(0) < (1l << 16) && plain_rows(x) && plain_rows(w) && a.is_contiguous() && aligned(a) &&
-      b.is_contiguous() && aligned(b) && meta.size() == 10 && meta[0] == x.size(0) && meta[1] <= a.size(0) &&
+      b.is_contiguous() && aligned(b) && meta.size() == 11 && meta[0] == x.size(0) && meta[1] <= a.size(0) &&
       buf.device() == x.device() && buf.scalar_type() == at::kInt && buf.is_contiguous() &&
       (!scales.has_value() || (scales->dim() == 1 && scales->size(0) == a.size(0) && scales->is_contiguous() &&
                                scales->scalar_type() == at::kFloat && scales->device() == x.device() &&
@@ -198,7 +205,7 @@ torch::Tensor adapter_linear(torch::Tensor x, torch::Tensor w, torch::Tensor a, 
     return AdapterLinear::apply(x, w, a, b, buf, meta, scale, scales, a_main, b_main, w_main);
   const c10::cuda::CUDAGuard guard(x.device());
   if (x.size(0) == 0) return at::empty({0, w.size(0)}, x.options().requires_grad(false));
-  return joint(x, w, shrink(x, a, false, buf, meta, scale, scales), b, false, buf, meta);
+  return products(x, w, a, b, false, false, true, buf, meta, scale, scales).y;
 }
 
 int64_t adapter_error_code() { return bb::adapter_error_code(); }

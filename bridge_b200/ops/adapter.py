@@ -59,7 +59,8 @@ def _lay_out(cu: list[int], slots: list[int]) -> tuple[np.ndarray, list[int]]:
     * ``row_slot [T]``;
     * per tile of 256 rows, the slots that it meets: ``tile_start [tiles + 1]`` into ``pairs [., 12]`` =
       (slot, 0, 0, 0, 8 words with the bits of the rows that are NOT the slot's);
-    * the same by tiles of 128 rows, each pair by itself: ``units [., 8]`` = (tile, slot, 0, 0, 4 words);
+    * the same by tiles of 128 rows, each pair by itself: ``unit_start [tiles + 1]`` into ``units [., 8]`` = (tile,
+      slot, 0, 0, 4 words);
     * per slot, its rows in blocks of at most 64: ``block_start [slots + 1]`` into ``blocks [., 4]`` = (first
       row, rows, slot, 0).  A block ends where the slot's rows end, so that it holds no other request's row.
     """
@@ -77,6 +78,8 @@ def _lay_out(cu: list[int], slots: list[int]) -> tuple[np.ndarray, list[int]]:
     pair, half = np.nonzero((halves != -1).any(axis=2))
     units = np.zeros((len(pair), 8), np.int32)
     units[:, 0], units[:, 1], units[:, 4:] = keys[pair] // max(top, 1) * 2 + half, pairs[pair, 0], halves[pair, half]
+    units = units[np.argsort(units[:, 0], kind="stable")]
+    unit_start = np.searchsorted(units[:, 0], np.arange(2 * tiles + 1))
     tile_start = np.searchsorted(keys // max(top, 1), np.arange(tiles + 1))
 
     first = np.flatnonzero(np.diff(row_slot, prepend=-2))            # runs of one slot, whatever their requests
@@ -92,7 +95,7 @@ def _lay_out(cu: list[int], slots: list[int]) -> tuple[np.ndarray, list[int]]:
     block_start = np.searchsorted(owner[order], np.arange(top + 1))
 
     parts, where, total = [], [], 0
-    for part in (row_slot, tile_start, pairs, units, block_start, blocks[order]):
+    for part in (row_slot, tile_start, pairs, unit_start, units, block_start, blocks[order]):
         flat = np.asarray(part, np.int32).reshape(-1)
         where.append(total)
         parts.append(np.concatenate((flat, np.zeros(-len(flat) % 4, np.int32))))      # each begins at 16 bytes

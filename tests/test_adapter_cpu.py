@@ -51,11 +51,11 @@ def test_plan(seed):
     for n in lengths:
         cu.append(cu[-1] + n)
     rows = adapter_rows(cu, slots, device="cpu")
-    total, top, units, blocks, o_row, o_tile, o_pair, o_unit, o_start, o_block = rows.meta
+    total, top, units, blocks, o_row, o_tile, o_pair, o_first, o_unit, o_start, o_block = rows.meta
     table = rows.table.tolist()
     want = row_slots(cu, slots, "cpu").tolist()
     assert total == cu[-1] and top == max(slots) + 1 and table[o_row:o_row + total] == want
-    assert all(o % 4 == 0 for o in (o_row, o_tile, o_pair, o_unit, o_start, o_block))
+    assert all(o % 4 == 0 for o in (o_row, o_tile, o_pair, o_first, o_unit, o_start, o_block))
     seen = [-1] * total
     for t in range(-(-total // 256)):
         for p in range(table[o_tile + t], table[o_tile + t + 1]):
@@ -68,6 +68,7 @@ def test_plan(seed):
     seen = [-1] * total
     for u in range(units):
         unit = table[o_unit + 8 * u:o_unit + 8 * u + 8]
+        assert table[o_first + unit[0]] <= u < table[o_first + unit[0] + 1]
         here = [i for i in range(128) if not unit[4 + i // 32] >> (i % 32) & 1]
         assert here
         for i in here:
