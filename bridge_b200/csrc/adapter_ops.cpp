@@ -3,6 +3,9 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
+#include <tuple>
+
 #include "adapter_linear.h"
 
 torch::Tensor gemm(torch::Tensor a, torch::Tensor b, bool a_mn, bool b_mn, c10::optional<torch::Tensor> out,
@@ -206,6 +209,94 @@ torch::Tensor adapter_linear(torch::Tensor x, torch::Tensor w, torch::Tensor a, 
   const c10::cuda::CUDAGuard guard(x.device());
   if (x.size(0) == 0) return at::empty({0, w.size(0)}, x.options().requires_grad(false));
   return products(x, w, a, b, false, false, true, buf, meta, scale, scales).y;
+}
+
+// The plan of a batch on `device`, laid out as ops/adapter.py's _lay_out says (which makes the same without CUDA), and
+// its meta.  The copy is complete when this returns: kernels read a plan before they wait for the stream.
+std::tuple<torch::Tensor, Meta> adapter_plan(const std::vector<int64_t>& cu, const std::vector<int64_t>& slots,
+                                             const torch::Device& device) {
+  const int64_t rows = cu.back(), tiles = (rows + 255) / 256;
+  const int64_t top = slots.empty() ? 0 : *std::max_element(slots.begin(), slots.end()) + 1;
+  struct Pair {
+    int32_t slot;
+    uint32_t off[8];
+  };
+  struct Block {
+    int32_t row, n;
+  };
+  std::vector<int32_t> row_slot(rows), tile_start{0}, unit_start{0}, units;
+  std::vector<Pair> pairs;
+  std::vector<int64_t> seen(top, -1);              // tile in which a slot was met last
+  std::vector<std::vector<Block>> blocks(top);
+  int64_t open = -1, begin = 0;                    // the run of rows of one slot that is under way
+  const auto close = [&](int64_t end) {
+    for (int64_t r = begin; open >= 0 && r < end; r += 64)
+      blocks[open].push_back({(int32_t)r, (int32_t)std::min<int64_t>(64, end - r)});
+  };
+  for (size_t i = 0; i < slots.size(); ++i) {
+    if (cu[i] == cu[i + 1]) continue;
+    std::fill(row_slot.begin() + cu[i], row_slot.begin() + cu[i + 1], (int32_t)slots[i]);
+    if (slots[i] != open) close(cu[i]), open = slots[i], begin = cu[i];
+  }
+  close(rows);
+  for (int64_t t = 0; t < tiles; ++t) {
+    const int64_t lo = t * 256, hi = std::min(rows, lo + 256);
+    std::vector<int32_t> here;
+    for (int64_t r = lo; r < hi; ++r)
+      if (const int32_t s = row_slot[r]; s >= 0 && seen[s] != t) seen[s] = t, here.push_back(s);
+    std::sort(here.begin(), here.end());
+    const size_t first = pairs.size();
+    for (const int32_t s : here) {
+      Pair p{s, {}};
+      std::fill(p.off, p.off + 8, 0xffffffffu);
+      pairs.push_back(p);
+    }
+    for (int64_t r = lo; r < hi; ++r)
+      if (const int32_t s = row_slot[r]; s >= 0) {
+        const size_t at = first + (std::lower_bound(here.begin(), here.end(), s) - here.begin());
+        pairs[at].off[(r - lo) / 32] &= ~(1u << ((r - lo) % 32));
+      }
+    tile_start.push_back((int32_t)pairs.size());
+    for (int half = 0; half < 2; ++half) {
+      for (size_t k = first; k < pairs.size(); ++k) {
+        const uint32_t* off = pairs[k].off + 4 * half;
+        if ((off[0] & off[1] & off[2] & off[3]) == 0xffffffffu) continue;
+        units.insert(units.end(), {(int32_t)(2 * t + half), pairs[k].slot, 0, 0});
+        for (int w = 0; w < 4; ++w) units.push_back((int32_t)off[w]);
+      }
+      unit_start.push_back((int32_t)(units.size() / 8));
+    }
+  }
+  std::vector<int32_t> flat;
+  Meta meta{rows, top, (int64_t)units.size() / 8, 0};
+  const auto begin_part = [&] {
+    flat.resize((flat.size() + 3) / 4 * 4);        // each part begins at 16 bytes
+    meta.push_back((int64_t)flat.size());
+  };
+  const auto part = [&](const std::vector<int32_t>& v) {
+    begin_part();
+    flat.insert(flat.end(), v.begin(), v.end());
+  };
+  part(row_slot);
+  part(tile_start);
+  begin_part();
+  for (const Pair& p : pairs) {
+    flat.insert(flat.end(), {p.slot, 0, 0, 0});
+    for (const uint32_t w : p.off) flat.push_back((int32_t)w);
+  }
+  part(unit_start);
+  part(units);
+  std::vector<int32_t> block_start{0}, list;
+  for (int64_t s = 0; s < top; ++s) {
+    for (const Block& b : blocks[s]) list.insert(list.end(), {b.row, b.n, (int32_t)s, 0});
+    block_start.push_back((int32_t)(list.size() / 4));
+  }
+  meta[3] = (int64_t)list.size() / 4;
+  part(block_start);
+  part(list);
+  flat.resize((flat.size() + 3) / 4 * 4);
+  const auto host = torch::from_blob(flat.data(), {(int64_t)flat.size()}, at::kInt);
+  return {host.to(device, /*non_blocking=*/false, /*copy=*/true), meta};
 }
 
 int64_t adapter_error_code() { return bb::adapter_error_code(); }

@@ -143,6 +143,9 @@ torch::Tensor adapter_linear(torch::Tensor x, torch::Tensor w, torch::Tensor a, 
                              std::vector<int64_t> meta, double scale, c10::optional<torch::Tensor> scales,
                              c10::optional<torch::Tensor> a_main, c10::optional<torch::Tensor> b_main,
                              c10::optional<torch::Tensor> w_main);
+std::tuple<torch::Tensor, std::vector<int64_t>> adapter_plan(const std::vector<int64_t>& cu,
+                                                             const std::vector<int64_t>& slots,
+                                                             const torch::Device& device);
 int64_t adapter_error_code();
 torch::Tensor clip_grad_norm(const std::vector<torch::Tensor>& grads, bool per_slot, double grad_scale, bool clip,
                              double max_norm, c10::optional<torch::Tensor> max_norms,
@@ -222,6 +225,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("grouped_gemm", &grouped_gemm, "MoE grouped tcgen05 GEMM (device expert offsets)");
   m.def("grouped_gemm_wgrad", &grouped_gemm_wgrad, "MoE grouped weight gradient, FP32 accumulate");
   m.def("adapter_linear", &adapter_linear, "shared projection beside the low-rank adapters of the rows' requests");
+  m.def("adapter_plan", &adapter_plan, "which rows of a batch use which adapter, for the kernels");
   m.def("adapter_error_code", &adapter_error_code);
   m.def("clip_grad_norm", &clip_grad_norm, "norm over many gradients, of all or by slot, and the scaling to a bound");
   m.def("launch_count", &bb_launch_count,

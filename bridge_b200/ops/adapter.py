@@ -29,7 +29,7 @@ import numpy as np
 import torch
 from torch import Tensor
 
-from ._ext import kernels, on_gpu
+from ._ext import kernels, on_gpu, reference_forced
 from .norm import _main_grad
 
 MAX_RANK = 128
@@ -44,8 +44,11 @@ class AdapterRows:
         self.cu_seqlens, self.slots = cu_seqlens, slots
         self.num_rows = cu_seqlens[-1]
         self.num_slots = max(slots, default=-1) + 1       # a stack needs at least as many
-        table, self.meta = _lay_out(cu_seqlens, slots)
-        self.table = torch.from_numpy(table).to(device)
+        if device.type == "cuda" and not reference_forced():
+            self.table, self.meta = kernels().adapter_plan(cu_seqlens, slots, device)
+        else:
+            table, self.meta = _lay_out(cu_seqlens, slots)
+            self.table = torch.from_numpy(table).to(device)
         self.device = self.table.device
 
     def rows_of(self, slot: int) -> list[tuple[int, int]]:
@@ -54,7 +57,7 @@ class AdapterRows:
 
 
 def _lay_out(cu: list[int], slots: list[int]) -> tuple[np.ndarray, list[int]]:
-    """The plan as the kernels read it, one int32 buffer, and ``[rows, slots, units, blocks, where its parts begin]``.
+    """The plan as the kernels read it (``csrc/adapter_ops.cpp`` lays out the same for them), one int32 buffer, and ``[rows, slots, units, blocks, where its parts begin]``.
 
     * ``row_slot [T]``;
     * per tile of 256 rows, the slots that it meets: ``tile_start [tiles + 1]`` into ``pairs [., 12]`` =
@@ -108,7 +111,7 @@ def adapter_rows(cu_seqlens: Sequence[int], slots: Sequence[int], device=None) -
 
     Both are host lists; ``device`` is where the batch lives (the current CUDA device unless given, else the CPU).
     Requests may be empty, share slots, and come in any order.  One plan serves any number of calls."""
-    cu, slots = [int(c) for c in cu_seqlens], [int(s) for s in slots]
+    cu, slots = list(map(int, cu_seqlens)), list(map(int, slots))
     if len(cu) != len(slots) + 1 or cu[0] != 0 or any(b < a for a, b in zip(cu, cu[1:])):
         raise ValueError(f"adapter_rows: cu_seqlens must rise from 0 and have one entry more than the {len(slots)} slots")
     if any(s < -1 for s in slots):

@@ -100,6 +100,19 @@ def test_an_adapter_spoils_its_own_rows_only(t):
     assert not torch.isfinite(_train(x, w, a * math.nan, b, rows, 1.0, dy)["y"]).any()
 
 
+@pytest.mark.parametrize("seed", range(12))
+def test_plan_is_the_one_laid_out_without_cuda(seed):
+    g = torch.Generator().manual_seed(seed)
+    count = int(torch.randint(0, 60, (), generator=g))
+    lengths = torch.randint(0, [3, 40, 900][seed % 3], (count,), generator=g).tolist()
+    slots = torch.randint(-1, [1, 5, 40, 3][seed // 3], (count,), generator=g).tolist()
+    cu = [0]
+    for n in lengths:
+        cu.append(cu[-1] + n)
+    host, dev = adapter_rows(cu, slots, device="cpu"), adapter_rows(cu, slots, device=DEV)
+    assert host.meta == list(dev.meta) and torch.equal(host.table, dev.table.cpu())
+
+
 def test_no_adapter_is_the_projection():
     x, w, a, b, dy = _inputs(300, 256, 512, 2, 8, torch.bfloat16)
     got = _train(x, w, a * math.nan, b * math.inf, adapter_rows([0, 300], [-1], device=DEV), 1.0, dy)
