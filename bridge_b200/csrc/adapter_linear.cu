@@ -613,6 +613,7 @@ struct JointParams {
   uint16_t* y;
   float* sums;             // [units of cut tiles][256 / 4 columns][256 rows][4]
   int T, N, R, nk;
+  int group;                  // tiles of rows that go through the columns together
   int whole, slices, units;   // tiles that are not cut, cuts of each other one, pieces of work in all
   uint32_t idesc;
   bool half;
@@ -636,8 +637,9 @@ __device__ __forceinline__ Piece piece_at(const JointParams& p, int q) {
       w.sum = j, w.last = slice == p.slices - 1;
     }
   }
-  // groups of 8 tiles of rows, so that a tile of W serves 8 from L2
-  const int per_group = 8 * n_tiles, first = tile / per_group * 8, gm = min(8, m_tiles - first), r = tile % per_group;
+  // groups of tiles of rows, so that a tile of W serves all of a group from L2
+  const int per_group = p.group * n_tiles, first = tile / per_group * p.group, gm = min(p.group, m_tiles - first);
+  const int r = tile % per_group;
   w.mt = first + r % gm;
   w.nt = r / gm;
   return w;
@@ -1391,6 +1393,10 @@ cudaError_t run_joint(const AdapterProduct& a, cudaStream_t stream) {
   p.sums = static_cast<float*>(a.workspace);
   p.T = a.T, p.N = a.N, p.R = a.R;
   p.nk = (a.K + BK - 1) / BK;
+  // Wide products like larger groups (W is read once per group), tall ones smaller: 8192 rows, 2560 -> 19456, groups of 4,
+  // 8, 16, 32: 643, 623, 607, 609 us under a sustained power cap; 9728 -> 2560: 316, 320, 324, 338.
+  const int m_tiles = (a.T + 255) / 256, n_tiles = (a.N + 255) / 256;
+  p.group = n_tiles >= 2 * m_tiles ? 16 : m_tiles >= 2 * n_tiles ? 4 : 8;
   p.whole = c.whole, p.slices = c.slices, p.units = c.units;
   p.idesc = sm100::umma_idesc_bf16(256, 256, false, MN) & ~(a.half ? sm100::kIdescBf16 : 0u);
   p.half = a.half;
