@@ -24,7 +24,7 @@ import torch
 import torch.nn as nn
 from torch import Tensor
 
-from ..ops.adapter import AdapterRows, adapter_linear, adapter_rows
+from ..ops.adapter import MAX_RANK, AdapterRows, adapter_linear, adapter_rows
 from ..ops.grad_norm import clip_grad_norm
 from ..parallel.tp import ColumnParallelLinear, RowParallelLinear, tp_size
 
@@ -58,6 +58,8 @@ class AdapterSet(nn.Module):
             raise ValueError(f"AdapterSet: the model has no projection named one of {targets}")
         if any(tp_size(m.group) > 1 for _, m in found):
             raise NotImplementedError("AdapterSet: tensor-parallel projections are not adapted")
+        if any(m.weight.is_cuda for _, m in found) and (rank % 8 or rank > MAX_RANK):
+            raise ValueError(f"AdapterSet: on CUDA the rank is a multiple of 8 up to {MAX_RANK}, got {rank}")
         if any(m.adapter is not None for _, m in found):
             raise ValueError("AdapterSet: the model has adapters already; remove() them first")
         self.slots, self.rank, self.scale = slots, rank, (rank if alpha is None else alpha) / rank

@@ -110,7 +110,8 @@ def adapter_rows(cu_seqlens: Sequence[int], slots: Sequence[int], device=None) -
     """The plan of a packed batch: request ``i`` has rows ``cu_seqlens[i]:cu_seqlens[i+1]`` and slot ``slots[i]`` (-1: none).
 
     Both are host lists; ``device`` is where the batch lives (the current CUDA device unless given, else the CPU).
-    Requests may be empty, share slots, and come in any order.  One plan serves any number of calls."""
+    Requests may be empty, share slots, and come in any order.  One plan serves any number of calls; it is made outside
+    of CUDA graphs (its copy to the device is waited for) and lives as long as a graph that was captured with it."""
     cu, slots = list(map(int, cu_seqlens)), list(map(int, slots))
     if len(cu) != len(slots) + 1 or cu[0] != 0 or any(b < a for a, b in zip(cu, cu[1:])):
         raise ValueError(f"adapter_rows: cu_seqlens must rise from 0 and have one entry more than the {len(slots)} slots")
@@ -120,7 +121,10 @@ def adapter_rows(cu_seqlens: Sequence[int], slots: Sequence[int], device=None) -
         raise ValueError("adapter_rows: at most 2^30 rows and 2^16 slots")
     if device is None:
         device = torch.device("cuda", torch.cuda.current_device()) if torch.cuda.is_available() else "cpu"
-    return AdapterRows(cu, slots, torch.device(device))
+    device = torch.device(device)
+    if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("adapter_rows: a plan cannot be made while a CUDA graph is captured; make it before")
+    return AdapterRows(cu, slots, device)
 
 
 def adapter_linear_reference(x: Tensor, weight: Tensor, a: Tensor, b: Tensor, rows: AdapterRows,

@@ -129,6 +129,26 @@ def test_one_slot_on_gpu(preset):
     assert torch.isfinite(got).all() and (got - base.float()).norm() > 0.01 * base.float().norm()
 
 
+@pytest.mark.gpu
+def test_refusals_on_gpu():
+    model = build_model(get_config("tiny"), seed=1, device="cuda")
+    for rank in (4, 12, 136):
+        with pytest.raises(ValueError, match="multiple of 8"):
+            AdapterSet(model, slots=1, rank=rank)
+    adapters = AdapterSet(model, slots=1, rank=8)
+    g = torch.cuda.CUDAGraph()
+    x = torch.zeros(8, 256, device="cuda", dtype=torch.bfloat16)
+    adapters.active = 0
+    plan = adapters.rows_for(x)                 # made before: the capture takes it
+    with torch.cuda.graph(g):
+        assert adapters.rows_for(x) is plan
+        with pytest.raises(RuntimeError, match="captured"):
+            adapter_rows([0, 8], [0], device="cuda")
+        x.add_(1.0)
+    g.replay()
+    assert (x == 1).all()
+
+
 def test_refusals():
     model = build_model(get_config("tiny"), seed=1)
     with pytest.raises(ValueError, match="slot"):
