@@ -325,8 +325,32 @@ def bench_vocab_rows(t: Timer, small: bool):
     _report("topk_distill_fwd_bwd", {"U": U, "V": V, "k": k}, ms, bytes_=2 * nb)
 
 
+def bench_adapters(t: Timer, small: bool):
+    """Projections with the adapters of four policies beside them (rank 16), their gradients, and clipping those."""
+    from bridge_b200.ops import adapter_linear, adapter_rows, clip_grad_norm
+
+    K, N, R, S = 2560, 6144, 16, 4
+    w = (torch.randn(N, K, device="cuda") / math.sqrt(K)).to(torch.bfloat16)
+    a = (torch.randn(S, R, K, device="cuda") / math.sqrt(K)).to(torch.bfloat16)
+    b = torch.randn(S, N, R, device="cuda").to(torch.bfloat16)
+    for T in (1, 32, 4608 if not small else 2048):
+        x = torch.randn(T, K, device="cuda").to(torch.bfloat16)
+        rows = adapter_rows([0, T // 3, T // 2, T], [0, 3, 1], device="cuda")
+        fl, nb = 2.0 * T * K * N + 2.0 * T * R * (K + N), 2.0 * (T * (K + N) + N * K + 3 * R * (K + N))
+        ms = t(lambda: adapter_linear(x, w, a, b, rows, 2.0))
+        _report("adapter_linear", {"T": T, "K": K, "N": N, "R": R}, ms, bytes_=nb, flops=fl if T > 128 else 0.0)
+    xg, ag, bg = (v.detach().requires_grad_() for v in (x, a, b))
+    dy = torch.randn(T, N, device="cuda").to(torch.bfloat16)
+    ms = t(lambda: torch.autograd.grad(adapter_linear(xg, w, ag, bg, rows, 2.0), (xg, ag, bg), dy))
+    _report("adapter_linear_fwd_bwd", {"T": T, "K": K, "N": N, "R": R}, ms, flops=2 * fl + 2.0 * T * R * (K + N))
+    grads = [torch.randn(S, R, K, device="cuda") for _ in range(18 if small else 288)]
+    ms = t(lambda: clip_grad_norm(grads, 1.0, per_slot=True))
+    _report("clip_grad_norm", {"tensors": len(grads), "slots": S}, ms, bytes_=8.0 * len(grads) * S * R * K)
+
+
 OPS = {"gemm": bench_gemm, "attention": bench_attention, "elementwise": bench_elementwise,
-       "logprob": bench_logprob, "vocab_rows": bench_vocab_rows, "ppo": bench_ppo, "gdn": bench_gdn, "moe": bench_moe}
+       "logprob": bench_logprob, "vocab_rows": bench_vocab_rows, "adapters": bench_adapters,
+       "ppo": bench_ppo, "gdn": bench_gdn, "moe": bench_moe}
 
 
 def main(argv=None):
