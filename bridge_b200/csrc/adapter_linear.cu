@@ -222,6 +222,115 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
+// The same for a few rows, where a cluster's start and joining would take longer than the reading: a block makes two
+// columns of u for four of a slot's rows, its four warps taking 256 values of K in turn.
+// Ordinary FP32 arithmetic; nothing to allocate, no barrier but one at the end.
+constexpr int kDotWarps = 4, kDotRows = 4;
+
+struct DotsParams {
+  AdapterPlan plan;
+  const uint16_t *x, *op;
+  uint16_t* u;
+  const float* scales;
+  float scale;
+  long ldx;
+  int K, R;
+};
+
+__device__ __forceinline__ float2 unpack2(uint32_t v, bool half) {
+  if (half) return __half22float2(*reinterpret_cast<const __half2*>(&v));
+  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+}
+__device__ __forceinline__ float dot8(const uint4& a, const uint4& b, float s, bool half) {
+  const uint32_t p[4] = {a.x, a.y, a.z, a.w}, q[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = unpack2(p[i], half), g = unpack2(q[i], half);
+    s = fmaf(f.x, g.x, s);
+    s = fmaf(f.y, g.y, s);
+  }
+  return s;
+}
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
+template <bool HALF>
+__global__ void __launch_bounds__(32 * kDotWarps) adapter_dots_kernel(const DotsParams p) {
+  __shared__ float sums[kDotWarps][2 * kDotRows];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int* unit = p.plan.units + (size_t)(blockIdx.x / (p.R / 2)) * 8;
+  const int tile = __ldg(unit), slot = __ldg(unit + 1), r0 = blockIdx.x % (p.R / 2) * 2;
+  const uint16_t* a = p.op + ((size_t)slot * p.R + r0) * p.K;
+  constexpr int kStep = 256 * kDotWarps, kUnroll = 4;
+  const int k0 = warp * 256 + lane * 8;
+  uint32_t mine[4];
+  int skip = kDotRows * blockIdx.y;       // rows of the slot that other blocks take
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    mine[w] = ~(uint32_t)__ldg(unit + 4 + w);
+    for (; skip > 0 && mine[w]; --skip) mine[w] &= mine[w] - 1;
+  }
+  if (!(mine[0] | mine[1] | mine[2] | mine[3])) return;
+  for (int k = k0; k < p.K; k += kStep) prefetch_l2(a + k), prefetch_l2(a + p.K + k);
+  wait_for_previous();
+  let_next_begin();
+  const float f = p.scales ? p.scales[slot] : p.scale;
+  int row[kDotRows], n = 0;
+#pragma unroll
+  for (int j = 0; j < kDotRows; ++j) {
+    row[j] = -1;
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      if (row[j] < 0 && mine[w]) row[j] = 32 * w + __ffs(mine[w]) - 1, mine[w] &= mine[w] - 1, ++n;
+  }
+  const uint16_t* x[kDotRows];
+  float s[2 * kDotRows];
+#pragma unroll
+  for (int j = 0; j < kDotRows; ++j) {
+    x[j] = p.x + (size_t)(tile * BM + max(row[j], 0)) * p.ldx;
+    s[2 * j] = s[2 * j + 1] = 0.f;
+  }
+  for (int k = k0; k < p.K; k += kUnroll * kStep) {
+    uint4 q[kUnroll][2], v[kUnroll][kDotRows];
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i)
+      if (k + i * kStep < p.K) {
+        q[i][0] = *reinterpret_cast<const uint4*>(a + k + i * kStep);
+        q[i][1] = *reinterpret_cast<const uint4*>(a + p.K + k + i * kStep);
+#pragma unroll
+        for (int j = 0; j < kDotRows; ++j)
+          if (j < n) v[i][j] = *reinterpret_cast<const uint4*>(x[j] + k + i * kStep);
+      }
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i)
+      if (k + i * kStep < p.K)
+#pragma unroll
+        for (int j = 0; j < kDotRows; ++j)
+          if (j < n) {
+            s[2 * j] = dot8(q[i][0], v[i][j], s[2 * j], HALF);
+            s[2 * j + 1] = dot8(q[i][1], v[i][j], s[2 * j + 1], HALF);
+          }
+  }
+#pragma unroll
+  for (int j = 0; j < 2 * kDotRows; ++j) {
+    s[j] = bb::warp_sum(s[j]);
+    if (lane == 0) sums[warp][j] = s[j];
+  }
+  __syncthreads();
+  if (threadIdx.x < kDotRows) {
+    const int j = threadIdx.x;
+    int r = -1;
+#pragma unroll
+    for (int i = 0; i < kDotRows; ++i)
+      if (i == j) r = row[i];
+    if (r >= 0) {
+      float t0 = 0.f, t1 = 0.f;
+#pragma unroll
+      for (int w = 0; w < kDotWarps; ++w) t0 += sums[w][2 * j], t1 += sums[w][2 * j + 1];
+      *reinterpret_cast<uint32_t*>(p.u + (size_t)(tile * BM + r) * p.R + r0) = pack2(f * t0, f * t1, HALF);
+    }
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ few rows
 struct FewParams {
   AdapterPlan plan;
@@ -397,10 +506,6 @@ struct TokenParams {
   bool half;
 };
 
-__device__ __forceinline__ float2 unpack2(uint32_t v, bool half) {
-  if (half) return __half22float2(*reinterpret_cast<const __half2*>(&v));
-  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
-}
 __device__ __forceinline__ float unpack1(uint16_t v, bool half) {
   return half ? __half2float(__ushort_as_half(v)) : __bfloat162float(__ushort_as_bfloat16(v));
 }
@@ -409,8 +514,6 @@ __device__ __forceinline__ float ld_cluster1(uint32_t addr) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
-
 // A few rows of few slots, in one kernel: every cluster (128 columns of y, each of its blocks a stretch of K) makes
 // u for itself as it goes, from the slots' rows of A beside W's: more reading from L2, but no second kernel to start, to
 // end and to wait for.  The accumulator holds y's 128 columns and the products with every slot's A, of which a row takes
@@ -1186,11 +1289,11 @@ cudaError_t allow_smem(Kernel kernel, int bytes, std::atomic<unsigned long long>
 // The kernel may begin while the one before it in the stream ends (it waits by itself for what that one wrote).
 // `cluster`: blocks of one, 0 where the kernel says it itself.
 template <typename... P, typename... A>
-cudaError_t launch(void (*kernel)(P...), int grid, int threads, int smem, int cluster, cudaStream_t stream,
+cudaError_t launch(void (*kernel)(P...), dim3 grid, int threads, int smem, int cluster, cudaStream_t stream,
                    const A&... args) {
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[2];
-  cfg.gridDim = dim3(grid);
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -1281,6 +1384,22 @@ cudaError_t run_shrink(const AdapterProduct& a, cudaStream_t stream) {
   return launch(adapter_shrink_kernel<OP_MN>, a.plan.num_units * p.ranks, kThreads, smem, p.ranks, stream, x, op, p);
 }
 
+cudaError_t run_dots(const AdapterProduct& a, cudaStream_t stream) {
+  DotsParams p{};
+  p.plan = a.plan;
+  p.x = static_cast<const uint16_t*>(a.x), p.op = static_cast<const uint16_t*>(a.op), p.u = static_cast<uint16_t*>(a.u);
+  p.scales = a.scales, p.scale = a.scale;
+  p.ldx = a.ldx, p.K = a.K, p.R = a.R;
+  const dim3 grid(a.plan.num_units * (a.R / 2), (a.T + kDotRows - 1) / kDotRows);
+  return a.half ? launch(adapter_dots_kernel<true>, grid, 32 * kDotWarps, 0, 0, stream, p)
+                : launch(adapter_dots_kernel<false>, grid, 32 * kDotWarps, 0, 0, stream, p);
+}
+
+// Rows and ranks up to which u is made by dot products: 2560 -> 6144, whole calls, dots and tensor cores: 8 rows of 8 slots,
+// rank 16, 11.7 and 13.9 us; 64 rows of 2, rank 16, 16.7 and 17.6; 8 rows of 8 slots, rank 64, 15.2 and 14.1; 64 rows of 8
+// slots, rank 32, over 9728 32 and 24.
+bool few_dots(const AdapterProduct& a) { return !a.mn && a.R <= 32 && a.T * a.R <= 1024; }
+
 // Which kernel makes the joint product.  Up to 128 rows the read of W is all there is, and clusters that split K read it
 // fastest; further on as long as tiles of 128 x 128 are few (to a cluster of 3 blocks or more each) and K is long:
 // 4096 -> 2560, 256 rows (40 tiles): 18 us, on pairs of SMs 23; 2560 -> 6144, 256 rows (96 tiles): 22 and 18; 256 -> 512,
@@ -1319,12 +1438,12 @@ cudaError_t run_few(const AdapterProduct& a, cudaStream_t stream) {
 }
 
 // Columns of the accumulator that a batch's slots take beside y's 128 in the one-kernel form, or 0 where it does not apply.
-// Its low-rank part goes by rows x rank, its reading by the slots: 2560 -> 6144, one and two kernels: 1 row of rank 16
-// 10.8 and 11.9 us, 16 rows 12.5 and 13.4, 32 rows 14.5 and 14.2 (and a launch less), 16 rows of rank 64 19 and 15; 4 slots
-// 11.8 and 13.2, 8 slots 20 and 15.
+// Its low-rank part goes by rows x rank, its reading by the slots; what it saves is a launch (4 us of the host's 11).
+// 2560 -> 6144 on the device, one kernel and two: 1 row of rank 16 10.7 and 11.1 us, 4 rows of 2 slots 11.3 and 11.1, 8 rows
+// of 4 slots 12.5 and 11.4, 32 rows of 4 slots 21.5 and 13.5; calls of 1 row, host included, 9.8 and 12.5.
 int token_columns(const AdapterProduct& a) {
   const int each = a.mn ? (a.R + 63) / 64 * 64 : (a.R + 15) / 16 * 16, all = a.plan.num_units * each;
-  return a.T * a.R <= 512 && all <= 64 ? all : 0;
+  return a.T * a.R <= 64 && all <= (a.mn ? 64 : 32) ? all : 0;
 }
 
 template <bool MN>
@@ -1413,6 +1532,7 @@ cudaError_t run_joint(const AdapterProduct& a, cudaStream_t stream) {
 cudaError_t launch_adapter_shrink(const AdapterProduct& a, cudaStream_t stream) {
   const cudaError_t e = have_context();
   if (e != cudaSuccess || a.plan.num_units == 0) return e;
+  if (few_dots(a)) return run_dots(a, stream);
   return a.mn ? run_shrink<true>(a, stream) : run_shrink<false>(a, stream);
 }
 
