@@ -335,12 +335,12 @@ __global__ void __launch_bounds__(32 * kDotWarps) adapter_dots_kernel(const Dots
 struct FewParams {
   AdapterPlan plan;
   uint16_t* y;
-  int T, N, R, rows, stages, nk, ranks;   // rows of a tile: 128, or T up to the next 8
+  int T, N, R, rows, cols, stages, nk, ranks;   // a tile: 128 rows, or T up to the next 8; columns of y
   uint32_t idesc;
   bool half;
 };
 
-// Few rows: bound by the read of W.  A cluster of `ranks` blocks takes 128 columns of y (and 128 rows), each block a
+// Few rows: bound by the read of W.  A cluster of `ranks` blocks takes `cols` columns of y (and 128 rows), each block a
 // stretch of K and some of the slots' low-rank products; the partial sums meet in shared memory.  Only the rows that there are get
 // loaded: the matrix instruction's other rows read whatever lies behind, and nobody reads what becomes of them.  u is
 // waited for when W has been asked for, so that this kernel streams W while the one before it still makes u.
@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(kThreads)
                        const FewParams p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int x_bytes = p.rows * 128, stage_bytes = x_bytes + kXBytes;
+  const int x_bytes = p.rows * 128, stage_bytes = x_bytes + p.cols * 128, tmem_cols = p.cols <= 128 ? 128 : 256;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + p.stages * stage_bytes);
   uint64_t* empty = full + p.stages;
   uint64_t* done = empty + p.stages;
@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(kThreads)
   int* my_slot = reinterpret_cast<int*>(my_mask + BM);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tile = blockIdx.x / p.ranks, m_tiles = (p.T + BM - 1) / BM;    // neighbours share columns of W
-  const int rank = (int)sm100::cluster_ctarank(), mt = tile % m_tiles, m0 = mt * BM, n0 = tile / m_tiles * BM;
+  const int rank = (int)sm100::cluster_ctarank(), mt = tile % m_tiles, m0 = mt * BM, n0 = tile / m_tiles * p.cols;
   const int rows = min(BM, p.T - m0);
   const int kb0 = (int)((long)p.nk * rank / p.ranks), kb1 = (int)((long)p.nk * (rank + 1) / p.ranks);
   const int rank_blocks = (p.R + BK - 1) / BK;
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(kThreads)
     sm100::prefetch_tmap(&map_x);
     sm100::prefetch_tmap(&map_w);
   }
-  if (warp == 1) sm100::tmem_alloc(tmem_word, 128);
+  if (warp == 1) sm100::tmem_alloc(tmem_word, tmem_cols);
   if (warp >= 2 && (int)threadIdx.x - 64 < units) {        // (one at a time in the loops below, each would be a wait)
     const int4* unit = reinterpret_cast<const int4*>(p.plan.units) + 2 * (size_t)(unit0 + (threadIdx.x - 64) * p.ranks);
     my_slot[threadIdx.x - 64] = __ldg(unit).y;
@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(kThreads)
     sm100::umma_commit(done);
   }
   __syncwarp();
-  constexpr int kRow = BM + 4;     // floats: rows 16 bytes apart in the banks
+  const int row_floats = p.cols + 4;     // rows 16 bytes apart in the banks
   float* part = reinterpret_cast<float*>(smem);
   if (warp >= 2) {
     const int quarter = warp & 3, row = quarter * 32 + lane;
@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(kThreads)
     __syncwarp();
     sm100::tc_fence_after();
     if (quarter * 32 < rows)
-      for (int c = 0; c < BM; c += 32) {
+      for (int c = 0; c < p.cols; c += 32) {
         uint32_t r[32];
         sm100::tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + c, r);
         sm100::tmem_ld_wait();
@@ -470,27 +470,28 @@ __global__ void __launch_bounds__(kThreads)
         if (row < rows)
 #pragma unroll
           for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<uint4*>(part + row * kRow + c + i) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
+            if (c + i < p.cols)
+              *reinterpret_cast<uint4*>(part + row * row_floats + c + i) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
       }
     sm100::tc_fence_before();
   }
   __syncthreads();
   sm100::cluster_sync();
-  // this block's share of the 16 groups of 8 columns
-  const int lo = 16 * rank / p.ranks, groups = 16 * (rank + 1) / p.ranks - lo;
+  // this block's share of the groups of 8 columns
+  const int lo = p.cols / 8 * rank / p.ranks, groups = p.cols / 8 * (rank + 1) / p.ranks - lo;
   const uint32_t base = sm100::smem_addr(part);
   for (int i = threadIdx.x; i < groups * rows; i += kThreads) {
     const int c = (lo + i % groups) * 8, t = i / groups;
     if (n0 + c >= p.N) continue;
     float v[8];
-    joined8(base, t * kRow + c, p.ranks, v);
+    joined8(base, t * row_floats + c, p.ranks, v);
     *reinterpret_cast<uint4*>(p.y + (size_t)(m0 + t) * p.N + n0 + c) =
         make_uint4(pack2(v[0], v[1], p.half), pack2(v[2], v[3], p.half), pack2(v[4], v[5], p.half), pack2(v[6], v[7], p.half));
   }
   sm100::cluster_sync();   // the peers' sums stay until all have read them
   if (warp == 1) {
     sm100::tc_fence_after();
-    sm100::tmem_dealloc(tmem, 128);
+    sm100::tmem_dealloc(tmem, tmem_cols);
   }
 }
 
@@ -1412,27 +1413,35 @@ bool few_rows(int T, int K, int N) {
 template <bool MN>
 cudaError_t run_few(const AdapterProduct& a, cudaStream_t stream) {
   alignas(64) CUtensorMap x, w, u, low;
-  const int rows = std::min(BM, (a.T + 7) / 8 * 8);
+  const int rows = std::min(BM, (a.T + 7) / 8 * 8), m_tiles = (a.T + BM - 1) / BM;
+  // Where tiles of 128 columns are a few more than SMs, some SMs would have two and the rest one: wider tiles, one to each.
+  // 2560 -> 19456, 152 tiles of 128 and 136 of 144: 1 row 19.4 and 18.7 us, 61 rows 23.2 and 21.4, 128 rows 27.9 and 25.5;
+  // 176 tiles and 141: 19.0 and 18.5; 282 tiles and 141 of 256: 31.9 and 32.5.
+  constexpr int kWidest = 176;
+  int cols = BM;
+  if (!MN && m_tiles * ((a.N + kWidest - 1) / kWidest) <= sm_count())
+    while (m_tiles * ((a.N + cols - 1) / cols) > sm_count()) cols += 16;
   bool ok = encode(&x, a.x, a.K, a.T, a.ldx, 0, rows, a.half) && encode(&u, a.u, a.R, a.T, a.R, 0, rows, a.half);
   if (MN) ok = ok && encode(&w, a.w, a.N, a.K, a.ldw, 0, 64, a.half) && encode(&low, a.low, a.N, a.R, a.N, a.S, 64, a.half);
-  else ok = ok && encode(&w, a.w, a.K, a.N, a.ldw, 0, BM, a.half) && encode(&low, a.low, a.R, a.N, a.R, a.S, BM, a.half);
+  else ok = ok && encode(&w, a.w, a.K, a.N, a.ldw, 0, cols, a.half) && encode(&low, a.low, a.R, a.N, a.R, a.S, cols, a.half);
   if (!ok) return cudaErrorInvalidValue;
   FewParams p{};
   p.plan = a.plan;
   p.y = static_cast<uint16_t*>(a.y);
-  p.T = a.T, p.N = a.N, p.R = a.R, p.rows = rows;
+  p.T = a.T, p.N = a.N, p.R = a.R, p.rows = rows, p.cols = cols;
   p.nk = (a.K + BK - 1) / BK;
-  const int tiles = (a.T + BM - 1) / BM * ((a.N + BM - 1) / BM);
+  const int tiles = m_tiles * ((a.N + cols - 1) / cols), stage = (rows + cols) * 128;
   // 69 to 128 KB; where tiles outnumber the SMs, little enough for two blocks to an SM.  (128 rows, 4 stages: 14.7 us with
   // 2 blocks a cluster and one to an SM, 18 with 3 stages and more of them; 152 tiles: 27 us with 3 stages, 42 with 4.)
-  p.stages = tiles > sm_count() ? std::min(4, 110 * 1024 / (kXBytes + rows * 128)) : 4;
-  p.idesc = sm100::umma_idesc_bf16(BM, BM, false, MN) & ~(a.half ? sm100::kIdescBf16 : 0u);
+  p.stages = tiles > sm_count() ? std::min(4, 110 * 1024 / stage) : 4;
+  p.idesc = sm100::umma_idesc_bf16(BM, cols, false, MN) & ~(a.half ? sm100::kIdescBf16 : 0u);
   p.half = a.half;
-  const int smem = std::max(p.stages * (kXBytes + rows * 128), std::min(BM, a.T) * (BM + 4) * 4) + 256 + BM * 20 + 1024;
+  int smem = std::max(p.stages * stage, std::min(BM, a.T) * (cols + 4) * 4) + 256 + BM * 20 + 1024;
+  if (cols > 128) smem = std::max(smem, 80 * 1024);      // (with 256 columns of TMEM: see the gradients)
   static std::atomic<unsigned long long> done{0};
   const cudaError_t e = allow_smem(adapter_few_kernel<MN>, kMaxSmem, done);
   if (e != cudaSuccess) return e;
-  p.ranks = split(adapter_few_kernel<MN>, smem, 128, tiles, p.nk);
+  p.ranks = split(adapter_few_kernel<MN>, smem, cols <= 128 ? 128 : 256, tiles, p.nk);
   return launch(adapter_few_kernel<MN>, tiles * p.ranks, kThreads, smem, p.ranks, stream, x, w, u,
                 low, p);
 }
@@ -1440,10 +1449,11 @@ cudaError_t run_few(const AdapterProduct& a, cudaStream_t stream) {
 // Columns of the accumulator that a batch's slots take beside y's 128 in the one-kernel form, or 0 where it does not apply.
 // Its low-rank part goes by rows x rank, its reading by the slots; what it saves is a launch (4 us of the host's 11).
 // 2560 -> 6144 on the device, one kernel and two: 1 row of rank 16 10.7 and 11.1 us, 4 rows of 2 slots 11.3 and 11.1, 8 rows
-// of 4 slots 12.5 and 11.4, 32 rows of 4 slots 21.5 and 13.5; calls of 1 row, host included, 9.8 and 12.5.
+// of 4 slots 12.5 and 11.4, 32 rows of 4 slots 21.5 and 13.5; calls of 1 row, host included, 9.8 and 12.5.  Larger W, where
+// the host is not what counts: 1 row, 2048 -> 12352 15.2 and 13.7, 9728 -> 2560 16.0 and 14.5, 2560 -> 19456 28.3 and 20.6.
 int token_columns(const AdapterProduct& a) {
   const int each = a.mn ? (a.R + 63) / 64 * 64 : (a.R + 15) / 16 * 16, all = a.plan.num_units * each;
-  return a.T * a.R <= 64 && all <= (a.mn ? 64 : 32) ? all : 0;
+  return a.T * a.R <= 64 && all <= (a.mn ? 64 : 32) && (long)a.K * a.N <= 1 << 24 ? all : 0;
 }
 
 template <bool MN>

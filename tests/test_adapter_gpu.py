@@ -77,6 +77,13 @@ def test_sizes(k, n, r, t):
     _compare(x, w, a, b, cu, [3, 0, 1], 2.0, dy)
 
 
+@pytest.mark.parametrize("t,n", [(3, 19456), (70, 19208), (128, 37000), (5, 40000)])
+def test_more_columns_than_multiprocessors(t, n):
+    """Few rows and tiles that are a few more than there are SMs."""
+    x, w, a, b, dy = _inputs(t, 136, n, 3, 16, torch.bfloat16, seed=n)
+    _compare(x, w, a, b, [0, t // 3, t - 1, t], [2, 0, -1], 1.0, dy)
+
+
 @pytest.mark.parametrize("t", [9, 300, 2500])
 def test_an_adapter_spoils_its_own_rows_only(t):
     """Infinite and NaN adapters, and rows that hold them, beside requests that share their tiles and blocks."""
