@@ -1592,8 +1592,9 @@ cudaError_t launch_adapter_grads(const AdapterGrads& a, cudaStream_t stream) {
   static std::atomic<unsigned long long> done{0};
   e = allow_smem(adapter_grads_kernel, kMaxSmem, done);
   if (e != cudaSuccess) return e;
-  const int tiles = p.tiles_a + p.tiles_b;
-  p.ranks = split(adapter_grads_kernel, smem, p.cols == 64 ? 256 : 512, tiles, std::max(1, a.plan.num_blocks));
+  // (cut as for both gradients, so that one does not depend on whether the other is asked for)
+  const int tiles = p.tiles_a + p.tiles_b, both = (a.K + BM - 1) / BM + (a.N + BM - 1) / BM;
+  p.ranks = split(adapter_grads_kernel, smem, p.cols == 64 ? 256 : 512, both, std::max(1, a.plan.num_blocks));
   return launch(adapter_grads_kernel, tiles * p.ranks, kThreads, smem, p.ranks, stream, x, dy, u, du, p);
 }
 
