@@ -53,7 +53,10 @@ __device__ __forceinline__ uint16_t pack1(float a, bool half) {
 
 __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
   float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
 }
 
@@ -117,7 +120,9 @@ struct ShrinkParams {
 };
 
 // A cluster of `ranks` blocks takes one slot's rows of a tile of 128, each block a stretch of K; the partial sums meet in
-// shared memory.  Rows without an adapter are not written: nothing reads them.
+// shared memory.  Rows without an adapter are not written: nothing reads them.  Bound by what an SM takes in by TMA (56
+// GB/s from DRAM: x and the adapter's part for every 128 rows), and by start and joining, some 8 us: 4608 rows of 2560,
+// rank 16, 12 us; 8192 rows of 9728, rank 64, 45 us (3.5 TB/s of x).
 template <bool OP_MN>
 __global__ void __launch_bounds__(kThreads)
     adapter_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_op,
@@ -224,7 +229,8 @@ __global__ void __launch_bounds__(kThreads)
 
 // The same for a few rows, where a cluster's start and joining would take longer than the reading: a block makes two
 // columns of u for four of a slot's rows, its four warps taking 256 values of K in turn.
-// Ordinary FP32 arithmetic; nothing to allocate, no barrier but one at the end.
+// Ordinary FP32 arithmetic; nothing to allocate, no barrier but one at the end.  32 rows of 16 slots, 4096 -> 2560, rank 16:
+// the whole call 14.4 us, with the kernel above 17.6.
 constexpr int kDotWarps = 4, kDotRows = 4;
 
 struct DotsParams {
@@ -341,9 +347,11 @@ struct FewParams {
 };
 
 // Few rows: bound by the read of W.  A cluster of `ranks` blocks takes `cols` columns of y (and 128 rows), each block a
-// stretch of K and some of the slots' low-rank products; the partial sums meet in shared memory.  Only the rows that there are get
-// loaded: the matrix instruction's other rows read whatever lies behind, and nobody reads what becomes of them.  u is
-// waited for when W has been asked for, so that this kernel streams W while the one before it still makes u.
+// stretch of K and some of the slots' low-rank products; the partial sums meet in shared memory.  Only the rows that
+// there are get loaded: the matrix instruction's other rows read whatever lies behind, and nobody reads what becomes of
+// them.  u is waited for when W has been asked for, so that this kernel streams W while the one before it still makes
+// u.  2560 -> 6144 without adapters, back to back: 1 row 9.6 us (3.3 TB/s; 5 us of it start and joining), 128 rows 14.3;
+// 2560 -> 19456, 61 rows 21.5 (4.8 TB/s).
 template <bool MN>
 __global__ void __launch_bounds__(kThreads)
     adapter_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
@@ -502,7 +510,8 @@ struct TokenParams {
   const uint16_t* low;
   const float* scales;
   float scale;
-  int T, N, R, rows, slot_cols, stages, nk, ranks, columns;   // slot_cols: of a slot in the accumulator; columns: of TMEM
+  int T, N, R, rows, stages, nk, ranks;
+  int slot_cols, columns;   // of a slot in the accumulator; of TMEM
   uint32_t idesc;
   bool half;
 };
@@ -519,7 +528,8 @@ __device__ __forceinline__ float ld_cluster1(uint32_t addr) {
 // u for itself as it goes, from the slots' rows of A beside W's: more reading from L2, but no second kernel to start, to
 // end and to wait for.  The accumulator holds y's 128 columns and the products with every slot's A, of which a row takes
 // its own slot's.  Where the partial sums meet, each block adds up u, rounds it as the other kernels do, and makes its
-// share of the columns: a few FP32 products a value.  The first cluster keeps u if it is asked for.
+// share of the columns: a few FP32 products a value.  The first cluster keeps u if it is asked for.  1 row, 2560 -> 6144,
+// rank 16: 10.7 us back to back.
 template <bool MN>
 __global__ void __launch_bounds__(kThreads)
     adapter_token_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
@@ -702,6 +712,9 @@ __global__ void __launch_bounds__(kThreads)
 // A pair of blocks (two SMs) computes tiles of 256 x 256: each holds its 128 rows of x and its half of W's 256, so that
 // every block of K costs an SM 32 KB for 2 x 128 x 256 x 64 products.  Accumulators are double-buffered in TMEM: a tile's
 // stores overlap the next one's products.
+//
+// Bound by the matrix units (85% of their cycles at 4096 x 9728 x 2560) and, when calls follow each other, by the power
+// cap: 8192 rows, 2560 -> 19456, 0.53 ms alone (1.55 PFLOP/s), 0.60 sustained (1.35 at 1.34 GHz; the library's 0.61).
 //
 // Tiles go round the pairs; those of a last round that would leave most pairs idle are cut along K into `slices`, whose
 // FP32 sums adapter_join_kernel adds up in slice order.
@@ -1029,7 +1042,8 @@ struct GradTile {
         const float4 o = *dst;
         *dst = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
       } else {
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + to) = make_uint2(pack2(v.x, v.y, half), pack2(v.z, v.w, half));
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + to) =
+            make_uint2(pack2(v.x, v.y, half), pack2(v.z, v.w, half));
       }
     } else {
       const size_t to = ((size_t)slot * R + c) * limit + m0 + r;
@@ -1051,7 +1065,9 @@ struct GradTile {
 // A cluster takes 128 columns of dy (or x) and the rows of all slots, cut evenly over its blocks whatever the slots'
 // shares: D_s [128, R] = sum over slot s's rows of dy^T u (x^T du).  A slot whose rows all fall to one block is written
 // by it at once, from the accumulator, while the next slot's products go into another one; of the slots that begin or end
-// in another block (at most two a block) the partial sums meet in shared memory at the end, in the blocks' order.
+// in another block (at most two a block) the partial sums meet in shared memory at the end, in the blocks' order.  Bound
+// like the shrink: 4608 rows of 2560 and 6144 columns, rank 16, 28 us (80 MB); 8192 rows of 9728 and 2560, rank 64, 45 us
+// (201 MB).
 __global__ void __launch_bounds__(kThreads)
     adapter_grads_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_dy,
                          const __grid_constant__ CUtensorMap map_u, const __grid_constant__ CUtensorMap map_du,
@@ -1353,9 +1369,10 @@ int split(void (*kernel)(P...), int smem, int columns, int clusters, int nk) {
     known.push_back(f);
     fit = &known.back();
   }
-  const int per_sm = std::max(1, std::min(kMaxSmem / (smem + 1024), 512 / columns));
+  const int sms = sm_count(), per_sm = std::max(1, std::min(kMaxSmem / (smem + 1024), 512 / columns));
   int ranks = 8;
-  while (ranks > 1 && (clusters > per_sm * fit->fits[ranks] || nk < (clusters * ranks > sm_count() ? 8 : 4) * ranks)) --ranks;
+  const auto fits = [&](int r) { return clusters <= per_sm * fit->fits[r] && nk >= (clusters * r > sms ? 8 : 4) * r; };
+  while (ranks > 1 && !fits(ranks)) --ranks;
   return ranks;
 }
 
@@ -1399,7 +1416,7 @@ cudaError_t run_dots(const AdapterProduct& a, cudaStream_t stream) {
 // Rows and ranks up to which u is made by dot products: 2560 -> 6144, whole calls, dots and tensor cores: 8 rows of 8 slots,
 // rank 16, 11.7 and 13.9 us; 64 rows of 2, rank 16, 16.7 and 17.6; 8 rows of 8 slots, rank 64, 15.2 and 14.1; 64 rows of 8
 // slots, rank 32, over 9728 32 and 24.
-bool few_dots(const AdapterProduct& a) { return !a.mn && a.R <= 32 && a.T * a.R <= 1024; }
+bool few_dots(const AdapterProduct& a) { return !a.mn && a.R <= 32 && (long)a.T * a.R <= 1024; }
 
 // Which kernel makes the joint product.  Up to 128 rows the read of W is all there is, and clusters that split K read it
 // fastest; further on as long as tiles of 128 x 128 are few (to a cluster of 3 blocks or more each) and K is long:
@@ -1452,8 +1469,8 @@ cudaError_t run_few(const AdapterProduct& a, cudaStream_t stream) {
 // of 4 slots 12.5 and 11.4, 32 rows of 4 slots 21.5 and 13.5; calls of 1 row, host included, 9.8 and 12.5.  Larger W, where
 // the host is not what counts: 1 row, 2048 -> 12352 15.2 and 13.7, 9728 -> 2560 16.0 and 14.5, 2560 -> 19456 28.3 and 20.6.
 int token_columns(const AdapterProduct& a) {
-  const int each = a.mn ? (a.R + 63) / 64 * 64 : (a.R + 15) / 16 * 16, all = a.plan.num_units * each;
-  return a.T * a.R <= 64 && all <= (a.mn ? 64 : 32) && (long)a.K * a.N <= 1 << 24 ? all : 0;
+  const long each = a.mn ? (a.R + 63) / 64 * 64 : (a.R + 15) / 16 * 16, all = a.plan.num_units * each;
+  return (long)a.T * a.R <= 64 && all <= (a.mn ? 64 : 32) && (long)a.K * a.N <= 1 << 24 ? all : 0;
 }
 
 template <bool MN>

@@ -47,7 +47,8 @@ struct Products {
   torch::Tensor u, y;      // undefined where not asked for
 };
 
-// u = scale A x and y = W x + B u from (x, W, A, B); du = scale B^T dy and dx = W^T dy + A^T du from (dy, W, B, A) with `mn`.
+// u = scale A x and y = W x + B u from (x, W, A, B); with `mn` du = scale B^T dy and dx = W^T dy + A^T du from
+// (dy, W, B, A).
 Products products(const torch::Tensor& x, const torch::Tensor& w, const torch::Tensor& op, const torch::Tensor& low, bool mn,
                   bool want_u, bool want_y, const torch::Tensor& buf, const Meta& meta, double scale,
                   const OptTensor& scales) {

@@ -51,13 +51,10 @@ class AdapterRows:
             self.table = torch.from_numpy(table).to(device)
         self.device = self.table.device
 
-    def rows_of(self, slot: int) -> list[tuple[int, int]]:
-        """``(first, end)`` of the requests that use ``slot``."""
-        return [(a, b) for a, b, s in zip(self.cu_seqlens, self.cu_seqlens[1:], self.slots) if s == slot and b > a]
-
 
 def _lay_out(cu: list[int], slots: list[int]) -> tuple[np.ndarray, list[int]]:
-    """The plan as the kernels read it (``csrc/adapter_ops.cpp`` lays out the same for them), one int32 buffer, and ``[rows, slots, units, blocks, where its parts begin]``.
+    """The plan as the kernels read it (``csrc/adapter_ops.cpp`` lays out the same for them): one int32 buffer, and
+    ``[rows, slots, units, blocks, where its parts begin]``.
 
     * ``row_slot [T]``;
     * per tile of 256 rows, the slots that it meets: ``tile_start [tiles + 1]`` into ``pairs [., 12]`` =
@@ -175,7 +172,8 @@ def _check_cuda(x, weight, a) -> None:
         raise TypeError(f"adapter_linear: bfloat16 or float16 on CUDA, got {x.dtype}")
     s, r, k = a.shape
     if s < 1 or k < 8 or k % 8 or weight.shape[0] < 8 or weight.shape[0] % 8:
-        raise ValueError(f"adapter_linear: K ({k}) and N ({weight.shape[0]}) must be multiples of 8, and the stack not empty")
+        raise ValueError(f"adapter_linear: K ({k}) and N ({weight.shape[0]}) must be multiples of 8, and the stack must "
+                         "not be empty")
     if r < 8 or r % 8 or r > MAX_RANK:
         raise ValueError(f"adapter_linear: rank {r} must be a multiple of 8 up to {MAX_RANK} (smaller ones: pad with zeros)")
     if weight.requires_grad and x.dtype == torch.float16:

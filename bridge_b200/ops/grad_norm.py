@@ -6,8 +6,8 @@ Stacked gradients (``[S, ...]``, as those of :func:`~bridge_b200.ops.adapter.ada
     norm_s = sqrt(sum over tensors and values of g_s^2) / grad_scale
     out_s  = g_s min(1, max_norm / (norm_s + 1e-6)) / grad_scale
 
-``grad_scale`` is the loss scale that the gradients carry.  The norm is the one of :class:`~bridge_b200.engine.optim.MixedPrecisionAdamW`,
-summed in 64 bits: no finite gradient overflows it.  A NaN or infinite gradient makes the norm NaN or infinite and,
+``grad_scale`` is the loss scale that the gradients carry.  The norm is the one of
+:class:`~bridge_b200.engine.optim.MixedPrecisionAdamW`, summed in 64 bits: no finite gradient overflows it.  A NaN or infinite gradient makes the norm NaN or infinite and,
 times the factor (NaN or 0), its slot's gradients NaN where they were not finite.  Subnormal FP32 gradients count as 0
 on CUDA.  Results do not depend on timing
 (``csrc/grad_norm.cu``); on CPU the PyTorch form runs.  Nothing here is differentiable.
