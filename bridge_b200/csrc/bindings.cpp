@@ -147,9 +147,8 @@ std::tuple<torch::Tensor, std::vector<int64_t>> adapter_plan(const std::vector<i
                                                              const std::vector<int64_t>& slots,
                                                              const torch::Device& device);
 int64_t adapter_error_code();
-torch::Tensor clip_grad_norm(const std::vector<torch::Tensor>& grads, bool per_slot, double grad_scale, bool clip,
-                             double max_norm, c10::optional<torch::Tensor> max_norms,
-                             const std::vector<torch::Tensor>& out);
+torch::Tensor clip_grad_norm(const pybind11::object& grads, bool per_slot, double grad_scale, bool clip,
+                             double max_norm, c10::optional<torch::Tensor> max_norms, const pybind11::object& out);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "bridge_b200 sm_100a kernels";

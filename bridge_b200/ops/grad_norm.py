@@ -25,12 +25,28 @@ from ._ext import kernels, on_gpu
 
 
 def _check(grads, grad_scale: float) -> list[Tensor]:
-    grads = list(grads)
-    if not grads or any(not isinstance(g, Tensor) for g in grads):
+    if not isinstance(grads, (list, tuple)):
+        grads = list(grads)
+    if not grads or not isinstance(grads[0], Tensor):
         raise ValueError("clip_grad_norm: needs a list of gradient tensors, without None")
     if not (grad_scale > 0 and math.isfinite(grad_scale)):
         raise ValueError(f"clip_grad_norm: grad_scale must be positive and finite, got {grad_scale}")
     return grads
+
+
+def _tensors(*lists) -> None:
+    """(The binding looks at every entry by itself: on CUDA this only finds the words for what it refused.)"""
+    for entries in lists:
+        if any(not isinstance(t, Tensor) for t in entries):
+            raise ValueError("clip_grad_norm: needs lists of tensors, without None")
+
+
+def _run(*args):
+    try:
+        return kernels().clip_grad_norm(*args)
+    except TypeError:
+        _tensors(args[0], args[-1])
+        raise
 
 
 def _detached(tensors) -> None:
@@ -68,7 +84,8 @@ def global_grad_norm(grads: Sequence[Tensor], *, per_slot: bool = False, grad_sc
     """2-norm over all tensors, FP32 ``[]``; with ``per_slot`` ``[S]``, each slot's own.  No host synchronisation."""
     grads = _check(grads, grad_scale)
     if on_gpu(grads[0]):
-        return kernels().clip_grad_norm(grads, per_slot, grad_scale, False, 0.0, None, [])
+        return _run(grads, per_slot, grad_scale, False, 0.0, None, [])
+    _tensors(grads)
     _detached(grads)
     with torch.no_grad():
         return clip_grad_norm_reference(grads, 0.0, per_slot, grad_scale, None)
@@ -81,17 +98,17 @@ def clip_grad_norm(grads: Sequence[Tensor], max_norm: Tensor | float, *, per_slo
     The gradients (dense FP32, BF16 or FP16 tensors of any mix, on one device) are overwritten, or left and written to
     ``out``, tensors like them that may be FP32.  ``max_norm`` is a number, or FP32 ``[S]`` with ``per_slot``."""
     grads = _check(grads, grad_scale)
+    if out is not None and not isinstance(out, (list, tuple)):
+        out = list(out)
     if out is not None and len(out) != len(grads):
         raise ValueError(f"clip_grad_norm: one output per gradient, got {len(out)} for {len(grads)}")
-    out = [] if out is None else list(out)
-    if any(not isinstance(o, Tensor) for o in out):
-        raise ValueError("clip_grad_norm: outputs are tensors")
+    out = [] if out is None else out
     bounds = isinstance(max_norm, Tensor)
     if not bounds and not max_norm >= 0:
         raise ValueError(f"clip_grad_norm: max_norm must not be negative, got {max_norm}")
     if on_gpu(grads[0]):
-        return kernels().clip_grad_norm(grads, per_slot, grad_scale, True, 0.0 if bounds else max_norm,
-                                        max_norm if bounds else None, out)
-    _detached(grads + out)
+        return _run(grads, per_slot, grad_scale, True, 0.0 if bounds else max_norm, max_norm if bounds else None, out)
+    _tensors(grads, out)
+    _detached([*grads, *out])
     with torch.no_grad():
         return clip_grad_norm_reference(grads, max_norm, per_slot, grad_scale, out or grads)

@@ -168,6 +168,16 @@ def test_in_place_is_seen_by_autograd():
 
 def test_refusals():
     g = torch.randn(8, 16, device=DEV)
+    for bad in ([g, None], [g, 1.0], [None, g]):
+        with pytest.raises(ValueError, match="without None"):
+            global_grad_norm(bad)
+    with pytest.raises(ValueError, match="without None"):
+        clip_grad_norm([g, g.clone()], 1.0, out=[g, None])
+    assert torch.equal(global_grad_norm(x for x in (g, g)), global_grad_norm((g, g)))
+    with pytest.raises(RuntimeError, match="differentiable"):
+        global_grad_norm([g, g.clone().requires_grad_()])
+    with torch.no_grad():
+        assert global_grad_norm([g.clone().requires_grad_()]) == global_grad_norm([g])
     with pytest.raises(TypeError, match="float32"):
         global_grad_norm([g.double()])
     with pytest.raises(TypeError, match="cpu"):
