@@ -398,7 +398,7 @@ torch::Tensor clip_grad_norm(const pybind11::object& grad_list, bool per_slot, d
   TORCH_CHECK_VALUE(!per_slot || (slots >= 1 && slots < (1 << 16)), "clip_grad_norm: per_slot needs gradients stacked by slot");
   const bool in_place = out.empty();
   TORCH_CHECK_VALUE(in_place || out.size() == grads.size(), "clip_grad_norm: one output per gradient");
-  const bool watched = at::GradMode::is_enabled();
+  const bool watched = at::GradMode::is_enabled(), inference = c10::InferenceMode::is_enabled();
   const c10::cuda::CUDAGuard guard(device);
   int64_t total = 0, bytes = 0;
   for (size_t i = 0; i < grads.size(); ++i) total += grads[i].numel(), bytes += grads[i].numel() * grads[i].element_size();
@@ -416,6 +416,8 @@ torch::Tensor clip_grad_norm(const pybind11::object& grad_list, bool per_slot, d
     TORCH_CHECK_TYPE(g.device() == device, "clip_grad_norm: gradients are on ", device, " and ", g.device());
     TORCH_CHECK(!watched || !(g.requires_grad() || (clip && o.requires_grad())),
                 "clip_grad_norm: norms and clipped gradients are not differentiable; detach the tensors");
+    TORCH_CHECK(!clip || inference || !o.is_inference(),
+                "clip_grad_norm: inference tensors are overwritten in inference mode only");
     Entry e{};
     e.kind = kind_of(g);
     const bool dense = per_slot ? g.is_contiguous() : (g.is_contiguous() || g.is_non_overlapping_and_dense());
@@ -469,6 +471,7 @@ torch::Tensor clip_grad_norm(const pybind11::object& grad_list, bool per_slot, d
     }
   }
   const Tensors& changed = in_place ? grads : out;
-  for (size_t i = 0; clip && i < changed.size(); ++i) changed[i].unsafeGetTensorImpl()->bump_version();
+  for (size_t i = 0; clip && i < changed.size(); ++i)
+    if (!changed[i].is_inference()) changed[i].unsafeGetTensorImpl()->bump_version();   // (those have no version)
   return norm;
 }

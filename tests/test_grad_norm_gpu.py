@@ -166,6 +166,20 @@ def test_in_place_is_seen_by_autograd():
     assert g._version > before
 
 
+def test_inference_tensors():
+    with torch.inference_mode():
+        g = torch.randn(100, device=DEV)
+        before = g.clone()
+        norm = clip_grad_norm([g], 1.0)
+        assert torch.allclose(g, before / (norm + 1e-6), rtol=2 ** -21, atol=0)     # (three roundings here, two there)
+        before = g.clone()
+    assert global_grad_norm([g]) == global_grad_norm([before])
+    with pytest.raises(RuntimeError, match="inference"):
+        clip_grad_norm([g], 0.5)
+    assert torch.equal(g, before)
+    clip_grad_norm([g], 0.5, out=[torch.empty(100, device=DEV)])
+
+
 def test_refusals():
     g = torch.randn(8, 16, device=DEV)
     for bad in ([g, None], [g, 1.0], [None, g]):
