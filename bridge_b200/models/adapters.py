@@ -65,6 +65,7 @@ class AdapterSet(nn.Module):
         self.slots, self.rank, self.scale = slots, rank, (rank if alpha is None else alpha) / rank
         self.active: AdapterRows | int | None = None
         self._plans: dict[tuple[int, int, str], AdapterRows] = {}
+        self._captured: dict[tuple[int, int, str], AdapterRows] = {}     # those that a CUDA graph may read again
         self._modules_of = [m for _, m in found]        # (a list: the model's modules do not become this one's)
         g = torch.Generator().manual_seed(seed)
         self.a, self.b = nn.ParameterDict(), nn.ParameterDict()
@@ -104,11 +105,19 @@ class AdapterSet(nn.Module):
             return None
         t = x.numel() // x.shape[-1]
         key = (t, self.active, str(x.device))
-        if key not in self._plans:
+        plan = self._plans.get(key) or self._captured.get(key)
+        if plan is None:
             if len(self._plans) >= 256:
                 self._plans.clear()
-            self._plans[key] = adapter_rows([0, t], [self.active], device=x.device)
-        return self._plans[key]
+            plan = self._plans[key] = adapter_rows([0, t], [self.active], device=x.device)
+        if x.is_cuda:
+            with torch.cuda.device(x.device):
+                if torch.cuda.is_current_stream_capturing():
+                    self._captured[key] = plan
+                else:
+                    # (a plan that leaves the list may have readers on other streams than the one it was made on)
+                    plan.table.record_stream(torch.cuda.current_stream())
+        return plan
 
     def gradients(self) -> list[Tensor]:
         """The stacks' gradients (FP32 ``main_grad`` where an optimizer keeps one), of those that have any."""

@@ -1,5 +1,8 @@
 """Adapters on whole models, with the clipping and the optimizer that follow: a run of them as it would be used."""
 
+import gc
+import weakref
+
 import pytest
 import torch
 
@@ -127,6 +130,28 @@ def test_one_slot_on_gpu(preset):
         with adapters.use(adapter_rows([0, 50, 130], [1, 1])):
             assert torch.equal(model(ids, pos, 130).float(), got)
     assert torch.isfinite(got).all() and (got - base.float()).norm() > 0.01 * base.float().norm()
+
+
+@pytest.mark.gpu
+def test_captured_plan_outlives_the_list():
+    """A graph reads the plan of its slot again after hundreds of other lengths have come by."""
+    model = build_model(get_config("tiny"), seed=1, device="cuda")
+    adapters = _filled(model)
+    p = next(m for m in adapters._modules_of)
+    x = torch.randn(40, p.weight.shape[1], device="cuda", dtype=p.weight.dtype)
+    with torch.no_grad(), adapters.use(1):
+        want = p.adapter(x, p.weight)
+        plan = weakref.ref(adapters.rows_for(x))
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = p.adapter(x, p.weight)
+        for t in range(41, 641):
+            adapters.rows_for(x.expand(t, 40, -1)[:, 0])
+        gc.collect()
+        assert plan() is not None and adapters.rows_for(x) is plan()
+        assert len(adapters._plans) <= 256
+        g.replay()
+    assert torch.equal(y, want)
 
 
 @pytest.mark.gpu
