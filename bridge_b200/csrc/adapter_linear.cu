@@ -910,7 +910,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
   } else {
     const int quarter = warp & 3;
-    int acc = 0;
+    int acc = 0, turn = 0;      // turn: which of the warp's two store buffers is next, through all of its tiles
     uint32_t acc_phase = 0;
     for (int q = pair; q < p.units; q += pairs) {
       const bool got = sm100::mbar_wait_cluster(&tfull[acc], acc_phase, &g_error, 44);
@@ -934,7 +934,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
       } else {
         // 32 rows x 64 columns at a time through shared memory (128-byte swizzle: 16-byte piece j of row i lies at
-        // j ^ i % 8), so that y is written in whole lines; straight from the registers its sectors went out in halves
+        // j ^ i % 8), so that y is written in whole lines; straight from the registers its sectors went out in halves.
+        // The two buffers take turns from store to store, not from column to column: a tile at the right edge may have
+        // an odd number of stores, and the wait below is for all but the last one.
         const int row0 = w.mt * 256 + 128 * rank + quarter * 32;
 #pragma unroll 1
         for (int c = 0; c < 256; c += 64) {
@@ -946,7 +948,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           sm100::tmem_ld_wait();
           sm100::tmem_regs_ready(r);
           sm100::tmem_regs_ready(r2);
-          unsigned char* buf = store + (quarter * 2 + (c / 64 & 1)) * kStoreBytes;
+          unsigned char* buf = store + (quarter * 2 + turn) * kStoreBytes;
+          turn ^= 1;
           if (lane == 0) sm100::tma_store_wait_read<1>();      // the store before the last one has left this buffer
           __syncwarp();
 #pragma unroll

@@ -33,3 +33,14 @@ def test_slots_are_read_before_they_are_refilled():
     assert body.rindex("__syncwarp()") > body.rindex("read<3>(")
     # and every read of a slot goes through it
     assert len(re.findall(r"\bread<\d>\(ring", text)) == len(re.findall(r"\bread<\d>\(ring", body)) == 4
+
+
+def test_store_buffers_take_turns_across_tiles():
+    """A wait for all but the last store frees the other buffer only if every store takes the buffer that the one before
+    it did not, through all tiles of a warp."""
+    text = dict(_sources())["adapter_linear.cu"]
+    body = re.search(r"\n    adapter_joint_kernel\(.*?\n}\n", text, re.S).group(0)
+    assert len(re.findall(r"tma_store_2d\(", body)) == len(re.findall(r"tma_store_wait_read<1>", body)) == 1
+    assert re.search(r"buf = store \+ \(quarter \* 2 \+ turn\) \* kStoreBytes;\s+turn \^= 1;", body)
+    assert len(re.findall(r"\bturn\b", re.sub(r"//[^\n]*", "", body))) == 3
+    assert body.index("turn = 0") < body.rindex("for (int q = pair;") < body.index("+ turn)")
