@@ -8,7 +8,8 @@ model's forward takes each row through its request's slot; outside of it the mod
     optimizer = MixedPrecisionAdamW(adapters, AdamWConfig(grad_clip=0.0))
     with adapters.use(adapter_rows(cu_seqlens, slots)):
         hidden = model(ids, positions)
-    loss.backward()
+        ...
+        loss.backward()                            # inside, where activations are computed again
     norms = adapters.clip_grad_norm_(1.0)          # each policy by its own norm
     optimizer.step()
 
@@ -64,6 +65,8 @@ class AdapterSet(nn.Module):
             raise ValueError("AdapterSet: the model has adapters already; remove() them first")
         self.slots, self.rank, self.scale = slots, rank, (rank if alpha is None else alpha) / rank
         self.active: AdapterRows | int | None = None
+        self._open = 0              # use() blocks under way
+        self._used = False          # whether one of them had adapters
         self._plans: dict[tuple[int, int, str], AdapterRows] = {}
         self._captured: dict[tuple[int, int, str], AdapterRows] = {}     # those that a CUDA graph may read again
         self._modules_of = [m for _, m in found]        # (a list: the model's modules do not become this one's)
@@ -86,19 +89,29 @@ class AdapterSet(nn.Module):
     @contextlib.contextmanager
     def use(self, rows: AdapterRows | int | None):
         """Forwards inside run ``rows``' requests through their slots; an integer: every row through that slot;
-        ``None``: the model as it was.  One setting at a time, for all threads (a recomputed forward sees it too)."""
+        ``None``: the model as it was.  One setting at a time, for all threads.
+
+        A forward that a backward pass computes again (activation checkpointing) takes the setting of that moment, so the
+        backward belongs inside the block of its forward.  Outside of every block it is refused rather than taken
+        through the model without its adapters."""
         if isinstance(rows, int) and not -1 <= rows < self.slots:
             raise ValueError(f"AdapterSet: slot {rows} of {self.slots}")
         if not (rows is None or isinstance(rows, (int, AdapterRows))):
             raise TypeError("AdapterSet: use() takes adapter_rows(), a slot or None")
         before, self.active = self.active, rows
+        self._open += 1
+        self._used = self._used or rows is not None
         try:
             yield self
         finally:
+            self._open -= 1
             self.active = before
 
     def rows_for(self, x: Tensor) -> AdapterRows | None:
         """The plan of a projection's input, or None for the model as it was."""
+        if self.active is None and self._used and not self._open and torch._C._current_graph_task_id() != -1:
+            raise RuntimeError("AdapterSet: a backward pass computes a forward again outside of use(); run the backward inside "
+                               "the block of its forward (use(None) for the model as it was)")
         if not isinstance(self.active, int):
             return self.active
         if self.active < 0:
