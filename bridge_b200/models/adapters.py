@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import contextlib
 import math
+import warnings
 
 import torch
 import torch.nn as nn
@@ -28,6 +29,7 @@ from torch import Tensor
 from ..ops.adapter import MAX_RANK, AdapterRows, adapter_linear, adapter_rows
 from ..ops.grad_norm import clip_grad_norm
 from ..parallel.tp import ColumnParallelLinear, RowParallelLinear, tp_size
+from .moe import MoELayer
 
 TARGETS = ("qkv", "o_proj", "in_proj", "out_proj", "fc1", "fc2")
 
@@ -46,7 +48,8 @@ class _Adapted:
 class AdapterSet(nn.Module):
     """Adapters of ``slots`` policies on the ``targets`` projections of ``model`` (unsharded; its weights are frozen).
 
-    ``scale`` is ``alpha / rank`` (``alpha`` is the rank unless given)."""
+    ``scale`` is ``alpha / rank`` (``alpha`` is the rank unless given).  The experts of mixture-of-experts layers, routed and
+    shared, get no adapters; a warning says so where ``targets`` name MLP projections."""
 
     def __init__(self, model: nn.Module, *, slots: int, rank: int, alpha: float | None = None,
                  targets: tuple[str, ...] = TARGETS, seed: int = 0) -> None:
@@ -63,6 +66,10 @@ class AdapterSet(nn.Module):
             raise ValueError(f"AdapterSet: on CUDA the rank is a multiple of 8 up to {MAX_RANK}, got {rank}")
         if any(m.adapter is not None for _, m in found):
             raise ValueError("AdapterSet: the model has adapters already; remove() them first")
+        experts = [name for name, m in model.named_modules() if isinstance(m, MoELayer)]
+        if experts and {"fc1", "fc2"} & set(targets):
+            warnings.warn(f"AdapterSet: the routed and shared experts of {len(experts)} mixture-of-experts layers get no "
+                          f"adapters ({experts[0]} the first)", stacklevel=2)
         self.slots, self.rank, self.scale = slots, rank, (rank if alpha is None else alpha) / rank
         self.active: AdapterRows | int | None = None
         self._open = 0              # use() blocks under way
