@@ -129,12 +129,19 @@ class TPREngine:
             return run_tpr_forward_backward(self, data[TPR_REQUEST_KEY])
         return run_tpr_forward_backward_batch(self, data, loss_function, forward_only=forward_only)
 
+    def _own_weights_only(self) -> None:
+        if any(getattr(m, "adapter", None) is not None for m in self.model.modules()):
+            raise NotImplementedError("the engine's optimizer steps the model's own weights, which adapters have frozen: step an "
+                                      "optimizer over the AdapterSet, or remove() the adapters first")
+
     def optimizer_step(self) -> torch.Tensor:
+        self._own_weights_only()
         norm = self.optimizer.step()
         self.optimizer.zero_grad()
         return norm
 
     def train_step(self, data: Any, loss_function=None) -> dict:
+        self._own_weights_only()
         out = self.forward_backward_batch(data, loss_function)
         out["grad_norm"] = self.optimizer_step()
         if self.symm_heap is not None:

@@ -64,6 +64,8 @@ class MixedPrecisionAdamW:
     def __init__(self, module: nn.Module, cfg: AdamWConfig = AdamWConfig()) -> None:
         self.cfg = cfg
         params = [p for p in module.parameters() if p.requires_grad]
+        if not params:
+            raise ValueError("the optimizer's module has no parameter that takes a gradient (is its model frozen by adapters?)")
         dev = params[0].device
         self.arenas = []
         for dt in (torch.bfloat16, torch.float32):
@@ -253,6 +255,8 @@ class ShardedNVLinkAdamW(MixedPrecisionAdamW):
         self.heap = heap
         self.tp_group = tp_group
         groups = bucket_groups(module)
+        if not groups:
+            raise ValueError("the optimizer's module has no parameter that takes a gradient (is its model frozen by adapters?)")
         self.arenas = []
         for dt in (torch.bfloat16, torch.float32):
             g = [(label, [p for p in ps if p.dtype == dt]) for label, ps in groups]

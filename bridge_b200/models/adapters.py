@@ -14,6 +14,10 @@ model's forward takes each row through its request's slot; outside of it the mod
     optimizer.step()
 
 ``B`` begins at zero, so that a fresh slot is the reference policy.
+
+With an engine: ``forward_backward_batch`` inside ``use(slot)`` gives one slot's gradients (its executors take a batch apart,
+so a plan of several requests does not fit their rows); over data-parallel ranks the caller adds them up.  ``train_step`` and
+``optimizer_step``, which step the model's own weights, are refused.
 """
 
 from __future__ import annotations
