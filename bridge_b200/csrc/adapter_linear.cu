@@ -480,6 +480,7 @@ __global__ void __launch_bounds__(kThreads)
           for (int i = 0; i < 32; i += 4)
             if (c + i < p.cols)
               *reinterpret_cast<uint4*>(part + row * row_floats + c + i) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
+        __syncwarp();        // (the next load from TMEM takes the whole warp)
       }
     sm100::tc_fence_before();
   }
@@ -647,6 +648,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
           for (int i = 0; i < 16; i += 4)
             *reinterpret_cast<uint4*>(part + row * row_floats + c + i) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
+        __syncwarp();        // (the next load from TMEM takes the whole warp)
       }
     sm100::tc_fence_before();
   }
@@ -1197,6 +1199,7 @@ __global__ void __launch_bounds__(kThreads)
             if (c + j < p.R)
               g.put(slot, quarter * 32 + lane, c + j, make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]),
                                                                   __uint_as_float(r[j + 2]), __uint_as_float(r[j + 3])));
+          __syncwarp();      // (rows behind the last one leave `put` early; the next load from TMEM takes the whole warp)
         }
       }
       sm100::tc_fence_before();

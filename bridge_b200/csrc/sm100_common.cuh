@@ -222,6 +222,7 @@ __device__ __forceinline__ uint32_t mapa(uint32_t a, uint32_t rank) {
   return r;
 }
 __device__ __forceinline__ void cluster_sync() {
+  __syncwarp();      // (.aligned: the whole warp has to arrive together, also from a loop that its lanes leave one by one)
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {

@@ -44,3 +44,15 @@ def test_store_buffers_take_turns_across_tiles():
     assert re.search(r"buf = store \+ \(quarter \* 2 \+ turn\) \* kStoreBytes;\s+turn \^= 1;", body)
     assert len(re.findall(r"\bturn\b", re.sub(r"//[^\n]*", "", body))) == 3
     assert body.index("turn = 0") < body.rindex("for (int q = pair;") < body.index("+ turn)")
+
+
+def test_aligned_cluster_barriers_take_whole_warps():
+    """An aligned barrier is for a converged warp; after a loop of which each lane has its own number of rounds nothing but
+    a warp barrier says that it is."""
+    seen = 0
+    for name, text in _sources():
+        for m in re.finditer(r"barrier\.cluster\.arrive[\w.]*\.aligned", text):
+            seen += 1
+            before = re.sub(r"//[^\n]*", "", text[:m.start()])
+            assert re.search(r"__syncwarp\(\);\s*asm volatile\(\s*\"$", before), name
+    assert seen
