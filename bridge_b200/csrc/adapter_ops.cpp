@@ -1,5 +1,6 @@
 // Torch entry points of the adapter kernels (adapter_linear.cu): argument checks, allocation, autograd.
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -176,6 +177,15 @@ class AdapterLinear : public torch::autograd::Function<AdapterLinear> {
   }
 };
 
+// A plan lies inside an object that its owner may let go while kernels of another stream than the one it was made on still
+// read it: its memory is not handed out again before they are done.  (One that a graph is captured with has to be kept.)
+void read_by(const torch::Tensor& buf, const at::cuda::CUDAStream& stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  check(cudaStreamIsCapturing(stream, &status));
+  if (status == cudaStreamCaptureStatusNone)
+    c10::cuda::CUDACachingAllocator::recordStream(buf.storage().data_ptr(), stream);
+}
+
 bool main_fits(const OptTensor& m, const torch::Tensor& p) {
   return !m.has_value() || (m->scalar_type() == at::kFloat && m->is_contiguous() && m->numel() == p.numel() &&
                             m->device() == p.device() && aligned(*m));
@@ -205,9 +215,10 @@ torch::Tensor adapter_linear(torch::Tensor x, torch::Tensor w, torch::Tensor a, 
   if (!fits) return {};
   for (const auto& t : {x, w, a, b})
     TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), "adapter_linear has no forward-mode derivative");
+  const c10::cuda::CUDAGuard guard(x.device());
+  if (x.size(0)) read_by(buf, at::cuda::getCurrentCUDAStream());
   if (at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || a.requires_grad() || b.requires_grad()))
     return AdapterLinear::apply(x, w, a, b, buf, meta, scale, scales, a_main, b_main, w_main);
-  const c10::cuda::CUDAGuard guard(x.device());
   if (x.size(0) == 0) return at::empty({0, w.size(0)}, x.options().requires_grad(false));
   return products(x, w, a, b, false, false, true, buf, meta, scale, scales).y;
 }

@@ -138,9 +138,6 @@ class AdapterSet(nn.Module):
             with torch.cuda.device(x.device):
                 if torch.cuda.is_current_stream_capturing():
                     self._captured[key] = plan
-                else:
-                    # (a plan that leaves the list may have readers on other streams than the one it was made on)
-                    plan.table.record_stream(torch.cuda.current_stream())
         return plan
 
     def gradients(self) -> list[Tensor]:

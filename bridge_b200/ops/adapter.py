@@ -107,8 +107,9 @@ def adapter_rows(cu_seqlens: Sequence[int], slots: Sequence[int], device=None) -
     """The plan of a packed batch: request ``i`` has rows ``cu_seqlens[i]:cu_seqlens[i+1]`` and slot ``slots[i]`` (-1: none).
 
     Both are host lists; ``device`` is where the batch lives (the current CUDA device unless given, else the CPU).
-    Requests may be empty, share slots, and come in any order.  One plan serves any number of calls; it is made outside
-    of CUDA graphs (its copy to the device is waited for) and lives as long as a graph that was captured with it."""
+    Requests may be empty, share slots, and come in any order.  One plan serves any number of calls, on any streams, and may
+    be let go after the last one; with a CUDA graph it is made before the capture and kept as long as the graph.  Its
+    copy to the device is waited for, behind what the current stream has under way."""
     cu, slots = list(map(int, cu_seqlens)), list(map(int, slots))
     if len(cu) != len(slots) + 1 or cu[0] != 0 or any(b < a for a, b in zip(cu, cu[1:])):
         raise ValueError(f"adapter_rows: cu_seqlens must rise from 0 and have one entry more than the {len(slots)} slots")
