@@ -529,8 +529,9 @@ __device__ __forceinline__ float ld_cluster1(uint32_t addr) {
 // u for itself as it goes, from the slots' rows of A beside W's: more reading from L2, but no second kernel to start, to
 // end and to wait for.  The accumulator holds y's 128 columns and the products with every slot's A, of which a row takes
 // its own slot's.  Where the partial sums meet, each block adds up u, rounds it as the other kernels do, and makes its
-// share of the columns: a few FP32 products a value.  The first cluster keeps u if it is asked for.  1 row, 2560 -> 6144,
-// rank 16: 10.7 us back to back.
+// share of the columns: a few FP32 products a value.  The first cluster keeps u if it is asked for, but only y's: du, whose
+// sums here go by the columns of dx, comes from the kernels above whether dx is asked for or not, so that dA is the same
+// either way.  1 row, 2560 -> 6144, rank 16: 10.7 us back to back.
 template <bool MN>
 __global__ void __launch_bounds__(kThreads)
     adapter_token_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
@@ -1489,7 +1490,7 @@ cudaError_t run_token(const AdapterProduct& a, int u_cols, cudaStream_t stream) 
   if (!ok) return cudaErrorInvalidValue;
   TokenParams p{};
   p.plan = a.plan;
-  p.y = static_cast<uint16_t*>(a.y), p.u = a.keep_u ? static_cast<uint16_t*>(a.u) : nullptr;
+  p.y = static_cast<uint16_t*>(a.y), p.u = a.keep_u && !MN ? static_cast<uint16_t*>(a.u) : nullptr;
   p.low = static_cast<const uint16_t*>(a.low);
   p.scales = a.scales, p.scale = a.scale;
   p.T = a.T, p.N = a.N, p.R = a.R, p.rows = rows, p.slot_cols = each;
@@ -1580,8 +1581,11 @@ cudaError_t launch_adapter_product(const AdapterProduct& a, cudaStream_t stream)
   cudaError_t e = have_context();
   if (e != cudaSuccess) return e;
   if (a.plan.num_units)
-    if (const int columns = token_columns(a))
+    if (const int columns = token_columns(a)) {
+      if (a.mn && a.keep_u) e = launch_adapter_shrink(a, stream);
+      if (e != cudaSuccess) return e;
       return a.mn ? run_token<true>(a, columns, stream) : run_token<false>(a, columns, stream);
+    }
   e = launch_adapter_shrink(a, stream);
   if (e != cudaSuccess) return e;
   if (few_rows(a.T, a.K, a.N)) return a.mn ? run_few<true>(a, stream) : run_few<false>(a, stream);
