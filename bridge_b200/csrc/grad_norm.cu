@@ -16,7 +16,9 @@
 // 0.69 ms (0.178 and 0.511); 16 tensors of 53 thousand values 6.6 us.
 //
 // Squares are FP32 in sums of eight, which are added up in 64 bits; sums outside [1e-25, 1e37] (infinite or vanishing
-// squares, and zeros) are taken again value by value in 64 bits, so that no finite gradient overflows or disappears.
+// squares, and zeros) are taken again value by value in 64 bits, so that no finite gradient overflows or disappears.  The
+// factor is 64-bit too; where it leaves [1e-30, 1e30] the values are scaled by two factors, so that neither is a
+// subnormal, which would count as 0, or infinite.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cooperative_groups.h>
@@ -148,8 +150,22 @@ __device__ __forceinline__ double block_sum_f64(double v, double* scratch) {
   return s;
 }
 
+// A factor as two: f alone (g = 1), or f in [0.5, 1) times a power of two where one FP32 value could not hold it.
+struct Factor {
+  float f, g;
+  __device__ __forceinline__ float operator*(float v) const { return (f * v) * g; }
+};
+
+__device__ __forceinline__ Factor split(double factor) {
+  if (!(fabs(factor) > 0.0 && (fabs(factor) < 1e-30 || fabs(factor) > 1e30)) || isinf(factor)) return {(float)factor, 1.f};
+  int e;
+  const double m = frexp(factor, &e);
+  const int at = min(max(e, -126), 127);
+  return {(float)ldexp(m, e - at), (float)ldexp(1.0, at)};
+}
+
 template <int NT, typename T, typename O>
-__device__ void chunk_scale(const T* x, O* y, long n, float f, int tid) {
+__device__ void chunk_scale(const T* x, O* y, long n, const Factor& f, int tid) {
   constexpr int V = 16 / sizeof(T);
   const long head = lead(x, n), vecs = (n - head) / V;
   const Vec<T>* body = reinterpret_cast<const Vec<T>*>(x + head);
@@ -195,8 +211,8 @@ __device__ double sum_of(const Entry& e, const Chunk& c, int tid) {
 }
 
 template <int NT>
-__device__ void scale_of(const Entry& e, const Chunk& c, float f, int tid) {
-  if (f == 1.f && e.in == e.out) return;
+__device__ void scale_of(const Entry& e, const Chunk& c, const Factor& f, int tid) {
+  if (f.f == 1.f && f.g == 1.f && e.in == e.out) return;
   if (e.kind == kF32) {
     chunk_scale<NT>(static_cast<const float*>(e.in) + c.begin, static_cast<float*>(e.out) + c.begin, c.n, f, tid);
   } else if (e.kind == kBF16) {
@@ -217,12 +233,12 @@ struct Bound {
   bool scale;
 };
 
-__device__ __forceinline__ float finish(const Bound& b, int slot, double sum, bool write) {
+__device__ __forceinline__ Factor finish(const Bound& b, int slot, double sum, bool write) {
   const double n = sqrt(sum) / b.grad_scale;
   if (write) b.norm[slot] = (float)n;
   const double most = b.max_norms ? (double)b.max_norms[slot] : b.max_norm;
   // (a NaN norm makes the factor NaN)
-  return (float)((n + 1e-6 <= most ? 1.0 : most / (n + 1e-6)) / b.grad_scale);
+  return split((n + 1e-6 <= most ? 1.0 : most / (n + 1e-6)) / b.grad_scale);
 }
 
 template <int N>
@@ -233,18 +249,18 @@ __global__ void __launch_bounds__(kThreads) sums_kernel(const __grid_constant__ 
   if (threadIdx.x == 0) parts[(long)c.slot * t.per_slot + c.part] = s;
 }
 
-__global__ void __launch_bounds__(1024) finish_kernel(const double* parts, int per_slot, const Bound b, float* factor) {
+__global__ void __launch_bounds__(1024) finish_kernel(const double* parts, int per_slot, const Bound b, Factor* factor) {
   __shared__ double scratch[32];
   double s = 0.0;
   for (int i = threadIdx.x; i < per_slot; i += 1024) s += parts[(long)blockIdx.x * per_slot + i];
   s = block_sum_f64(s, scratch);
   if (threadIdx.x) return;
-  const float f = finish(b, blockIdx.x, s, true);
+  const Factor f = finish(b, blockIdx.x, s, true);
   if (b.scale) factor[blockIdx.x] = f;
 }
 
 template <int N>
-__global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ Table<N> t, const float* factor) {
+__global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ Table<N> t, const Factor* factor) {
   const Chunk c = locate(t, t.total - 1 - blockIdx.x);
   scale_of<kThreads>(t.e[c.entry], c, factor[c.slot], threadIdx.x);
 }
@@ -256,7 +272,7 @@ template <int N>
 __global__ void __cluster_dims__(kSmallBlocks, 1, 1) __launch_bounds__(32 * kSmallWarps)
     small_kernel(const __grid_constant__ Table<N> t, const Bound b) {
   __shared__ double sums[kSmallWarps][kSmallSlots];
-  __shared__ float factor[kSmallSlots];
+  __shared__ Factor factor[kSmallSlots];
   cg::cluster_group cluster = cg::this_cluster();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int first = blockIdx.x * kSmallWarps + warp, step = kSmallBlocks * kSmallWarps;
@@ -371,7 +387,7 @@ void run_small(const std::vector<Entry>& all, int slots, int per_slot, long chun
 }
 
 template <int N>
-void run(const std::vector<Entry>& all, int slots, int per_slot, long chunk, double* parts, const float* factor,
+void run(const std::vector<Entry>& all, int slots, int per_slot, long chunk, double* parts, const Factor* factor,
          cudaStream_t stream) {
   // (the scaling takes the lists backwards too)
   const size_t lists = (all.size() + N - 1) / N;
@@ -460,7 +476,7 @@ torch::Tensor clip_grad_norm(const pybind11::object& grad_list, bool per_slot, d
   } else {
     auto parts = at::empty({slots * per + slots}, f32.dtype(at::kDouble));     // sums, then factors
     double* sums = parts.data_ptr<double>();
-    float* factor = reinterpret_cast<float*>(sums + slots * per);
+    auto* factor = reinterpret_cast<Factor*>(sums + slots * per);
     if (few) run<kFew>(all, (int)slots, (int)per, chunk, sums, nullptr, stream);
     else run<kMany>(all, (int)slots, (int)per, chunk, sums, nullptr, stream);
     finish_kernel<<<(int)slots, 1024, 0, stream>>>(sums, (int)per, bound, factor);

@@ -7,9 +7,10 @@ Stacked gradients (``[S, ...]``, as those of :func:`~bridge_b200.ops.adapter.ada
     out_s  = g_s min(1, max_norm / (norm_s + 1e-6)) / grad_scale
 
 ``grad_scale`` is the loss scale that the gradients carry.  The norm is the one of
-:class:`~bridge_b200.engine.optim.MixedPrecisionAdamW`, summed in 64 bits: no finite gradient overflows it.  A NaN or infinite gradient makes the norm NaN or infinite and,
-times the factor (NaN or 0), its slot's gradients NaN where they were not finite.  Subnormal FP32 gradients count as 0
-on CUDA.  Results do not depend on timing
+:class:`~bridge_b200.engine.optim.MixedPrecisionAdamW`; its sum and the factor are 64-bit, so that finite gradients are
+scaled right whatever their size (the norm itself is returned in FP32, infinite above 3.4e38).  A NaN or infinite gradient
+makes the norm NaN or infinite and, times the factor (NaN or 0), its slot's gradients NaN where they were not finite.
+Subnormal FP32 gradients count as 0 on CUDA, and so do FP32 results that would be subnormal.  Results do not depend on timing
 (``csrc/grad_norm.cu``); on CPU the PyTorch form runs.  Nothing here is differentiable.
 """
 
@@ -73,10 +74,9 @@ def clip_grad_norm_reference(grads: list[Tensor], max_norm, per_slot: bool, grad
     norm = total.sqrt() / grad_scale
     if out is not None:
         bound = max_norm.double().reshape(-1) if isinstance(max_norm, Tensor) else torch.full_like(norm, max_norm)
-        factor = (torch.where(norm + 1e-6 <= bound, torch.ones_like(norm), bound / (norm + 1e-6)) / grad_scale).float()
+        factor = torch.where(norm + 1e-6 <= bound, torch.ones_like(norm), bound / (norm + 1e-6)) / grad_scale
         for g, o in zip(grads, out):
-            wide = torch.promote_types(g.dtype, torch.float32)
-            o.copy_((_groups(g, per_slot, slots).to(wide) * factor[:, None].to(wide)).view(g.shape))
+            o.copy_((_groups(g, per_slot, slots).double() * factor[:, None]).view(g.shape))
     return norm.float() if per_slot else norm.float()[0]
 
 
