@@ -15,6 +15,11 @@ tile of rows holds, and a row takes nothing from another request: an adapter tha
 NaN spoils its own rows and gradients only.  Results do not depend on timing.  On CPU, and as the library
 baseline, the PyTorch form runs, in any floating type.
 
+The rounding of ``u`` and ``du`` is one of range too.  In FP16 a value above 65504 makes its row of ``y`` (``dx``), and its
+slot's ``dB`` (``dA``), infinite or NaN also where they would be finite themselves, never finite and wrong; and below 6e-5, as
+``du`` is while ``B`` is still near zero, steps of 6e-8 are what is left of it: carry a loss scale that keeps ``B^T dy`` above that.
+BF16 has FP32's range.
+
 ``K``, ``N`` and ``R`` are multiples of 8 on CUDA and ``R`` is at most 128; adapters of different ranks share a
 stack by rows and columns of zeros.  A slot without rows has zero gradients.  A parameter's FP32
 ``main_grad`` (``A``, ``B`` and ``W`` alike) is added to in place of a returned gradient.  The gradient of ``W``
