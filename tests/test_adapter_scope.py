@@ -5,7 +5,7 @@ import warnings
 import pytest
 import torch
 
-from bridge_b200.engine import EngineConfig, TPREngine
+from bridge_b200.engine import AdamWConfig, EngineConfig, MixedPrecisionAdamW, TPREngine
 from bridge_b200.models import AdapterSet, build_model, get_config
 from tests.helpers import flat_ppo_loss, rel_err, set_old_log_probs, tree_batch
 
@@ -75,3 +75,35 @@ def test_the_engine_does_not_step_a_model_with_adapters():
     eng.model.requires_grad_(True)
     eng.train_step(batch)
     assert any(not torch.equal(p, q) for p, q in zip(eng.model.parameters(), before))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", ["retain", "recompute"])
+def test_one_slot_through_the_engine_on_gpu(mode):
+    """As above in BF16, into the FP32 accumulators of an optimizer over the adapters: some 40 roundings (half a step: 2^-8)
+    of activations, low-rank values and gradients on the way through three layers, in other places: sqrt(40) 2^-8 = 2.5% of
+    a gradient's length, allowed three times."""
+    cfg = get_config("tiny", hidden_size=512, num_heads=8, num_kv_heads=2, head_dim=128, intermediate_size=1024,
+                     num_layers=3)
+    batch = tree_batch(n_trees=2, prefix=200, siblings=4, resp=96, seed=5)
+    ref = build_model(cfg, device="cuda", seed=0)
+    set_old_log_probs(ref, batch)
+    plain = _filled(ref)
+    with plain.use(1):
+        loss, _ = flat_ppo_loss(ref, batch)
+        loss.backward()
+    eng = TPREngine(cfg, EngineConfig(forest_mode=mode, token_budget=1024), device="cuda",
+                    model=build_model(cfg, device="cuda", seed=0))
+    adapters = _filled(eng.model)
+    optimizer = MixedPrecisionAdamW(adapters, AdamWConfig(grad_clip=0.0))
+    with adapters.use(1):
+        out = eng.forward_backward_batch(batch)
+    assert abs(out["loss"][0] - loss.item()) <= 2e-3 * abs(loss.item()) + 1e-4
+    for (name, p), q in zip(adapters.named_parameters(), plain.parameters()):
+        got, want = p.main_grad[1], q.grad[1].float()
+        assert (p.main_grad[0] == 0).all() and (got - want).norm() <= 0.075 * want.norm(), name
+    before = [p.detach().clone() for p in adapters.parameters()]
+    adapters.clip_grad_norm_(1.0)
+    optimizer.step()
+    assert all(torch.isfinite(p).all() for p in adapters.parameters())
+    assert any(not torch.equal(p[1], q[1]) for p, q in zip(adapters.parameters(), before))
