@@ -11,7 +11,9 @@
 // even a product with zero (which would carry that adapter's infinities over).  The gradients' sums run over rows, so
 // there the blocks of rows end where a slot's rows end, and the rows behind are cleared in both operands.
 //
-// u and du are rounded to the operands' 16 bits once (they feed matrix instructions); every sum is FP32.
+// u and du feed matrix instructions, so they are rounded to the operands' 16 bits, and every sum is FP32.  y and dx take
+// them as they are then, which costs them less than their own rounding; dA and dB, which are made of nothing else, take them in
+// two parts, the rounded value and, rounded too, what it left, or their error would be 1.4 times that of their own rounding.
 #include "adapter_linear.h"
 
 #include <c10/util/Exception.h>
@@ -49,6 +51,22 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, bool half) {
 __device__ __forceinline__ uint16_t pack1(float a, bool half) {
   if (half) return __half_as_ushort(__float2half_rn(a));
   return __bfloat16_as_ushort(__float2bfloat16_rn(a));
+}
+
+// f v as 16-bit values, and what they leave of it.
+__device__ __forceinline__ float unpack1(uint16_t v, bool half) {
+  return half ? __half2float(__ushort_as_half(v)) : __bfloat162float(__ushort_as_bfloat16(v));
+}
+__device__ __forceinline__ uint32_t rest2(float a, float b, uint32_t rounded, bool half) {
+  return pack2(a - unpack1((uint16_t)(rounded & 0xffff), half), b - unpack1((uint16_t)(rounded >> 16), half), half);
+}
+__device__ __forceinline__ uint4 scaled8(const float (&v)[8], float f, bool half) {
+  return make_uint4(pack2(f * v[0], f * v[1], half), pack2(f * v[2], f * v[3], half), pack2(f * v[4], f * v[5], half),
+                    pack2(f * v[6], f * v[7], half));
+}
+__device__ __forceinline__ uint4 rest8(const float (&v)[8], float f, const uint4& r, bool half) {
+  return make_uint4(rest2(f * v[0], f * v[1], r.x, half), rest2(f * v[2], f * v[3], r.y, half),
+                    rest2(f * v[4], f * v[5], r.z, half), rest2(f * v[6], f * v[7], r.w, half));
 }
 
 __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
@@ -111,7 +129,7 @@ __device__ __forceinline__ void joined8(uint32_t part, int at, int ranks, float 
 // ------------------------------------------------------------------------------------------------ shrink
 struct ShrinkParams {
   AdapterPlan plan;
-  uint16_t* u;
+  uint16_t *u, *rest;         // rest: what u's rounding leaves, or null
   const float* scales;
   float scale;
   int T, R, cols, op_bytes, stages, nk, ranks;
@@ -216,9 +234,10 @@ __global__ void __launch_bounds__(kThreads)
     if (__ldg(unit + 4 + r / 32) >> (r % 32) & 1) continue;      // another request's row
     float v[8];
     joined8(base, r * (p.cols + 4) + c, p.ranks, v);
-    *reinterpret_cast<uint4*>(p.u + (size_t)(tile * BM + r) * p.R + c) =
-        make_uint4(pack2(f * v[0], f * v[1], p.half), pack2(f * v[2], f * v[3], p.half),
-                   pack2(f * v[4], f * v[5], p.half), pack2(f * v[6], f * v[7], p.half));
+    const size_t at = (size_t)(tile * BM + r) * p.R + c;
+    const uint4 out = scaled8(v, f, p.half);
+    *reinterpret_cast<uint4*>(p.u + at) = out;
+    if (p.rest) *reinterpret_cast<uint4*>(p.rest + at) = rest8(v, f, out, p.half);
   }
   sm100::cluster_sync();   // the peers' sums stay until all have read them
   if (warp == 1) {
@@ -236,7 +255,7 @@ constexpr int kDotWarps = 4, kDotRows = 4;
 struct DotsParams {
   AdapterPlan plan;
   const uint16_t *x, *op;
-  uint16_t* u;
+  uint16_t *u, *rest;
   const float* scales;
   float scale;
   long ldx;
@@ -332,7 +351,10 @@ __global__ void __launch_bounds__(32 * kDotWarps) adapter_dots_kernel(const Dots
       float t0 = 0.f, t1 = 0.f;
 #pragma unroll
       for (int w = 0; w < kDotWarps; ++w) t0 += sums[w][2 * j], t1 += sums[w][2 * j + 1];
-      *reinterpret_cast<uint32_t*>(p.u + (size_t)(tile * BM + r) * p.R + r0) = pack2(f * t0, f * t1, HALF);
+      const size_t at = (size_t)(tile * BM + r) * p.R + r0;
+      const uint32_t out = pack2(f * t0, f * t1, HALF);
+      *reinterpret_cast<uint32_t*>(p.u + at) = out;
+      if (p.rest) *reinterpret_cast<uint32_t*>(p.rest + at) = rest2(f * t0, f * t1, out, HALF);
     }
   }
 }
@@ -517,9 +539,6 @@ struct TokenParams {
   bool half;
 };
 
-__device__ __forceinline__ float unpack1(uint16_t v, bool half) {
-  return half ? __half2float(__ushort_as_half(v)) : __bfloat162float(__ushort_as_bfloat16(v));
-}
 __device__ __forceinline__ float ld_cluster1(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
@@ -666,10 +685,12 @@ __global__ void __launch_bounds__(kThreads)
     float v[8];
     joined8(base, t * row_floats + BM + at * p.slot_cols + c, p.ranks, v);
     const float f = p.scales ? p.scales[slot] : p.scale;
-    const uint4 out = make_uint4(pack2(f * v[0], f * v[1], p.half), pack2(f * v[2], f * v[3], p.half),
-                                 pack2(f * v[4], f * v[5], p.half), pack2(f * v[6], f * v[7], p.half));
+    const uint4 out = scaled8(v, f, p.half);
     *reinterpret_cast<uint4*>(u + t * p.R + c) = out;
-    if (p.u && blockIdx.x == 0) *reinterpret_cast<uint4*>(p.u + (size_t)t * p.R + c) = out;
+    if (p.u && blockIdx.x == 0) {
+      *reinterpret_cast<uint4*>(p.u + (size_t)t * p.R + c) = out;
+      *reinterpret_cast<uint4*>(p.u + ((size_t)p.T + t) * p.R + c) = rest8(v, f, out, p.half);
+    }
   }
   __syncthreads();
   // this block's columns of y
@@ -1022,7 +1043,8 @@ __global__ void __launch_bounds__(256) adapter_join_kernel(const __grid_constant
 }
 
 // ------------------------------------------------------------------------------------------------ grads
-constexpr int kGradStages = 4;
+// Stages of 32 KB (three, so that two blocks fit an SM), or of 48 where the rank is above 64.
+constexpr int grad_stages(int cols) { return cols == 64 ? 3 : 4; }
 
 struct GradParams {
   AdapterPlan plan;
@@ -1072,19 +1094,19 @@ struct GradTile {
 // shares: D_s [128, R] = sum over slot s's rows of dy^T u (x^T du).  A slot whose rows all fall to one block is written
 // by it at once, from the accumulator, while the next slot's products go into another one; of the slots that begin or end
 // in another block (at most two a block) the partial sums meet in shared memory at the end, in the blocks' order.  Bound
-// like the shrink: 4608 rows of 2560 and 6144 columns, rank 16, 28 us (80 MB); 8192 rows of 9728 and 2560, rank 64, 45 us
-// (201 MB).
+// like the shrink: 4608 rows of 2560 and 6144 columns, rank 16, 32 us (80 MB); 8192 rows of 9728 and 2560, rank 64, 57 us
+// (201 MB); 3.5 and 12 us of it for the second parts of u and du.
 __global__ void __launch_bounds__(kThreads)
     adapter_grads_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_dy,
                          const __grid_constant__ CUtensorMap map_u, const __grid_constant__ CUtensorMap map_du,
                          const GradParams p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int low_bytes = p.cols / 64 * 8192, stage_bytes = kXBytes + low_bytes;
+  const int low_bytes = p.cols / 64 * 8192, stage_bytes = kXBytes + 2 * low_bytes, stages = grad_stages(p.cols);
   const int part_floats = BM * (p.cols + 4), tmem_cols = p.cols == 64 ? 256 : 512;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + max(kGradStages * stage_bytes, 2 * part_floats * 4));
-  uint64_t* empty = full + kGradStages;
-  uint64_t* tfull = empty + kGradStages;     // of the three accumulators
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + max(stages * stage_bytes, 2 * part_floats * 4));
+  uint64_t* empty = full + stages;
+  uint64_t* tfull = empty + stages;     // of the three accumulators
   uint64_t* tempty = tfull + 3;
   uint32_t* tmem_word = reinterpret_cast<uint32_t*>(tempty + 3);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -1101,7 +1123,7 @@ __global__ void __launch_bounds__(kThreads)
   const bool began = b1 > b0 && __ldg(p.plan.block_start + __ldg(&blocks[b0]).z) < b0;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kGradStages; ++s) {
+    for (int s = 0; s < stages; ++s) {
       sm100::mbar_init(&full[s], 1);
       sm100::mbar_init(&empty[s], 1);
     }
@@ -1133,9 +1155,9 @@ __global__ void __launch_bounds__(kThreads)
         sm100::mbar_expect_tx(&full[stage], stage_bytes);
         sm100::tma_load_2d(dst, map_wide, &full[stage], g.m0, row);
         sm100::tma_load_2d(dst + 8192, map_wide, &full[stage], g.m0 + 64, row);
-        for (int i = 0; i < p.cols / 64; ++i)
-          sm100::tma_load_2d(dst + kXBytes + i * 8192, map_thin, &full[stage], 64 * i, row);
-        if (++stage == kGradStages) stage = 0, phase ^= 1;
+        for (int i = 0; i < p.cols / 32; ++i)      // both parts of u
+          sm100::tma_load_3d(dst + kXBytes + i * 8192, map_thin, &full[stage], i % (p.cols / 64) * 64, row, i / (p.cols / 64));
+        if (++stage == stages) stage = 0, phase ^= 1;
       }
     }
   } else if (warp == 1) {
@@ -1160,7 +1182,7 @@ __global__ void __launch_bounds__(kThreads)
       if (n < steps * 16) {
         // rows of other requests behind the block: a row is 128 bytes of every 64 columns, in whatever order
         const int lines = (steps * 16 - n) * 8;
-        for (int i = lane; i < lines * (2 + p.cols / 64); i += 32)
+        for (int i = lane; i < lines * (2 + p.cols / 32); i += 32)
           *reinterpret_cast<uint4*>(at + i / lines * 8192 + n * 128 + i % lines * 16) = make_uint4(0, 0, 0, 0);
         sm100::fence_proxy_async_smem();
       }
@@ -1169,12 +1191,15 @@ __global__ void __launch_bounds__(kThreads)
         sm100::tc_fence_after();
         const uint32_t a = sm100::smem_addr(at), w = a + kXBytes;
         for (int kk = 0; kk < steps; ++kk)
-          sm100::umma_bf16(tmem + acc * p.cols, sm100::umma_desc_sw128(a + kk * 2048, 8192, 1024),
-                           sm100::umma_desc_sw128(w + kk * 2048, 8192, 1024), p.idesc, !fresh || kk > 0);
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+            sm100::umma_bf16(tmem + acc * p.cols, sm100::umma_desc_sw128(a + kk * 2048, 8192, 1024),
+                             sm100::umma_desc_sw128(w + half * low_bytes + kk * 2048, 8192, 1024), p.idesc,
+                             !fresh || kk > 0 || half > 0);
         sm100::umma_commit(&empty[stage]);
       }
       __syncwarp();
-      if (++stage == kGradStages) stage = 0, phase ^= 1;
+      if (++stage == stages) stage = 0, phase ^= 1;
     }
     if (slot >= 0 && lane == 0) sm100::umma_commit(&tfull[acc]);
   } else {
@@ -1383,6 +1408,9 @@ int split(void (*kernel)(P...), int smem, int columns, int clusters, int nk) {
   return ranks;
 }
 
+uint16_t* rest_of(const AdapterProduct& a) {
+  return a.keep_u ? static_cast<uint16_t*>(a.u) + (size_t)a.T * a.R : nullptr;
+}
 
 template <bool OP_MN>
 cudaError_t run_shrink(const AdapterProduct& a, cudaStream_t stream) {
@@ -1393,7 +1421,7 @@ cudaError_t run_shrink(const AdapterProduct& a, cudaStream_t stream) {
     return cudaErrorInvalidValue;
   ShrinkParams p{};
   p.plan = a.plan;
-  p.u = static_cast<uint16_t*>(a.u);
+  p.u = static_cast<uint16_t*>(a.u), p.rest = rest_of(a);
   p.scales = a.scales, p.scale = a.scale;
   p.T = a.T, p.R = a.R, p.cols = cols;
   p.op_bytes = cols * 128;
@@ -1413,6 +1441,7 @@ cudaError_t run_dots(const AdapterProduct& a, cudaStream_t stream) {
   DotsParams p{};
   p.plan = a.plan;
   p.x = static_cast<const uint16_t*>(a.x), p.op = static_cast<const uint16_t*>(a.op), p.u = static_cast<uint16_t*>(a.u);
+  p.rest = rest_of(a);
   p.scales = a.scales, p.scale = a.scale;
   p.ldx = a.ldx, p.K = a.K, p.R = a.R;
   const dim3 grid(a.plan.num_units * (a.R / 2), (a.T + kDotRows - 1) / kDotRows);
@@ -1599,8 +1628,8 @@ cudaError_t launch_adapter_grads(const AdapterGrads& a, cudaStream_t stream) {
   // (an operand that is not asked for has no pointer: any valid map stands in for its own)
   const bool ok = encode(&x, a.da ? a.x : a.dy, a.da ? a.K : a.N, a.T, a.da ? a.ldx : a.lddy, 0, 64, a.half) &&
                   encode(&dy, a.db ? a.dy : a.x, a.db ? a.N : a.K, a.T, a.db ? a.lddy : a.ldx, 0, 64, a.half) &&
-                  encode(&u, a.db ? a.u : a.du, a.R, a.T, a.R, 0, 64, a.half) &&
-                  encode(&du, a.da ? a.du : a.u, a.R, a.T, a.R, 0, 64, a.half);
+                  encode(&u, a.db ? a.u : a.du, a.R, a.T, a.R, 2, 64, a.half) &&
+                  encode(&du, a.da ? a.du : a.u, a.R, a.T, a.R, 2, 64, a.half);
   if (!ok) return cudaErrorInvalidValue;
   GradParams p{};
   p.plan = a.plan;
@@ -1611,11 +1640,10 @@ cudaError_t launch_adapter_grads(const AdapterGrads& a, cudaStream_t stream) {
   p.tiles_b = a.db ? (a.N + BM - 1) / BM : 0;
   p.idesc = sm100::umma_idesc_bf16(BM, p.cols, true, true) & ~(a.half ? sm100::kIdescBf16 : 0u);
   p.add_a = a.add_a, p.add_b = a.add_b, p.half = a.half;
-  int smem = std::max(kGradStages * (kXBytes + p.cols * 128), 2 * BM * (p.cols + 4) * 4) + 256 + 1024;
+  const int smem = std::max(grad_stages(p.cols) * (kXBytes + p.cols * 256), 2 * BM * (p.cols + 4) * 4) + 256 + 1024;
   // Blocks that hold all of an SM's TMEM have the SM for themselves: of two clusters that wait for each other's, each in
-  // another SM, neither would end.  (All other blocks here take 69 KB of shared memory
-  // or more, 80 with 256 columns: what room there is for blocks is room for their columns.)
-  if (p.cols > 64) smem = std::max(smem, 160 * 1024);
+  // another SM, neither would end.  (With 512 columns they take 193 KB of shared memory, with 256 97; all other blocks here
+  // 69 KB or more, 80 with 256 columns: what room there is for blocks is room for their columns.)
   static std::atomic<unsigned long long> done{0};
   e = allow_smem(adapter_grads_kernel, kMaxSmem, done);
   if (e != cudaSuccess) return e;

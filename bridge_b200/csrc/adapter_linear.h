@@ -28,7 +28,7 @@ struct AdapterProduct {
   const void* op;          // [S, R, K], or [S, K, R] with `mn`
   const void* w;           // [N, K], or [K, N]; row stride ldw
   const void* low;         // [S, N, R], or [S, R, N]
-  void *u, *y;             // [T, R], [T, N]
+  void *u, *y;             // [T, R] (with keep_u [2, T, R]: and what u's rounding left, rounded too), [T, N]
   void* workspace;
   const float* scales;     // [S], or null: `scale`
   float scale;
@@ -46,7 +46,7 @@ struct AdapterNeeds {
 // db[s, n, r] = sum_t dy[t, n] u[t, r],  da[s, r, k] = sum_t du[t, r] x[t, k] over the rows of slot s
 struct AdapterGrads {
   const void *x, *dy;      // [T, K], [T, N]
-  const void *u, *du;      // [T, R]
+  const void *u, *du;      // [2, T, R], as above
   void *da, *db;           // null: not asked for
   bool add_a, add_b;       // FP32, added to; else the inputs' type, written
   long ldx, lddy;

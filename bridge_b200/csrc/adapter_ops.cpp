@@ -49,7 +49,7 @@ struct Products {
 };
 
 // u = scale A x and y = W x + B u from (x, W, A, B); with `mn` du = scale B^T dy and dx = W^T dy + A^T du from
-// (dy, W, B, A).
+// (dy, W, B, A).  u is for the gradients, in two parts.
 Products products(const torch::Tensor& x, const torch::Tensor& w, const torch::Tensor& op, const torch::Tensor& low, bool mn,
                   bool want_u, bool want_y, const torch::Tensor& buf, const Meta& meta, double scale,
                   const OptTensor& scales) {
@@ -68,7 +68,7 @@ Products products(const torch::Tensor& x, const torch::Tensor& w, const torch::T
   const bb::AdapterNeeds needs = want_y ? bb::adapter_product_needs(a) : bb::AdapterNeeds{true, 0};
   Products out;
   if (needs.u) {
-    out.u = at::empty({a.T, a.R}, opts);
+    out.u = at::empty({want_u ? 2 : 1, a.T, a.R}, opts);
     a.u = out.u.data_ptr();
   }
   if (!want_y) {

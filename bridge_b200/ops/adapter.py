@@ -10,7 +10,7 @@ policy next to the policies that are trained from it).  With ``W [N, K]`` and a 
 
 :func:`adapter_rows` lays out once per batch which rows use which slot; every projection of the model takes
 the same plan.  On CUDA (``csrc/adapter_linear.cu``; BF16 or FP16, sums in FP32, ``u`` and ``du`` rounded to
-the inputs' type) the low-rank products join the projection's own accumulators, whatever mix of slots a
+the inputs' type for ``y`` and ``dx``, in two parts of it for ``dB`` and ``dA``) the low-rank products join the projection's own accumulators, whatever mix of slots a
 tile of rows holds, and a row takes nothing from another request: an adapter that has gone to infinity or
 NaN spoils its own rows and gradients only.  Results do not depend on timing.  On CPU, and as the library
 baseline, the PyTorch form runs, in any floating type.
