@@ -1094,8 +1094,8 @@ struct GradTile {
 // shares: D_s [128, R] = sum over slot s's rows of dy^T u (x^T du).  A slot whose rows all fall to one block is written
 // by it at once, from the accumulator, while the next slot's products go into another one; of the slots that begin or end
 // in another block (at most two a block) the partial sums meet in shared memory at the end, in the blocks' order.  Bound
-// like the shrink: 4608 rows of 2560 and 6144 columns, rank 16, 32 us (80 MB); 8192 rows of 9728 and 2560, rank 64, 57 us
-// (201 MB); 3.5 and 12 us of it for the second parts of u and du.
+// like the shrink: alone and with nothing in L2, 4608 rows of 2560 and 6144 columns, rank 16, 33 us (80 MB); 8192 rows of 9728
+// and 2560, rank 64, 71 us (201 MB); 3.5 and 12 us of it for the second parts of u and du.
 __global__ void __launch_bounds__(kThreads)
     adapter_grads_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_dy,
                          const __grid_constant__ CUtensorMap map_u, const __grid_constant__ CUtensorMap map_du,
